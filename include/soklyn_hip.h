@@ -227,6 +227,97 @@ int32_t skl_dense_error_from_sum_noalloc(skl_ctx *ctx, const skl_dense_desc *blk
  * accumulation as backward_wmma.cu:39-63). */
 int32_t skl_dense_input_grad(skl_ctx *ctx, const skl_dense_desc *blk, uint32_t batch, float *dx);
 
+/* ---- residual joins (no counterpart in the reference) ------------------------ */
+/* The join between two blocks of a residual network, one kernel:
+ *   u = post(y)                        the norm behind the block whose output y is
+ *   h = scale * x + gate_act(gate) * u the residual stream, rounded to its type
+ *   n = pre(h)                         the norm before the next block, of h as stored
+ * y, n, gate and the norm parameters are T of `dtype`, the stream x and h of
+ * `stream_dtype` (SKL_F32, or SKL_F16 with fp16 blocks); all are [rows x cols]
+ * row-major but gate [gate_rows x cols], gate_rows 1 (one gate for every row) or
+ * rows, and the norm parameters [1 x cols].  Norms are SKL_NORM_DISABLED, _RMS
+ * (weight) or _LAYER (weight and bias), with the blocks' 1e-6 under the root;
+ * gate_act is Identity, Sigmoid or Tanh.  x NULL: no stream yet (h = gate * u).
+ * y NULL: no block yet (h = scale * x; no post norm, no gate).  gate NULL with
+ * gate_rows 0: a gate of 1.  h NULL: not stored.  n NULL: no norm before (pre_norm
+ * is not looked at).  stats (fp32 [4 x rows], or NULL): mean and 1/deviation of y's
+ * norm, then of h's, as the backward reads them (0 and 1 where there is none).
+ * h may be x and n may be y, in place; no other output may overlap an input.
+ * 1 <= cols <= 8192. */
+int32_t skl_residual_forward(skl_ctx *ctx, uint32_t dtype, uint32_t stream_dtype, uint32_t rows, uint32_t cols,
+                             uint32_t post_norm, uint32_t pre_norm, uint32_t gate_act, uint32_t gate_rows,
+                             float scale, const void *x, const void *y, const void *gate, const void *post_w,
+                             const void *post_b, const void *pre_w, const void *pre_b, void *h, void *n,
+                             float *stats);
+/* Its backward, from dn (the gradient of n; NULL: n was not used) and dh (the
+ * gradient that reaches h from behind; NULL: none), h, y and stats as the forward
+ * left them: dx = scale * d, dy (what skl_dense_error_from_sum takes for the block
+ * that made y), dgate [gate_rows x cols], and dparam [4 x cols]: the gradients of
+ * post_w, post_b, pre_w and pre_b summed over the rows (zeros where there is no such
+ * parameter).  Gradients are fp32 and linear in dn and dh (a loss scale passes
+ * through).  Any output may be NULL.  work: skl_residual_work_bytes(rows, cols) bytes
+ * of the caller's, 4-byte aligned, for the column sums (dparam, and dgate of one gate
+ * row); NULL where none is wanted.  What it holds does not outlive the call; calls that
+ * overlap in time need a work of their own.  dx may be dh, in place; no other output
+ * may overlap an input. */
+int32_t skl_residual_backward(skl_ctx *ctx, uint32_t dtype, uint32_t stream_dtype, uint32_t rows, uint32_t cols,
+                              uint32_t post_norm, uint32_t pre_norm, uint32_t gate_act, uint32_t gate_rows,
+                              float scale, const void *h, const void *y, const void *gate, const void *post_w,
+                              const void *post_b, const void *pre_w, const float *stats, const float *dn,
+                              const float *dh, float *dx, float *dy, float *dgate, float *dparam, void *work,
+                              size_t work_bytes);
+/* Host side; 0 where rows or cols is. */
+size_t skl_residual_work_bytes(uint32_t rows, uint32_t cols);
+
+/* ---- distillation (no counterpart in the reference) -------------------------- */
+/* skl_dense_output_error for a head that learns from a teacher's top logits.
+ * blk: an output layer without a norm whose activation is Identity, so that the
+ * first `rows` rows of out hold its logits z.  The teacher: `top` classes and their
+ * logits per row (int32 top_index, fp32 top_logit, [rows x top], top <= 1024); a slot
+ * whose class is not in [0, outputs) is empty, classes may repeat (their shares add
+ * up).  label (int32 [rows]; a value outside [0, outputs): no label), needed where
+ * alpha < 1.  With t = temperature, q = softmax(top_logit / t) over the held slots,
+ * p = softmax(z / t), p1 = softmax(z):
+ *   loss = alpha t^2 sum q log(q / p) - (1 - alpha) log p1[label]
+ *   d loss / d z = alpha t (p - q) + (1 - alpha) (p1 - [label])
+ * The gradient times LOSS_SCALE goes to grad and d_prenorm (and d_prenorm_h), as
+ * skl_dense_backward and the layer below read it; loss (fp32 [rows], or NULL) is
+ * unscaled.  A row without held slots has no first term, without a label no second,
+ * and a row whose logits are all -inf neither.  out is left as it is; rows past
+ * `rows` are neither read nor written. */
+int32_t skl_dense_distill_error(skl_ctx *ctx, const skl_dense_desc *blk, const void *top_index,
+                                const float *top_logit, uint32_t top, const void *label, uint32_t rows,
+                                float temperature, float alpha, float *loss);
+
+/* ---- 4-bit microscaled floats (no counterpart in the reference) -------------- */
+/* A matrix of n vectors of k elements as MXFP4: codes [n x kp / 2] bytes (16-byte
+ * aligned) and scales [n x kp / 32] bytes (4-byte aligned), kp = k rounded up to 128.
+ * Element i of a vector is the low (i even) or high half of byte i / 2: sign, two
+ * exponent bits, one mantissa bit (0, 0.5, 1, 1.5, 2, 3, 4, 6), times 2^(s - 127) with
+ * s the scale byte of its block of 32.  s is 2 below the exponent of the block's
+ * largest magnitude (0 at the least); elements round to the nearest code, ties to the
+ * even one, past 6 to 6.  A block with an infinity or NaN has s = 255 and stands for
+ * NaN.  Elements past k are 0.
+ * The vectors are the rows of src [rows x cols] (down = 0) or its columns (down = 1:
+ * the weights [inputs x outputs] of a block). */
+int32_t skl_mxfp4_quantise(skl_ctx *ctx, const void *src, uint32_t dtype, uint32_t rows, uint32_t cols,
+                           uint32_t down, void *codes, void *scales);
+/* The values, rounded to dtype, into dst [rows x cols]. */
+int32_t skl_mxfp4_dequantise(skl_ctx *ctx, const void *codes, const void *scales, uint32_t rows, uint32_t cols,
+                             uint32_t down, void *dst, uint32_t dtype);
+/* skl_dense_forward of a block that is only used, with 4-bit weights: w_codes and
+ * w_scales are its W [inputs x outputs] quantised down, the input is quantised along
+ * its rows on the way, Z = Q(in) . Q(W) (+b) is summed in fp32, then norm and
+ * activation (no dropout).  blk->w may be NULL.  Without a norm only out is written.
+ * in may not overlap what is written.  work: skl_mxfp4_work_bytes(inputs, batch) bytes
+ * of the caller's, 16-byte aligned; what it holds does not outlive the call, and calls
+ * that overlap in time need a work of their own (as they need an out of their own). */
+int32_t skl_dense_forward_mxfp4(skl_ctx *ctx, const skl_dense_desc *blk, const void *in, uint32_t in_rows,
+                                uint32_t in_cols, uint32_t batch, const void *w_codes, const void *w_scales,
+                                void *work, size_t work_bytes);
+/* Host side. */
+size_t skl_mxfp4_work_bytes(uint32_t inputs, uint32_t batch);
+
 #ifdef __cplusplus
 }
 #endif

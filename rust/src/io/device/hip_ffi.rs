@@ -137,4 +137,27 @@ extern "C" {
     pub fn skl_dense_error_from_sum_noalloc(ctx: *mut SklCtx, blk: *const SklDenseDesc, s: *const f32,
                                             batch: u32) -> i32;
     pub fn skl_dense_input_grad(ctx: *mut SklCtx, blk: *const SklDenseDesc, batch: u32, dx: *mut f32) -> i32;
+    pub fn skl_residual_forward(ctx: *mut SklCtx, dtype: u32, stream_dtype: u32, rows: u32, cols: u32,
+                                post_norm: u32, pre_norm: u32, gate_act: u32, gate_rows: u32, scale: f32,
+                                x: *const c_void, y: *const c_void, gate: *const c_void, post_w: *const c_void,
+                                post_b: *const c_void, pre_w: *const c_void, pre_b: *const c_void,
+                                h: *mut c_void, n: *mut c_void, stats: *mut f32) -> i32;
+    pub fn skl_residual_backward(ctx: *mut SklCtx, dtype: u32, stream_dtype: u32, rows: u32, cols: u32,
+                                 post_norm: u32, pre_norm: u32, gate_act: u32, gate_rows: u32, scale: f32,
+                                 h: *const c_void, y: *const c_void, gate: *const c_void, post_w: *const c_void,
+                                 post_b: *const c_void, pre_w: *const c_void, stats: *const f32, dn: *const f32,
+                                 dh: *const f32, dx: *mut f32, dy: *mut f32, dgate: *mut f32, dparam: *mut f32,
+                                 work: *mut c_void, work_bytes: usize) -> i32;
+    pub fn skl_residual_work_bytes(rows: u32, cols: u32) -> usize;
+    pub fn skl_dense_distill_error(ctx: *mut SklCtx, blk: *const SklDenseDesc, top_index: *const c_void,
+                                   top_logit: *const f32, top: u32, label: *const c_void, rows: u32,
+                                   temperature: f32, alpha: f32, loss: *mut f32) -> i32;
+    pub fn skl_mxfp4_quantise(ctx: *mut SklCtx, src: *const c_void, dtype: u32, rows: u32, cols: u32, down: u32,
+                              codes: *mut c_void, scales: *mut c_void) -> i32;
+    pub fn skl_mxfp4_dequantise(ctx: *mut SklCtx, codes: *const c_void, scales: *const c_void, rows: u32,
+                                cols: u32, down: u32, dst: *mut c_void, dtype: u32) -> i32;
+    pub fn skl_dense_forward_mxfp4(ctx: *mut SklCtx, blk: *const SklDenseDesc, input: *const c_void,
+                                   in_rows: u32, in_cols: u32, batch: u32, w_codes: *const c_void,
+                                   w_scales: *const c_void, work: *mut c_void, work_bytes: usize) -> i32;
+    pub fn skl_mxfp4_work_bytes(inputs: u32, batch: u32) -> usize;
 }

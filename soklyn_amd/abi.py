@@ -85,6 +85,20 @@ _SIGS = {
     "skl_dense_error_from_sum": (C.c_int32, [_VP, C.POINTER(SklDenseDesc), _VP, C.c_uint32]),
     "skl_dense_error_from_sum_noalloc": (C.c_int32, [_VP, C.POINTER(SklDenseDesc), _VP, C.c_uint32]),
     "skl_dense_input_grad": (C.c_int32, [_VP, C.POINTER(SklDenseDesc), C.c_uint32, _VP]),
+    "skl_residual_forward": (C.c_int32, [_VP, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32,
+                                         C.c_uint32, C.c_uint32, C.c_uint32, C.c_float, _VP, _VP, _VP, _VP, _VP,
+                                         _VP, _VP, _VP, _VP, _VP]),
+    "skl_residual_backward": (C.c_int32, [_VP, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32,
+                                          C.c_uint32, C.c_uint32, C.c_uint32, C.c_float, _VP, _VP, _VP, _VP,
+                                          _VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, C.c_size_t]),
+    "skl_residual_work_bytes": (C.c_size_t, [C.c_uint32, C.c_uint32]),
+    "skl_dense_distill_error": (C.c_int32, [_VP, C.POINTER(SklDenseDesc), _VP, _VP, C.c_uint32, _VP, C.c_uint32,
+                                            C.c_float, C.c_float, _VP]),
+    "skl_mxfp4_quantise": (C.c_int32, [_VP, _VP, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32, _VP, _VP]),
+    "skl_mxfp4_dequantise": (C.c_int32, [_VP, _VP, _VP, C.c_uint32, C.c_uint32, C.c_uint32, _VP, C.c_uint32]),
+    "skl_dense_forward_mxfp4": (C.c_int32, [_VP, C.POINTER(SklDenseDesc), _VP, C.c_uint32, C.c_uint32,
+                                            C.c_uint32, _VP, _VP, _VP, C.c_size_t]),
+    "skl_mxfp4_work_bytes": (C.c_size_t, [C.c_uint32, C.c_uint32]),
 }
 
 EXPORTED = tuple(_SIGS)
@@ -143,6 +157,14 @@ def train_ctx(opt: SklOptimiser, norm_opt: SklOptimiser, batch_size: int, learn_
     return SklTrainCtx(opt, norm_opt, batch_size, learn_rate, grad_clamp)
 
 
+def need(name: str, t, dtype, shape: tuple, device: int) -> int:
+    """The address of tensor t, which has to be contiguous, of this type and shape and on GPU `device`."""
+    if t.dtype is not dtype or t.shape != shape or not t.is_contiguous() or t.get_device() != device:
+        raise ValueError(f"{name}: a contiguous {dtype} tensor {list(shape)} on GPU {device} is wanted, "
+                         f"got {t.dtype} {list(t.shape)} on {t.device}, strides {t.stride()}")
+    return t.data_ptr()
+
+
 class Context:
     """GpuContext (src/io/device.rs:22-183) over the C ABI."""
 
@@ -150,6 +172,7 @@ class Context:
         h = C.c_void_p()
         call("skl_ctx_create", ordinal, tile_dim, C.byref(h))
         self.h = h
+        self.device = ordinal
         if stream is not None:
             call("skl_ctx_set_stream", self.h, C.c_void_p(stream))
 

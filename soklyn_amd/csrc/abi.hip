@@ -17,8 +17,11 @@
 #include <hip/hip_runtime.h>
 
 #include "../../include/soklyn_hip.h"
+#include "distill.h"
 #include "gemm_cost.h"
 #include "launch.h"
+#include "mxfp4.h"
+#include "residual.h"
 
 using namespace skl;
 
@@ -1700,6 +1703,309 @@ int32_t skl_dense_input_grad(skl_ctx *ctx, const skl_dense_desc *b, uint32_t bat
             c.valid = false;
         else
             c.call = ctx->calls;
+    }
+    return finish(ctx);
+}
+
+// ---- residual joins -------------------------------------------------------------------
+// The checks of these operators come before anything that needs the context or the device.
+
+static bool aligned_to(const void *p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
+
+namespace {
+
+struct Span {
+    const void *p;
+    size_t bytes;
+};
+
+// No written span may overlap a read one, except where the two are the same buffer and the pair is
+// `same` (a call that can run in place).
+bool spans_clash(const Span *out, size_t outs, const Span *in, size_t ins, const void *same_out0 = nullptr,
+                 const void *same_out1 = nullptr) {
+    for (size_t i = 0; i < outs; ++i)
+        for (size_t j = 0; j < ins; ++j) {
+            const bool in_place = (i == 0 && j == 0 && same_out0 && in[0].p == same_out0 && out[0].p == same_out0) ||
+                                  (i == 1 && j == 1 && same_out1 && in[1].p == same_out1 && out[1].p == same_out1);
+            if (!in_place && overlaps(out[i].p, out[i].bytes, in[j].p, in[j].bytes)) return true;
+        }
+    return false;
+}
+
+bool outputs_clash(const Span *out, size_t outs) {
+    for (size_t i = 0; i < outs; ++i)
+        for (size_t j = i + 1; j < outs; ++j)
+            if (overlaps(out[i].p, out[i].bytes, out[j].p, out[j].bytes)) return true;
+    return false;
+}
+
+// What the join and its backward check alike.
+int32_t check_join(uint32_t dtype, uint32_t stream_dtype, uint32_t rows, uint32_t cols, uint32_t post, uint32_t pre,
+                   uint32_t gate_act, uint32_t gate_rows, float scale, const void *y, const void *gate,
+                   const void *post_w, const void *post_b, bool with_pre, const void *pre_w) {
+    SKL_CHECK(dtype <= SKL_F16 && stream_dtype <= dtype, SKL_ERR_INVALID_CONFIGURATION);
+    SKL_CHECK(cols > 0 && cols <= kJoinCols, SKL_ERR_INVALID_CONFIGURATION);
+    SKL_CHECK(rows > 0, SKL_ERR_INVALID_BATCH_SIZE);
+    SKL_CHECK(post <= SKL_NORM_LAYER && (!with_pre || pre <= SKL_NORM_LAYER), SKL_ERR_INVALID_CONFIGURATION);
+    SKL_CHECK(gate_act == SKL_ACT_IDENTITY || gate_act == SKL_ACT_SIGMOID || gate_act == SKL_ACT_TANH,
+              SKL_ERR_INVALID_CONFIGURATION);
+    SKL_CHECK(std::isfinite(scale), SKL_ERR_INVALID_CONFIGURATION);
+    SKL_CHECK(y || (post == SKL_NORM_DISABLED && !gate), SKL_ERR_INVALID_CONFIGURATION);
+    SKL_CHECK(gate ? gate_rows == 1 || gate_rows == rows : gate_rows == 0, SKL_ERR_MISMATCHED_DIMENSIONS);
+    SKL_CHECK(post == SKL_NORM_DISABLED || post_w, SKL_ERR_NULL_POINTER);
+    SKL_CHECK(post != SKL_NORM_LAYER || post_b, SKL_ERR_NULL_POINTER);
+    SKL_CHECK(!with_pre || pre == SKL_NORM_DISABLED || pre_w, SKL_ERR_NULL_POINTER);
+    return SKL_OK;
+}
+
+}  // namespace
+
+int32_t skl_residual_forward(skl_ctx *ctx, uint32_t dtype, uint32_t stream_dtype, uint32_t rows, uint32_t cols,
+                             uint32_t post_norm, uint32_t pre_norm, uint32_t gate_act, uint32_t gate_rows,
+                             float scale, const void *x, const void *y, const void *gate, const void *post_w,
+                             const void *post_b, const void *pre_w, const void *pre_b, void *h, void *n,
+                             float *stats) {
+    SKL_CHECK(ctx, SKL_ERR_NULL_POINTER);
+    int32_t r;
+    if ((r = check_join(dtype, stream_dtype, rows, cols, post_norm, pre_norm, gate_act, gate_rows, scale, y, gate,
+                        post_w, post_b, n != nullptr, pre_w)))
+        return r;
+    SKL_CHECK(!n || pre_norm != SKL_NORM_LAYER || pre_b, SKL_ERR_NULL_POINTER);
+    SKL_CHECK((x || y) && (h || n), SKL_ERR_NULL_POINTER);
+    const size_t t = dtype == SKL_F16 ? 2 : 4, st = stream_dtype == SKL_F16 ? 2 : 4, e = (size_t)rows * cols;
+    const Span out[] = {{h, e * st}, {n, e * t}, {stats, (size_t)rows * 16}};
+    const Span in[] = {{x, e * st}, {y, e * t}, {gate, gate_rows * (size_t)cols * t},
+                       {post_w, cols * t}, {post_b, cols * t}, {pre_w, cols * t}, {pre_b, cols * t}};
+    SKL_CHECK(!spans_clash(out, 3, in, 7, x, y) && !outputs_clash(out, 3), SKL_ERR_INVALID_CONFIGURATION);
+    if ((r = enter(ctx))) return r;
+    JoinArgs a{};
+    a.rows = rows;
+    a.cols = cols;
+    a.post = post_norm;
+    a.pre = pre_norm;
+    a.gate_act = gate_act;
+    a.gate_rows = gate_rows;
+    a.scale = scale;
+    a.x = x;
+    a.y = y;
+    a.gate = gate;
+    a.post_w = post_w;
+    a.post_b = post_b;
+    a.pre_w = pre_w;
+    a.pre_b = pre_b;
+    a.h = h;
+    a.n = n;
+    a.stats = stats;
+    SKL_TRY(launch_join(a, dtype, stream_dtype, ctx->stream));
+    return finish(ctx);
+}
+
+size_t skl_residual_work_bytes(uint32_t rows, uint32_t cols) {
+    return rows && cols ? (size_t)residual_planes(rows, cols) * kPlanes * cols * sizeof(float) : 0;
+}
+
+int32_t skl_residual_backward(skl_ctx *ctx, uint32_t dtype, uint32_t stream_dtype, uint32_t rows, uint32_t cols,
+                              uint32_t post_norm, uint32_t pre_norm, uint32_t gate_act, uint32_t gate_rows,
+                              float scale, const void *h, const void *y, const void *gate, const void *post_w,
+                              const void *post_b, const void *pre_w, const float *stats, const float *dn,
+                              const float *dh, float *dx, float *dy, float *dgate, float *dparam, void *work,
+                              size_t work_bytes) {
+    SKL_CHECK(ctx, SKL_ERR_NULL_POINTER);
+    int32_t r;
+    if ((r = check_join(dtype, stream_dtype, rows, cols, post_norm, pre_norm, gate_act, gate_rows, scale, y, gate,
+                        post_w, post_b, dn != nullptr, pre_w)))
+        return r;
+    SKL_CHECK(stats && (dn || dh), SKL_ERR_NULL_POINTER);
+    SKL_CHECK(!dn || pre_norm == SKL_NORM_DISABLED || h, SKL_ERR_NULL_POINTER);
+    SKL_CHECK((!dy || y) && (!dgate || gate), SKL_ERR_NULL_POINTER);
+    const bool sums = dparam || (dgate && gate_rows == 1);
+    SKL_CHECK(!sums || work, SKL_ERR_NULL_POINTER);
+    SKL_CHECK(!sums || work_bytes >= skl_residual_work_bytes(rows, cols), SKL_ERR_ALLOCATION_LIMIT);
+    SKL_CHECK(!sums || aligned_to(work, 4), SKL_ERR_HARDWARE_CONSTRAINT);
+    const size_t t = dtype == SKL_F16 ? 2 : 4, st = stream_dtype == SKL_F16 ? 2 : 4, e = (size_t)rows * cols;
+    const Span out[] = {{dx, e * 4}, {dy, e * 4}, {dgate, gate_rows * (size_t)cols * 4}, {dparam, (size_t)cols * 16},
+                        {sums ? work : nullptr, skl_residual_work_bytes(rows, cols)}};
+    const Span in[] = {{dh, e * 4}, {dn, e * 4}, {h, e * st}, {y, e * t}, {gate, gate_rows * (size_t)cols * t},
+                       {post_w, cols * t}, {post_b, cols * t}, {pre_w, cols * t}, {stats, (size_t)rows * 16}};
+    SKL_CHECK(!spans_clash(out, 5, in, 9, dh) && !outputs_clash(out, 5), SKL_ERR_INVALID_CONFIGURATION);
+    if ((r = enter(ctx))) return r;
+    UnjoinArgs a{};
+    a.rows = rows;
+    a.cols = cols;
+    a.post = post_norm;
+    a.pre = dn ? pre_norm : 0;
+    a.gate_act = gate_act;
+    a.gate_rows = gate_rows;
+    a.scale = scale;
+    a.h = h;
+    a.y = y;
+    a.gate = gate;
+    a.post_w = post_w;
+    a.post_b = post_b;
+    a.pre_w = pre_w;
+    a.stats = stats;
+    a.dn = dn;
+    a.dh = dh;
+    a.dx = dx;
+    a.dy = dy;
+    a.dgate = dgate && gate_rows > 1 ? dgate : nullptr;
+    a.gate_sum = dgate && gate_rows == 1 ? dgate : nullptr;
+    a.dparam = dparam;
+    a.planes = (dparam && a.post ? 1u : 0u) | (dparam && a.post == SKL_NORM_LAYER ? 2u : 0u) |
+               (dparam && a.pre ? 4u : 0u) | (dparam && a.pre == SKL_NORM_LAYER ? 8u : 0u) | (a.gate_sum ? 16u : 0u);
+    a.work = sums ? reinterpret_cast<float *>(work) : nullptr;
+    SKL_TRY(launch_unjoin(a, dtype, stream_dtype, ctx->stream));
+    return finish(ctx);
+}
+
+// ---- distillation ---------------------------------------------------------------------
+
+int32_t skl_dense_distill_error(skl_ctx *ctx, const skl_dense_desc *b, const void *top_index, const float *top_logit,
+                                uint32_t top, const void *label, uint32_t rows, float temperature, float alpha,
+                                float *loss) {
+    SKL_CHECK(ctx && b, SKL_ERR_NULL_POINTER);
+    SKL_CHECK(b->dtype <= SKL_F16 && b->outputs > 0 && b->max_batch > 0, SKL_ERR_INVALID_CONFIGURATION);
+    SKL_CHECK(b->norm == SKL_NORM_DISABLED && b->act == SKL_ACT_IDENTITY, SKL_ERR_INVALID_CONFIGURATION);
+    SKL_CHECK(b->is_training, SKL_ERR_TRAINING_MODE_REQUIRED);
+    SKL_CHECK(rows > 0, SKL_ERR_INVALID_BATCH_SIZE);
+    SKL_CHECK(rows <= b->max_batch, SKL_ERR_ALLOCATION_LIMIT);
+    SKL_CHECK(b->outputs <= 0x7fffffffu && top <= kDistillTop, SKL_ERR_INVALID_CONFIGURATION);
+    SKL_CHECK(std::isfinite(temperature) && temperature > 0.0f, SKL_ERR_INVALID_CONFIGURATION);
+    SKL_CHECK(alpha >= 0.0f && alpha <= 1.0f, SKL_ERR_INVALID_CONFIGURATION);
+    SKL_CHECK(!top || (top_index && top_logit), SKL_ERR_NULL_POINTER);
+    SKL_CHECK(alpha == 1.0f || label, SKL_ERR_NULL_POINTER);
+    SKL_CHECK(b->out && b->grad && b->d_prenorm, SKL_ERR_NULL_POINTER);
+    SKL_CHECK(b->dtype != SKL_F16 || b->d_prenorm_h, SKL_ERR_NULL_POINTER);
+    const size_t e = (size_t)rows * b->outputs, t = b->dtype == SKL_F16 ? 2 : 4, slots = (size_t)rows * top * 4;
+    const Span out[] = {{b->grad, e * 4}, {b->d_prenorm, e * 4}, {b->dtype == SKL_F16 ? b->d_prenorm_h : nullptr, e * 2},
+                        {loss, (size_t)rows * 4}};
+    const Span in[] = {{b->out, e * t}, {top ? top_index : nullptr, slots}, {top ? top_logit : nullptr, slots},
+                       {label, (size_t)rows * 4}};
+    SKL_CHECK(!spans_clash(out, 4, in, 4) && !outputs_clash(out, 4), SKL_ERR_INVALID_CONFIGURATION);
+    int32_t r = enter(ctx);
+    if (r) return r;
+    DistillArgs a{};
+    a.rows = rows;
+    a.n = b->outputs;
+    a.top = top;
+    a.tau = temperature;
+    a.alpha = alpha;
+    a.logits = b->out;
+    a.index = reinterpret_cast<const int32_t *>(top_index);
+    a.value = top_logit;
+    a.label = alpha < 1.0f ? reinterpret_cast<const int32_t *>(label) : nullptr;
+    a.loss = loss;
+    a.grad = b->grad;
+    a.d_prenorm = b->d_prenorm;
+    a.d_prenorm_h = b->dtype == SKL_F16 ? reinterpret_cast<half_t *>(b->d_prenorm_h) : nullptr;
+    note_rewrite(ctx, b);
+    ctx->cs.valid = false;
+    SKL_TRY(launch_distill(a, b->dtype, ctx->stream));
+    return finish(ctx);
+}
+
+// ---- 4-bit microscaled floats -------------------------------------------------------------
+
+static int32_t mx_cast(skl_ctx *ctx, const void *values, uint32_t dtype, uint32_t rows, uint32_t cols, uint32_t down,
+                       const void *codes, const void *scales, bool back) {
+    SKL_CHECK(ctx, SKL_ERR_NULL_POINTER);
+    SKL_CHECK(dtype <= SKL_F16 && down <= 1, SKL_ERR_INVALID_CONFIGURATION);
+    SKL_CHECK((down ? rows : cols) <= 0x7fffff80u, SKL_ERR_INVALID_CONFIGURATION);
+    if (rows == 0 || cols == 0) return SKL_OK;
+    SKL_CHECK(values && codes && scales, SKL_ERR_NULL_POINTER);
+    SKL_CHECK(aligned16(codes) && aligned_to(scales, 4), SKL_ERR_HARDWARE_CONSTRAINT);
+    MxCastArgs a{};
+    a.n = down ? cols : rows;
+    a.k = down ? rows : cols;
+    const size_t kp = mx_pad(a.k), nv = (size_t)rows * cols * (dtype == SKL_F16 ? 2 : 4);
+    const Span v{values, nv}, c{codes, a.n * kp / 2}, sc{scales, a.n * kp / 32};
+    SKL_CHECK(!overlaps(v.p, v.bytes, c.p, c.bytes) && !overlaps(v.p, v.bytes, sc.p, sc.bytes) &&
+                  !overlaps(c.p, c.bytes, sc.p, sc.bytes),
+              SKL_ERR_INVALID_CONFIGURATION);
+    int32_t r = enter(ctx);
+    if (r) return r;
+    a.values = const_cast<void *>(values);
+    a.codes = reinterpret_cast<uint8_t *>(const_cast<void *>(codes));
+    a.scales = reinterpret_cast<uint8_t *>(const_cast<void *>(scales));
+    SKL_TRY((back ? launch_mx_dequantise : launch_mx_quantise)(a, dtype, down != 0, ctx->stream));
+    return finish(ctx);
+}
+
+int32_t skl_mxfp4_quantise(skl_ctx *ctx, const void *src, uint32_t dtype, uint32_t rows, uint32_t cols,
+                           uint32_t down, void *codes, void *scales) {
+    return mx_cast(ctx, src, dtype, rows, cols, down, codes, scales, false);
+}
+
+int32_t skl_mxfp4_dequantise(skl_ctx *ctx, const void *codes, const void *scales, uint32_t rows, uint32_t cols,
+                             uint32_t down, void *dst, uint32_t dtype) {
+    return mx_cast(ctx, dst, dtype, rows, cols, down, codes, scales, true);
+}
+
+size_t skl_mxfp4_work_bytes(uint32_t inputs, uint32_t batch) { return mx_work_bytes(inputs, batch); }
+
+int32_t skl_dense_forward_mxfp4(skl_ctx *ctx, const skl_dense_desc *b, const void *in, uint32_t in_rows,
+                                uint32_t in_cols, uint32_t batch, const void *w_codes, const void *w_scales,
+                                void *work, size_t work_bytes) {
+    SKL_CHECK(ctx && b, SKL_ERR_NULL_POINTER);
+    SKL_CHECK(b->dtype <= SKL_F16 && b->inputs > 0 && b->outputs > 0 && b->max_batch > 0 &&
+                  b->norm <= SKL_NORM_BATCH && b->act <= SKL_ACT_MISH && b->inputs <= 0x7fffff80u,
+              SKL_ERR_INVALID_CONFIGURATION);
+    int32_t r;
+    if ((r = check_input(b, in, in_rows, in_cols, batch))) return r;
+    if ((r = check_act_batch(b, batch))) return r;
+    if ((r = check_norm_cache(b))) return r;
+    const bool normed = b->norm != SKL_NORM_DISABLED;
+    SKL_CHECK(w_codes && w_scales && b->out, SKL_ERR_NULL_POINTER);
+    SKL_CHECK(!normed || (b->preact && b->predrop), SKL_ERR_NULL_POINTER);
+    SKL_CHECK(b->norm == SKL_NORM_BATCH || b->b, SKL_ERR_NULL_POINTER);
+    SKL_CHECK(aligned16(w_codes) && aligned_to(w_scales, 4), SKL_ERR_HARDWARE_CONSTRAINT);
+    const size_t need = mx_work_bytes(b->inputs, batch);
+    SKL_CHECK(!need || work, SKL_ERR_NULL_POINTER);
+    SKL_CHECK(work_bytes >= need, SKL_ERR_ALLOCATION_LIMIT);
+    SKL_CHECK(aligned16(work), SKL_ERR_HARDWARE_CONSTRAINT);
+    const size_t t = b->dtype == SKL_F16 ? 2 : 4, e = (size_t)batch * b->outputs * t;
+    const size_t kp = mx_pad(b->inputs), nb = b->outputs * t;
+    const Span read[] = {{in, (size_t)batch * in_cols * t}, {w_codes, b->outputs * kp / 2},
+                         {w_scales, b->outputs * kp / 32}, {b->b, nb}, {normed ? b->norm_w : nullptr, nb},
+                         {normed ? b->norm_b : nullptr, nb}};
+    const Span out[] = {{b->out, e}, {need ? work : nullptr, need}, {normed ? b->prenorm : nullptr, e},
+                        {normed ? b->centered : nullptr, e}, {normed ? b->preact : nullptr, e},
+                        {normed ? b->predrop : nullptr, e}};
+    SKL_CHECK(!spans_clash(out, 6, read, 6) && !outputs_clash(out, 2), SKL_ERR_INVALID_CONFIGURATION);
+    if ((r = check_tile(ctx, b))) return r;
+    if ((r = enter(ctx))) return r;
+    MxForwardArgs a{};
+    a.m = batch;
+    a.n = b->outputs;
+    a.k = b->inputs;
+    a.x = in;
+    a.w_codes = reinterpret_cast<const uint8_t *>(w_codes);
+    a.w_scales = reinterpret_cast<const uint8_t *>(w_scales);
+    a.bias = b->norm == SKL_NORM_BATCH ? nullptr : b->b;
+    a.act = normed ? (uint32_t)SKL_ACT_IDENTITY : b->act;
+    a.leaky = b->act == SKL_ACT_LEAKY_RELU ? b->leaky : 0.0f;
+    a.out = normed ? b->prenorm : b->out;
+    a.work = work;
+    SKL_TRY(launch_mx_forward(a, b->dtype, ctx->stream));
+    if (normed) {
+        RowNormArgs n{};
+        n.dtype = b->dtype;
+        n.m = batch;
+        n.n = b->outputs;
+        n.norm = b->norm;
+        n.act = b->act;
+        n.leaky = a.leaky;
+        n.prenorm = b->prenorm;
+        n.norm_w = b->norm_w;
+        n.norm_b = b->norm_b;
+        n.centered = b->centered;
+        n.preact = b->preact;
+        n.predrop = b->predrop;
+        n.out = b->out;
+        n.mask = b->mask;
+        n.norm_rstd = b->norm_rstd;
+        float *stats = n.norm == SKL_NORM_BATCH ? norm_scratch(ctx, norm_cols_scratch(n.m, n.n)) : nullptr;
+        SKL_TRY(launch_norm_act(n, stats, ctx->norm.done, ctx->stream));
     }
     return finish(ctx);
 }

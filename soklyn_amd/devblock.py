@@ -34,6 +34,7 @@ _READS = {
     "forward": (("w", "b", "out", "predrop", "preact", "mask"), _NORM_CACHES),
     "output_error": (_ERROR + ("out",), _ERROR_NORM),
     "error": (_ERROR + ("predrop", "mask"), _ERROR_NORM),
+    "distill": (("out", "grad", "d_prenorm", "d_prenorm_h"), ()),
     "input_grad": (("w", "d_prenorm", "d_prenorm_h"), ()),
     "above": (("w", "d_prenorm", "d_prenorm_h"), ()),
     "update": (_UPDATE, _UPDATE_NORM),
@@ -45,6 +46,40 @@ _PTR_AT = {n: getattr(abi.SklDenseDesc, n).offset // 8 for n in abi.DESC_POINTER
 
 def _ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
+
+
+def _distill(ctx, desc, index, value, label, temperature, alpha, loss):
+    device, (rows, top) = ctx.device, index.shape
+    i = abi.need("index", index, torch.int32, (rows, top), device)
+    v = abi.need("value", value, torch.float32, (rows, top), device)
+    y = None if label is None else abi.need("label", label, torch.int32, (rows,), device)
+    to = None if loss is None else abi.need("loss", loss, torch.float32, (rows,), device)
+    abi.call("skl_dense_distill_error", ctx.h, desc, i, v, top, y, rows, temperature, alpha, to)
+
+
+def distill_error(ctx: abi.Context, logits: torch.Tensor, index: torch.Tensor, value: torch.Tensor,
+                  label: torch.Tensor | None = None, *, temperature: float = 1.0, alpha: float = 1.0,
+                  grad: torch.Tensor, d_prenorm: torch.Tensor, d_prenorm_h: torch.Tensor | None = None,
+                  loss: torch.Tensor | None = None) -> None:
+    """skl_dense_distill_error over tensors that are not a DeviceBlock's: logits [rows x classes]
+    (fp16 or fp32), the teacher's classes (int32) and logits (fp32) [rows x top], labels int32
+    [rows] where alpha < 1; writes grad and d_prenorm (fp32), d_prenorm_h (fp16; fp16 logits only)
+    and loss [rows] where given."""
+    rows, classes = logits.shape
+    half = logits.dtype is torch.float16
+    d = abi.SklDenseDesc()
+    d.dtype, d.inputs, d.outputs, d.max_batch, d.is_training = abi.F16 if half else abi.F32, 1, classes, rows, 1
+    dev, shape = ctx.device, (rows, classes)
+    d.out = abi.need("logits", logits, torch.float16 if half else torch.float32, shape, dev)
+    d.grad = abi.need("grad", grad, torch.float32, shape, dev)
+    d.d_prenorm = abi.need("d_prenorm", d_prenorm, torch.float32, shape, dev)
+    if half:
+        if d_prenorm_h is None:
+            raise ValueError("d_prenorm_h: fp16 logits need one")
+        d.d_prenorm_h = abi.need("d_prenorm_h", d_prenorm_h, torch.float16, shape, dev)
+    if index.shape[0] != rows:
+        raise ValueError(f"index: {index.shape[0]} rows, logits have {rows}")
+    _distill(ctx, C.byref(d), index, value, label, temperature, alpha, loss)
 
 
 class DeviceBlock:
@@ -141,6 +176,13 @@ class DeviceBlock:
         rows, cols = target.shape[0], target.shape[1]
         abi.call("skl_dense_output_error", self.ctx.h, self._fill("output_error"), target.data_ptr(), rows, cols, loss,
                  act, leaky)
+
+    def distill_error(self, index: torch.Tensor, value: torch.Tensor, label: torch.Tensor | None = None, *,
+                      temperature: float = 1.0, alpha: float = 1.0, loss: torch.Tensor | None = None):
+        """The error of the first index.shape[0] rows against a teacher's top logits: classes index
+        (int32) and logits value (fp32) [rows x top], labels int32 [rows] where alpha < 1; loss [rows]
+        (fp32) is written where given."""
+        _distill(self.ctx, self._fill("distill"), index, value, label, temperature, alpha, loss)
 
     def hidden_error(self, nxt: "DeviceBlock", batch: int):
         abi.call("skl_dense_hidden_error", self.ctx.h, self._fill("hidden"), nxt._fill("above"), batch)
