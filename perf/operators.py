@@ -372,8 +372,8 @@ def _kernels(s):
         mxfp4.quantise(_ctx(), s["src"], down=c["down"], codes=s["codes"], scales=s["scales"])
         return mxfp4.dequantise(_ctx(), s["codes"], s["scales"], s["values"], down=c["down"])
     if "layer" not in s:
-        s["layer"] = mxfp4.Layer(_ctx(), c["inputs"], c["outputs"], c["batch"], s["codes"], s["scales"],
-                                 half=c["dtype"] == "f16", act=ACTS[c["act"]], b=s["bias"], out=s["out"])
+        s["layer"] = mxfp4.Layer(_ctx(), c["inputs"], c["outputs"], c["batch"], s["codes"].to(torch.uint8),
+                                 s["scales"], half=c["dtype"] == "f16", act=ACTS[c["act"]], b=s["bias"], out=s["out"])
     return s["layer"].forward(s["x"], c["batch"])
 
 
