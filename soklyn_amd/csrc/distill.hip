@@ -67,7 +67,7 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT) distill_kernel(DistillArg
     extern __shared__ f32x4 lds[];
     __shared__ float red[3][W > 0 ? W : 1];
     const uint32_t tid = threadIdx.x % NT, lane = threadIdx.x % LANES, n = a.n, top = a.top;
-    float *table = reinterpret_cast<float *>(lds) + (threadIdx.x / NT) * (distill_words(NT, E, TABLE) + 4 * top);
+    float *table = reinterpret_cast<float *>(lds) + sub_row<NT>() * (distill_words(NT, E, TABLE) + 4 * top);
     uint32_t *marks = reinterpret_cast<uint32_t *>(table + (TABLE ? NT * E : 0));
     int32_t *at = reinterpret_cast<int32_t *>(marks + kMarks);
     float *value = reinterpret_cast<float *>(at + top), *q = value + top, *z_at = q + top;
@@ -76,7 +76,7 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT) distill_kernel(DistillArg
     if constexpr (!TABLE)
         while ((n + V - 1) >> group >= kMarks * 32u) ++group;
 
-    for (uint32_t row = blockIdx.x * RPG + threadIdx.x / NT; row < a.rows; row += gridDim.x * RPG) {
+    for (uint32_t row = blockIdx.x * RPG + sub_row<NT>(); row < a.rows; row += gridDim.x * RPG) {
         const uint64_t row_at = (uint64_t)row * n;
         // A row of an odd width starts anywhere.  Its threads take its vectors from the last of the
         // matrix's own vectors that begins at or before it, so that every whole one is aligned if

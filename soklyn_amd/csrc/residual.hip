@@ -4,10 +4,10 @@
 //   h = scale x + act(gate) u      the residual stream, rounded to its type
 //   n = pre(h)                     the norm before the next block, of h as stored
 //
-// A row is held in registers, 8 or 16 elements a thread, from its loads to its stores, so each
-// tensor crosses HBM once; the norms' sums are two-pass (mean, then squared deviations).
-#include "launch.h"
+// A row is held in registers from its loads to its stores, so each tensor crosses HBM once; the
+// norms' sums are two-pass (mean, then squared deviations).
 #include "residual.h"
+#include "launch.h"
 #include "rows.h"
 
 namespace skl {
@@ -16,9 +16,22 @@ constexpr float kNormEps = 1e-6f;   // the blocks' own norms add the same
 
 namespace {
 
+// tanh to about 2 units in the last place: its series up to |x| = 0.4 (the first term left out is
+// 0.0036 x^13), else (1 - e) / (1 + e) with e = exp(-2 |x|), whose difference cancels no more than
+// one bit there.
+__device__ __forceinline__ float tanh_gate(float x) {
+    const float q = x * x;
+    float s = fmaf(q, -0.008863235529902197f, 0.02186948853615520f);
+    s = fmaf(q, s, -0.05396825396825397f);
+    s = fmaf(q, s, 0.1333333333333333f);
+    s = fmaf(q, s, -0.3333333333333333f);
+    const float e = __expf(-2.0f * fabsf(x));
+    const float far = copysignf((1.0f - e) * __builtin_amdgcn_rcpf(1.0f + e), x);
+    return fabsf(x) < 0.4f ? fmaf(x * q, s, x) : far;
+}
 __device__ __forceinline__ float gate_value(uint32_t act, float g) {
-    if (act == 1) return 1.0f / (1.0f + expf(-g));
-    if (act == 4) return tanhf(g);
+    if (act == 1) return sigmoid_fast(g);
+    if (act == 4) return tanh_gate(g);
     return g;
 }
 // The gate's slope from its value a.
@@ -29,105 +42,105 @@ __device__ __forceinline__ float gate_slope(uint32_t act, float a) {
 }
 
 // Mean and reciprocal deviation of a row's values v (zero past its end).
-template <int NT, int E, int V>
-__device__ __forceinline__ void row_stats(const float (&v)[E], uint32_t tid, uint32_t cols, uint32_t norm, float *slots,
+template <int NT, int E>
+__device__ __forceinline__ void row_stats(const float (&v)[E + 1], const RowMap<NT> &map, uint32_t norm, float *slots,
                                           float &mean, float &rstd) {
     mean = 0.0f;
     rstd = 1.0f;
     if (norm == 0) return;
-    const float inv = 1.0f / (float)cols;
+    const float inv = 1.0f / (float)map.cols;
     if (norm == 2) {
-        float s = 0.0f;
+        float s[1] = {0.0f};
 #pragma unroll
-        for (int e = 0; e < E; ++e) s += v[e];
-        mean = row_sum<NT>(s, slots) * inv;
+        for (int e = 0; e <= E; ++e) s[0] += v[e];
+        row_sums<NT>(s, slots);
+        mean = s[0] * inv;
     }
-    float q = 0.0f;
+    float q[1] = {0.0f};
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-        const uint32_t col = ((uint32_t)(e / V) * NT + tid) * V + e % V;
-        const float d = col < cols ? v[e] - mean : 0.0f;
-        q += d * d;
+    for (int e = 0; e <= E; ++e) {
+        const float d = (e < E ? map.whole(e / 4) : map.tailed()) ? v[e] - mean : 0.0f;
+        q[0] += d * d;
     }
-    rstd = 1.0f / sqrtf(row_sum<NT>(q, slots + NT / 64) * inv + kNormEps);
+    row_sums<NT>(q, slots + NT / 64);
+    rstd = 1.0f / sqrtf(q[0] * inv + kNormEps);
 }
 
-// One row per NT threads (four rows per workgroup where a wave is enough for one).
+// One row per NT threads (several to a workgroup of 256 where a wave, or a quarter, holds one).
 template <typename T, typename R, int NT, int E>
 __global__ void __launch_bounds__(NT < 256 ? 256 : NT) join_kernel(JoinArgs a) {
-    constexpr int V = 16 / sizeof(T), C = E / V;
     constexpr int RPG = NT < 256 ? 256 / NT : 1;
-    __shared__ float slots[4 * (NT / 64)];
-    const uint32_t tid = threadIdx.x % NT;
-    const uint32_t cols = a.cols;
-    auto chunk = [&](int c) { return ((uint32_t)c * NT + tid) * V; };
-    auto part = [&](float (&v)[E], int c) -> float (&)[V] { return *reinterpret_cast<float (*)[V]>(&v[c * V]); };
-    for (uint32_t row = blockIdx.x * RPG + threadIdx.x / NT; row < a.rows; row += gridDim.x * RPG) {
-    const uint64_t at = (uint64_t)row * cols;
-    float h[E], u[E];
+    __shared__ float slots[4 * (NT < 64 ? 1 : NT / 64)];
+    const RowMap<NT> map{threadIdx.x % NT, a.cols};
+    for (uint32_t row = blockIdx.x * RPG + sub_row<NT>(); row < a.rows; row += gridDim.x * RPG) {
+        const uint64_t at = (uint64_t)row * a.cols;
+        float mean = 0.0f, rstd = 1.0f;
+        RowPart<R, E> x;
+        RowPart<T, E> y, g;
+        if (a.x) map.template read<R, E>(reinterpret_cast<const R *>(a.x) + at, x);
+        if (a.y) map.template read<T, E>(reinterpret_cast<const T *>(a.y) + at, y);
+        if (a.gate) map.template read<T, E>(reinterpret_cast<const T *>(a.gate) + (a.gate_rows > 1 ? at : 0), g);
+        float h[E + 1];
+        if (a.x) {
+            map.template floats<R, E>(x, h);
 #pragma unroll
-    for (int c = 0; c < C; ++c) {
-        if (a.x)
-            load_row<R, V>(reinterpret_cast<const R *>(a.x) + at, chunk(c), cols, part(h, c));
-        else
+            for (int e = 0; e <= E; ++e) h[e] *= a.scale;
+        } else {
 #pragma unroll
-            for (int e = 0; e < V; ++e) h[c * V + e] = 0.0f;
-        if (a.y) load_row<T, V>(reinterpret_cast<const T *>(a.y) + at, chunk(c), cols, part(u, c));
-    }
+            for (int e = 0; e <= E; ++e) h[e] = 0.0f;
+        }
+        if (a.y) {
+            float u[E + 1];
+            map.template floats<T, E>(y, u);
+            row_stats<NT, E>(u, map, a.post, slots, mean, rstd);
+            if (a.post) {
+                float w[E + 1];
+                map.template read<T, E>(a.post_w, w);
 #pragma unroll
-    for (int e = 0; e < E; ++e) h[e] *= a.scale;
-    if (a.y) {
-        float mean, rstd;
-        row_stats<NT, E, V>(u, tid, cols, a.post, slots, mean, rstd);
-        if (a.stats && tid == 0) {
+                for (int e = 0; e <= E; ++e) u[e] = (u[e] - mean) * rstd * w[e];
+                if (a.post == 2) {
+                    map.template read<T, E>(a.post_b, w);
+#pragma unroll
+                    for (int e = 0; e <= E; ++e) u[e] += w[e];
+                }
+            }
+            if (a.gate) {
+                float v[E + 1];
+                map.template floats<T, E>(g, v);
+#pragma unroll
+                for (int e = 0; e <= E; ++e) u[e] *= gate_value(a.gate_act, v[e]);
+            }
+#pragma unroll
+            for (int e = 0; e <= E; ++e) h[e] += u[e];
+        }
+        if (a.stats && map.tid == 0) {
             a.stats[row] = mean;
             a.stats[(uint64_t)a.rows + row] = rstd;
         }
 #pragma unroll
-        for (int c = 0; c < C; ++c) {
-            float w[V], b[V], g[V];
-            if (a.post) load_row<T, V>(a.post_w, chunk(c), cols, w);
-            if (a.post == 2) load_row<T, V>(a.post_b, chunk(c), cols, b);
-            if (a.gate)
-                load_row<T, V>(reinterpret_cast<const T *>(a.gate) + (a.gate_rows > 1 ? at : 0), chunk(c), cols, g);
+        for (int e = 0; e <= E; ++e) h[e] = (float)(R)h[e];
+        if (a.h) map.template write<R, E>(reinterpret_cast<R *>(a.h) + at, h);
+        mean = 0.0f;
+        rstd = 1.0f;
+        if (a.n) row_stats<NT, E>(h, map, a.pre, slots + 2 * (NT / 64), mean, rstd);
+        if (a.stats && map.tid == 0) {
+            a.stats[2 * (uint64_t)a.rows + row] = mean;
+            a.stats[3 * (uint64_t)a.rows + row] = rstd;
+        }
+        if (!a.n) continue;
+        if (a.pre) {
+            // past the row's end w is 0, and what is there is not written
+            float w[E + 1];
+            map.template read<T, E>(a.pre_w, w);
 #pragma unroll
-            for (int e = 0; e < V; ++e) {
-                float v = u[c * V + e];
-                if (a.post) v = (v - mean) * rstd * w[e];
-                if (a.post == 2) v += b[e];
-                if (a.gate) v *= gate_value(a.gate_act, g[e]);
-                h[c * V + e] += v;
+            for (int e = 0; e <= E; ++e) h[e] = (h[e] - mean) * rstd * w[e];
+            if (a.pre == 2) {
+                map.template read<T, E>(a.pre_b, w);
+#pragma unroll
+                for (int e = 0; e <= E; ++e) h[e] += w[e];
             }
         }
-    } else if (a.stats && tid == 0) {
-        a.stats[row] = 0.0f;
-        a.stats[(uint64_t)a.rows + row] = 1.0f;
-    }
-#pragma unroll
-    for (int e = 0; e < E; ++e) h[e] = (float)(R)h[e];
-    if (a.h)
-#pragma unroll
-        for (int c = 0; c < C; ++c) store_row<R, V>(reinterpret_cast<R *>(a.h) + at, chunk(c), cols, part(h, c));
-    float mean = 0.0f, rstd = 1.0f;
-    if (a.n) row_stats<NT, E, V>(h, tid, cols, a.pre, slots + 2 * (NT / 64), mean, rstd);
-    if (a.stats && tid == 0) {
-        a.stats[2 * (uint64_t)a.rows + row] = mean;
-        a.stats[3 * (uint64_t)a.rows + row] = rstd;
-    }
-    if (!a.n) continue;
-#pragma unroll
-    for (int c = 0; c < C; ++c) {
-        float w[V], b[V], o[V];
-        if (a.pre) load_row<T, V>(a.pre_w, chunk(c), cols, w);
-        if (a.pre == 2) load_row<T, V>(a.pre_b, chunk(c), cols, b);
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-            o[e] = h[c * V + e];
-            if (a.pre) o[e] = (o[e] - mean) * rstd * w[e];
-            if (a.pre == 2) o[e] += b[e];
-        }
-        store_row<T, V>(reinterpret_cast<T *>(a.n) + at, chunk(c), cols, o);
-    }
+        map.template write<T, E>(reinterpret_cast<T *>(a.n) + at, h);
     }
 }
 
@@ -136,146 +149,200 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT) join_kernel(JoinArgs a) {
 //   dx = scale d,   du = act(g) d,   dgate = act'(g) d u
 //   b = du w_post,  dy = r_y (b - y^ <b y^> - <b>)
 // and the column sums of du y^, du, dn h^, dn (and of dgate for one gate row) over the rows.
-// A workgroup walks rows blockIdx, blockIdx + grid, ... with its columns' parameters and column
-// sums in registers, and writes its sums as one plane of a.work [grid x kPlanes x cols]; the
-// next kernel adds the planes.
-template <typename T, typename R, int NT, int E>
+// A workgroup walks rows blockIdx, blockIdx + grid, ... with its column sums in registers and the
+// next row's tensors on their way, and writes its sums as one plane of a.work [grid x kPlanes x
+// cols]; the next kernel adds the planes.  BIAS: a Layer norm is there, so that du and dn are summed.
+// Rows of more than 4096 columns leave no registers for the next row, nor for the sums but dn's,
+// which each thread then keeps in LDS.
+template <typename T, typename R, int NT, int E, bool BIAS>
 __global__ void __launch_bounds__(NT < 256 ? 256 : NT) unjoin_kernel(UnjoinArgs a) {
-    constexpr int V = 16 / sizeof(T), C = E / V;
-    constexpr int RPG = NT < 256 ? 256 / NT : 1;
-    __shared__ float slots[2][4][NT / 64];
-    const uint32_t tid = threadIdx.x % NT, sub = threadIdx.x / NT;
-    const uint32_t cols = a.cols;
-    const float inv = 1.0f / (float)cols;
-    auto chunk = [&](int c) { return ((uint32_t)c * NT + tid) * V; };
-    auto part = [&](float (&v)[E], int c) -> float (&)[V] { return *reinterpret_cast<float (*)[V]>(&v[c * V]); };
-    float sum[kPlanes][E];
+    constexpr int RPG = NT < 256 ? 256 / NT : 1, S = NT < 64 ? 1 : NT / 64;
+    __shared__ float slots[2][4 * S];
+    __shared__ float join[RPG > 1 ? RPG : 1][RPG > 1 ? NT * E + 4 : 1];
+    const uint32_t sub = sub_row<NT>();
+    const RowMap<NT> map{threadIdx.x % NT, a.cols};
+    const float inv = 1.0f / (float)a.cols;
+    constexpr bool kWide = E * NT > 4096;
+    constexpr int kKept = BIAS ? 4 : 3;   // 32 KB each
+    __shared__ f32x4 kept[kWide ? kKept : 1][kWide ? E / 4 : 1][kWide ? NT : 1];
+    float sum[kPlanes][E + 1];
 #pragma unroll
     for (int p = 0; p < kPlanes; ++p)
 #pragma unroll
-        for (int e = 0; e < E; ++e) sum[p][e] = 0.0f;
-    uint32_t turn = 0;
-    for (uint32_t row = blockIdx.x * RPG + sub; row < a.rows; row += gridDim.x * RPG, turn ^= 1u) {
-        const uint64_t at = (uint64_t)row * cols;
-        float d[E], hat[E], t[E];
-        float s1 = 0.0f, s0 = 0.0f;
-        const float h_mean = a.stats[2 * (uint64_t)a.rows + row], h_rstd = a.stats[3 * (uint64_t)a.rows + row];
+        for (int e = 0; e <= E; ++e) sum[p][e] = 0.0f;
+    if constexpr (kWide)
 #pragma unroll
-        for (int c = 0; c < C; ++c) {
-            if (a.dh)
-                load_row<float, V>(a.dh + at, chunk(c), cols, part(d, c));
+        for (int i = 0; i < kKept * (E / 4); ++i) kept[i / (E / 4)][i % (E / 4)][threadIdx.x] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    // adds v to column sum p
+    auto add = [&](int p, const float (&v)[E + 1]) {
+        if (kWide && p != 3) {
+#pragma unroll
+            for (int c = 0; c < E / 4; ++c) {
+                f32x4 &k = kept[p == 1 ? 3 : p / 2][c][threadIdx.x];
+                k += f32x4{v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]};
+            }
+            sum[p][E] += v[E];
+        } else {
+#pragma unroll
+            for (int e = 0; e <= E; ++e) sum[p][e] += v[e];
+        }
+    };
+    struct Parts {
+        RowPart<float, E> dn, dh;
+        RowPart<R, E> h;
+        RowPart<T, E> y;
+    } in;
+    auto read = [&](uint32_t row) {
+        const uint64_t at = (uint64_t)row * a.cols;
+        if (a.dn) map.template read<float, E>(a.dn + at, in.dn);
+        if (!kWide && a.dh) map.template read<float, E>(a.dh + at, in.dh);
+        if (a.pre) map.template read<R, E>(reinterpret_cast<const R *>(a.h) + at, in.h);
+        if (!kWide && a.y) map.template read<T, E>(reinterpret_cast<const T *>(a.y) + at, in.y);
+    };
+    uint32_t turn = 0, row = blockIdx.x * RPG + sub;
+    if (!kWide && row < a.rows) read(row);
+    for (; row < a.rows; row += gridDim.x * RPG, turn ^= 1u) {
+        const uint64_t at = (uint64_t)row * a.cols;
+        float d[E + 1], t[E + 1], hat[E + 1], y[E + 1];
+        if constexpr (kWide) read(row);
+        // from behind the join, once the sums of what comes from the next block are taken
+        auto behind = [&] {
+            if (kWide && a.dh)
+                map.template read<float, E>(a.dh + at, d);
+            else if (a.dh)
+                map.template floats<float, E>(in.dh, d);
             else
 #pragma unroll
-                for (int e = 0; e < V; ++e) d[c * V + e] = 0.0f;
-            if (!a.dn) continue;
-            load_row<float, V>(a.dn + at, chunk(c), cols, part(t, c));
-            if (!a.pre) continue;
-            float w[V];
-            load_row<R, V>(reinterpret_cast<const R *>(a.h) + at, chunk(c), cols, part(hat, c));
-            load_row<T, V>(a.pre_w, chunk(c), cols, w);
+                for (int e = 0; e <= E; ++e) d[e] = 0.0f;
+        };
+        if constexpr (!kWide) behind();
+        if (a.dn) map.template floats<float, E>(in.dn, t);
+        if (a.pre) map.template floats<R, E>(in.h, hat);
+        if (!kWide && a.y) map.template floats<T, E>(in.y, y);
+        if (!kWide && row + gridDim.x * RPG < a.rows) read(row + gridDim.x * RPG);
+        if (a.dn && a.pre) {
+            const float mean = a.stats[2 * (uint64_t)a.rows + row], rstd = a.stats[3 * (uint64_t)a.rows + row];
+            float w[E + 1], s[2] = {0.0f, 0.0f};
+            map.template read<T, E>(a.pre_w, w);
+            float product[E + 1];
 #pragma unroll
-            for (int e = 0; e < V; ++e) {
-                const int i = c * V + e;
-                hat[i] = (hat[i] - h_mean) * h_rstd;
-                sum[2][i] += t[i] * hat[i];
-                sum[3][i] += t[i];
-                t[i] *= w[e];
-                s1 += t[i] * hat[i];
-                s0 += t[i];
+            for (int e = 0; e <= E; ++e) {
+                hat[e] = (hat[e] - mean) * rstd;
+                product[e] = t[e] * hat[e];
             }
+            add(2, product);
+            if constexpr (BIAS) add(3, t);
+#pragma unroll
+            for (int e = 0; e <= E; ++e) {
+                t[e] *= w[e];   // 0 past the row's end
+                s[0] += t[e] * hat[e];
+                s[1] += t[e];
+            }
+            row_sums<NT>(s, slots[turn]);
+            s[0] *= inv;
+            s[1] = a.pre == 2 ? s[1] * inv : 0.0f;
+            if constexpr (kWide) behind();
+#pragma unroll
+            for (int e = 0; e <= E; ++e) d[e] += rstd * (t[e] - hat[e] * s[0] - s[1]);
+        } else {
+            if constexpr (kWide) behind();
+            if (a.dn)
+#pragma unroll
+                for (int e = 0; e <= E; ++e) d[e] += t[e];
         }
-        if (a.dn) {
-            if (a.pre) {
-                s1 = row_sum<NT>(s1, slots[turn][0]) * inv;
-                s0 = a.pre == 2 ? row_sum<NT>(s0, slots[turn][1]) * inv : 0.0f;
+        if (a.dx) {
 #pragma unroll
-                for (int e = 0; e < E; ++e) d[e] += h_rstd * (t[e] - hat[e] * s1 - s0);
-            } else {
-#pragma unroll
-                for (int e = 0; e < E; ++e) d[e] += t[e];
-            }
+            for (int e = 0; e <= E; ++e) t[e] = a.scale * d[e];
+            map.template write<float, E>(a.dx + at, t);
         }
-        if (a.dx)
-#pragma unroll
-            for (int c = 0; c < C; ++c) {
-                float o[V];
-#pragma unroll
-                for (int e = 0; e < V; ++e) o[e] = a.scale * d[c * V + e];
-                store_row<float, V>(a.dx + at, chunk(c), cols, o);
-            }
         if (!a.y) continue;
-        // y^ in hat, du in d, then du w_post in t
-        const float y_mean = a.stats[row], y_rstd = a.stats[(uint64_t)a.rows + row];
-        float t1 = 0.0f, t0 = 0.0f;
+        const float mean = a.stats[row], rstd = a.stats[(uint64_t)a.rows + row];
+        if constexpr (kWide) map.template read<T, E>(reinterpret_cast<const T *>(a.y) + at, y);
+        float w[E + 1];
+        if (a.post) {
+            map.template read<T, E>(a.post_w, w);
 #pragma unroll
-        for (int c = 0; c < C; ++c) {
-            float w[V], b[V], g[V], o[V];
-            load_row<T, V>(reinterpret_cast<const T *>(a.y) + at, chunk(c), cols, part(hat, c));
-            if (a.post) load_row<T, V>(a.post_w, chunk(c), cols, w);
-            if (a.post == 2) load_row<T, V>(a.post_b, chunk(c), cols, b);
-            if (a.gate)
-                load_row<T, V>(reinterpret_cast<const T *>(a.gate) + (a.gate_rows > 1 ? at : 0), chunk(c), cols, g);
+            for (int e = 0; e <= E; ++e) y[e] = (y[e] - mean) * rstd;
+        }
+        if (a.gate) {
+            float u[E + 1];
 #pragma unroll
-            for (int e = 0; e < V; ++e) {
-                const int i = c * V + e;
-                float u = hat[i];
-                if (a.post) {
-                    hat[i] = (hat[i] - y_mean) * y_rstd;
-                    u = hat[i] * w[e];
-                    if (a.post == 2) u += b[e];
-                }
-                if (a.gate) {
-                    const float v = gate_value(a.gate_act, g[e]);
-                    o[e] = d[i] * u * gate_slope(a.gate_act, v);
-                    sum[4][i] += o[e];
-                    d[i] *= v;
-                }
-                t[i] = d[i];
-                if (a.post) {
-                    sum[0][i] += d[i] * hat[i];
-                    sum[1][i] += d[i];
-                    t[i] *= w[e];
-                    t1 += t[i] * hat[i];
-                    t0 += t[i];
-                }
+            for (int e = 0; e <= E; ++e) u[e] = a.post ? y[e] * w[e] : y[e];
+            if (BIAS && a.post == 2) {
+                map.template read<T, E>(a.post_b, t);
+#pragma unroll
+                for (int e = 0; e <= E; ++e) u[e] += t[e];
             }
-            if (a.gate && a.dgate && a.gate_rows > 1) store_row<float, V>(a.dgate + at, chunk(c), cols, o);
+            map.template read<T, E>(reinterpret_cast<const T *>(a.gate) + (a.gate_rows > 1 ? at : 0), t);
+#pragma unroll
+            for (int e = 0; e <= E; ++e) {
+                const float v = gate_value(a.gate_act, t[e]);
+                u[e] = d[e] * u[e] * gate_slope(a.gate_act, v);
+                d[e] *= v;
+            }
+            if (a.gate_sum) add(4, u);
+            if (a.dgate) map.template write<float, E>(a.dgate + at, u);
         }
         if (a.post) {
-            t1 = row_sum<NT>(t1, slots[turn][2]) * inv;
-            t0 = a.post == 2 ? row_sum<NT>(t0, slots[turn][3]) * inv : 0.0f;
+            float s[2] = {0.0f, 0.0f}, product[E + 1];
 #pragma unroll
-            for (int e = 0; e < E; ++e) t[e] = y_rstd * (t[e] - hat[e] * t1 - t0);
+            for (int e = 0; e <= E; ++e) product[e] = d[e] * y[e];
+            add(0, product);
+            if constexpr (BIAS) add(1, d);
+#pragma unroll
+            for (int e = 0; e <= E; ++e) {
+                d[e] *= w[e];
+                s[0] += d[e] * y[e];
+                s[1] += d[e];
+            }
+            row_sums<NT>(s, slots[turn] + 2 * S);
+            s[0] *= inv;
+            s[1] = a.post == 2 ? s[1] * inv : 0.0f;
+#pragma unroll
+            for (int e = 0; e <= E; ++e) d[e] = rstd * (d[e] - y[e] * s[0] - s[1]);
         }
-        if (a.dy)
-#pragma unroll
-            for (int c = 0; c < C; ++c) store_row<float, V>(a.dy + at, chunk(c), cols, part(t, c));
+        if (a.dy) map.template write<float, E>(a.dy + at, d);
     }
     if (!a.work) return;
 #pragma unroll
     for (int p = 0; p < kPlanes; ++p) {
         if (!(a.planes >> p & 1u)) continue;
+        if (kWide && p != 3 && (BIAS || p != 1))
 #pragma unroll
-        for (int c = 0; c < C; ++c) {
-            float *plane = a.work + ((uint64_t)(blockIdx.x * RPG + sub) * kPlanes + p) * cols;
-            store_row<float, V>(plane, chunk(c), cols, part(sum[p], c));
+            for (int e = 0; e < E; ++e) sum[p][e] = kept[p == 1 ? 3 : p / 2][e / 4][threadIdx.x][e % 4];
+        float *plane = a.work + ((uint64_t)blockIdx.x * kPlanes + p) * a.cols;
+        if constexpr (RPG == 1) {
+            map.template write<float, E>(plane, sum[p]);
+        } else {
+            __syncthreads();
+            map.template write<float, E>(join[sub], sum[p]);
+            __syncthreads();
+            for (uint32_t col = threadIdx.x; col < a.cols; col += 256) {
+                float s = 0.0f;
+#pragma unroll
+                for (int i = 0; i < RPG; ++i) s += join[i][col];
+                plane[col] = s;
+            }
         }
     }
 }
 
-// Column sums: the planes of a.work added in a fixed order, four slices of planes per column and
-// then the slices.  Column sums that the configuration does not have are written as zeros.
-__global__ void __launch_bounds__(256) unjoin_sums_kernel(UnjoinArgs a, uint32_t count) {
-    __shared__ float part[4][64];
-    const uint32_t lane = threadIdx.x & 63u, slice = threadIdx.x >> 6, p = blockIdx.y;
-    const uint32_t col = blockIdx.x * 64 + lane;
+// Column sums: the planes of a.work added in a fixed order, 32 slices of them per column and then
+// the slices.  Column sums that the configuration does not have are written as zeros.
+__global__ void __launch_bounds__(1024) unjoin_sums_kernel(UnjoinArgs a, uint32_t count) {
+    __shared__ float part[32][33];
+    const uint32_t lane = threadIdx.x & 31u, slice = threadIdx.x >> 5, p = blockIdx.y;
+    const uint32_t col = blockIdx.x * 32 + lane;
     float s = 0.0f;
     if (col < a.cols && (a.planes >> p & 1u))
-        for (uint32_t g = slice; g < count; g += 4) s += a.work[((uint64_t)g * kPlanes + p) * a.cols + col];
+#pragma unroll 8
+        for (uint32_t g = slice; g < count; g += 32) s += a.work[((uint64_t)g * kPlanes + p) * a.cols + col];
     part[slice][lane] = s;
     __syncthreads();
     if (slice || col >= a.cols) return;
-    s = (part[0][lane] + part[1][lane]) + (part[2][lane] + part[3][lane]);
+    s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) s += part[i][lane];
     if (p < 4) {
         if (a.dparam) a.dparam[(uint64_t)p * a.cols + col] = s;
     } else if (a.gate_sum) {
@@ -286,29 +353,35 @@ __global__ void __launch_bounds__(256) unjoin_sums_kernel(UnjoinArgs a, uint32_t
 template <typename T, typename R, int NT, int E> hipError_t join_t(const JoinArgs &a, hipStream_t s) {
     constexpr uint32_t rpg = NT < 256 ? 256 / NT : 1;
     const uint32_t groups = (a.rows + rpg - 1) / rpg;
-    hipLaunchKernelGGL((join_kernel<T, R, NT, E>), dim3(groups < (1u << 20) ? groups : 1u << 20), dim3(NT < 256 ? 256 : NT), 0, s, a);
+    hipLaunchKernelGGL((join_kernel<T, R, NT, E>), dim3(groups < (1u << 20) ? groups : 1u << 20),
+                       dim3(NT < 256 ? 256 : NT), 0, s, a);
     return hipGetLastError();
 }
 
 template <typename T, typename R> hipError_t join_c(const JoinArgs &a, hipStream_t s) {
-    if (a.cols <= 512) return join_t<T, R, 64, 8>(a, s);
+    if (a.cols <= 64) return join_t<T, R, 16, 4>(a, s);
+    if (a.cols <= 256) return join_t<T, R, 64, 4>(a, s);
     if (a.cols <= 1024) return join_t<T, R, 64, 16>(a, s);
     if (a.cols <= 2048) return join_t<T, R, 256, 8>(a, s);
-    if (a.cols <= 4096) return join_t<T, R, 512, 8>(a, s);
-    return join_t<T, R, 1024, 8>(a, s);
+    if (a.cols <= 4096) return join_t<T, R, 256, 16>(a, s);
+    return join_t<T, R, 512, 16>(a, s);
 }
 
 template <typename T, typename R, int NT, int E> hipError_t unjoin_t(const UnjoinArgs &a, hipStream_t s) {
-    constexpr uint32_t rpg = NT < 256 ? 256 / NT : 1;
-    const uint32_t planes = residual_planes(a.rows, a.cols);
-    hipLaunchKernelGGL((unjoin_kernel<T, R, NT, E>), dim3(planes / rpg), dim3(NT < 256 ? 256 : NT), 0, s, a);
+    const uint32_t groups = residual_planes(a.rows, a.cols);
+    const bool bias = a.pre == 2 || a.post == 2;
+    hipLaunchKernelGGL((bias ? unjoin_kernel<T, R, NT, E, true> : unjoin_kernel<T, R, NT, E, false>), dim3(groups),
+                       dim3(NT < 256 ? 256 : NT), 0, s, a);
     if (a.work)
-        hipLaunchKernelGGL(unjoin_sums_kernel, dim3((a.cols + 63) / 64, kPlanes), dim3(256), 0, s, a, planes);
+        hipLaunchKernelGGL(unjoin_sums_kernel, dim3((a.cols + 31) / 32, kPlanes), dim3(1024), 0, s, a, groups);
     return hipGetLastError();
 }
 
 template <typename T, typename R> hipError_t unjoin_c(const UnjoinArgs &a, hipStream_t s) {
+    if (a.cols <= 64) return unjoin_t<T, R, 16, 4>(a, s);
+    if (a.cols <= 256) return unjoin_t<T, R, 64, 4>(a, s);
     if (a.cols <= 512) return unjoin_t<T, R, 64, 8>(a, s);
+    if (a.cols <= 1024) return unjoin_t<T, R, 256, 4>(a, s);
     if (a.cols <= 2048) return unjoin_t<T, R, 256, 8>(a, s);
     if (a.cols <= 4096) return unjoin_t<T, R, 512, 8>(a, s);
     return unjoin_t<T, R, 512, 16>(a, s);

@@ -68,18 +68,81 @@ template <int LANES = 64> __device__ __forceinline__ float lanes_max(float v) {
     return lanes_all<LANES>(v, [](float a, float b) { return fmaxf(a, b); });
 }
 
-// The sum of v over the NT threads of a row, in every one of them, in a fixed order.  slot: NT / 64
-// floats of LDS that no other sum uses until every thread has passed another barrier.
-template <int NT> __device__ __forceinline__ float row_sum(float v, float *slot) {
-    v = lanes_sum(v);
-    if constexpr (NT > 64) {
-        if ((threadIdx.x & 63u) == 0) slot[threadIdx.x >> 6] = v;
-        __syncthreads();
-        v = 0.0f;
+// Which of a workgroup's rows a thread has a part in, with NT threads to a row: known to be the
+// same in a whole wave where it is, so that the row's addresses stay in scalar registers.
+template <int NT> __device__ __forceinline__ uint32_t sub_row() {
+    if constexpr (NT >= 256) return 0;
+    if constexpr (NT >= 64) return (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x / NT));
+    return threadIdx.x / NT;
+}
+
+// A row of `cols` elements over NT threads: thread t has the vectors of 4 at columns 4 (t + NT c) and,
+// of the up to three columns behind the last whole vector, the t-th, as its element E.
+template <typename T, int E> struct RowPart {
+    typename Unaligned<T, 4>::type v[E / 4];
+    T last;
+};
+template <int NT> struct RowMap {
+    uint32_t tid, cols;
+    __device__ __forceinline__ uint32_t col(int c) const { return (c * NT + tid) * 4; }
+    __device__ __forceinline__ uint32_t tail() const { return (cols & ~3u) + tid; }
+    __device__ __forceinline__ bool whole(int c) const { return col(c) + 4 <= cols; }
+    __device__ __forceinline__ bool tailed() const { return tid < (cols & 3u); }
+
+    // Elements past the row's end are 0.
+    template <typename T, int E> __device__ __forceinline__ void read(const void *row, RowPart<T, E> &to) const {
+        const T *p = reinterpret_cast<const T *>(row);
+        typedef typename Unaligned<T, 4>::type Vec;
 #pragma unroll
-        for (int w = 0; w < NT / 64; ++w) v += slot[w];
+        for (int c = 0; c < E / 4; ++c) {
+            to.v[c] = Vec{};
+            if (whole(c)) to.v[c] = *reinterpret_cast<const Vec *>(p + col(c));
+        }
+        to.last = tailed() ? p[tail()] : (T)0;
     }
-    return v;
+    template <typename T, int E> __device__ __forceinline__ void read(const void *row, float (&to)[E + 1]) const {
+        RowPart<T, E> part;
+        read<T, E>(row, part);
+        floats<T, E>(part, to);
+    }
+    template <typename T, int E> __device__ __forceinline__ static void floats(const RowPart<T, E> &part, float (&to)[E + 1]) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) to[e] = (float)part.v[e / 4][e % 4];
+        to[E] = (float)part.last;
+    }
+    template <typename T, int E> __device__ __forceinline__ void write(void *row, const float (&from)[E + 1]) const {
+        T *p = reinterpret_cast<T *>(row);
+        typedef typename Unaligned<T, 4>::type Vec;
+#pragma unroll
+        for (int c = 0; c < E / 4; ++c) {
+            Vec w;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[e] = (T)from[4 * c + e];
+            if (whole(c)) *reinterpret_cast<Vec *>(p + col(c)) = w;
+        }
+        if (tailed()) p[tail()] = (T)from[E];
+    }
+};
+
+// The sums of N values over the NT threads of a row (16 or 64: lanes of one wave), in every one of
+// them, in a fixed order.  slots: N NT / 64 floats of LDS that no other sum uses until every
+// thread has passed another barrier.
+template <int NT, int N> __device__ __forceinline__ void row_sums(float (&v)[N], float *slots) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = lanes_sum<(NT < 64 ? NT : 64)>(v[i]);
+    if constexpr (NT > 64) {
+        constexpr int W = NT / 64;
+        if ((threadIdx.x & 63u) == 0)
+#pragma unroll
+            for (int i = 0; i < N; ++i) slots[i * W + (threadIdx.x >> 6)] = v[i];
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            v[i] = 0.0f;
+#pragma unroll
+            for (int w = 0; w < W; ++w) v[i] += slots[i * W + w];
+        }
+    }
 }
 
 }  // namespace skl
