@@ -30,11 +30,11 @@ struct UnjoinArgs {
     float *work;       // null: no column sums wanted
 };
 
-// Workgroups of the backward of [rows x cols], each of which writes a plane of column sums.
+// The most workgroups of the backward of [rows x cols], each of which writes a plane of column sums.
 inline uint32_t residual_planes(uint32_t rows, uint32_t cols) {
     const uint32_t rpg = cols <= 64 ? 16 : cols <= 512 ? 4 : 1;
-    const uint32_t groups = (rows + rpg - 1) / rpg;
-    return groups < 512 ? groups : 512;
+    const uint32_t groups = (rows + rpg - 1) / rpg, most = cols <= 1024 ? 1280 : cols <= 2048 ? 768 : 256;
+    return groups < most ? groups : most;
 }
 
 hipError_t launch_join(const JoinArgs &a, uint32_t dtype, uint32_t stream_dtype, hipStream_t s);

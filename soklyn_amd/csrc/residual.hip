@@ -6,6 +6,8 @@
 //
 // A row is held in registers from its loads to its stores, so each tensor crosses HBM once; the
 // norms' sums are two-pass (mean, then squared deviations).
+#include <algorithm>
+
 #include "residual.h"
 #include "launch.h"
 #include "rows.h"
@@ -367,24 +369,43 @@ template <typename T, typename R> hipError_t join_c(const JoinArgs &a, hipStream
     return join_t<T, R, 512, 16>(a, s);
 }
 
-template <typename T, typename R, int NT, int E> hipError_t unjoin_t(const UnjoinArgs &a, hipStream_t s) {
-    const uint32_t groups = residual_planes(a.rows, a.cols);
-    const bool bias = a.pre == 2 || a.post == 2;
-    hipLaunchKernelGGL((bias ? unjoin_kernel<T, R, NT, E, true> : unjoin_kernel<T, R, NT, E, false>), dim3(groups),
-                       dim3(NT < 256 ? 256 : NT), 0, s, a);
+// Workgroups of `kernel` that the current GPU holds at once.
+template <class K> uint32_t resident(K kernel, int threads) {
+    int dev = 0, cus = 0, per_cu = 0;
+    if (hipGetDevice(&dev) != hipSuccess ||
+        hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess ||
+        hipOccupancyMaxActiveBlocksPerMultiprocessor(&per_cu, kernel, threads, 0) != hipSuccess || cus * per_cu <= 0)
+        return 256;
+    return (uint32_t)(cus * per_cu);
+}
+
+// As many workgroups as the GPU holds at once, each with as many rows as the next (16384 x 2048
+// fp16: 150 us on 768 workgroups, three to a CU; 175 on 512, 183 on 1024); two rows at least once
+// there is one for every CU, which halves the planes (500 x 777 fp32: 14.4 and 15.6 us).
+template <typename T, typename R, int NT, int E, bool BIAS> hipError_t unjoin_t(const UnjoinArgs &a, hipStream_t s) {
+    constexpr uint32_t rpg = NT < 256 ? 256 / NT : 1, threads = NT < 256 ? 256 : NT;
+    static const uint32_t held = resident(unjoin_kernel<T, R, NT, E, BIAS>, threads);
+    const uint32_t groups = (a.rows + rpg - 1) / rpg, most = std::min(held, residual_planes(a.rows, a.cols));
+    const uint32_t each = std::max((groups + most - 1) / most, groups > 256 ? 2u : 1u);
+    const uint32_t grid = (groups + each - 1) / each;
+    hipLaunchKernelGGL((unjoin_kernel<T, R, NT, E, BIAS>), dim3(grid), dim3(threads), 0, s, a);
     if (a.work)
-        hipLaunchKernelGGL(unjoin_sums_kernel, dim3((a.cols + 31) / 32, kPlanes), dim3(1024), 0, s, a, groups);
+        hipLaunchKernelGGL(unjoin_sums_kernel, dim3((a.cols + 31) / 32, kPlanes), dim3(1024), 0, s, a, grid);
     return hipGetLastError();
 }
 
+template <typename T, typename R, int NT, int E> hipError_t unjoin_n(const UnjoinArgs &a, hipStream_t s) {
+    return a.pre == 2 || a.post == 2 ? unjoin_t<T, R, NT, E, true>(a, s) : unjoin_t<T, R, NT, E, false>(a, s);
+}
+
 template <typename T, typename R> hipError_t unjoin_c(const UnjoinArgs &a, hipStream_t s) {
-    if (a.cols <= 64) return unjoin_t<T, R, 16, 4>(a, s);
-    if (a.cols <= 256) return unjoin_t<T, R, 64, 4>(a, s);
-    if (a.cols <= 512) return unjoin_t<T, R, 64, 8>(a, s);
-    if (a.cols <= 1024) return unjoin_t<T, R, 256, 4>(a, s);
-    if (a.cols <= 2048) return unjoin_t<T, R, 256, 8>(a, s);
-    if (a.cols <= 4096) return unjoin_t<T, R, 512, 8>(a, s);
-    return unjoin_t<T, R, 512, 16>(a, s);
+    if (a.cols <= 64) return unjoin_n<T, R, 16, 4>(a, s);
+    if (a.cols <= 256) return unjoin_n<T, R, 64, 4>(a, s);
+    if (a.cols <= 512) return unjoin_n<T, R, 64, 8>(a, s);
+    if (a.cols <= 1024) return unjoin_n<T, R, 256, 4>(a, s);
+    if (a.cols <= 2048) return unjoin_n<T, R, 256, 8>(a, s);
+    if (a.cols <= 4096) return unjoin_n<T, R, 512, 8>(a, s);
+    return unjoin_n<T, R, 512, 16>(a, s);
 }
 
 }  // namespace

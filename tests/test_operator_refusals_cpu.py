@@ -177,7 +177,7 @@ def test_work_sizes():
     assert lib.skl_residual_work_bytes(0, 64) == lib.skl_residual_work_bytes(64, 0) == 0
     assert lib.skl_residual_work_bytes(1, 64) >= 5 * 64 * 4
     # workspaces do not grow with the rows without end
-    assert lib.skl_residual_work_bytes(1 << 31, 8192) <= 2048 * 5 * 8192 * 4
+    assert lib.skl_residual_work_bytes(1 << 31, 8192) <= 256 * 5 * 8192 * 4
 
 
 class NoContext:
