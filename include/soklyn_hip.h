@@ -309,14 +309,14 @@ int32_t skl_mxfp4_dequantise(skl_ctx *ctx, const void *codes, const void *scales
  * w_scales are its W [inputs x outputs] quantised down, the input is quantised along
  * its rows on the way, Z = Q(in) . Q(W) (+b) is summed in fp32, then norm and
  * activation (no dropout).  blk->w may be NULL.  Without a norm only out is written.
- * in may not overlap what is written.  work: skl_mxfp4_work_bytes(inputs, batch) bytes
- * of the caller's, 16-byte aligned; what it holds does not outlive the call, and calls
+ * in may not overlap what is written.  work: skl_mxfp4_work_bytes(inputs, outputs,
+ * batch) bytes of the caller's, 16-byte aligned; what it holds does not outlive the call, and calls
  * that overlap in time need a work of their own (as they need an out of their own). */
 int32_t skl_dense_forward_mxfp4(skl_ctx *ctx, const skl_dense_desc *blk, const void *in, uint32_t in_rows,
                                 uint32_t in_cols, uint32_t batch, const void *w_codes, const void *w_scales,
                                 void *work, size_t work_bytes);
-/* Host side. */
-size_t skl_mxfp4_work_bytes(uint32_t inputs, uint32_t batch);
+/* Host side; grows with the batch, and is 0 where the batch or the layer is small. */
+size_t skl_mxfp4_work_bytes(uint32_t inputs, uint32_t outputs, uint32_t batch);
 
 #ifdef __cplusplus
 }

@@ -159,5 +159,5 @@ extern "C" {
     pub fn skl_dense_forward_mxfp4(ctx: *mut SklCtx, blk: *const SklDenseDesc, input: *const c_void,
                                    in_rows: u32, in_cols: u32, batch: u32, w_codes: *const c_void,
                                    w_scales: *const c_void, work: *mut c_void, work_bytes: usize) -> i32;
-    pub fn skl_mxfp4_work_bytes(inputs: u32, batch: u32) -> usize;
+    pub fn skl_mxfp4_work_bytes(inputs: u32, outputs: u32, batch: u32) -> usize;
 }

@@ -98,7 +98,7 @@ _SIGS = {
     "skl_mxfp4_dequantise": (C.c_int32, [_VP, _VP, _VP, C.c_uint32, C.c_uint32, C.c_uint32, _VP, C.c_uint32]),
     "skl_dense_forward_mxfp4": (C.c_int32, [_VP, C.POINTER(SklDenseDesc), _VP, C.c_uint32, C.c_uint32,
                                             C.c_uint32, _VP, _VP, _VP, C.c_size_t]),
-    "skl_mxfp4_work_bytes": (C.c_size_t, [C.c_uint32, C.c_uint32]),
+    "skl_mxfp4_work_bytes": (C.c_size_t, [C.c_uint32, C.c_uint32, C.c_uint32]),
 }
 
 EXPORTED = tuple(_SIGS)

@@ -1941,7 +1941,9 @@ int32_t skl_mxfp4_dequantise(skl_ctx *ctx, const void *codes, const void *scales
     return mx_cast(ctx, dst, dtype, rows, cols, down, codes, scales, true);
 }
 
-size_t skl_mxfp4_work_bytes(uint32_t inputs, uint32_t batch) { return mx_work_bytes(inputs, batch); }
+size_t skl_mxfp4_work_bytes(uint32_t inputs, uint32_t outputs, uint32_t batch) {
+    return inputs && outputs ? mx_work(inputs, outputs, batch).bytes : 0;
+}
 
 int32_t skl_dense_forward_mxfp4(skl_ctx *ctx, const skl_dense_desc *b, const void *in, uint32_t in_rows,
                                 uint32_t in_cols, uint32_t batch, const void *w_codes, const void *w_scales,
@@ -1959,7 +1961,7 @@ int32_t skl_dense_forward_mxfp4(skl_ctx *ctx, const skl_dense_desc *b, const voi
     SKL_CHECK(!normed || (b->preact && b->predrop), SKL_ERR_NULL_POINTER);
     SKL_CHECK(b->norm == SKL_NORM_BATCH || b->b, SKL_ERR_NULL_POINTER);
     SKL_CHECK(aligned16(w_codes) && aligned_to(w_scales, 4), SKL_ERR_HARDWARE_CONSTRAINT);
-    const size_t need = mx_work_bytes(b->inputs, batch);
+    const size_t need = mx_work(b->inputs, b->outputs, batch).bytes;
     SKL_CHECK(!need || work, SKL_ERR_NULL_POINTER);
     SKL_CHECK(work_bytes >= need, SKL_ERR_ALLOCATION_LIMIT);
     SKL_CHECK(aligned16(work), SKL_ERR_HARDWARE_CONSTRAINT);

@@ -31,9 +31,33 @@ struct MxForwardArgs {
     uint32_t act;
     float leaky;
     void *out;                          // T [m x n]
-    void *work;                         // mx_work_bytes(k, m)
+    void *work;                         // mx_work(k, n, m).bytes
 };
-inline size_t mx_work_bytes(uint32_t, uint32_t) { return 0; }
+
+// The tile edge of the product, 0: the kernel for few rows, which needs no workspace.
+inline uint32_t mx_tile(uint32_t m, uint32_t n) {
+    const uint64_t t256 = (uint64_t)((m + 255) / 256) * ((n + 255) / 256);
+    const uint64_t t128 = (uint64_t)((m + 127) / 128) * ((n + 127) / 128);
+    return t256 >= 192 ? 256 : t128 >= 64 ? 128 : 0;
+}
+
+// The workspace of the tiled product: x's codes, then both scales in the product's order.
+struct MxWork {
+    uint32_t mp, np, k2;
+    size_t codes, xs, ws, bytes;
+};
+inline MxWork mx_work(uint32_t k, uint32_t n, uint32_t m) {
+    MxWork w{};
+    if (mx_tile(m, n) == 0) return w;
+    w.mp = (m + 255u) / 256u * 256u;
+    w.np = (n + 255u) / 256u * 256u;
+    w.k2 = (k + 255u) / 256u * 256u;
+    w.codes = (size_t)w.mp * (w.k2 / 2);
+    w.xs = (size_t)w.mp * (w.k2 / 32);
+    w.ws = (size_t)w.np * (w.k2 / 32);
+    w.bytes = w.codes + w.xs + w.ws;
+    return w;
+}
 hipError_t launch_mx_forward(const MxForwardArgs &a, uint32_t dtype, hipStream_t s);
 
 }  // namespace skl

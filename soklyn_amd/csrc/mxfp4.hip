@@ -1,13 +1,11 @@
 // mxfp4.hip — matrices to 4-bit microscaled floats and back, and the product of two.
+#include "mx_gemm.h"
 #include "mxfp4.h"
 #include "rows.h"
 
 namespace skl {
 
 namespace {
-
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-typedef int intx8 __attribute__((ext_vector_type(8)));
 
 // The scale byte of a block from its largest magnitude: 2^(e - 2) with 2^e the largest power of
 // two up to it, so that it lies in [4, 8) of the scale (6 is the largest code; past it values
@@ -141,12 +139,6 @@ __device__ __forceinline__ u32x4 mx_block(const T *row, uint32_t i, uint32_t k, 
     return u32x4{mx_codes(v[0], scale), mx_codes(v[1], scale), mx_codes(v[2], scale), mx_codes(v[3], scale)};
 }
 
-__device__ __forceinline__ void mx_mma(f32x4 &acc, u32x4 w, uint32_t ws, u32x4 x, uint32_t xs) {
-    const intx8 a = {(int)w[0], (int)w[1], (int)w[2], (int)w[3], 0, 0, 0, 0};
-    const intx8 b = {(int)x[0], (int)x[1], (int)x[2], (int)x[3], 0, 0, 0, 0};
-    acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, acc, 4, 4, 0, (int)ws, 0, (int)xs);
-}
-
 // x in 4 bits times w, tiles of 16 MT rows by 16 columns.  The operand of v_mfma_scale_16x16x128 is
 // one block of 32 consecutive elements of one vector per lane (vector lane % 16, block lane / 16)
 // with that block's scale, so w goes from memory to the matrix cores as it is stored, and a lane
@@ -172,7 +164,9 @@ template <typename T, int MT> __global__ void __launch_bounds__(512) mx_forward_
             const uint32_t row = min(m0 + 16u * i + r, a.m - 1);
             uint32_t xs;
             const u32x4 x = mx_block(reinterpret_cast<const T *>(a.x) + (uint64_t)row * a.k, k, a.k, xs);
-            mx_mma(acc[i], w, ws, x, xs);
+            const intx8 wop = {(int)w[0], (int)w[1], (int)w[2], (int)w[3], 0, 0, 0, 0};
+            const intx8 xop = {(int)x[0], (int)x[1], (int)x[2], (int)x[3], 0, 0, 0, 0};
+            acc[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wop, xop, acc[i], 4, 4, 0, (int)ws, 0, (int)xs);
         }
     }
 #pragma unroll
@@ -195,7 +189,70 @@ template <typename T, int MT> __global__ void __launch_bounds__(512) mx_forward_
     }
 }
 
+// What the tiled product reads: x [m x k] as codes [mp x k2 / 2], and both operands' scales in its
+// order (mx_gemm.h).  A workgroup takes 64 vectors by 128 elements, a thread one block; the first
+// `xtiles` workgroups x, the others w's scales.  Vectors and elements past the matrix are 0.
+struct MxStageArgs {
+    uint32_t m, n, k, kp, k2, xtiles;
+    const void *x;
+    const uint8_t *w_scales;
+    uint8_t *codes, *xs, *ws;
+};
+template <typename T> __global__ void __launch_bounds__(256) mx_stage_kernel(MxStageArgs a) {
+    __shared__ uint32_t words[4][16];
+    const uint32_t ktiles = a.k2 / 128u, vec = threadIdx.x >> 2, block = threadIdx.x & 3u;
+    const bool is_w = blockIdx.x >= a.xtiles;
+    const uint32_t tile = is_w ? blockIdx.x - a.xtiles : blockIdx.x, group = tile / ktiles, kt = tile % ktiles;
+    const uint32_t v = group * 64u + vec, kb = kt * 4u + block;
+    uint32_t scale = 0;
+    if (is_w) {
+        if (v < a.n && kb < a.kp / 32u) scale = a.w_scales[(uint64_t)v * (a.kp / 32u) + kb];
+    } else {
+        u32x4 c = {0, 0, 0, 0};
+        if (v < a.m) c = mx_block(reinterpret_cast<const T *>(a.x) + (uint64_t)v * a.k, kb * 32u, a.k, scale);
+        *reinterpret_cast<u32x4 *>(a.codes + (uint64_t)v * (a.k2 / 2u) + kb * 16u) = c;
+    }
+    reinterpret_cast<uint8_t *>(words)[block * 64u + (vec & 15u) * 4u + (vec >> 4)] = (uint8_t)scale;
+    __syncthreads();
+    if (threadIdx.x < 64)
+        reinterpret_cast<uint32_t *>(is_w ? a.ws : a.xs)[((uint64_t)group * (a.k2 / 32u) + kt * 4u) * 16u + threadIdx.x] =
+            words[threadIdx.x >> 4][threadIdx.x & 15u];
+}
+
+template <typename T, int BT> hipError_t mx_tiles_t(const MxForwardArgs &f, hipStream_t s) {
+    const MxWork w = mx_work(f.k, f.n, f.m);
+    MxStageArgs st{};
+    MxGemmArgs a{};
+    a.m = st.m = f.m;
+    a.n = st.n = f.n;
+    st.k = f.k;
+    a.kp = st.kp = mx_pad(f.k);
+    a.k2 = st.k2 = w.k2;
+    st.x = f.x;
+    st.w_scales = f.w_scales;
+    st.codes = reinterpret_cast<uint8_t *>(f.work);
+    st.xs = st.codes + w.codes;
+    st.ws = st.xs + w.xs;
+    a.x = st.codes;
+    a.xs = st.xs;
+    a.ws = st.ws;
+    a.w = f.w_codes;
+    a.bias = f.bias;
+    a.act = f.act;
+    a.leaky = f.leaky;
+    a.out = f.out;
+    a.tiles_m = (f.m + BT - 1) / BT;
+    a.tiles_n = (f.n + BT - 1) / BT;
+    st.xtiles = w.mp / 64u * (w.k2 / 128u);
+    hipLaunchKernelGGL(mx_stage_kernel<T>, dim3(st.xtiles + w.np / 64u * (w.k2 / 128u)), dim3(256), 0, s, st);
+    hipLaunchKernelGGL((mx_gemm_kernel<T, BT>), dim3(a.tiles_m * a.tiles_n), dim3(2 * BT), 0, s, a);
+    return hipGetLastError();
+}
+
 template <typename T> hipError_t mx_forward_t(const MxForwardArgs &a, hipStream_t s) {
+    const uint32_t bt = mx_tile(a.m, a.n);
+    if (bt == 256) return mx_tiles_t<T, 256>(a, s);
+    if (bt == 128) return mx_tiles_t<T, 128>(a, s);
     if (a.m <= 16)
         hipLaunchKernelGGL((mx_forward_kernel<T, 1>), dim3((a.n + 15) / 16), dim3(512), 0, s, a);
     else

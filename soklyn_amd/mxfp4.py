@@ -86,7 +86,7 @@ class Layer:
             for cache in ("prenorm", "centered", "preact", "predrop"):
                 setattr(self, cache, own(cache, None, (m, n), torch.zeros))
             self.norm_rstd = own("norm_rstd", None, (max(m, n),), torch.zeros)
-        size = abi.load().skl_mxfp4_work_bytes(inputs, max_batch)
+        size = abi.load().skl_mxfp4_work_bytes(inputs, outputs, max_batch)
         self.work = torch.empty(size, device=f"cuda:{dev}", dtype=torch.uint8)
         d = self._desc = abi.SklDenseDesc()
         d.dtype, d.inputs, d.outputs, d.max_batch = abi.F16 if half else abi.F32, inputs, outputs, max_batch

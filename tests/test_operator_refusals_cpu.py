@@ -153,7 +153,7 @@ def test_casts(back, code, change):
 def serve_status(d=None, **change):
     blk, at = desc(**(d or {}))
     a = dict(ctx=CTX, blk=C.byref(blk), x=at(), rows=8, cols=64, batch=8, codes=at(), scales=at(), work=at(),
-             size=abi.load().skl_mxfp4_work_bytes(64, 16))
+             size=abi.load().skl_mxfp4_work_bytes(64, 32, 16))
     a.update(change)
     return abi.status("skl_dense_forward_mxfp4", *a.values())
 
@@ -178,6 +178,14 @@ def test_work_sizes():
     assert lib.skl_residual_work_bytes(1, 64) >= 5 * 64 * 4
     # workspaces do not grow with the rows without end
     assert lib.skl_residual_work_bytes(1 << 31, 8192) <= 256 * 5 * 8192 * 4
+
+
+def test_work_of_a_layer_covers_its_smaller_batches():
+    need = abi.load().skl_mxfp4_work_bytes
+    for inputs, outputs in ((64, 32), (4096, 4096), (777, 1531), (300, 20000), (5000, 100)):
+        sizes = [need(inputs, outputs, b) for b in (0, 1, 16, 17, 64, 65, 128, 500, 1000, 2048, 4096, 8192, 100000)]
+        assert sizes == sorted(sizes) and sizes[0] == 0 and sizes[-1] > 0
+    assert need(0, 64, 64) == need(64, 0, 64) == 0
 
 
 class NoContext:
