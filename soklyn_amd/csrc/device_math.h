@@ -67,6 +67,20 @@ __device__ __forceinline__ float sigmoid_fast(float x) {
     return __builtin_amdgcn_rcpf(1.0f + __expf(-x));
 }
 
+// tanh to about 2 units in the last place: its series up to |x| = 0.4 (the first term left out is
+// 0.0036 x^13), else (1 - e) / (1 + e) with e = exp(-2 |x|), whose difference cancels at most one
+// bit there.
+__device__ __forceinline__ float tanh_fast(float x) {
+    const float q = x * x;
+    float s = fmaf(q, -0.008863235529902197f, 0.02186948853615520f);
+    s = fmaf(q, s, -0.05396825396825397f);
+    s = fmaf(q, s, 0.1333333333333333f);
+    s = fmaf(q, s, -0.3333333333333333f);
+    const float e = __expf(-2.0f * fabsf(x));
+    const float far = copysignf((1.0f - e) * __builtin_amdgcn_rcpf(1.0f + e), x);
+    return fabsf(x) < 0.4f ? fmaf(x * q, s, x) : far;
+}
+
 // Mish for fp16 blocks (util.cu:28-39) and its derivative (util.cu:75-87) from
 // one hardware exp and reciprocal per element: with u = e^x and n = u (u + 2),
 // tanh(softplus(x)) = n / (n + 2) and 1 - tanh^2 = 4 (n + 1) / (n + 2)^2.  Above

@@ -48,6 +48,24 @@ template <> struct Each<0> {
     template <class Fn> __device__ __forceinline__ static void run(Fn) {}
 };
 
+// The activation of several values, chosen once for them; the fast forms of device_math.h, a few
+// units in the last place of fp32 each.
+template <int N> __device__ __forceinline__ void activate(uint32_t act, float leaky, float (&v)[N]) {
+    auto each = [&](auto f) {
+#pragma unroll
+        for (int c = 0; c < N; ++c) v[c] = f(v[c]);
+    };
+    switch (act) {
+    case 1: each([](float x) { return sigmoid_fast(x); }); break;
+    case 2: each([](float x) { return fmaxf(0.0f, x); }); break;
+    case 3: each([&](float x) { return x > 0.0f ? x : leaky * x; }); break;
+    case 4: each([](float x) { return tanh_fast(x); }); break;
+    case 6: each([](float x) { return x * sigmoid_fast(x); }); break;
+    case 7: each([](float x) { return mish_fast(x); }); break;
+    default: break;
+    }
+}
+
 struct MxGemmArgs {
     uint32_t m, n, kp, k2;          // kp: W's padded k; k2: of X's codes and both scales, a multiple of 256
     uint32_t tiles_m, tiles_n;
@@ -58,7 +76,12 @@ struct MxGemmArgs {
     void *out;
 };
 
-// BT: tile edge; 256 with 8 waves (wave tile 128 x 64), 128 with 4 (64 x 64, two workgroups a CU).
+// BT: tile edge.  256: eight waves, two to a SIMD, each 128 x 64 of the tile; X's fragments are read
+// in place, each behind its last MFMA, as 128 accumulators leave no room for two sets.  128: four
+// waves of 64 x 64, two workgroups to a CU, both operands' fragments double.  (256 on four waves of
+// 128 x 128 with double fragments has the faster k loop, 51 us per 4096 of k over 8192 x 4096 against
+// 53, but one wave per SIMD hides nothing in the epilogue: 8192 x 4096 x 4096 with SiLU 82 us
+// against 78.)
 template <typename T, int BT>
 __global__ void __launch_bounds__(2 * BT) __attribute__((amdgpu_waves_per_eu(2, 2))) mx_gemm_kernel(MxGemmArgs a) {
     constexpr int NW = BT / 32, WN = BT / 64, TWM = BT / 2, MT = TWM / 16, NTL = 4;
@@ -67,6 +90,7 @@ __global__ void __launch_bounds__(2 * BT) __attribute__((amdgpu_waves_per_eu(2, 
     constexpr int STAGE = 2 * OP + 2 * SC;
     constexpr int IPO = BT / 8 / NW;                    // 1 KB loads of a wave per operand and tile
     constexpr int SLOADS = 2 * SC / 1024;               // of the whole workgroup for the scales
+    constexpr bool kInPlace = BT == 256;
     static_assert(SLOADS <= NW && SC % 1024 == 0, "at most one scale load per wave");
     __shared__ __attribute__((aligned(16))) char smem[2 * STAGE];
     lds_char *lsm = (lds_char *)(smem);
@@ -102,7 +126,6 @@ __global__ void __launch_bounds__(2 * BT) __attribute__((amdgpu_waves_per_eu(2, 
                                                  (int)off, (int)add, 0, 0);
     };
     // load q of this wave for k-tile kt
-    constexpr int NDMA = 2 * IPO + 1;
     auto load = [&](int kt, uint32_t stage, int q) {
         lds_char *st = lsm + stage;
         if (q < IPO) {
@@ -127,30 +150,36 @@ __global__ void __launch_bounds__(2 * BT) __attribute__((amdgpu_waves_per_eu(2, 
             asm volatile("s_nop 1" : "+a"(acc[i][j]));   // two wait states before its first use
         }
 
-    // fragments: X's are read in place behind their last use, W's and the scales are double
     const uint32_t lds0 = (uint32_t)(uintptr_t)lsm, swz = g ^ ((r >> 1) & 7u);
     const uint32_t xf = lds0 + (wm * TWM + r) * 128u, wf = lds0 + OP + (wn * 64u + r) * 128u;
     const uint32_t xsf = lds0 + 2 * OP + wm * MG * 512u + g * 64u + r * 4u;
     const uint32_t wsf = lds0 + 2 * OP + SC + wn * 512u + g * 64u + r * 4u;
-    u32x4 fx[MT], fw[2][NTL];
+    u32x4 fx[kInPlace ? 1 : 2][MT], fw[2][NTL];
     uint32_t sx[2][MG], sw[2];
-    auto read_w = [&](auto set, uint32_t stage, auto ks) {
-        constexpr int S = decltype(set)::value, KS = decltype(ks)::value;
+    constexpr int NDMA = 2 * IPO + 1;
+    // W's fragments and both scales of step KS of the tile in `stage`, into set KS; X's fragment I
+    auto read_w = [&](uint32_t stage, auto ks) {
+        constexpr int KS = decltype(ks)::value;
         const uint32_t at = wf + stage + ((4u * KS) ^ swz) * 16u;
-        Each<NTL>::run([&](auto j) { ds_read16<decltype(j)::value * 2048>(fw[S][j], at); });
-        ds_read4<KS * 256>(sw[S], wsf + stage);
-        Each<MG>::run([&](auto q) { ds_read4<decltype(q)::value * 512 + KS * 256>(sx[S][q], xsf + stage); });
+        Each<NTL>::run([&](auto j) { ds_read16<decltype(j)::value * 2048>(fw[KS][j], at); });
+        ds_read4<KS * 256>(sw[KS], wsf + stage);
+        Each<MG>::run([&](auto q) { ds_read4<decltype(q)::value * 512 + KS * 256>(sx[KS][q], xsf + stage); });
     };
     auto read_x = [&](auto i, uint32_t stage, auto ks) {
-        ds_read16<decltype(i)::value * 2048>(fx[i], xf + stage + ((4u * decltype(ks)::value) ^ swz) * 16u);
+        constexpr int KS = decltype(ks)::value;
+        ds_read16<decltype(i)::value * 2048>(fx[kInPlace ? 0 : KS][i], xf + stage + ((4u * KS) ^ swz) * 16u);
     };
-    auto pin_w = [&](auto set) {
-        constexpr int S = decltype(set)::value;
+    auto pin_w = [&](auto ks) {
+        constexpr int KS = decltype(ks)::value;
 #pragma unroll
-        for (int j = 0; j < NTL; ++j) pin(fw[S][j]);
-        pin(sw[S]);
+        for (int j = 0; j < NTL; ++j) pin(fw[KS][j]);
+        pin(sw[KS]);
 #pragma unroll
-        for (int q = 0; q < MG; ++q) pin(sx[S][q]);
+        for (int q = 0; q < MG; ++q) pin(sx[KS][q]);
+    };
+    auto pin_x = [&](auto ks) {
+#pragma unroll
+        for (int i = 0; i < MT; ++i) pin(fx[kInPlace ? 0 : decltype(ks)::value][i]);
     };
     typedef std::integral_constant<int, 0> Zero;
     typedef std::integral_constant<int, 1> One;
@@ -158,10 +187,40 @@ __global__ void __launch_bounds__(2 * BT) __attribute__((amdgpu_waves_per_eu(2, 
     // pending, the other MT - 1; before row i > 0 the rest of those and what rows 0 .. i - 1 issued.
     constexpr int W0 = MT - 1, W1 = MT - 1 + NTL + 1 + MG;
     static_assert(W1 <= 15, "the counter's range");
-    auto row = [&](auto i, auto set) {
-        constexpr int I = decltype(i)::value, S = decltype(set)::value;
-        Each<NTL>::run([&](auto j) {
-            mx_mma<decltype(j)::value, I % 4>(acc[I][j], fw[S][j], sw[S], fx[I], sx[S][I / 4]);
+    // Step KS: row by row of X's fragments its MFMAs, then the reads of the step after it (of the
+    // tile in `from`) and, in the second step, the loads of k-tile kn into `to`.  X's fragment I is
+    // read behind its own row (in place) or the row before it.
+    auto step = [&](auto ks, uint32_t from, int kn, uint32_t to) {
+        constexpr int KS = decltype(ks)::value;
+        typedef std::integral_constant<int, 1 - KS> Next;
+        Each<MT>::run([&](auto i) {
+            constexpr int I = decltype(i)::value;
+            if constexpr (KS == 0) {
+                if constexpr (!kInPlace) {
+                    if constexpr (I == 0) {
+                        wait_lgkmcnt<0>();
+                        pin_w(ks);
+                        pin_x(ks);
+                    }
+                } else if constexpr (I == 0) {
+                    wait_lgkmcnt<W0>();
+                    pin_w(ks);
+                    pin(fx[0][0]);
+                } else {
+                    wait_lgkmcnt<W1>();
+                    pin(fx[0][I]);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            Each<NTL>::run([&](auto j) {
+                mx_mma<decltype(j)::value, I % 4>(acc[I][j], fw[KS][j], sw[KS], fx[kInPlace ? 0 : KS][I], sx[KS][I / 4]);
+                __builtin_amdgcn_sched_barrier(0);
+            });
+            if constexpr (KS == 1)
+#pragma unroll
+                for (int q = I * NDMA / MT; q < (I + 1) * NDMA / MT; ++q) load(kn, to, q);
+            if constexpr (I == 0) read_w(from, Next());
+            read_x(i, from, Next());
             __builtin_amdgcn_sched_barrier(0);
         });
     };
@@ -172,91 +231,101 @@ __global__ void __launch_bounds__(2 * BT) __attribute__((amdgpu_waves_per_eu(2, 
     __builtin_amdgcn_s_barrier();
 #pragma unroll
     for (int q = 0; q < NDMA; ++q) load(min(1, nk - 1), STAGE, q);
-    read_w(Zero(), 0u, Zero());
+    read_w(0u, Zero());
     Each<MT>::run([&](auto i) { read_x(i, 0u, Zero()); });
     uint32_t stage = 0;
     for (int kt = 0; kt < nk; ++kt) {
-        Each<MT>::run([&](auto i) {   // first step, the second's fragments behind it
-            constexpr int I = decltype(i)::value;
-            if constexpr (I == 0) {
-                wait_lgkmcnt<W0>();
-                pin_w(Zero());
-            } else {
-                wait_lgkmcnt<W1>();
-            }
-            pin(fx[I]);
-            __builtin_amdgcn_sched_barrier(0);
-            row(i, Zero());
-            if constexpr (I == 0) read_w(One(), stage, One());
-            read_x(i, stage, One());
-            __builtin_amdgcn_sched_barrier(0);
-        });
-        // the next tile has landed and every read of this one's stage is done
+        step(Zero(), stage, 0, 0u);
+        // the next tile has landed, and every read of this one's stage is done
         wait_vmcnt<0>();
         wait_lgkmcnt<0>();
         pin_w(One());
-#pragma unroll
-        for (int i = 0; i < MT; ++i) pin(fx[i]);
+        pin_x(One());
         __builtin_amdgcn_s_barrier();
         __builtin_amdgcn_sched_barrier(0);
-        const int kn = min(kt + 2, nk - 1);   // past the end: the last tile again, not used
-        const uint32_t other = stage ^ 0u ? 0u : (uint32_t)STAGE;
-        Each<MT>::run([&](auto i) {   // second step, the refill of this stage and the next tile's fragments
-            constexpr int I = decltype(i)::value;
-            row(i, One());
-            constexpr int Q0 = I * NDMA / MT, Q1 = (I + 1) * NDMA / MT;
-#pragma unroll
-            for (int q = Q0; q < Q1; ++q) load(kn, stage, q);
-            if constexpr (I == 0) read_w(Zero(), other, Zero());
-            read_x(i, other, Zero());
-            __builtin_amdgcn_sched_barrier(0);
-        });
+        const uint32_t other = STAGE - stage;
+        // past the end: the last tile again, not used
+        step(One(), other, min(kt + 2, nk - 1), stage);
         stage = other;
     }
     wait_vmcnt<0>();
     wait_lgkmcnt<0>();
     pin_w(Zero());
-#pragma unroll
-    for (int i = 0; i < MT; ++i) pin(fx[i]);
+    pin_x(Zero());
     // wait states before the last sums are read (and those reads stay below)
     asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 7" ::: "memory");
 #pragma unroll
     for (int i = 0; i < MT; ++i)
 #pragma unroll
         for (int j = 0; j < NTL; ++j) asm volatile("" : "+a"(acc[i][j]));
-    __syncthreads();
 
-    // Epilogue: a wave puts 64 of its rows at a time into LDS of its own, then takes them row-wise, 8
-    // columns a lane, so that 8 lanes store a row's 64 columns.  (The loop over them is not
-    // unrolled: the activation is chosen at run time, and its code once is enough.)
-    constexpr int PITCH = 68;
-    static_assert(NW * 64 * PITCH * 4 <= 2 * STAGE, "the epilogue's rows fit the stages");
-    float *e = reinterpret_cast<float *>(smem) + wave * 64 * PITCH;
-    const uint32_t col = n0 + wn * 64u + (lane & 7u) * 8u;
-    float bias[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-    if (a.bias && col < a.n) load_row<T, 8>(a.bias, col, a.n, bias);
+    // Epilogue, from the registers: a lane's block holds columns 16 j + 4 g .. + 3 of row 16 i + r.
+    // For fp16 the lanes of two neighbouring g exchange halves of two blocks, so that each has 8
+    // columns of one, and an instruction stores 16 rows by 64 bytes.  A loop over the rows of blocks,
+    // with the accumulators (whose registers are fixed) taken by a switch: unrolled, the activations
+    // would be 300 KB of code for a 64 KB instruction cache.
+    const uint32_t nw = n0 + wn * 64u;
+    float bias[NTL * 4];
 #pragma unroll
-    for (int p = 0; p < MT / 4; ++p) {
+    for (int j = 0; j < NTL; ++j) {
+        float b[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (a.bias && nw + 16u * j + 4u * g < a.n) load_row<T, 4>(a.bias, nw + 16u * j + 4u * g, a.n, b);
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int j = 0; j < NTL; ++j)
-                *reinterpret_cast<f32x4 *>(e + (i * 16 + r) * PITCH + j * 16 + 4 * g) = acc[4 * p + i][j];
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
+        for (int c = 0; c < 4; ++c) bias[4 * j + c] = b[c];
+    }
 #pragma unroll 1
-        for (uint32_t b = 0; b < 8; ++b) {
-            const uint32_t er = b * 8u + (lane >> 3), m = m0 + wm * TWM + p * 64u + er;
-            float v[8];
+    for (int i = 0; i < MT; ++i) {
+        const uint32_t m = m0 + wm * TWM + 16u * i + r;
+        T *to = reinterpret_cast<T *>(a.out) + (uint64_t)m * a.n;
+        float v[NTL * 4];
+        auto take = [&](auto row) {
 #pragma unroll
-            for (int c = 0; c < 8; ++c) v[c] = e[er * PITCH + (lane & 7u) * 8u + c] + bias[c];
-            if (a.act)
-#pragma unroll
-                for (int c = 0; c < 8; ++c) v[c] = activation<float>(a.act, v[c], a.leaky);
-            if (m < a.m && col < a.n) store_row<T, 8>(reinterpret_cast<T *>(a.out) + (uint64_t)m * a.n, col, a.n, v);
+            for (int c = 0; c < NTL * 4; ++c) v[c] = acc[decltype(row)::value][c / 4][c % 4] + bias[c];
+        };
+        switch (i) {
+        case 0: take(std::integral_constant<int, 0>()); break;
+        case 1: take(std::integral_constant<int, 1>()); break;
+        case 2: take(std::integral_constant<int, 2>()); break;
+        case 3: take(std::integral_constant<int, 3>()); break;
+        case 4: take(std::integral_constant<int, (MT > 4 ? 4 : 0)>()); break;
+        case 5: take(std::integral_constant<int, (MT > 4 ? 5 : 0)>()); break;
+        case 6: take(std::integral_constant<int, (MT > 4 ? 6 : 0)>()); break;
+        default: take(std::integral_constant<int, (MT > 4 ? 7 : 0)>()); break;
         }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
+        activate(a.act, a.leaky, v);
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int j = 0; j < NTL; ++j) {
+                const uint32_t col = nw + 16u * j + 4u * g;
+                const float w[4] = {v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]};
+                if (m < a.m && col < a.n) store_row<T, 4>(to, col, a.n, w);
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < NTL; j += 2) {
+                typedef T T2 __attribute__((ext_vector_type(2)));
+                typedef T T8 __attribute__((ext_vector_type(8)));
+                u32x4 w;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const uint32_t lo = __builtin_bit_cast(uint32_t, T2{(T)v[4 * j + 2 * h], (T)v[4 * j + 2 * h + 1]});
+                    const uint32_t hi = __builtin_bit_cast(uint32_t, T2{(T)v[4 * j + 4 + 2 * h], (T)v[4 * j + 4 + 2 * h + 1]});
+                    const auto both = __builtin_amdgcn_permlane16_swap(lo, hi, false, false);
+                    w[h] = both[0];
+                    w[2 + h] = both[1];
+                }
+                const uint32_t col = nw + 16u * (j + (g & 1u)) + 8u * (g >> 1);
+                if (m >= a.m || col >= a.n) continue;
+                if (col + 8u <= a.n) {
+                    *reinterpret_cast<typename Unaligned<T, 8>::type *>(to + col) = __builtin_bit_cast(T8, w);
+                } else {
+                    const T8 part = __builtin_bit_cast(T8, w);
+#pragma unroll
+                    for (int c = 0; c < 8; ++c)
+                        if (col + c < a.n) to[col + c] = part[c];
+                }
+            }
+        }
     }
 }
 

@@ -18,22 +18,9 @@ constexpr float kNormEps = 1e-6f;   // the blocks' own norms add the same
 
 namespace {
 
-// tanh to about 2 units in the last place: its series up to |x| = 0.4 (the first term left out is
-// 0.0036 x^13), else (1 - e) / (1 + e) with e = exp(-2 |x|), whose difference cancels no more than
-// one bit there.
-__device__ __forceinline__ float tanh_gate(float x) {
-    const float q = x * x;
-    float s = fmaf(q, -0.008863235529902197f, 0.02186948853615520f);
-    s = fmaf(q, s, -0.05396825396825397f);
-    s = fmaf(q, s, 0.1333333333333333f);
-    s = fmaf(q, s, -0.3333333333333333f);
-    const float e = __expf(-2.0f * fabsf(x));
-    const float far = copysignf((1.0f - e) * __builtin_amdgcn_rcpf(1.0f + e), x);
-    return fabsf(x) < 0.4f ? fmaf(x * q, s, x) : far;
-}
 __device__ __forceinline__ float gate_value(uint32_t act, float g) {
     if (act == 1) return sigmoid_fast(g);
-    if (act == 4) return tanh_gate(g);
+    if (act == 4) return tanh_fast(g);
     return g;
 }
 // The gate's slope from its value a.
