@@ -139,53 +139,143 @@ __device__ __forceinline__ u32x4 mx_block(const T *row, uint32_t i, uint32_t k, 
     return u32x4{mx_codes(v[0], scale), mx_codes(v[1], scale), mx_codes(v[2], scale), mx_codes(v[3], scale)};
 }
 
-// x in 4 bits times w, tiles of 16 MT rows by 16 columns.  The operand of v_mfma_scale_16x16x128 is
-// one block of 32 consecutive elements of one vector per lane (vector lane % 16, block lane / 16)
-// with that block's scale, so w goes from memory to the matrix cores as it is stored, and a lane
-// turns 32 elements of x into its operand by itself.  The eight waves of a workgroup take every
-// eighth step of 128 of the k axis, and their sums are joined in LDS in the order of the waves.
-template <typename T, int MT> __global__ void __launch_bounds__(512) mx_forward_kernel(MxForwardArgs a) {
+__device__ __forceinline__ void mx_mma_plain(f32x4 &acc, const u32x4 &w, uint32_t ws, const u32x4 &x, uint32_t xs) {
+    const intx8 a = {(int)w[0], (int)w[1], (int)w[2], (int)w[3], 0, 0, 0, 0};
+    const intx8 b = {(int)x[0], (int)x[1], (int)x[2], (int)x[3], 0, 0, 0, 0};
+    acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, acc, 4, 4, 0, (int)ws, 0, (int)xs);
+}
+
+// 16 x 16 outputs of a wave: lane holds columns col .. + 3 of a row.
+template <typename T>
+__device__ __forceinline__ void mx_store(const MxForwardArgs &a, f32x4 s, uint32_t row, uint32_t col) {
+    if (row >= a.m || col >= a.n) return;
+    float v[4], b[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (a.bias) load_row<T, 4>(a.bias, col, a.n, b);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = s[e] + b[e];
+    activate(a.act, a.leaky, v);
+    store_row<T, 4>(reinterpret_cast<T *>(a.out) + (uint64_t)row * a.n, col, a.n, v);
+}
+
+// Few rows: x in 4 bits times w in one launch, tiles of 16 MT rows by 16 columns.  The operand of
+// v_mfma_scale_16x16x128 is one block of 32 consecutive elements of one vector per lane (vector
+// lane % 16, block lane / 16) with that block's scale, so w goes from memory to the matrix cores
+// as it is stored, and a lane turns 32 elements of x into its operand by itself.  The eight waves
+// of a workgroup take every eighth step of 128 of the k axis, with the loads of U steps in flight,
+// and their sums are joined in LDS in the order of the waves.
+template <typename T, int MT, int U> __global__ void __launch_bounds__(512) mx_rows_kernel(MxForwardArgs a) {
     constexpr int WV = 8;
+    typedef typename Unaligned<T, 8>::type Vec;
     __shared__ f32x4 part[WV][MT][64];
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, r = lane & 15u, g = lane >> 4;
-    const uint32_t kp = mx_pad(a.k), ntiles = (a.n + 15u) / 16u;
-    const uint32_t n0 = blockIdx.x % ntiles * 16u, m0 = blockIdx.x / ntiles * 16u * MT;
+    const uint32_t n0 = blockIdx.x * 16u;
+    const uint32_t kp = mx_pad(a.k);
     // rows past an operand's end read its last one; what they give is not stored
     const uint32_t wn = min(n0 + r, a.n - 1);
     const uint8_t *wc = a.w_codes + (uint64_t)wn * (kp / 2), *wsc = a.w_scales + (uint64_t)wn * (kp / 32);
+    const T *x[MT];
     f32x4 acc[MT];
 #pragma unroll
-    for (int i = 0; i < MT; ++i) acc[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    for (uint32_t k = wave * 128u + g * 32u; k < kp; k += WV * 128u) {
-        const u32x4 w = *reinterpret_cast<const u32x4 *>(wc + k / 2);
-        const uint32_t ws = wsc[k / 32];
+    for (int i = 0; i < MT; ++i) {
+        x[i] = reinterpret_cast<const T *>(a.x) + (uint64_t)min(16u * i + r, a.m - 1) * a.k;
+        acc[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    for (uint32_t k0 = wave * 128u; k0 < kp; k0 += U * WV * 128u) {
+        u32x4 w[U];
+        uint32_t ws[U];
+        Vec v[U][MT][4];
 #pragma unroll
-        for (int i = 0; i < MT; ++i) {
-            const uint32_t row = min(m0 + 16u * i + r, a.m - 1);
-            uint32_t xs;
-            const u32x4 x = mx_block(reinterpret_cast<const T *>(a.x) + (uint64_t)row * a.k, k, a.k, xs);
-            const intx8 wop = {(int)w[0], (int)w[1], (int)w[2], (int)w[3], 0, 0, 0, 0};
-            const intx8 xop = {(int)x[0], (int)x[1], (int)x[2], (int)x[3], 0, 0, 0, 0};
-            acc[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wop, xop, acc[i], 4, 4, 0, (int)ws, 0, (int)xs);
+        for (int u = 0; u < U; ++u) {
+            const uint32_t k = k0 + u * WV * 128u + g * 32u;
+            if (k >= kp) break;
+            w[u] = *reinterpret_cast<const u32x4 *>(wc + k / 2);
+            ws[u] = wsc[k / 32];
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    const uint32_t e0 = k + 8 * c;
+                    v[u][i][c] = Vec{};
+                    if (e0 + 8 <= a.k)
+                        v[u][i][c] = *reinterpret_cast<const Vec *>(x[i] + e0);
+                    else
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            if (e0 + e < a.k) v[u][i][c][e] = x[i][e0 + e];
+                }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (k0 + u * WV * 128u >= kp) break;
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+                uint32_t big = 0;
+                float f[4][8];
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        f[c][e] = (float)v[u][i][c][e];
+                        big = max(big, magnitude(f[c][e]));
+                    }
+                const uint32_t xs = mx_scale(big);
+                const u32x4 xc = {mx_codes(f[0], xs), mx_codes(f[1], xs), mx_codes(f[2], xs), mx_codes(f[3], xs)};
+                mx_mma_plain(acc[i], w[u], ws[u], xc, xs);
+            }
         }
     }
 #pragma unroll
     for (int i = 0; i < MT; ++i) part[wave][i][lane] = acc[i];
     __syncthreads();
-    // wave i joins row block i: lane holds columns n0 + 4 g .. + 3 of row m0 + 16 i + r
-    for (uint32_t i = wave; i < MT; i += WV) {
-        f32x4 s = part[0][i][lane];
+    if (wave >= MT) return;
+    f32x4 s = part[0][wave][lane];
 #pragma unroll
-        for (int w = 1; w < WV; ++w) s += part[w][i][lane];
-        const uint32_t row = m0 + 16u * i + r, col = n0 + 4u * g;
-        if (row >= a.m) continue;
-        float v[4];
+    for (int w = 1; w < WV; ++w) s += part[w][wave][lane];
+    mx_store<T>(a, s, 16u * wave + r, n0 + 4u * g);
+}
+
+// Ordinary batches: 64 x 64 tiles over staged codes and scales (below), whose waves split the k axis
+// as above, fragments straight from memory to registers.
+template <typename T> __global__ void __launch_bounds__(512) mx_split_kernel(MxForwardArgs a, MxGemmArgs t) {
+    constexpr int WV = 8;
+    __shared__ f32x4 part[WV][16][64];
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, r = lane & 15u, g = lane >> 4;
+    uint32_t tm, tn;
+    tile_coords(blockIdx.x, t.tiles_m, t.tiles_n, tm, tn);
+    const uint32_t m0 = tm * 64u, n0 = tn * 64u, xp = t.k2 / 2, wp = t.kp / 2;
+    const uint8_t *x = t.x + (uint64_t)(m0 + r) * xp + g * 16u, *w[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            v[e] = s[e] + (a.bias && col + e < a.n ? to_f32(reinterpret_cast<const T *>(a.bias)[col + e]) : 0.0f);
-            v[e] = activation<float>(a.act, v[e], a.leaky);
-        }
-        if (col < a.n) store_row<T, 4>(reinterpret_cast<T *>(a.out) + (uint64_t)row * a.n, col, a.n, v);
+    for (int j = 0; j < 4; ++j) w[j] = t.w + (uint64_t)min(n0 + 16u * j + r, a.n - 1) * wp + g * 16u;
+    const uint32_t *xs = reinterpret_cast<const uint32_t *>(t.xs) + ((uint64_t)tm * (t.k2 / 32) + g) * 16u + r;
+    const uint32_t *ws = reinterpret_cast<const uint32_t *>(t.ws) + ((uint64_t)tn * (t.k2 / 32) + g) * 16u + r;
+    f32x4 acc[4][4];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) acc[i / 4][i % 4] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 2
+    for (uint32_t step = wave; step < t.kp / 128u; step += WV) {
+        u32x4 fx[4], fw[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) fx[i] = *reinterpret_cast<const u32x4 *>(x + 16u * i * xp + step * 64u);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) fw[j] = *reinterpret_cast<const u32x4 *>(w[j] + step * 64u);
+        const uint32_t sx = xs[step * 64u], sw = ws[step * 64u];
+        Each<16>::run([&](auto q) {
+            constexpr int I = decltype(q)::value / 4, J = decltype(q)::value % 4;
+            const intx8 wo = {(int)fw[J][0], (int)fw[J][1], (int)fw[J][2], (int)fw[J][3], 0, 0, 0, 0};
+            const intx8 xo = {(int)fx[I][0], (int)fx[I][1], (int)fx[I][2], (int)fx[I][3], 0, 0, 0, 0};
+            acc[I][J] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wo, xo, acc[I][J], 4, 4, J, (int)sw, I, (int)sx);
+        });
+    }
+#pragma unroll
+    for (int q = 0; q < 16; ++q) part[wave][q][lane] = acc[q / 4][q % 4];
+    __syncthreads();
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const uint32_t q = 2 * wave + h;
+        f32x4 s = part[0][q][lane];
+#pragma unroll
+        for (int v = 1; v < WV; ++v) s += part[v][q][lane];
+        mx_store<T>(a, s, m0 + 16u * (q / 4) + r, n0 + 16u * (q % 4) + 4u * g);
     }
 }
 
@@ -219,6 +309,7 @@ template <typename T> __global__ void __launch_bounds__(256) mx_stage_kernel(MxS
             words[threadIdx.x >> 4][threadIdx.x & 15u];
 }
 
+// BT: the tile edge, 64, 128 or 256.
 template <typename T, int BT> hipError_t mx_tiles_t(const MxForwardArgs &f, hipStream_t s) {
     const MxWork w = mx_work(f.k, f.n, f.m);
     MxStageArgs st{};
@@ -245,18 +336,26 @@ template <typename T, int BT> hipError_t mx_tiles_t(const MxForwardArgs &f, hipS
     a.tiles_n = (f.n + BT - 1) / BT;
     st.xtiles = w.mp / 64u * (w.k2 / 128u);
     hipLaunchKernelGGL(mx_stage_kernel<T>, dim3(st.xtiles + w.np / 64u * (w.k2 / 128u)), dim3(256), 0, s, st);
-    hipLaunchKernelGGL((mx_gemm_kernel<T, BT>), dim3(a.tiles_m * a.tiles_n), dim3(2 * BT), 0, s, a);
+    if constexpr (BT == 64)
+        hipLaunchKernelGGL(mx_split_kernel<T>, dim3(a.tiles_m * a.tiles_n), dim3(512), 0, s, f, a);
+    else
+        hipLaunchKernelGGL((mx_gemm_kernel<T, BT>), dim3(a.tiles_m * a.tiles_n), dim3(2 * BT), 0, s, a);
     return hipGetLastError();
 }
 
 template <typename T> hipError_t mx_forward_t(const MxForwardArgs &a, hipStream_t s) {
-    const uint32_t bt = mx_tile(a.m, a.n);
-    if (bt == 256) return mx_tiles_t<T, 256>(a, s);
-    if (bt == 128) return mx_tiles_t<T, 128>(a, s);
+    switch (mx_tile(a.m, a.n)) {
+    case 256: return mx_tiles_t<T, 256>(a, s);
+    case 128: return mx_tiles_t<T, 128>(a, s);
+    case 64: return mx_tiles_t<T, 64>(a, s);
+    default: break;
+    }
+    // fewer elements in flight where a row's are twice as large or there are twice as many rows
+    constexpr int U = sizeof(T) == 2 ? 4 : 2;
     if (a.m <= 16)
-        hipLaunchKernelGGL((mx_forward_kernel<T, 1>), dim3((a.n + 15) / 16), dim3(512), 0, s, a);
+        hipLaunchKernelGGL((mx_rows_kernel<T, 1, U>), dim3((a.n + 15) / 16), dim3(512), 0, s, a);
     else
-        hipLaunchKernelGGL((mx_forward_kernel<T, 4>), dim3((a.n + 15) / 16 * ((a.m + 63) / 64)), dim3(512), 0, s, a);
+        hipLaunchKernelGGL((mx_rows_kernel<T, 2, U / 2>), dim3((a.n + 15) / 16), dim3(512), 0, s, a);
     return hipGetLastError();
 }
 
