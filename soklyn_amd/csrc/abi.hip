@@ -1910,13 +1910,15 @@ static int32_t mx_cast(skl_ctx *ctx, const void *values, uint32_t dtype, uint32_
                        const void *codes, const void *scales, bool back) {
     SKL_CHECK(ctx, SKL_ERR_NULL_POINTER);
     SKL_CHECK(dtype <= SKL_F16 && down <= 1, SKL_ERR_INVALID_CONFIGURATION);
-    SKL_CHECK((down ? rows : cols) <= 0x7fffff80u, SKL_ERR_INVALID_CONFIGURATION);
+    // elements of a vector and 256-element pieces of the matrix are counted in 32 bits
+    const uint64_t k = down ? rows : cols, n = down ? cols : rows;
+    SKL_CHECK(k <= 0x7fffff80u && n * ((k + 255) / 256) <= 0xffffffffu, SKL_ERR_INVALID_CONFIGURATION);
     if (rows == 0 || cols == 0) return SKL_OK;
     SKL_CHECK(values && codes && scales, SKL_ERR_NULL_POINTER);
     SKL_CHECK(aligned16(codes) && aligned_to(scales, 4), SKL_ERR_HARDWARE_CONSTRAINT);
     MxCastArgs a{};
-    a.n = down ? cols : rows;
-    a.k = down ? rows : cols;
+    a.n = (uint32_t)n;
+    a.k = (uint32_t)k;
     const size_t kp = mx_pad(a.k), nv = (size_t)rows * cols * (dtype == SKL_F16 ? 2 : 4);
     const Span v{values, nv}, c{codes, a.n * kp / 2}, sc{scales, a.n * kp / 32};
     SKL_CHECK(!overlaps(v.p, v.bytes, c.p, c.bytes) && !overlaps(v.p, v.bytes, sc.p, sc.bytes) &&

@@ -32,96 +32,200 @@ __device__ __forceinline__ uint32_t mx_codes(const float (&v)[8], uint32_t scale
 
 __device__ __forceinline__ uint32_t magnitude(float v) { return __builtin_bit_cast(uint32_t, v) & 0x7fffffffu; }
 
-// The value of a code: its magnitude is exact in fp32, and so is its product with any scale.
-__device__ __forceinline__ float mx_value(uint32_t code, uint32_t scale) {
-    const uint32_t c = code & 7u;
-    // 0, 0.5, then 1.m 2^(e - 1)
-    float v = c < 2u ? 0.5f * (float)c : __builtin_bit_cast(float, ((c >> 1) + 126u) << 23 | (c & 1u) << 22);
-    v = code & 8u ? -v : v;
-    return scale == 255u ? __builtin_nanf("") : ldexpf(v, (int)scale - 127);
+// Eight codes, the first in the lowest half byte, as the values they stand for: the convert's are
+// exact, and so is their product with any scale.
+__device__ __forceinline__ void mx_values(uint32_t codes, uint32_t scale, float (&v)[8]) {
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    const f32x2 p[4] = {
+        __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, 1.0f, 0), __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, 1.0f, 1),
+        __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, 1.0f, 2), __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, 1.0f, 3)};
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+        v[e] = scale == 255u ? __builtin_nanf("") : ldexpf(p[e / 2][e % 2], (int)scale - 127);
 }
 
-// Vectors along the rows of a [n x k] matrix: four lanes to a block of 32, eight elements each.
+// Vectors along the rows of a [n x k] matrix: E elements to a lane, a wave to 64 E elements of a row or
+// to several rows that are shorter.
+struct MxRows {
+    uint32_t lanes, per_row, rows;   // lanes of a vector, waves of a vector, vectors of a wave
+    uint64_t waves;
+};
+template <int E> __host__ __device__ __forceinline__ MxRows mx_rows(uint32_t n, uint32_t k) {
+    MxRows r;
+    r.lanes = mx_pad(k) / E;
+    r.per_row = (r.lanes + 63) / 64;
+    r.rows = r.lanes < 64 ? 64 / r.lanes : 1;
+    r.waves = (uint64_t)((n + r.rows - 1) / r.rows) * r.per_row;
+    return r;
+}
+// For every lane that has elements of a vector use(vector, lane of the vector, what load(...) of
+// these gave): the loads of U pieces before the first is used, or a wave would have a kilobyte on its
+// way at a time.
+template <int E, int U, class Load, class Use>
+__device__ __forceinline__ void mx_each(uint32_t n, uint32_t k, Load load, Use use) {
+    const MxRows r = mx_rows<E>(n, k);
+    const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t sub = r.rows > 1 ? lane / r.lanes : 0;
+    // (32-bit divisions, once for U pieces: in 64 bits and for each they took longer than the stores)
+    const uint32_t waves = (uint32_t)r.waves, stride = gridDim.x * 4 * U;
+    for (uint32_t w0 = (blockIdx.x * 4 + wave) * U; w0 < waves; w0 += stride) {
+        decltype(load(0u, 0u)) got[U];
+        uint32_t vec[U], l[U], row = w0 / r.per_row, part = w0 - row * r.per_row;
+        bool on[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            vec[u] = row * r.rows + sub;
+            l[u] = part * 64 + lane - sub * r.lanes;
+            on[u] = w0 + u < waves && sub < r.rows && l[u] < r.lanes && vec[u] < n;
+            if (on[u]) got[u] = load(vec[u], l[u]);
+            if (++part == r.per_row) {
+                part = 0;
+                ++row;
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (on[u]) use(vec[u], l[u], got[u]);
+        if (w0 + stride < w0) break;   // past 32 bits
+    }
+}
+
+template <typename T, int E> struct MxPiece {
+    float v[E];
+};
 template <typename T> __global__ void __launch_bounds__(256) mx_quantise_kernel(MxCastArgs a) {
-    const uint32_t kp = mx_pad(a.k), lanes = kp / 8;   // lanes of a vector
-    const uint64_t total = (uint64_t)a.n * lanes;
-    for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (uint64_t)gridDim.x * 256) {
-        const uint32_t row = (uint32_t)(i / lanes), l = (uint32_t)(i % lanes);
-        float v[8];
-        load_row<T, 8>(reinterpret_cast<const T *>(a.values) + (uint64_t)row * a.k, l * 8, a.k, v);
-        uint32_t big = 0;
+    mx_each<8, 2>(
+        a.n, a.k,
+        [&](uint32_t vec, uint32_t l) {
+            MxPiece<T, 8> p;
+            load_row<T, 8>(reinterpret_cast<const T *>(a.values) + (uint64_t)vec * a.k, l * 8, a.k, p.v);
+            return p;
+        },
+        [&](uint32_t vec, uint32_t l, const MxPiece<T, 8> &p) {
+            uint32_t big = 0;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) big = max(big, magnitude(v[e]));
-        big = max(big, (uint32_t)__shfl_xor((int)big, 1, 64));
-        big = max(big, (uint32_t)__shfl_xor((int)big, 2, 64));
-        const uint32_t scale = mx_scale(big);
-        reinterpret_cast<uint32_t *>(a.codes)[i] = mx_codes(v, scale);
-        if ((l & 3u) == 0) a.scales[i / 4] = (uint8_t)scale;
-    }
+            for (int e = 0; e < 8; ++e) big = max(big, magnitude(p.v[e]));
+            // a block's four lanes are here together
+            big = max(big, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)big, 0xB1, 0xf, 0xf, true));   // quad_perm 1 0 3 2
+            big = max(big, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)big, 0x4E, 0xf, 0xf, true));   // quad_perm 2 3 0 1
+            const uint32_t scale = mx_scale(big);
+            const uint64_t at = (uint64_t)vec * (mx_pad(a.k) / 8) + l;
+            reinterpret_cast<uint32_t *>(a.codes)[at] = mx_codes(p.v, scale);
+            if ((l & 3u) == 0) a.scales[at / 4] = (uint8_t)scale;
+        });
 }
 
+// 16 bytes of values to a lane, so that a wave writes 1 KB without gaps.
+template <typename T> constexpr int kValues = 16 / sizeof(T);
+struct MxPair {
+    uint32_t codes, scale;
+};
 template <typename T> __global__ void __launch_bounds__(256) mx_dequantise_kernel(MxCastArgs a) {
-    const uint32_t lanes = mx_pad(a.k) / 8;
-    const uint64_t total = (uint64_t)a.n * lanes;
-    for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (uint64_t)gridDim.x * 256) {
-        const uint32_t row = (uint32_t)(i / lanes), l = (uint32_t)(i % lanes);
-        const uint32_t c = reinterpret_cast<const uint32_t *>(a.codes)[i], scale = a.scales[i / 4];
-        float v[8];
+    constexpr int E = kValues<T>;
+    typedef typename std::conditional<E == 8, uint32_t, uint16_t>::type Codes;
+    mx_each<E, 4>(
+        a.n, a.k,
+        [&](uint32_t vec, uint32_t l) {
+            const uint64_t at = (uint64_t)vec * (mx_pad(a.k) / E) + l;
+            return MxPair{reinterpret_cast<const Codes *>(a.codes)[at], a.scales[at / (32 / E)]};
+        },
+        [&](uint32_t vec, uint32_t l, const MxPair &p) {
+            float v[8], o[E];
+            mx_values(p.codes, p.scale, v);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = mx_value(c >> 4 * e, scale);
-        if (l * 8 < a.k) store_row<T, 8>(reinterpret_cast<T *>(a.values) + (uint64_t)row * a.k, l * 8, a.k, v);
-    }
+            for (int e = 0; e < E; ++e) o[e] = v[e];
+            if (l * E < a.k) store_row<T, E>(reinterpret_cast<T *>(a.values) + (uint64_t)vec * a.k, l * E, a.k, o);
+        });
 }
 
-// Vectors down the columns of a [k x n] matrix: a workgroup takes 64 columns by 128 rows, a wave
-// one block of 32 rows (a row's 64 elements are one load); the codes go through LDS, so that each
-// vector's 64 bytes are written together.
+// Vectors down the columns of a [k x n] matrix: a workgroup takes 64 CV columns by 128 rows, a wave one
+// block of 32 rows, a lane CV columns next to each other (256 bytes of a row to a load); the codes go
+// through LDS, so that each vector's 64 bytes are written together.
+template <typename T> constexpr int kDownCols = 4 / sizeof(T);   // columns of a lane
+
 template <typename T> __global__ void __launch_bounds__(256) mx_quantise_down_kernel(MxCastArgs a) {
-    __shared__ u32x4 codes[64][5];
-    __shared__ uint8_t scales[64][4];
-    const uint32_t kp = mx_pad(a.k), ntiles = (a.n + 63u) / 64u;
+    constexpr int CV = kDownCols<T>, COLS = 64 * CV;
+    typedef typename Unaligned<T, CV>::type Vec;
+    __shared__ u32x4 codes[COLS][5];
+    __shared__ uint8_t scales[COLS][4];
+    const uint32_t kp = mx_pad(a.k), ntiles = (a.n + COLS - 1) / COLS;
     const uint32_t ntile = blockIdx.x % ntiles, ktile = blockIdx.x / ntiles;
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
-    const uint32_t k0 = ktile * 128u + wave * 32u, col = ntile * 64u + lane;
-    float v[32];
-    uint32_t big = 0;
+    const uint32_t k0 = ktile * 128u + wave * 32u, n0 = ntile * COLS, col = n0 + lane * CV;
+    Vec v[32];
 #pragma unroll
     for (int e = 0; e < 32; ++e) {
-        v[e] = col < a.n && k0 + e < a.k ? (float)reinterpret_cast<const T *>(a.values)[(uint64_t)(k0 + e) * a.n + col] : 0.0f;
-        big = max(big, magnitude(v[e]));
-    }
-    const uint32_t scale = mx_scale(big);
-    u32x4 c;
+        const T *p = reinterpret_cast<const T *>(a.values) + (uint64_t)(k0 + e) * a.n;
+        v[e] = Vec{};
+        if (k0 + e < a.k) {
+            if (col + CV <= a.n)
+                v[e] = *reinterpret_cast<const Vec *>(p + col);
+            else
 #pragma unroll
-    for (int e = 0; e < 4; ++e) c[e] = mx_codes(*reinterpret_cast<const float (*)[8]>(&v[8 * e]), scale);
-    codes[lane][wave] = c;
-    scales[lane][wave] = (uint8_t)scale;
+                for (int c = 0; c < CV; ++c)
+                    if (col + c < a.n) v[e][c] = p[col + c];
+        }
+    }
+#pragma unroll
+    for (int c = 0; c < CV; ++c) {
+        uint32_t big = 0;
+#pragma unroll
+        for (int e = 0; e < 32; ++e) big = max(big, magnitude((float)v[e][c]));
+        const uint32_t scale = mx_scale(big);
+        u32x4 o;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            float f[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f[e] = (float)v[8 * q + e][c];
+            o[q] = mx_codes(f, scale);
+        }
+        codes[lane * CV + c][wave] = o;
+        scales[lane * CV + c][wave] = (uint8_t)scale;
+    }
     __syncthreads();
-    const uint32_t vec = threadIdx.x >> 2, part = threadIdx.x & 3u, to = ntile * 64u + vec;
-    if (to < a.n)
-        reinterpret_cast<u32x4 *>(a.codes + (uint64_t)to * (kp / 2) + ktile * 64u)[part] = codes[vec][part];
-    if (threadIdx.x < 64 && col < a.n)
-        *reinterpret_cast<uint32_t *>(a.scales + (uint64_t)col * (kp / 32) + ktile * 4u) =
-            *reinterpret_cast<const uint32_t *>(scales[lane]);
+    for (uint32_t i = threadIdx.x; i < COLS * 4; i += 256) {
+        const uint32_t vec = i >> 2, part = i & 3u;
+        if (n0 + vec < a.n)
+            reinterpret_cast<u32x4 *>(a.codes + (uint64_t)(n0 + vec) * (kp / 2) + ktile * 64u)[part] = codes[vec][part];
+    }
+    for (uint32_t vec = threadIdx.x; vec < COLS; vec += 256)
+        if (n0 + vec < a.n)
+            *reinterpret_cast<uint32_t *>(a.scales + (uint64_t)(n0 + vec) * (kp / 32) + ktile * 4u) =
+                *reinterpret_cast<const uint32_t *>(scales[vec]);
 }
 
 template <typename T> __global__ void __launch_bounds__(256) mx_dequantise_down_kernel(MxCastArgs a) {
-    __shared__ u32x4 codes[64][5];
-    const uint32_t kp = mx_pad(a.k), ntiles = (a.n + 63u) / 64u;
+    constexpr int CV = kDownCols<T>, COLS = 64 * CV;
+    __shared__ u32x4 codes[COLS][5];
+    const uint32_t kp = mx_pad(a.k), ntiles = (a.n + COLS - 1) / COLS;
     const uint32_t ntile = blockIdx.x % ntiles, ktile = blockIdx.x / ntiles;
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
-    const uint32_t vec = threadIdx.x >> 2, part = threadIdx.x & 3u, from = ntile * 64u + vec;
-    if (from < a.n)
-        codes[vec][part] = reinterpret_cast<const u32x4 *>(a.codes + (uint64_t)from * (kp / 2) + ktile * 64u)[part];
-    __syncthreads();
-    const uint32_t k0 = ktile * 128u + wave * 32u, col = ntile * 64u + lane;
-    if (col >= a.n) return;
-    const uint32_t scale = a.scales[(uint64_t)col * (kp / 32) + k0 / 32u];
-    const u32x4 c = codes[lane][wave];
+    const uint32_t k0 = ktile * 128u + wave * 32u, n0 = ntile * COLS, col = n0 + lane * CV;
+    for (uint32_t i = threadIdx.x; i < COLS * 4; i += 256) {
+        const uint32_t vec = i >> 2, part = i & 3u;
+        if (n0 + vec < a.n)
+            codes[vec][part] = reinterpret_cast<const u32x4 *>(a.codes + (uint64_t)(n0 + vec) * (kp / 2) + ktile * 64u)[part];
+    }
+    uint32_t scale[CV];
 #pragma unroll
-    for (int e = 0; e < 32; ++e)
-        if (k0 + e < a.k)
-            reinterpret_cast<T *>(a.values)[(uint64_t)(k0 + e) * a.n + col] = (T)mx_value(c[e / 8] >> 4 * (e % 8), scale);
+    for (int c = 0; c < CV; ++c) scale[c] = a.scales[(uint64_t)min(col + c, a.n - 1) * (kp / 32) + k0 / 32u];
+    __syncthreads();
+    if (col >= a.n) return;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        float f[CV][8];
+#pragma unroll
+        for (int c = 0; c < CV; ++c) mx_values(codes[lane * CV + c][wave][q], scale[c], f[c]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const uint32_t k = k0 + 8 * q + e;
+            float o[CV];
+#pragma unroll
+            for (int c = 0; c < CV; ++c) o[c] = f[c][e];
+            if (k < a.k) store_row<T, CV>(reinterpret_cast<T *>(a.values) + (uint64_t)k * a.n, col, a.n, o);
+        }
+    }
 }
 
 // A lane's block of 32 elements of x, from element i of a row of k, as the product's operand.
@@ -359,37 +463,31 @@ template <typename T> hipError_t mx_forward_t(const MxForwardArgs &a, hipStream_
     return hipGetLastError();
 }
 
-dim3 flat_grid(uint64_t items) { return dim3((uint32_t)(items / 256 + 1 < 8192 ? items / 256 + 1 : 8192)); }
-dim3 down_grid(const MxCastArgs &a) { return dim3((a.n + 63) / 64 * (mx_pad(a.k) / 128)); }
+template <typename T> hipError_t mx_cast(const MxCastArgs &a, bool down, bool back, hipStream_t s) {
+    if (a.n == 0 || a.k == 0) return hipSuccess;
+    if (down) {
+        constexpr uint32_t cols = 64 * kDownCols<T>;
+        const dim3 grid((a.n + cols - 1) / cols * (mx_pad(a.k) / 128));
+        hipLaunchKernelGGL((back ? mx_dequantise_down_kernel<T> : mx_quantise_down_kernel<T>), grid, dim3(256), 0, s, a);
+    } else {
+        const uint64_t waves = back ? mx_rows<kValues<T>>(a.n, a.k).waves : mx_rows<8>(a.n, a.k).waves;
+        // workgroups that loop: 8192 x 4096 fp16 to codes 17.4 us on 2048, 20.2 on one per piece; its
+        // values to fp32 34.0 us on 4096, 41.6
+        const uint64_t groups = (waves + 3) / 4, most = back ? 4096 : 2048;
+        const dim3 grid((uint32_t)(groups < most ? groups : most));
+        hipLaunchKernelGGL((back ? mx_dequantise_kernel<T> : mx_quantise_kernel<T>), grid, dim3(256), 0, s, a);
+    }
+    return hipGetLastError();
+}
 
 }  // namespace
 
 hipError_t launch_mx_quantise(const MxCastArgs &a, uint32_t dtype, bool down, hipStream_t s) {
-    if (a.n == 0 || a.k == 0) return hipSuccess;
-    const uint64_t items = (uint64_t)a.n * (mx_pad(a.k) / 8);
-    if (down && dtype)
-        hipLaunchKernelGGL(mx_quantise_down_kernel<half_t>, down_grid(a), dim3(256), 0, s, a);
-    else if (down)
-        hipLaunchKernelGGL(mx_quantise_down_kernel<float>, down_grid(a), dim3(256), 0, s, a);
-    else if (dtype)
-        hipLaunchKernelGGL(mx_quantise_kernel<half_t>, flat_grid(items), dim3(256), 0, s, a);
-    else
-        hipLaunchKernelGGL(mx_quantise_kernel<float>, flat_grid(items), dim3(256), 0, s, a);
-    return hipGetLastError();
+    return dtype ? mx_cast<half_t>(a, down, false, s) : mx_cast<float>(a, down, false, s);
 }
 
 hipError_t launch_mx_dequantise(const MxCastArgs &a, uint32_t dtype, bool down, hipStream_t s) {
-    if (a.n == 0 || a.k == 0) return hipSuccess;
-    const uint64_t items = (uint64_t)a.n * (mx_pad(a.k) / 8);
-    if (down && dtype)
-        hipLaunchKernelGGL(mx_dequantise_down_kernel<half_t>, down_grid(a), dim3(256), 0, s, a);
-    else if (down)
-        hipLaunchKernelGGL(mx_dequantise_down_kernel<float>, down_grid(a), dim3(256), 0, s, a);
-    else if (dtype)
-        hipLaunchKernelGGL(mx_dequantise_kernel<half_t>, flat_grid(items), dim3(256), 0, s, a);
-    else
-        hipLaunchKernelGGL(mx_dequantise_kernel<float>, flat_grid(items), dim3(256), 0, s, a);
-    return hipGetLastError();
+    return dtype ? mx_cast<half_t>(a, down, true, s) : mx_cast<float>(a, down, true, s);
 }
 
 hipError_t launch_mx_forward(const MxForwardArgs &a, uint32_t dtype, hipStream_t s) {

@@ -65,20 +65,17 @@ def distill_error(ctx: abi.Context, logits: torch.Tensor, index: torch.Tensor, v
     (fp16 or fp32), the teacher's classes (int32) and logits (fp32) [rows x top], labels int32
     [rows] where alpha < 1; writes grad and d_prenorm (fp32), d_prenorm_h (fp16; fp16 logits only)
     and loss [rows] where given."""
-    rows, classes = logits.shape
-    half = logits.dtype is torch.float16
-    d = abi.SklDenseDesc()
-    d.dtype, d.inputs, d.outputs, d.max_batch, d.is_training = abi.F16 if half else abi.F32, 1, classes, rows, 1
-    dev, shape = ctx.device, (rows, classes)
-    d.out = abi.need("logits", logits, torch.float16 if half else torch.float32, shape, dev)
-    d.grad = abi.need("grad", grad, torch.float32, shape, dev)
-    d.d_prenorm = abi.need("d_prenorm", d_prenorm, torch.float32, shape, dev)
-    if half:
-        if d_prenorm_h is None:
-            raise ValueError("d_prenorm_h: fp16 logits need one")
-        d.d_prenorm_h = abi.need("d_prenorm_h", d_prenorm_h, torch.float16, shape, dev)
+    shape = rows, classes = logits.shape
+    dev, half = ctx.device, logits.dtype is torch.float16
+    if half and d_prenorm_h is None:
+        raise ValueError("d_prenorm_h: fp16 logits need one")
     if index.shape[0] != rows:
         raise ValueError(f"index: {index.shape[0]} rows, logits have {rows}")
+    d = abi.SklDenseDesc(abi.F16 if half else abi.F32, 1, classes, rows, is_training=1,
+                         out=abi.need("logits", logits, torch.float16 if half else torch.float32, shape, dev),
+                         grad=abi.need("grad", grad, torch.float32, shape, dev),
+                         d_prenorm=abi.need("d_prenorm", d_prenorm, torch.float32, shape, dev),
+                         d_prenorm_h=abi.need("d_prenorm_h", d_prenorm_h, torch.float16, shape, dev) if half else None)
     _distill(ctx, C.byref(d), index, value, label, temperature, alpha, loss)
 
 

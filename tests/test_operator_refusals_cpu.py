@@ -142,7 +142,7 @@ def cast_status(back=False, **change):
 @pytest.mark.parametrize("back", [False, True])
 @pytest.mark.parametrize("code,change", [
     (NULL, dict(ctx=None)), (INVALID, dict(dtype=2)), (INVALID, dict(down=2)), (INVALID, dict(cols=0x7fffff81)),
-    (INVALID, dict(down=1, rows=0x7fffff81)), (0, dict(rows=0)), (0, dict(cols=0)), (NULL, dict(src=None)), (NULL, dict(codes=None)),
+    (INVALID, dict(down=1, rows=0x7fffff81)), (INVALID, dict(rows=1 << 31, cols=1 << 16)), (0, dict(rows=0)), (0, dict(cols=0)), (NULL, dict(src=None)), (NULL, dict(codes=None)),
     (NULL, dict(scales=None)), (HARDWARE, dict(codes=(1 << 50) + 8)), (HARDWARE, dict(scales=(1 << 50) + 2)),
     (INVALID, dict(src=1 << 50, codes=(1 << 50) + 1008)), (INVALID, dict(codes=1 << 50, scales=(1 << 50) + 4)),
 ])
@@ -198,7 +198,9 @@ class NoContext:
 def test_wrappers_refuse_tensors_that_the_calls_do_not_take():
     """Wrong types, shapes, strides and devices (these are on the CPU) never reach an address."""
     ctx, f, h = NoContext(), torch.zeros(4, 8), torch.zeros(4, 8, dtype=torch.float16)
-    join = Join(ctx, 8, post_w=f[:1], pre_w=f[:1])
+    with pytest.raises(ValueError, match="pre_w"):
+        Join(ctx, 8, pre_w=f[:1])
+    join = Join(ctx, 8)
     for x, y in ((f, None), (h, None), (f[:, :4], None), (None, f), (torch.zeros(8, 4).t(), None), (None, None)):
         with pytest.raises(ValueError):
             join.forward(x, y, n=torch.zeros(4, 8))
