@@ -276,8 +276,8 @@ size_t skl_residual_work_bytes(uint32_t rows, uint32_t cols);
  * logits per row (int32 top_index, fp32 top_logit, [rows x top], top <= 1024); a slot
  * whose class is not in [0, outputs) is empty, classes may repeat (their shares add
  * up).  label (int32 [rows]; a value outside [0, outputs): no label), needed where
- * alpha < 1.  With t = temperature, q = softmax(top_logit / t) over the held slots,
- * p = softmax(z / t), p1 = softmax(z):
+ * alpha < 1.  With t = temperature (2^-60 to 2^60), q = softmax(top_logit / t) over
+ * the held slots, p = softmax(z / t), p1 = softmax(z):
  *   loss = alpha t^2 sum q log(q / p) - (1 - alpha) log p1[label]
  *   d loss / d z = alpha t (p - q) + (1 - alpha) (p1 - [label])
  * The gradient times LOSS_SCALE goes to grad and d_prenorm (and d_prenorm_h), as
@@ -308,10 +308,11 @@ int32_t skl_mxfp4_dequantise(skl_ctx *ctx, const void *codes, const void *scales
 /* skl_dense_forward of a block that is only used, with 4-bit weights: w_codes and
  * w_scales are its W [inputs x outputs] quantised down, the input is quantised along
  * its rows on the way, Z = Q(in) . Q(W) (+b) is summed in fp32, then norm and
- * activation (no dropout).  blk->w may be NULL.  Without a norm only out is written.
- * in may not overlap what is written.  work: skl_mxfp4_work_bytes(inputs, outputs,
- * batch) bytes of the caller's, 16-byte aligned; what it holds does not outlive the call, and calls
- * that overlap in time need a work of their own (as they need an out of their own). */
+ * activation (no dropout).  blk->w may be NULL.  inputs <= 2^24.  Without a norm only
+ * out is written.  in may not overlap what is written.  work: skl_mxfp4_work_bytes(
+ * inputs, outputs, batch) bytes of the caller's, 16-byte aligned; what it holds does
+ * not outlive the call, and calls that overlap in time need a work of their own (as
+ * they need an out of their own). */
 int32_t skl_dense_forward_mxfp4(skl_ctx *ctx, const skl_dense_desc *blk, const void *in, uint32_t in_rows,
                                 uint32_t in_cols, uint32_t batch, const void *w_codes, const void *w_scales,
                                 void *work, size_t work_bytes);

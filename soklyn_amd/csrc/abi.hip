@@ -1870,7 +1870,8 @@ int32_t skl_dense_distill_error(skl_ctx *ctx, const skl_dense_desc *b, const voi
     SKL_CHECK(rows > 0, SKL_ERR_INVALID_BATCH_SIZE);
     SKL_CHECK(rows <= b->max_batch, SKL_ERR_ALLOCATION_LIMIT);
     SKL_CHECK(b->outputs <= 0x7fffffffu && top <= kDistillTop, SKL_ERR_INVALID_CONFIGURATION);
-    SKL_CHECK(std::isfinite(temperature) && temperature > 0.0f, SKL_ERR_INVALID_CONFIGURATION);
+    // (NaN too; the loss has its square)
+    SKL_CHECK(temperature >= 0x1p-60f && temperature <= 0x1p60f, SKL_ERR_INVALID_CONFIGURATION);
     SKL_CHECK(alpha >= 0.0f && alpha <= 1.0f, SKL_ERR_INVALID_CONFIGURATION);
     SKL_CHECK(!top || (top_index && top_logit), SKL_ERR_NULL_POINTER);
     SKL_CHECK(alpha == 1.0f || label, SKL_ERR_NULL_POINTER);
@@ -1952,7 +1953,7 @@ int32_t skl_dense_forward_mxfp4(skl_ctx *ctx, const skl_dense_desc *b, const voi
                                 void *work, size_t work_bytes) {
     SKL_CHECK(ctx && b, SKL_ERR_NULL_POINTER);
     SKL_CHECK(b->dtype <= SKL_F16 && b->inputs > 0 && b->outputs > 0 && b->max_batch > 0 &&
-                  b->norm <= SKL_NORM_BATCH && b->act <= SKL_ACT_MISH && b->inputs <= 0x7fffff80u,
+                  b->norm <= SKL_NORM_BATCH && b->act <= SKL_ACT_MISH && b->inputs <= kMxInputs,
               SKL_ERR_INVALID_CONFIGURATION);
     int32_t r;
     if ((r = check_input(b, in, in_rows, in_cols, batch))) return r;

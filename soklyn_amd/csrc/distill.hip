@@ -57,8 +57,9 @@ __host__ __device__ constexpr uint32_t distill_words(int NT, int E, bool table) 
 // vector are found by its whole wave, a slot to a lane.  2048 rows of 50257 classes with 64 slots:
 // 588 us when each lane looked through the slots by itself, 286 us so.
 //
-// A softmax's exponent is fma(z, k, c), c = -max k rounded once: c's rounding is the same in every
-// term and leaves the quotient alone.
+// A softmax's exponent is (z - max) k and not fma(z, k, -max k): the rounding of max k is the same in
+// every term, but past 2^31 (large logits, a small temperature) takes the largest term itself out of
+// range.
 template <typename T, int NT, int E, bool TABLE, bool MORE>
 __global__ void __launch_bounds__(NT < 256 ? 256 : NT) distill_kernel(DistillArgs a) {
     constexpr int W = NT / 64, C = E / V, RPG = NT < 256 ? 256 / NT : 1, LANES = NT < 64 ? NT : 64;
@@ -151,17 +152,17 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT) distill_kernel(DistillArg
 #pragma unroll 1
         for (uint32_t j = lane; j < top; j += LANES) t_max = fmaxf(t_max, value[j]);
         t_max = lanes_max<LANES>(t_max);
-        const float t_c = t_max == -INFINITY ? 0.0f : -t_max * k_soft;
+        t_max = t_max == -INFINITY ? 0.0f : t_max;
 #pragma unroll 1
         for (uint32_t j = lane; j < top; j += LANES)
-            t_sum += at[j] >= 0 ? __builtin_amdgcn_exp2f(fmaf(value[j], k_soft, t_c)) : 0.0f;
+            t_sum += at[j] >= 0 ? __builtin_amdgcn_exp2f((value[j] - t_max) * k_soft) : 0.0f;
         t_sum = lanes_sum<LANES>(t_sum);
         const bool taught = a.alpha > 0.0f && t_sum != 0.0f;   // NaN: taught, and NaN
         bool twice = false;
 #pragma unroll 1
         for (uint32_t j = tid; j < top; j += NT) {
             const uint32_t b = ((uint32_t)at[j] + (TABLE ? 0 : lo)) >> group, bit = 1u << (b & 31u);
-            q[j] = taught && at[j] >= 0 ? __builtin_amdgcn_exp2f(fmaf(value[j], k_soft, t_c)) / t_sum : 0.0f;
+            q[j] = taught && at[j] >= 0 ? __builtin_amdgcn_exp2f((value[j] - t_max) * k_soft) / t_sum : 0.0f;
             if (at[j] >= 0) twice = (atomicOr(&marks[b >> 5], bit) & bit) || twice;
         }
         if constexpr (!TABLE) {
@@ -201,17 +202,16 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT) distill_kernel(DistillArg
             }
         }
         const float base = m == -INFINITY ? 0.0f : m;
-        const float c_soft = -base * k_soft, c_hard = -base * kLog2e;
         float s_soft = 0.0f, s_hard = 0.0f;
         if (taught)
             each([&](uint32_t, const float (&v)[V], auto) {
 #pragma unroll
-                for (int e = 0; e < V; ++e) s_soft += __builtin_amdgcn_exp2f(fmaf(v[e], k_soft, c_soft));
+                for (int e = 0; e < V; ++e) s_soft += __builtin_amdgcn_exp2f((v[e] - base) * k_soft);
             });
         if (labelled)
             each([&](uint32_t, const float (&v)[V], auto) {
 #pragma unroll
-                for (int e = 0; e < V; ++e) s_hard += __builtin_amdgcn_exp2f(fmaf(v[e], kLog2e, c_hard));
+                for (int e = 0; e < V; ++e) s_hard += __builtin_amdgcn_exp2f((v[e] - base) * kLog2e);
             });
         s_soft = lanes_sum<LANES>(s_soft);
         s_hard = lanes_sum<LANES>(s_hard);
@@ -243,10 +243,10 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT) distill_kernel(DistillArg
             const bool mine = decltype(whole)::value ? p >= v0 * V && p < v1 * V : edged;
             float g[V];
 #pragma unroll
-            for (int e = 0; e < V; ++e) g[e] = soft ? w_soft * __builtin_amdgcn_exp2f(fmaf(v[e], k_soft, c_soft)) : 0.0f;
+            for (int e = 0; e < V; ++e) g[e] = soft ? w_soft * __builtin_amdgcn_exp2f((v[e] - base) * k_soft) : 0.0f;
             if (hard)
 #pragma unroll
-                for (int e = 0; e < V; ++e) g[e] += w_hard * __builtin_amdgcn_exp2f(fmaf(v[e], kLog2e, c_hard));
+                for (int e = 0; e < V; ++e) g[e] += w_hard * __builtin_amdgcn_exp2f((v[e] - base) * kLog2e);
             if constexpr (TABLE) {
                 if (!mine) return;
                 const f32x4 share = *reinterpret_cast<const f32x4 *>(table + p);
@@ -301,15 +301,15 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT) distill_kernel(DistillArg
         });
 
         if (a.loss && tid < 64) {
+            // in units of the logits, not of the exponents: these may pass fp32 where the loss does not
             float l = 0.0f;
-            const float log_p = __builtin_amdgcn_logf(s_soft), log_q = __builtin_amdgcn_logf(t_sum);
+            const float logs = a.tau * kLn2 * (__builtin_amdgcn_logf(s_soft) - __builtin_amdgcn_logf(t_sum));
             if (soft)
 #pragma unroll 1
                 for (uint32_t j = lane; j < top; j += LANES)
-                    if (q[j] != 0.0f)
-                        l += q[j] * ((fmaf(value[j], k_soft, t_c) - log_q) - (fmaf(z_at[j], k_soft, c_soft) - log_p));
-            l = lanes_sum<LANES>(l) * (a.alpha * a.tau * a.tau * kLn2);
-            if (hard) l -= (1.0f - a.alpha) * kLn2 * (fmaf(z_y, kLog2e, c_hard) - __builtin_amdgcn_logf(s_hard));
+                    if (q[j] != 0.0f) l += q[j] * (((value[j] - t_max) - (z_at[j] - base)) + logs);
+            l = lanes_sum<LANES>(l) * (a.alpha * a.tau);
+            if (hard) l -= (1.0f - a.alpha) * ((z_y - base) - kLn2 * __builtin_amdgcn_logf(s_hard));
             if (lane == 0) a.loss[row] = l;
         }
         row_sync<NT>();   // the next row's slots

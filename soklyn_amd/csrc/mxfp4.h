@@ -23,6 +23,8 @@ struct MxCastArgs {
 hipError_t launch_mx_quantise(const MxCastArgs &a, uint32_t dtype, bool down, hipStream_t s);
 hipError_t launch_mx_dequantise(const MxCastArgs &a, uint32_t dtype, bool down, hipStream_t s);
 
+constexpr uint32_t kMxInputs = 1u << 24;   // a tile's codes, 256 vectors, are within 2^32 bytes
+
 struct MxForwardArgs {
     uint32_t m, n, k;
     const void *x;                      // T [m x k]

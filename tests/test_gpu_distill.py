@@ -112,7 +112,7 @@ def check(ctx, z, index, value, label, tau, alpha, offset=0):
     rg, tg, rl, tl = reference(z, index, value, label if label is not None else torch.full((z.shape[0],), -1), tau, alpha)
     d = (g - rg).abs()
     assert (d <= tg).all(), f"gradient: {(d / tg).max().item():.3g} of its tolerance"
-    same = rl == l   # infinities
+    same = rl.float() == l.float()   # infinities: fp32's, where the loss is past its largest (3.4e38)
     e = (l - rl).abs()
     assert (same | (e <= tl)).all(), f"loss: {torch.where(same, 0, e / tl).max().item():.3g} of its tolerance"
     return g, l
@@ -220,6 +220,17 @@ def test_gradient_against_differences(ctx):
             w[at] += s
             zs.append(run(ctx, w, index, value, label, 2.0, 0.5)[1].sum())
         assert abs((zs[0] - zs[1]) / (2 * step) - g[at] / 512) < 2e-3
+
+
+@pytest.mark.parametrize("n", [10, 300, 1000, 9000])
+@pytest.mark.parametrize("std,tau", [(1e10, 1.0), (1e30, 2.0), (2.5, 2.0 ** -40), (2.5, 2.0 ** -60), (1e-3, 2.0 ** 60)])
+def test_large_logits_and_extreme_temperatures(ctx, n, std, tau):
+    """Exponents far past 2^31: the largest term is 1 all the same.  Beside a logit of 3e38, alpha tau^2
+    (3e38 / tau) + (1 - alpha) 3e38 is 4.5e38 at tau = 2, so that row's loss rounds to infinity."""
+    z, index, value, label = inputs(5, n, 4, False, 21, std)
+    z[1, n // 2] = z[1, 3] = z[1].max()   # two largest
+    z[2, 0] = 3e38
+    check(ctx, z, index, value, label, tau, 0.5)
 
 
 @pytest.mark.parametrize("half", [True, False])

@@ -119,7 +119,7 @@ def distill_status(d=None, **change):
     (INVALID, dict(max_batch=0), {}), (INVALID, dict(norm=1), {}), (INVALID, dict(act=6), {}), (TRAINING, dict(is_training=0), {}),
     (BATCH, {}, dict(rows=0)), (LIMIT, {}, dict(rows=17)), (INVALID, {}, dict(top=1025)), (INVALID, dict(outputs=1 << 31), {}),
     (INVALID, {}, dict(t=0.0)), (INVALID, {}, dict(t=-1.0)), (INVALID, {}, dict(t=INF)), (INVALID, {}, dict(t=NAN)),
-    (INVALID, {}, dict(alpha=-0.1)), (INVALID, {}, dict(alpha=1.5)), (INVALID, {}, dict(alpha=NAN)), (NULL, {}, dict(index=None)),
+    (INVALID, {}, dict(t=2.0 ** -61)), (INVALID, {}, dict(t=2.0 ** 61)), (INVALID, {}, dict(alpha=-0.1)), (INVALID, {}, dict(alpha=1.5)), (INVALID, {}, dict(alpha=NAN)), (NULL, {}, dict(index=None)),
     (NULL, {}, dict(value=None)), (NULL, {}, dict(label=None)), (NULL, dict(out=None), {}), (NULL, dict(grad=None), {}),
     (NULL, dict(d_prenorm=None), {}), (NULL, dict(d_prenorm_h=None), {}),
     (INVALID, dict(grad=1 << 50, out=1 << 50), {}), (INVALID, dict(grad=1 << 50, d_prenorm=(1 << 50) + 64), {}),
@@ -160,7 +160,8 @@ def serve_status(d=None, **change):
 
 @pytest.mark.parametrize("code,d,change", [
     (NULL, {}, dict(ctx=None)), (NULL, {}, dict(blk=None)), (INVALID, dict(dtype=2), {}), (INVALID, dict(inputs=0), {}),
-    (INVALID, dict(outputs=0), {}), (INVALID, dict(norm=4), {}), (INVALID, dict(act=8), {}), (NULL, {}, dict(x=None)),
+    (INVALID, dict(inputs=(1 << 24) + 1), dict(cols=(1 << 24) + 1)), (INVALID, dict(outputs=0), {}), (INVALID, dict(norm=4), {}),
+    (INVALID, dict(act=8), {}), (NULL, {}, dict(x=None)),
     (DIMS, {}, dict(rows=7)), (LIMIT, {}, dict(rows=17)), (DIMS, {}, dict(cols=65)), (INVALID, dict(act=5), {}),
     (BATCH, {}, dict(batch=0)), (BATCH, dict(norm=3), dict(batch=1)), (NULL, dict(norm=1, prenorm=None), {}),
     (NULL, dict(norm=1, preact=None), {}), (NULL, {}, dict(codes=None)), (NULL, {}, dict(scales=None)), (NULL, dict(out=None), {}),
