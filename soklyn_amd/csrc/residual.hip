@@ -59,9 +59,12 @@ __device__ __forceinline__ void row_stats(const float (&v)[E + 1], const RowMap<
 template <typename T, typename R, int NT, int E>
 __global__ void __launch_bounds__(NT < 256 ? 256 : NT) join_kernel(JoinArgs a) {
     constexpr int RPG = NT < 256 ? 256 / NT : 1;
-    __shared__ float slots[4 * (NT < 64 ? 1 : NT / 64)];
+    constexpr int S = NT < 64 ? 1 : NT / 64;
+    __shared__ float both[2][4 * S];   // in turns: a row may have one sum, and so one barrier
     const RowMap<NT> map{threadIdx.x % NT, a.cols};
-    for (uint32_t row = blockIdx.x * RPG + sub_row<NT>(); row < a.rows; row += gridDim.x * RPG) {
+    uint32_t turn = 0;
+    for (uint32_t row = blockIdx.x * RPG + sub_row<NT>(); row < a.rows; row += gridDim.x * RPG, turn ^= 1u) {
+        float *slots = both[turn];
         const uint64_t at = (uint64_t)row * a.cols;
         float mean = 0.0f, rstd = 1.0f;
         RowPart<R, E> x;
@@ -111,7 +114,7 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT) join_kernel(JoinArgs a) {
         if (a.h) map.template write<R, E>(reinterpret_cast<R *>(a.h) + at, h);
         mean = 0.0f;
         rstd = 1.0f;
-        if (a.n) row_stats<NT, E>(h, map, a.pre, slots + 2 * (NT / 64), mean, rstd);
+        if (a.n) row_stats<NT, E>(h, map, a.pre, slots + 2 * S, mean, rstd);
         if (a.stats && map.tid == 0) {
             a.stats[2 * (uint64_t)a.rows + row] = mean;
             a.stats[3 * (uint64_t)a.rows + row] = rstd;

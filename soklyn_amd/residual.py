@@ -18,7 +18,7 @@ _NONE, _RMS, _LAYER = abi.NORM_DISABLED, abi.NORM_RMS, abi.NORM_LAYER
 class Join:
     """One join: its norms' parameters (tensors [1 x cols] of the blocks' type, held by reference and
     read at each call, so an update in place is seen), gate activation and residual scale.  Calls of
-    one Join share its workspace and follow each other on one stream."""
+    one Join that are given no workspace share its own and follow each other on one stream."""
 
     def __init__(self, ctx: abi.Context, cols: int, *, half: bool = False, half_stream: bool = False,
                  post_norm: int = _NONE, pre_norm: int = _RMS, gate_act: int = abi.ACT_IDENTITY, scale: float = 1.0,
@@ -31,7 +31,7 @@ class Join:
         self.stream_dtype = torch.float16 if half_stream else torch.float32
         self.post_w, self.post_b, self.pre_w, self.pre_b = post_w, post_b, pre_w, pre_b
         self._call = abi.load().skl_residual_forward, abi.load().skl_residual_backward
-        self._work = None
+        self._work = []
         for name, t in zip(("post_w", "post_b", "pre_w", "pre_b"), (post_w, post_b, pre_w, pre_b)):
             if t is not None:
                 abi.need(name, t, self.dtype, (1, cols), ctx.device)
@@ -93,11 +93,10 @@ class Join:
         if dparam is not None or (dgate is not None and gates == 1):
             size = abi.load().skl_residual_work_bytes(rows, cols)
             if work is None:
-                if self._work is None or self._work.numel() * 4 < size:
-                    if self._work is not None:
-                        self.ctx.synchronize()   # a call may still write the smaller one
-                    self._work = torch.empty(size // 4, device=f"cuda:{self.ctx.device}", dtype=f32)
-                work = self._work
+                if not self._work or self._work[-1].numel() * 4 < size:
+                    # (smaller ones stay: calls in flight and captured ones write there)
+                    self._work.append(torch.empty(size // 4, device=f"cuda:{self.ctx.device}", dtype=f32))
+                work = self._work[-1]
             size = work.numel() * 4
         ph, py, pg, ps, pdn, pdh, pdx, pdy, pdg, pdp, pw = self._addresses((
             ("h", h, self.stream_dtype, wide), ("y", y, self.dtype, wide), ("gate", gate, self.dtype, (gates, cols)),

@@ -289,6 +289,21 @@ def test_many_rows(ctx):
         assert torch.equal(first[k], second[k]), k
 
 
+def test_more_rows_than_workgroups(ctx):
+    """Workgroups that go on to another row, with one sum (and one barrier) in each row."""
+    rows, cols = (1 << 20) + 9, 1030
+    g = torch.Generator(device="cuda").manual_seed(3)
+    few = torch.randn(8, cols, generator=g, device="cuda").half()
+    join = Join(ctx, cols, half=True, half_stream=True, pre_norm=RMS, pre_w=torch.ones(1, cols, device="cuda").half())
+    want, got = torch.empty_like(few), torch.empty(rows, cols, dtype=torch.float16, device="cuda")
+    y = few.repeat(-(-rows // 8), 1)[:rows].contiguous()
+    join.forward(None, few, n=want)
+    join.forward(None, y, n=got)
+    torch.cuda.synchronize()
+    whole = rows // 8 * 8
+    assert (got[:whole].view(-1, 8, cols) == want).all() and torch.equal(got[whole:], want[:rows - whole])
+
+
 def test_against_differences(ctx):
     """dx, dy, dgate and dparam against central differences of the fp32 forward: step 2^-6, whose
     third-order term and fp32 rounding (64 u |f| / step) stay under 1e-3 of the gradients' scale."""
@@ -355,6 +370,39 @@ def test_captured_and_replayed(ctx):
             assert torch.equal(eh, h) and torch.equal(en, n) and torch.equal(es, stats)
             for k in out:
                 assert torch.equal(want[k], out[k]), k
+    finally:
+        torch.cuda.synchronize()
+        cap.close()
+
+
+def test_a_captured_joins_own_workspace_outlives_larger_batches(ctx):
+    """A Join whose own workspace grows behind a capture leaves the captured call's alone."""
+    c = Case(ctx, 16, 512, True, True, RMS, RMS, 0, IDENTITY, 1.0)
+    side = torch.cuda.Stream()
+    cap = abi.Context(0, 16, stream=side.cuda_stream)
+    try:
+        j = Join(cap, 512, half=True, half_stream=True, post_norm=RMS, pre_norm=RMS, **c.p)
+        h, n, stats, dparam = torch.empty_like(c.x), torch.empty_like(c.y), torch.empty(4, 16, device="cuda"), torch.empty(4, 512, device="cuda")
+        torch.cuda.synchronize()
+        j.forward(c.x, c.y, h=h, n=n, stats=stats)
+        j.backward(h, c.y, None, stats, c.dn, c.dh, dparam=dparam)
+        torch.cuda.synchronize()
+        want, work = dparam.clone(), j._work[-1]
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side, capture_error_mode="thread_local"):
+            j.backward(h, c.y, None, stats, c.dn, c.dh, dparam=dparam)
+        big = Case(ctx, 600, 512, True, True, RMS, RMS, 0, IDENTITY, 1.0)
+        bh, bn, bs = torch.empty_like(big.x), torch.empty_like(big.y), torch.empty(4, 600, device="cuda")
+        torch.cuda.synchronize()
+        j.forward(big.x, big.y, h=bh, n=bn, stats=bs)
+        j.backward(bh, big.y, None, bs, big.dn, big.dh, dparam=torch.empty(4, 512, device="cuda"))
+        assert j._work[-1] is not work and j._work[0] is work
+        for _ in range(3):
+            dparam.fill_(float("nan"))
+            torch.cuda.synchronize()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(dparam, want)
     finally:
         torch.cuda.synchronize()
         cap.close()
