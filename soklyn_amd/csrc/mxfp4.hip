@@ -32,6 +32,15 @@ __device__ __forceinline__ uint32_t mx_codes(const float (&v)[8], uint32_t scale
 
 __device__ __forceinline__ uint32_t magnitude(float v) { return __builtin_bit_cast(uint32_t, v) & 0x7fffffffu; }
 
+// The largest magnitude of the block whose eight elements each of four neighbouring lanes has.
+__device__ __forceinline__ uint32_t mx_top4(const float (&v)[8]) {
+    uint32_t big = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) big = max(big, magnitude(v[e]));
+    big = max(big, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)big, 0xB1, 0xf, 0xf, true));          // quad_perm 1 0 3 2
+    return max(big, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)big, 0x4E, 0xf, 0xf, true));   // quad_perm 2 3 0 1
+}
+
 // Eight codes, the first in the lowest half byte, as the values they stand for: the convert's are
 // exact, and so is their product with any scale.
 __device__ __forceinline__ void mx_values(uint32_t codes, uint32_t scale, float (&v)[8]) {
@@ -90,25 +99,19 @@ __device__ __forceinline__ void mx_each(uint32_t n, uint32_t k, Load load, Use u
     }
 }
 
-template <typename T, int E> struct MxPiece {
-    float v[E];
+template <typename T> struct MxPiece {
+    float v[8];
 };
 template <typename T> __global__ void __launch_bounds__(256) mx_quantise_kernel(MxCastArgs a) {
     mx_each<8, 2>(
         a.n, a.k,
         [&](uint32_t vec, uint32_t l) {
-            MxPiece<T, 8> p;
+            MxPiece<T> p;
             load_row<T, 8>(reinterpret_cast<const T *>(a.values) + (uint64_t)vec * a.k, l * 8, a.k, p.v);
             return p;
         },
-        [&](uint32_t vec, uint32_t l, const MxPiece<T, 8> &p) {
-            uint32_t big = 0;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) big = max(big, magnitude(p.v[e]));
-            // a block's four lanes are here together
-            big = max(big, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)big, 0xB1, 0xf, 0xf, true));   // quad_perm 1 0 3 2
-            big = max(big, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)big, 0x4E, 0xf, 0xf, true));   // quad_perm 2 3 0 1
-            const uint32_t scale = mx_scale(big);
+        [&](uint32_t vec, uint32_t l, const MxPiece<T> &p) {
+            const uint32_t scale = mx_scale(mx_top4(p.v));   // a block's four lanes are here together
             const uint64_t at = (uint64_t)vec * (mx_pad(a.k) / 8) + l;
             reinterpret_cast<uint32_t *>(a.codes)[at] = mx_codes(p.v, scale);
             if ((l & 3u) == 0) a.scales[at / 4] = (uint8_t)scale;
@@ -226,21 +229,6 @@ template <typename T> __global__ void __launch_bounds__(256) mx_dequantise_down_
             if (k < a.k) store_row<T, CV>(reinterpret_cast<T *>(a.values) + (uint64_t)k * a.n, col, a.n, o);
         }
     }
-}
-
-// A lane's block of 32 elements of x, from element i of a row of k, as the product's operand.
-template <typename T>
-__device__ __forceinline__ u32x4 mx_block(const T *row, uint32_t i, uint32_t k, uint32_t &scale) {
-    float v[4][8];
-    uint32_t big = 0;
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
-        load_row<T, 8>(row, i + 8 * c, k, v[c]);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) big = max(big, magnitude(v[c][e]));
-    }
-    scale = mx_scale(big);
-    return u32x4{mx_codes(v[0], scale), mx_codes(v[1], scale), mx_codes(v[2], scale), mx_codes(v[3], scale)};
 }
 
 __device__ __forceinline__ void mx_mma_plain(f32x4 &acc, const u32x4 &w, uint32_t ws, const u32x4 &x, uint32_t xs) {
@@ -384,8 +372,10 @@ template <typename T> __global__ void __launch_bounds__(512) mx_split_kernel(MxF
 }
 
 // What the tiled product reads: x [m x k] as codes [mp x k2 / 2], and both operands' scales in its
-// order (mx_gemm.h).  A workgroup takes 64 vectors by 128 elements, a thread one block; the first
-// `xtiles` workgroups x, the others w's scales.  Vectors and elements past the matrix are 0.
+// order (mx_gemm.h).  The first `xtiles` workgroups take 64 vectors of x by 128 elements, 8 elements
+// of four vectors (16 apart: a word of scales) to a thread, so that a wave reads 256 bytes of a row
+// together; the others 64 vectors of w's scales by 512 elements.  Vectors and elements past the
+// matrix are 0.
 struct MxStageArgs {
     uint32_t m, n, k, kp, k2, xtiles;
     const void *x;
@@ -393,24 +383,64 @@ struct MxStageArgs {
     uint8_t *codes, *xs, *ws;
 };
 template <typename T> __global__ void __launch_bounds__(256) mx_stage_kernel(MxStageArgs a) {
-    __shared__ uint32_t words[4][16];
-    const uint32_t ktiles = a.k2 / 128u, vec = threadIdx.x >> 2, block = threadIdx.x & 3u;
-    const bool is_w = blockIdx.x >= a.xtiles;
-    const uint32_t tile = is_w ? blockIdx.x - a.xtiles : blockIdx.x, group = tile / ktiles, kt = tile % ktiles;
-    const uint32_t v = group * 64u + vec, kb = kt * 4u + block;
-    uint32_t scale = 0;
-    if (is_w) {
-        if (v < a.n && kb < a.kp / 32u) scale = a.w_scales[(uint64_t)v * (a.kp / 32u) + kb];
-    } else {
-        u32x4 c = {0, 0, 0, 0};
-        if (v < a.m) c = mx_block(reinterpret_cast<const T *>(a.x) + (uint64_t)v * a.k, kb * 32u, a.k, scale);
-        *reinterpret_cast<u32x4 *>(a.codes + (uint64_t)v * (a.k2 / 2u) + kb * 16u) = c;
+    const uint32_t tid = threadIdx.x, blocks = a.k2 / 32u;
+    if (blockIdx.x < a.xtiles) {
+        const uint32_t group = blockIdx.x / (blocks / 4u), kt = blockIdx.x % (blocks / 4u);
+        const uint32_t r = tid >> 4, l = tid & 15u, e0 = kt * 128u + l * 8u;
+        typedef typename Unaligned<T, 8>::type Vec;
+        Vec x[4];
+        const T *p = reinterpret_cast<const T *>(a.x) + (uint64_t)(group * 64u + r) * a.k + e0;
+        if (group * 64u + 64u <= a.m && kt * 128u + 128u <= a.k) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) x[q] = *reinterpret_cast<const Vec *>(p + (uint64_t)(16u * q) * a.k);
+        } else {
+            // what is past a row's end belongs to the next one and is dropped; a row's last elements one
+            // by one would wait for each other
+            const uint64_t end = (uint64_t)a.m * a.k;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const uint32_t vec = group * 64u + 16u * q + r;
+                const uint64_t at = (uint64_t)vec * a.k + e0;
+                x[q] = Vec{};
+                if (vec < a.m && e0 < a.k) {
+                    if (at + 8u <= end)
+                        x[q] = *reinterpret_cast<const Vec *>(reinterpret_cast<const T *>(a.x) + at);
+                    else
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            if (at + e < end) x[q][e] = reinterpret_cast<const T *>(a.x)[at + e];
+                }
+            }
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[q][e] = e0 + e < a.k ? x[q][e] : (T)0;
+        }
+        uint32_t word = 0;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = (float)x[q][e];
+            const uint32_t scale = mx_scale(mx_top4(v));
+            word |= scale << (8 * q);
+            reinterpret_cast<uint32_t *>(a.codes)[(uint64_t)(group * 64u + 16u * q + r) * (a.k2 / 8u) + e0 / 8u] =
+                mx_codes(v, scale);
+        }
+        if ((l & 3u) == 0) reinterpret_cast<uint32_t *>(a.xs)[((uint64_t)group * blocks + kt * 4u + l / 4u) * 16u + r] = word;
+        return;
     }
-    reinterpret_cast<uint8_t *>(words)[block * 64u + (vec & 15u) * 4u + (vec >> 4)] = (uint8_t)scale;
+    __shared__ uint8_t bytes[16][64];   // block, then 4 r + q of vector 16 q + r
+    const uint32_t quads = (blocks + 15u) / 16u, tile = blockIdx.x - a.xtiles, group = tile / quads, b0 = tile % quads * 16u;
+    const uint32_t vec = tid >> 2, b = b0 + (tid & 3u) * 4u;
+    uint32_t four = 0;
+    if (group * 64u + vec < a.n && b < a.kp / 32u)   // (kp / 32 is a multiple of 4)
+        four = *reinterpret_cast<const uint32_t *>(a.w_scales + (uint64_t)(group * 64u + vec) * (a.kp / 32u) + b);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) bytes[(tid & 3u) * 4u + c][(vec & 15u) * 4u + (vec >> 4)] = (uint8_t)(four >> (8 * c));
     __syncthreads();
-    if (threadIdx.x < 64)
-        reinterpret_cast<uint32_t *>(is_w ? a.ws : a.xs)[((uint64_t)group * (a.k2 / 32u) + kt * 4u) * 16u + threadIdx.x] =
-            words[threadIdx.x >> 4][threadIdx.x & 15u];
+    if (b0 + (tid >> 4) < blocks)
+        reinterpret_cast<uint32_t *>(a.ws)[((uint64_t)group * blocks + b0) * 16u + tid] = reinterpret_cast<const uint32_t *>(bytes)[tid];
 }
 
 // BT: the tile edge, 64, 128 or 256.
@@ -439,7 +469,7 @@ template <typename T, int BT> hipError_t mx_tiles_t(const MxForwardArgs &f, hipS
     a.tiles_m = (f.m + BT - 1) / BT;
     a.tiles_n = (f.n + BT - 1) / BT;
     st.xtiles = w.mp / 64u * (w.k2 / 128u);
-    hipLaunchKernelGGL(mx_stage_kernel<T>, dim3(st.xtiles + w.np / 64u * (w.k2 / 128u)), dim3(256), 0, s, st);
+    hipLaunchKernelGGL(mx_stage_kernel<T>, dim3(st.xtiles + w.np / 64u * ((w.k2 + 511u) / 512u)), dim3(256), 0, s, st);
     if constexpr (BT == 64)
         hipLaunchKernelGGL(mx_split_kernel<T>, dim3(a.tiles_m * a.tiles_n), dim3(512), 0, s, f, a);
     else
