@@ -37,10 +37,10 @@ struct MxForwardArgs {
 };
 
 // The tile edge of the product, 0: the kernel for few rows, which needs no workspace.  64 x 64 tiles,
-// whose waves split the k axis, while the GPU holds them all at once (256 rows by 4096 x 4096: 16.4 us,
-// 19.4 on 128 x 128; 512 rows: 27.4 and 20.8), 256 x 256 once they leave few CUs idle (3000 rows:
-// 48.7 us, 52.9 on 128 x 128; 2048 rows: 41.2 and 39.4), 128 x 128 between.  16 rows: 9.5 us without
-// staging, 14.9 with.
+// whose waves split the k axis, while the GPU holds them all at once (256 rows by 4096 x 4096: 15.9 us,
+// 18.8 on 128 x 128; 512 rows: 27.1 and 20.3), 256 x 256 once they leave few CUs idle (3000 rows:
+// 47.2 us, 50.6 on 128 x 128; 2048 rows: 40.7 and 36.4; 8192 rows: 95.3 and 110.6), 128 x 128 between.
+// 16 rows: 9.6 us without staging, 14.6 with; 32 rows: 12.9 and 14.8.
 inline uint32_t mx_tile(uint32_t m, uint32_t n) {
     auto tiles = [&](uint32_t t) { return (uint64_t)((m + t - 1) / t) * ((n + t - 1) / t); };
     return m <= 32 ? 0 : tiles(64) <= 256 ? 64 : tiles(256) >= 160 ? 256 : 128;
