@@ -1,8 +1,8 @@
 /*
  * soklyn_hip.h — C ABI of the MI355X-native DenseBlock hot path.
  *
- * Drop-in boundary for Felix1G/soklyn's device layer: every entry point here
- * replaces one crate-internal GpuContext method of the reference (the
+ * Drop-in boundary for Felix1G/soklyn's device layer: every entry point here,
+ * but for those marked as having no counterpart, replaces one crate-internal GpuContext method of the reference (the
  * `pub(crate)` functions in src/io/device/ffn_device.rs and
  * src/io/device/util_device.rs) or the context constructor in
  * src/io/device.rs.  A Rust caller builds one `skl_dense_desc` per DenseBlock
@@ -33,7 +33,8 @@
  *  - The context keeps padded copies of d_prenorm_h and column sums of
  *    d_prenorm between calls.  An error entry point on any context that
  *    rewrites those buffers makes them stale; a caller that rewrites d_prenorm,
- *    d_prenorm_h or dNorm with its own kernels between two calls must make one
+ *    d_prenorm_h or dNorm with its own kernels, or with an entry point on
+ *    another context that takes them as plain tensors, between two calls must make one
  *    more entry-point call on the context in between (any call does).
  */
 #ifndef SOKLYN_HIP_H
