@@ -57,9 +57,10 @@ __host__ __device__ constexpr uint32_t distill_words(int NT, int E, bool table) 
 // vector are found by its whole wave, a slot to a lane.  2048 rows of 50257 classes with 64 slots:
 // 588 us when each lane looked through the slots by itself, 286 us so.
 //
-// HBM bounds long rows (fp16: 2 bytes of a logit read, 10 written): 2048 rows of 50257 take 274 us,
-// 4.5 TB/s, with one workgroup of 16 waves to a CU, so that a row's sums are waited for; 8192 rows
-// of 8000 150 us, 5.2 TB/s.  Few short rows are launch and latency: 1024 rows of 1000 8.3 us.
+// HBM bounds long rows (fp16: 2 bytes of a logit read, 10 written): 8192 rows of 8000 take 150 us,
+// 5.2 TB/s, 4096 of 30000 308 us, 4.8 TB/s, 2048 of 50257 274 us, 4.5 TB/s (there two workgroups to a
+// CU instead of one, with 64 registers a thread, are not ahead: 294 us against 288 in one run).  Few
+// short rows are launch and latency: 1024 rows of 1000 8.3 us.
 //
 // A softmax's exponent is (z - max) k and not fma(z, k, -max k): the rounding of max k is the same in
 // every term, but past 2^31 (large logits, a small temperature) takes the largest term itself out of
