@@ -147,7 +147,8 @@ template <typename T> __global__ void __launch_bounds__(256) mx_dequantise_kerne
 
 // Vectors down the columns of a [k x n] matrix: a workgroup takes 64 CV columns by 128 rows, a wave one
 // block of 32 rows, a lane CV columns next to each other (256 bytes of a row to a load); the codes go
-// through LDS, so that each vector's 64 bytes are written together.
+// through LDS, so that each vector's 64 bytes are written together.  (Twice the columns: 4096 x 4096
+// fp32 18.7 and 17.2 us for 17.7 and 14.9, 777 x 1531 10.4 for 3.4.)
 template <typename T> constexpr int kDownCols = 4 / sizeof(T);   // columns of a lane
 
 template <typename T> __global__ void __launch_bounds__(256) mx_quantise_down_kernel(MxCastArgs a) {
