@@ -15,9 +15,9 @@ template <typename T, int V> struct Unaligned {
     typedef T type __attribute__((ext_vector_type(V), aligned(sizeof(T))));
 };
 
-// Elements [i, i + V) of p as floats; those from `end` on read as `fill` and are not touched.
+// Elements [i, i + V) of p as floats; those from `end` on read as 0 and are not touched.
 template <typename T, int V>
-__device__ __forceinline__ void load_row(const void *p, uint32_t i, uint32_t end, float (&v)[V], float fill = 0.0f) {
+__device__ __forceinline__ void load_row(const void *p, uint32_t i, uint32_t end, float (&v)[V]) {
     const T *q = reinterpret_cast<const T *>(p);
     if (i + V <= end) {
         const auto w = *reinterpret_cast<const typename Unaligned<T, V>::type *>(q + i);
@@ -25,7 +25,7 @@ __device__ __forceinline__ void load_row(const void *p, uint32_t i, uint32_t end
         for (int e = 0; e < V; ++e) v[e] = (float)w[e];
     } else {
 #pragma unroll
-        for (int e = 0; e < V; ++e) v[e] = i + e < end ? (float)q[i + e] : fill;
+        for (int e = 0; e < V; ++e) v[e] = i + e < end ? (float)q[i + e] : 0.0f;
     }
 }
 
