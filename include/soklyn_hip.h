@@ -278,8 +278,9 @@ size_t skl_residual_work_bytes(uint32_t rows, uint32_t cols);
  * whose class is not in [0, outputs) is empty, classes may repeat (their shares add
  * up).  label (int32 [rows]; a value outside [0, outputs): no label), needed where
  * alpha < 1.  With t = temperature (2^-60 to 2^60), q = softmax(top_logit / t) over
- * the held slots, p = softmax(z / t), p1 = softmax(z):
- *   loss = alpha t^2 sum q log(q / p) - (1 - alpha) log p1[label]
+ * the held slots and added up over those of each class, p = softmax(z / t),
+ * p1 = softmax(z):
+ *   loss = alpha t^2 sum q log(q / p) - (1 - alpha) log p1[label]   (over the classes)
  *   d loss / d z = alpha t (p - q) + (1 - alpha) (p1 - [label])
  * The gradient times LOSS_SCALE goes to grad and d_prenorm (and d_prenorm_h), as
  * skl_dense_backward and the layer below read it; loss (fp32 [rows], or NULL) is

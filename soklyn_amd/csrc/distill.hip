@@ -2,8 +2,8 @@
 // with z the layer's logits, v_j at class i_j the teacher's (j over the row's held slots), t the
 // temperature and y the label:
 //
-//   q = softmax_j(v / t),  p = softmax(z / t),  p1 = softmax(z)
-//   loss = alpha t^2 sum_j q_j (log q_j - log p[i_j]) - (1 - alpha) log p1[y]
+//   q = softmax_j(v / t), added up over the slots of each class,  p = softmax(z / t),  p1 = softmax(z)
+//   loss = alpha t^2 sum_c q_c (log q_c - log p_c) - (1 - alpha) log p1[y]
 //   d loss / d z = alpha t (p - q) + (1 - alpha) (p1 - [y])
 //
 // the gradient times the loss scale into grad and d_prenorm (and its fp16 copy).  A row without
@@ -168,7 +168,12 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT) distill_kernel(DistillArg
         for (uint32_t j = tid; j < top; j += NT) {
             const uint32_t b = ((uint32_t)at[j] + (TABLE ? 0 : lo)) >> group, bit = 1u << (b & 31u);
             q[j] = taught && at[j] >= 0 ? __builtin_amdgcn_exp2f((value[j] - t_max) * k_soft) / t_sum : 0.0f;
-            if (at[j] >= 0) twice = (atomicOr(&marks[b >> 5], bit) & bit) || twice;
+            const bool marked = at[j] >= 0 && (atomicOr(&marks[b >> 5], bit) & bit);
+            if (TABLE)
+                twice = twice || marked;
+            else if (marked && a.loss)   // its group was marked, perhaps by a neighbour; the loss asks for the class
+#pragma unroll 1
+                for (uint32_t i = 0; i < top; ++i) twice = twice || (i != j && at[i] == at[j]);
         }
         if constexpr (!TABLE) {
             const uint32_t b = ((uint32_t)y + lo) >> group;
@@ -188,25 +193,38 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT) distill_kernel(DistillArg
             twice = __any(twice);
             row_sync<NT>();
         }
-        if constexpr (TABLE) {
-            if (!twice) {
+        const float base = m == -INFINITY ? 0.0f : m;
+        if (!twice) {
 #pragma unroll 1
-                for (uint32_t j = tid; j < top; j += NT)
-                    if (at[j] >= 0) table[lo + at[j]] = q[j];
-            } else {
-#pragma unroll 1
-                for (uint32_t j = tid; j < top; j += NT) {
-                    float sum = 0.0f;
-                    bool first = at[j] >= 0;
-                    for (uint32_t i = 0; i < top; ++i) {
-                        sum += at[i] == at[j] ? q[i] : 0.0f;
-                        first = first && (i >= j || at[i] != at[j]);
-                    }
-                    if (first) table[lo + at[j]] = sum;
-                }
+            for (uint32_t j = tid; j < top; j += NT) {
+                if (TABLE && at[j] >= 0) table[lo + at[j]] = q[j];
+                z_at[j] -= base;
             }
         }
-        const float base = m == -INFINITY ? 0.0f : m;
+        // A class that several slots name has the sum of their shares, and as its logit tau log sum exp(v /
+        // tau).  The loss counts each slot with its own share and the class's logit: by how much that is
+        // above the slot's own goes off the class's z.
+        if (twice) {
+#pragma unroll 1
+            for (uint32_t j = tid; j < top; j += NT) {
+                float sum = 0.0f, v = -INFINITY;
+                bool first = at[j] >= 0;
+#pragma unroll 1
+                for (uint32_t i = 0; i < top; ++i)
+                    if (at[i] == at[j]) {
+                        sum += q[i];
+                        v = fmaxf(v, value[i]);
+                        first = first && i >= j;
+                    }
+                if (TABLE && first) table[lo + at[j]] = sum;
+                if (!a.loss) continue;
+                sum = 0.0f;
+#pragma unroll 1
+                for (uint32_t i = 0; i < top; ++i)
+                    if (at[i] == at[j]) sum += __builtin_amdgcn_exp2f((value[i] - v) * k_soft);
+                z_at[j] = (z_at[j] - base) - ((v - value[j]) + a.tau * kLn2 * __builtin_amdgcn_logf(sum));
+            }
+        }
         float s_soft = 0.0f, s_hard = 0.0f;
         if (taught)
             each([&](uint32_t, const float (&v)[V], auto) {
@@ -309,10 +327,10 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT) distill_kernel(DistillArg
             // in units of the logits, not of the exponents: these may pass fp32 where the loss does not
             float l = 0.0f;
             const float logs = a.tau * kLn2 * (__builtin_amdgcn_logf(s_soft) - __builtin_amdgcn_logf(t_sum));
-            if (soft)
+            if (soft)   // (opaque: addresses that are kept from the other loops take registers)
 #pragma unroll 1
-                for (uint32_t j = lane; j < top; j += LANES)
-                    if (q[j] != 0.0f) l += q[j] * (((value[j] - t_max) - (z_at[j] - base)) + logs);
+                for (uint32_t j = opaque(lane); j < top; j += LANES)
+                    if (q[j] != 0.0f) l += q[j] * (((value[j] - t_max) - z_at[j]) + logs);
             l = lanes_sum<LANES>(l) * (a.alpha * a.tau);
             if (hard) l -= (1.0f - a.alpha) * ((z_y - base) - kLn2 * __builtin_amdgcn_logf(s_hard));
             if (lane == 0) a.loss[row] = l;

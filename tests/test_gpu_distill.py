@@ -52,6 +52,7 @@ def reference(z, index, value, label, tau, alpha):
             at = index[r, held].long()
             lq, arg_q = torch.log_softmax(v, 0), v - v.max()
             q = lq.exp()
+            lq = torch.stack([lq[at == c].logsumexp(0) for c in at])   # of the class: all of its slots' shares
             lp = torch.log_softmax(z[r] / tau, 0)
             arg = (z[r] - z[r].max()) / tau
             p = lp.exp()
@@ -165,6 +166,41 @@ def test_a_class_named_twice_adds_its_shares(ctx, n):
     label[0] = 3
     label[1] = index[1, 0]
     check(ctx, z, index, value, label, 2.0, 0.5)
+
+
+# each form of the kernel, with a table of the columns and without
+@pytest.mark.parametrize("n,top", [(1, 2), (10, 4), (60, 33), (250, 64), (700, 8), (2000, 128), (4000, 64), (8000, 64), (9001, 300),
+                                   (40000, 64), (70001, 1024)])
+def test_the_loss_is_a_divergence_where_classes_repeat(ctx, n, top):
+    """sum Q (log Q - log p) over the classes, Q a class's shares added up: 0 where the layer has the
+    teacher's distribution, and never below."""
+    rows = 7
+    z, index, value, label = inputs(rows, n, min(top, n), False, n + top)
+    g = torch.Generator().manual_seed(n)
+    index, value = torch.zeros(rows, top, dtype=torch.int32), torch.randn(rows, top, generator=g)
+    index[1:] = torch.randint(0, n, (rows - 1, top), generator=g)      # some twice
+    index[2] = torch.randint(0, min(n, 3), (top,), generator=g)        # each many times
+    index[3, ::2] = index[3, 0]
+    value[3, top // 2:] -= 90.0                                        # shares that vanish beside the others
+    index[4, 1::2] = -1
+    value[5, ::2] = -INF
+    index[6, top // 2:] = (index[6, : top - top // 2] + 1) % n         # neighbours: one vector's columns
+    z[0] = -INF
+    z[0, 0] = 1.5                                                      # one class, the teacher's
+    _, l = check(ctx, z, index, value, None, 1.0, 1.0)
+    assert l[0].abs() <= (4 * top + 64) * U                            # (two sums of the same terms, in other orders)
+    check(ctx, z, index, value, label, 2.0, 0.5)
+    check(ctx, z.half(), index, value, label, 2.0, 0.5)
+    for tau in (0.5, 1.0, 4.0):
+        # the teacher's own distribution over its classes, mixed from all of its slots
+        same = torch.full((rows, n), -INF)
+        for r in range(rows):
+            v = torch.where(index[r] >= 0, value[r], -INF).double() / tau
+            for c in set(index[r].tolist()) - {-1}:
+                same[r, c] = (tau * v[index[r] == c].logsumexp(0)).float()
+        _, l = check(ctx, same, index, value, None, tau, 1.0)
+        # the logits round by u each, and the tolerance of a loss near 0 is that of its logarithms
+        assert (l.abs() <= tau * tau * (4 * top + n / 64 + 64 + 4 * 100 / tau) * U + tau * U * same.where(same > -INF, 0.0).abs().amax(1)).all()
 
 
 @pytest.mark.parametrize("n", [16, 1000, 3000, 20000])
