@@ -232,6 +232,20 @@ def test_widths(ctx, rows, cols, half, half_stream):
     check_backward(c, h, stats)
 
 
+@pytest.mark.parametrize("rows,cols,post,pre,gates,half,half_stream", [
+    (600, 5120, LAYER, LAYER, 1, True, True), (600, 5120, RMS, RMS, 1, True, False), (517, 8191, LAYER, RMS, 517, False, False),
+    (530, 4101, NONE, LAYER, 1, True, True), (700, 6000, RMS, NONE, 1, False, False)])
+def test_wide_rows_behind_each_other(ctx, rows, cols, post, pre, gates, half, half_stream):
+    """Workgroups with several rows of more than 4096 columns, whose column sums go from row to row."""
+    print(f"join {rows}x{cols} post={post} pre={pre}", flush=True)
+    c = Case(ctx, rows, cols, half, half_stream, post, pre, gates, SIGMOID, 0.75, seed=rows + cols)
+    h, _, stats = check_forward(c)
+    first = check_backward(c, h, stats)
+    second = check_backward(c, h, stats)
+    for k in first:
+        assert torch.equal(first[k], second[k]), k
+
+
 @pytest.mark.parametrize("post", [NONE, RMS, LAYER])
 @pytest.mark.parametrize("pre", [NONE, RMS, LAYER])
 @pytest.mark.parametrize("gates,act", [(0, IDENTITY), (1, IDENTITY), (1, TANH), (11, SIGMOID), (11, IDENTITY)])
