@@ -215,6 +215,41 @@ def test_large_grids(ctx):
     check_forward(ctx, 300, 1537, 1500, False, abi.ACT_IDENTITY)
 
 
+def tile_of(m, n):
+    """The tile edge that the product takes (0: the kernel for few rows)."""
+    def tiles(t):
+        return -(-m // t) * -(-n // t)
+    return 0 if m <= 32 else 64 if tiles(64) <= 256 else 256 if tiles(256) >= 160 else 128
+
+
+# every row and column of tiles of 256: whole and ragged, one k-tile, an odd number of them, the last one half there
+@pytest.mark.parametrize("M,K,N,half,act", [
+    (3000, 640, 4096, True, abi.ACT_SILU), (3333, 777, 3999, False, abi.ACT_TANH), (33, 300, 40967, True, abi.ACT_IDENTITY),
+    (40961, 128, 65, False, abi.ACT_SIGMOID), (2561, 2560, 4099, True, abi.ACT_LEAKY), (4096, 256, 2560, False, abi.ACT_RELU),
+    (3500, 1281, 3001, True, abi.ACT_TANH), (2570, 1024, 4010, False, abi.ACT_SILU)])
+def test_tiles_of_256(ctx, M, K, N, half, act):
+    print(f"mxfp4 forward {M}x{K}x{N} half={half}", flush=True)
+    assert tile_of(M, N) == 256
+    check_forward(ctx, K, N, M, half, act, seed=M + K + N)
+
+
+@pytest.mark.parametrize("M,K,N,half,act", [(1500, 400, 1100, True, abi.ACT_SILU), (1025, 900, 1090, False, abi.ACT_TANH),
+                                            (129, 128, 17001, True, abi.ACT_IDENTITY)])
+def test_tiles_of_128(ctx, M, K, N, half, act):
+    assert tile_of(M, N) == 128
+    check_forward(ctx, K, N, M, half, act, seed=M + K + N)
+
+
+def test_the_same_rows_in_every_tile(ctx):
+    """Each tile of 256 rows has the same rows, and so the same outputs, bit for bit."""
+    M, K, N = 256 * 12, 900, 256 * 14
+    assert tile_of(M, N) == 256
+    lay, _, _ = layer(ctx, K, N, M, True, abi.ACT_SILU, 12)
+    out = lay.forward(up(numbers(256, K, True, 13), True).repeat(12, 1), M)
+    torch.cuda.synchronize()
+    assert (out.view(12, 256, N) == out[:256]).all()
+
+
 def test_smaller_batches_of_a_layer(ctx):
     for M in (1, 16, 31, 100):
         check_forward(ctx, 500, 300, M, True, abi.ACT_IDENTITY, max_batch=160)
