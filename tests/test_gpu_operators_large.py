@@ -87,6 +87,33 @@ def test_distillation(ctx):
         assert torch.equal(far[k], few[k]), k
 
 
+# the threads to a row and rows to a workgroup of each: 16 / 16, 64 / 4, 256 / 1 with a table and without
+@pytest.mark.parametrize("rows,n", [((1 << 24) + 4096, 20), ((1 << 22) + 4096, 500), ((1 << 20) + 4096, 2052), ((1 << 20) + 4096, 4100)])
+def test_distillation_of_more_rows_than_workgroups(ctx, rows, n):
+    """Workgroups that go on to another row: what each of 4096 rows gives by itself, over and over."""
+    print(f"distill {rows}x{n}", flush=True)
+    base, top = 4096, 7
+    g = torch.Generator(device="cuda").manual_seed(n)
+    z = (torch.randn(base, n, generator=g, device="cuda") * 2.5).half()
+    index = torch.randint(-2, n, (base, top), generator=g, device="cuda", dtype=torch.int32)
+    value = torch.randn(base, top, generator=g, device="cuda")
+    label = torch.randint(-1, n, (base,), generator=g, device="cuda", dtype=torch.int32)
+
+    def run(z, index, value, label):
+        out = dict(grad=torch.empty(z.shape, device="cuda"), d_prenorm=torch.empty(z.shape, device="cuda"),
+                   d_prenorm_h=torch.empty_like(z), loss=torch.empty(z.shape[0], device="cuda"))
+        distill_error(ctx, z, index, value, label, temperature=2.0, alpha=0.5, **out)
+        torch.cuda.synchronize()
+        return out
+
+    few = run(z, index, value, label)
+    times = rows // base
+    far = run(z.repeat(times, 1), index.repeat(times, 1), value.repeat(times, 1), label.repeat(times))
+    for k, v in far.items():
+        for part in v.view(times, base, -1).split(64):
+            assert (part == few[k].view(base, -1)).all(), k
+
+
 @pytest.mark.parametrize("down", [False, True])
 def test_casts(ctx, down):
     v = far_rows(66048)
