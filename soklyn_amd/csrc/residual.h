@@ -30,10 +30,10 @@ struct UnjoinArgs {
     float *work;       // null: no column sums wanted
 };
 
-// The most workgroups of the backward of [rows x cols], each of which writes a plane of column sums.
+// The most workgroups of the backward of [rows x cols] (rows > 0), each of which writes a plane of column sums.
 inline uint32_t residual_planes(uint32_t rows, uint32_t cols) {
     const uint32_t rpg = cols <= 64 ? 16 : cols <= 512 ? 4 : 1;
-    const uint32_t groups = (rows + rpg - 1) / rpg, most = cols <= 1024 ? 1280 : cols <= 2048 ? 768 : 256;
+    const uint32_t groups = (rows - 1) / rpg + 1, most = cols <= 1024 ? 1280 : cols <= 2048 ? 768 : 256;
     return groups < most ? groups : most;
 }
 

@@ -65,7 +65,8 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT) join_kernel(JoinArgs a) {
     __shared__ float both[2][4 * S];   // in turns: a row may have one sum, and so one barrier
     const RowMap<NT> map{threadIdx.x % NT, a.cols};
     uint32_t turn = 0;
-    for (uint32_t row = blockIdx.x * RPG + sub_row<NT>(); row < a.rows; row += gridDim.x * RPG, turn ^= 1u) {
+    const uint32_t step = gridDim.x * RPG;
+    for (uint32_t row = blockIdx.x * RPG + sub_row<NT>(); row < a.rows; row = next_row(row, step, a.rows), turn ^= 1u) {
         float *slots = both[turn];
         const uint64_t at = (uint64_t)row * a.cols;
         float mean = 0.0f, rstd = 1.0f;
@@ -194,8 +195,9 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT) unjoin_kernel(UnjoinArgs 
         if (!kWide && a.y) map.template read<T, E>(reinterpret_cast<const T *>(a.y) + at, in.y);
     };
     uint32_t turn = 0, row = blockIdx.x * RPG + sub;
+    const uint32_t step = gridDim.x * RPG;
     if (!kWide && row < a.rows) read(row);
-    for (; row < a.rows; row += gridDim.x * RPG, turn ^= 1u) {
+    for (; row < a.rows; row = next_row(row, step, a.rows), turn ^= 1u) {
         const uint64_t at = (uint64_t)row * a.cols;
         float d[E + 1], t[E + 1], hat[E + 1], y[E + 1];
         if constexpr (kWide) read(row);
@@ -213,7 +215,7 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT) unjoin_kernel(UnjoinArgs 
         if (a.dn) map.template floats<float, E>(in.dn, t);
         if (a.pre) map.template floats<R, E>(in.h, hat);
         if (!kWide && a.y) map.template floats<T, E>(in.y, y);
-        if (!kWide && row + gridDim.x * RPG < a.rows) read(row + gridDim.x * RPG);
+        if (!kWide && step < a.rows - row) read(row + step);
         if (a.dn && a.pre) {
             const float mean = a.stats[2 * (uint64_t)a.rows + row], rstd = a.stats[3 * (uint64_t)a.rows + row];
             float w[E + 1], s[2] = {0.0f, 0.0f};
@@ -346,7 +348,7 @@ __global__ void __launch_bounds__(1024) unjoin_sums_kernel(UnjoinArgs a, uint32_
 
 template <typename T, typename R, int NT, int E> hipError_t join_t(const JoinArgs &a, hipStream_t s) {
     constexpr uint32_t rpg = NT < 256 ? 256 / NT : 1;
-    const uint32_t groups = (a.rows + rpg - 1) / rpg;
+    const uint32_t groups = (a.rows - 1) / rpg + 1;
     hipLaunchKernelGGL((join_kernel<T, R, NT, E>), dim3(groups < (1u << 20) ? groups : 1u << 20),
                        dim3(NT < 256 ? 256 : NT), 0, s, a);
     return hipGetLastError();
@@ -377,9 +379,9 @@ template <class K> uint32_t resident(K kernel, int threads) {
 template <typename T, typename R, int NT, int E, bool BIAS> hipError_t unjoin_t(const UnjoinArgs &a, hipStream_t s) {
     constexpr uint32_t rpg = NT < 256 ? 256 / NT : 1, threads = NT < 256 ? 256 : NT;
     static const uint32_t held = resident(unjoin_kernel<T, R, NT, E, BIAS>, threads);
-    const uint32_t groups = (a.rows + rpg - 1) / rpg, most = std::min(held, residual_planes(a.rows, a.cols));
-    const uint32_t each = std::max((groups + most - 1) / most, groups > 256 ? 2u : 1u);
-    const uint32_t grid = (groups + each - 1) / each;
+    const uint32_t groups = (a.rows - 1) / rpg + 1, most = std::min(held, residual_planes(a.rows, a.cols));
+    const uint32_t each = std::max((groups - 1) / most + 1, groups > 256 ? 2u : 1u);
+    const uint32_t grid = (groups - 1) / each + 1;
     hipLaunchKernelGGL((unjoin_kernel<T, R, NT, E, BIAS>), dim3(grid), dim3(threads), 0, s, a);
     if (a.work)
         hipLaunchKernelGGL(unjoin_sums_kernel, dim3((a.cols + 31) / 32, kPlanes), dim3(1024), 0, s, a, grid);

@@ -76,6 +76,11 @@ template <int NT> __device__ __forceinline__ uint32_t sub_row() {
     return threadIdx.x / NT;
 }
 
+// The row `step` behind `row`, or `rows` where there is none: row + step may be past 32 bits.
+__device__ __forceinline__ uint32_t next_row(uint32_t row, uint32_t step, uint32_t rows) {
+    return row + min(step, rows - row);
+}
+
 // A row of `cols` elements over NT threads: thread t has the vectors of 4 at columns 4 (t + NT c) and,
 // of the up to three columns behind the last whole vector, the t-th, as its element E.
 template <typename T, int E> struct RowPart {

@@ -87,6 +87,38 @@ def test_distillation(ctx):
         assert torch.equal(far[k], few[k]), k
 
 
+def test_a_join_of_the_most_rows(ctx):
+    """2^32 - 1 rows, where a row counter that goes on past the last one starts again at 0: in place, so that a
+    row done twice would show."""
+    rows = (1 << 32) - 1
+    j = Join(ctx, 1, half=True, half_stream=True, pre_norm=abi.NORM_DISABLED, scale=0.5)
+    x = torch.ones(rows, 1, dtype=torch.float16, device="cuda")
+    j.forward(x, None, h=x)
+    torch.cuda.synchronize()
+    assert (x == 0.5).all()
+    del x
+    # (of stats only y's part is read, and there is no y)
+    dh, stats = torch.ones(rows, 1, device="cuda"), torch.empty(4, rows, device="cuda")
+    dparam = torch.full((4, 1), 7.0, device="cuda")
+    j.backward(None, None, None, stats, None, dh, dx=dh, dparam=dparam)
+    torch.cuda.synchronize()
+    assert (dh == 0.5).all() and (dparam == 0).all()
+
+
+def test_a_gates_gradient_over_the_most_rows(ctx):
+    """A sum of 2^32 - 1 ones, each row's once: those of a thread and of a workgroup are exact, the 1280 planes
+    are added in slices of 40 and these 32 to each other, 72 roundings of at most u of the sum."""
+    rows = (1 << 32) - 1
+    j = Join(ctx, 1, half=True, half_stream=True, pre_norm=abi.NORM_DISABLED)
+    gate = torch.full((1, 1), 0.5, dtype=torch.float16, device="cuda")
+    y = torch.ones(rows, 1, dtype=torch.float16, device="cuda")
+    dh, stats = torch.ones(rows, 1, device="cuda"), torch.zeros(4, rows, device="cuda")
+    dgate = torch.zeros(1, 1, device="cuda")
+    j.backward(None, y, gate, stats, None, dh, dgate=dgate)
+    torch.cuda.synchronize()
+    assert abs(dgate.item() - rows) <= 72 * 2.0 ** -24 * rows
+
+
 # the threads to a row and rows to a workgroup of each: 16 / 16, 64 / 4, 256 / 1 with a table and without
 @pytest.mark.parametrize("rows,n", [((1 << 24) + 4096, 20), ((1 << 22) + 4096, 500), ((1 << 20) + 4096, 2052), ((1 << 20) + 4096, 4100)])
 def test_distillation_of_more_rows_than_workgroups(ctx, rows, n):

@@ -181,6 +181,14 @@ def test_work_sizes():
     assert lib.skl_residual_work_bytes(1 << 31, 8192) <= 256 * 5 * 8192 * 4
 
 
+@pytest.mark.parametrize("cols", [1, 64, 65, 512, 513, 8192])
+def test_work_of_a_join_of_the_most_rows(cols):
+    """Up to the last row that 32 bits count, as many planes as for a great many rows."""
+    need = abi.load().skl_residual_work_bytes
+    for rows in ((1 << 32) - (1 << 24), (1 << 32) - 20480, (1 << 32) - 16, (1 << 32) - 15, (1 << 32) - 1):
+        assert need(rows, cols) == need(1 << 31, cols) > 0, rows
+
+
 def test_work_of_a_layer_covers_its_smaller_batches():
     need = abi.load().skl_mxfp4_work_bytes
     for inputs, outputs in ((64, 32), (4096, 4096), (777, 1531), (300, 20000), (5000, 100)):
