@@ -37,13 +37,13 @@ __device__ __forceinline__ uint32_t opaque(uint32_t v) {
     return v;
 }
 
-// LDS words of one row, beside four per slot: marks, and the columns' shares where they have a
-// table.
+// LDS words of one row: the columns' shares where they have a table, marks, four words per slot, and without
+// a table the slots that found their mark made, and their classes.
 __host__ __device__ constexpr uint32_t distill_marks(int NT, bool table) {
     return NT == 16 ? 8 : NT == 64 ? 64 : table ? 128 : 256;
 }
-__host__ __device__ constexpr uint32_t distill_words(int NT, int E, bool table) {
-    return distill_marks(NT, table) + (table ? NT * E : 0);
+__host__ __device__ constexpr uint32_t distill_words(int NT, int E, bool table, uint32_t top) {
+    return distill_marks(NT, table) + (table ? NT * E + 4 * top : 6 * top + 1);
 }
 
 // NT threads to a row (16 or 64: several rows to a workgroup of 256).  They hold it in registers, E
@@ -52,10 +52,13 @@ __host__ __device__ constexpr uint32_t distill_words(int NT, int E, bool table) 
 //
 // What the teacher takes off a column.  TABLE: a table of the columns in LDS, filled by the slots (a
 // class that two of them name is seen when the second sets its bit in marks; then each slot looks
-// through all of them and the first of a class adds them up, in their order).  Otherwise marks has
+// through all of them and adds up those of its class, in their order).  Otherwise marks has
 // a bit for each 2^group columns that says whether a slot may be among them; the slots of a marked
 // vector are found by its whole wave, a slot to a lane.  2048 rows of 50257 classes with 64 slots:
-// 588 us when each lane looked through the slots by itself, 286 us so.
+// 588 us when each lane looked through the slots by itself, 286 us so.  There only the loss asks
+// whether a class repeats: slots that found their group marked go on a list, and each slot looks
+// through that (512 rows of 50257 fp16 with 1000 slots, no two alike: 696 us, 694 without the question
+// and 1002 when each of those looked through all slots; with two alike in half of the rows 790).
 //
 // HBM bounds long rows (fp16: 2 bytes of a logit read, 10 written): 8192 rows of 8000 take 150 us,
 // 5.2 TB/s, 4096 of 30000 308 us, 4.8 TB/s, 2048 of 50257 274 us, 4.5 TB/s (there two workgroups to a
@@ -73,10 +76,11 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT) distill_kernel(DistillArg
     extern __shared__ f32x4 lds[];
     __shared__ float red[3][W > 0 ? W : 1];
     const uint32_t tid = threadIdx.x % NT, lane = threadIdx.x % LANES, n = a.n, top = a.top;
-    float *table = reinterpret_cast<float *>(lds) + sub_row<NT>() * (distill_words(NT, E, TABLE) + 4 * top);
+    float *table = reinterpret_cast<float *>(lds) + sub_row<NT>() * distill_words(NT, E, TABLE, top);
     uint32_t *marks = reinterpret_cast<uint32_t *>(table + (TABLE ? NT * E : 0));
     int32_t *at = reinterpret_cast<int32_t *>(marks + kMarks);
     float *value = reinterpret_cast<float *>(at + top), *q = value + top, *z_at = q + top;
+    uint32_t *late = reinterpret_cast<uint32_t *>(z_at + top);   // without a table: their number, slots and classes
     const float k_soft = kLog2e / a.tau;
     uint32_t group = TABLE ? 0 : 2;   // without a table a vector lies in one group
     if constexpr (!TABLE)
@@ -136,6 +140,7 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT) distill_kernel(DistillArg
 
         // the teacher's slots and the label
         for (uint32_t j = tid; j < kMarks; j += NT) marks[j] = 0;
+        if (!TABLE && tid == 0) late[0] = 0;
         if constexpr (TABLE)
 #pragma unroll
             for (int c = 0; c < C; ++c) reinterpret_cast<f32x4 *>(table)[c * NT + tid] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -168,12 +173,14 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT) distill_kernel(DistillArg
         for (uint32_t j = tid; j < top; j += NT) {
             const uint32_t b = ((uint32_t)at[j] + (TABLE ? 0 : lo)) >> group, bit = 1u << (b & 31u);
             q[j] = taught && at[j] >= 0 ? __builtin_amdgcn_exp2f((value[j] - t_max) * k_soft) / t_sum : 0.0f;
-            const bool marked = at[j] >= 0 && (atomicOr(&marks[b >> 5], bit) & bit);
-            if (TABLE)
-                twice = twice || marked;
-            else if (marked && a.loss)   // its group was marked, perhaps by a neighbour; the loss asks for the class
-#pragma unroll 1
-                for (uint32_t i = 0; i < top; ++i) twice = twice || (i != j && at[i] == at[j]);
+            if (at[j] >= 0 && (atomicOr(&marks[b >> 5], bit) & bit)) {
+                twice = TABLE || a.loss;
+                if (!TABLE && a.loss) {
+                    uint32_t *entry = late + 1 + 2 * atomicAdd(&late[0], 1u);
+                    entry[0] = j;
+                    entry[1] = (uint32_t)at[j];
+                }
+            }
         }
         if constexpr (!TABLE) {
             const uint32_t b = ((uint32_t)y + lo) >> group;
@@ -193,6 +200,20 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT) distill_kernel(DistillArg
             twice = __any(twice);
             row_sync<NT>();
         }
+        // Without a table, where only the loss asks, a slot's group may have been marked by a neighbour: is
+        // there another slot of its class?
+        if (!TABLE && twice) {
+            uint32_t apart = 1;   // 0: no
+            const uint32_t found = late[0];
+#pragma unroll 1
+            for (uint32_t j = tid; j < top; j += NT) {
+                const uint32_t of = (uint32_t)at[j];
+#pragma unroll 4
+                for (uint32_t i = 0; i < found; ++i)
+                    apart = min(apart, late[1 + 2 * i] == j ? 1u : late[2 + 2 * i] ^ of);
+            }
+            twice = __syncthreads_or(apart == 0);
+        }
         const float base = m == -INFINITY ? 0.0f : m;
         if (!twice) {
 #pragma unroll 1
@@ -201,28 +222,19 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT) distill_kernel(DistillArg
                 z_at[j] -= base;
             }
         }
-        // A class that several slots name has the sum of their shares, and as its logit tau log sum exp(v /
-        // tau).  The loss counts each slot with its own share and the class's logit: by how much that is
-        // above the slot's own goes off the class's z.
+        // A class that several slots name has the sum of their shares.  The loss counts each slot with its own
+        // share and the logarithm of its class's: by how much that is above its own goes off the class's z.
+        // (Below 2^-126, where logarithms end, a share has no part in the loss.)
         if (twice) {
 #pragma unroll 1
             for (uint32_t j = tid; j < top; j += NT) {
-                float sum = 0.0f, v = -INFINITY;
-                bool first = at[j] >= 0;
-#pragma unroll 1
-                for (uint32_t i = 0; i < top; ++i)
-                    if (at[i] == at[j]) {
-                        sum += q[i];
-                        v = fmaxf(v, value[i]);
-                        first = first && i >= j;
-                    }
-                if (TABLE && first) table[lo + at[j]] = sum;
-                if (!a.loss) continue;
-                sum = 0.0f;
-#pragma unroll 1
-                for (uint32_t i = 0; i < top; ++i)
-                    if (at[i] == at[j]) sum += __builtin_amdgcn_exp2f((value[i] - v) * k_soft);
-                z_at[j] = (z_at[j] - base) - ((v - value[j]) + a.tau * kLn2 * __builtin_amdgcn_logf(sum));
+                const int32_t of = at[j];
+                float sum = 0.0f;   // the same, to the bit, for every slot of the class
+#pragma unroll 4
+                for (uint32_t i = 0; i < top; ++i) sum += at[i] == of ? q[i] : 0.0f;
+                if (TABLE && of >= 0) table[lo + of] = sum;
+                const float more = __builtin_amdgcn_logf(sum) - __builtin_amdgcn_logf(q[j]);
+                z_at[j] = (z_at[j] - base) - (q[j] >= 0x1p-126f ? a.tau * kLn2 * more : 0.0f);
             }
         }
         float s_soft = 0.0f, s_hard = 0.0f;
@@ -343,7 +355,7 @@ template <typename T, int NT, int E, bool TABLE, bool MORE = false> hipError_t d
     constexpr uint32_t rpg = NT < 256 ? 256 / NT : 1;
     const uint32_t groups = (a.rows + rpg - 1) / rpg;
     hipLaunchKernelGGL((distill_kernel<T, NT, E, TABLE, MORE>), dim3(groups < (1u << 20) ? groups : 1u << 20),
-                       dim3(NT < 256 ? 256 : NT), rpg * (distill_words(NT, E, TABLE) + 4 * a.top) * 4, s, a);
+                       dim3(NT < 256 ? 256 : NT), rpg * distill_words(NT, E, TABLE, a.top) * 4, s, a);
     return hipGetLastError();
 }
 
