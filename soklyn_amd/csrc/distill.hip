@@ -86,7 +86,7 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT) distill_kernel(DistillArg
     if constexpr (!TABLE)
         while ((n + V - 1) >> group >= kMarks * 32u) ++group;
 
-    for (uint32_t row = blockIdx.x * RPG + sub_row<NT>(); row < a.rows; row += gridDim.x * RPG) {
+    for (uint32_t row = blockIdx.x * RPG + sub_row<NT>(); row < a.rows; row = next_row(row, gridDim.x * RPG, a.rows)) {
         const uint64_t row_at = (uint64_t)row * n;
         // A row of an odd width starts anywhere.  Its threads take its vectors from the last of the
         // matrix's own vectors that begins at or before it, so that every whole one is aligned if
@@ -353,7 +353,7 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT) distill_kernel(DistillArg
 
 template <typename T, int NT, int E, bool TABLE, bool MORE = false> hipError_t distill_t(const DistillArgs &a, hipStream_t s) {
     constexpr uint32_t rpg = NT < 256 ? 256 / NT : 1;
-    const uint32_t groups = (a.rows + rpg - 1) / rpg;
+    const uint32_t groups = (a.rows - 1) / rpg + 1;
     hipLaunchKernelGGL((distill_kernel<T, NT, E, TABLE, MORE>), dim3(groups < (1u << 20) ? groups : 1u << 20),
                        dim3(NT < 256 ? 256 : NT), rpg * distill_words(NT, E, TABLE, a.top) * 4, s, a);
     return hipGetLastError();

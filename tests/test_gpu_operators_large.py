@@ -119,6 +119,20 @@ def test_a_gates_gradient_over_the_most_rows(ctx):
     assert abs(dgate.item() - rows) <= 72 * 2.0 ** -24 * rows
 
 
+def test_distillation_of_the_most_rows(ctx):
+    """2^32 - 1 rows of one class, whose probability is 1 and gradient 0, every one of them written."""
+    rows = (1 << 32) - 1
+    z = torch.ones(rows, 1, dtype=torch.float16, device="cuda")
+    label = torch.zeros(rows, dtype=torch.int32, device="cuda")
+    out = dict(grad=torch.full((rows, 1), 7.0, device="cuda"), d_prenorm=torch.full((rows, 1), 7.0, device="cuda"),
+               d_prenorm_h=torch.full((rows, 1), 7.0, dtype=torch.float16, device="cuda"))
+    none = torch.zeros(rows, 0, dtype=torch.int32, device="cuda")
+    distill_error(ctx, z, none, none.float(), label, alpha=0.5, **out)
+    torch.cuda.synchronize()
+    for k, v in out.items():
+        assert (v == 0).all(), k
+
+
 # the threads to a row and rows to a workgroup of each: 16 / 16, 64 / 4, 256 / 1 with a table and without
 @pytest.mark.parametrize("rows,n", [((1 << 24) + 4096, 20), ((1 << 22) + 4096, 500), ((1 << 20) + 4096, 2052), ((1 << 20) + 4096, 4100)])
 def test_distillation_of_more_rows_than_workgroups(ctx, rows, n):
