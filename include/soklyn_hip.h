@@ -310,8 +310,10 @@ int32_t skl_mxfp4_dequantise(skl_ctx *ctx, const void *codes, const void *scales
 /* skl_dense_forward of a block that is only used, with 4-bit weights: w_codes and
  * w_scales are its W [inputs x outputs] quantised down, the input is quantised along
  * its rows on the way, Z = Q(in) . Q(W) (+b) is summed in fp32, then norm and
- * activation (no dropout).  blk->w may be NULL.  inputs <= 2^24.  Without a norm only
- * out is written.  in may not overlap what is written.  work: skl_mxfp4_work_bytes(
+ * activation (no dropout).  blk->w may be NULL.  inputs <= 2^24, and a call whose
+ * kernels would need 2^32 threads is refused (SKL_ERR_INVALID_CONFIGURATION): about
+ * batch * inputs from 2^37 (at the least 256 inputs), or outputs from 2^27 with up to
+ * 32 rows.  Without a norm only out is written.  in may not overlap what is written.  work: skl_mxfp4_work_bytes(
  * inputs, outputs, batch) bytes of the caller's, 16-byte aligned; what it holds does
  * not outlive the call, and calls that overlap in time need a work of their own (as
  * they need an out of their own). */

@@ -1964,6 +1964,7 @@ int32_t skl_dense_forward_mxfp4(skl_ctx *ctx, const skl_dense_desc *b, const voi
     SKL_CHECK(!normed || (b->preact && b->predrop), SKL_ERR_NULL_POINTER);
     SKL_CHECK(b->norm == SKL_NORM_BATCH || b->b, SKL_ERR_NULL_POINTER);
     SKL_CHECK(aligned16(w_codes) && aligned_to(w_scales, 4), SKL_ERR_HARDWARE_CONSTRAINT);
+    SKL_CHECK(mx_fits(b->inputs, b->outputs, batch), SKL_ERR_INVALID_CONFIGURATION);
     const size_t need = mx_work(b->inputs, b->outputs, batch).bytes;
     SKL_CHECK(!need || work, SKL_ERR_NULL_POINTER);
     SKL_CHECK(work_bytes >= need, SKL_ERR_ALLOCATION_LIMIT);

@@ -14,6 +14,7 @@
 namespace skl {
 
 inline __host__ __device__ uint32_t mx_pad(uint32_t k) { return (k + 127u) / 128u * 128u; }
+inline __host__ __device__ uint32_t mx_ceil(uint32_t v, uint32_t by) { return v / by + (v % by != 0); }
 
 struct MxCastArgs {
     uint32_t n, k;          // vectors and their length
@@ -42,27 +43,37 @@ struct MxForwardArgs {
 // 47.2 us, 50.6 on 128 x 128; 2048 rows: 40.7 and 36.4; 8192 rows: 95.3 and 110.6), 128 x 128 between.
 // 16 rows: 9.6 us without staging, 14.6 with; 32 rows: 12.9 and 14.8.
 inline uint32_t mx_tile(uint32_t m, uint32_t n) {
-    auto tiles = [&](uint32_t t) { return (uint64_t)((m + t - 1) / t) * ((n + t - 1) / t); };
+    auto tiles = [&](uint32_t t) { return (uint64_t)mx_ceil(m, t) * mx_ceil(n, t); };
     return m <= 32 ? 0 : tiles(64) <= 256 ? 64 : tiles(256) >= 160 ? 256 : 128;
 }
 
 // The workspace of the tiled product: x's codes, then both scales in the product's order.
 struct MxWork {
-    uint32_t mp, np, k2;
+    size_t mp, np, k2;   // padded: rows, outputs, inputs
     size_t codes, xs, ws, bytes;
 };
 inline MxWork mx_work(uint32_t k, uint32_t n, uint32_t m) {
     MxWork w{};
     const uint32_t t = mx_tile(m, n);
     if (t == 0) return w;
-    w.mp = (m + t - 1) / t * t;
-    w.np = (n + t - 1) / t * t;
-    w.k2 = (k + 255u) / 256u * 256u;
-    w.codes = (size_t)w.mp * (w.k2 / 2);
-    w.xs = (size_t)w.mp * (w.k2 / 32);
-    w.ws = (size_t)w.np * (w.k2 / 32);
+    w.mp = (size_t)mx_ceil(m, t) * t;
+    w.np = (size_t)mx_ceil(n, t) * t;
+    w.k2 = (size_t)mx_ceil(k, 256) * 256;
+    w.codes = w.mp * (w.k2 / 2);
+    w.xs = w.mp * (w.k2 / 32);
+    w.ws = w.np * (w.k2 / 32);
     w.bytes = w.codes + w.xs + w.ws;
     return w;
+}
+
+// A launch has less than 2^32 threads.  Staging: 256 for 64 rows by 128 inputs, and for 64 outputs by 512.
+inline uint64_t mx_stage_x(const MxWork &w) { return w.mp / 64 * (w.k2 / 128); }
+inline uint64_t mx_stage_groups(const MxWork &w) { return mx_stage_x(w) + w.np / 64 * ((w.k2 + 511) / 512); }
+inline bool mx_fits(uint32_t k, uint32_t n, uint32_t m) {
+    const uint32_t t = mx_tile(m, n);
+    if (t == 0) return (uint64_t)mx_ceil(n, 16) * 512 <= 0xffffffffu;
+    return mx_stage_groups(mx_work(k, n, m)) * 256 <= 0xffffffffu &&
+           (uint64_t)mx_ceil(m, t) * mx_ceil(n, t) * 512 <= 0xffffffffu;
 }
 hipError_t launch_mx_forward(const MxForwardArgs &a, uint32_t dtype, hipStream_t s);
 

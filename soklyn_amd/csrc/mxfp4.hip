@@ -460,7 +460,7 @@ template <typename T, int BT> hipError_t mx_tiles_t(const MxForwardArgs &f, hipS
     a.n = st.n = f.n;
     st.k = f.k;
     a.kp = st.kp = mx_pad(f.k);
-    a.k2 = st.k2 = w.k2;
+    a.k2 = st.k2 = (uint32_t)w.k2;
     st.x = f.x;
     st.w_scales = f.w_scales;
     st.codes = reinterpret_cast<uint8_t *>(f.work);
@@ -474,10 +474,10 @@ template <typename T, int BT> hipError_t mx_tiles_t(const MxForwardArgs &f, hipS
     a.act = f.act;
     a.leaky = f.leaky;
     a.out = f.out;
-    a.tiles_m = (f.m + BT - 1) / BT;
-    a.tiles_n = (f.n + BT - 1) / BT;
-    st.xtiles = w.mp / 64u * (w.k2 / 128u);
-    hipLaunchKernelGGL(mx_stage_kernel<T>, dim3(st.xtiles + w.np / 64u * ((w.k2 + 511u) / 512u)), dim3(256), 0, s, st);
+    a.tiles_m = mx_ceil(f.m, BT);
+    a.tiles_n = mx_ceil(f.n, BT);
+    st.xtiles = (uint32_t)mx_stage_x(w);
+    hipLaunchKernelGGL(mx_stage_kernel<T>, dim3((uint32_t)mx_stage_groups(w)), dim3(256), 0, s, st);
     if constexpr (BT == 64)
         hipLaunchKernelGGL(mx_split_kernel<T>, dim3(a.tiles_m * a.tiles_n), dim3(512), 0, s, f, a);
     else
@@ -495,9 +495,9 @@ template <typename T> hipError_t mx_forward_t(const MxForwardArgs &a, hipStream_
     // fewer elements in flight where a row's are twice as large or there are twice as many rows
     constexpr int U = sizeof(T) == 2 ? 4 : 2;
     if (a.m <= 16)
-        hipLaunchKernelGGL((mx_rows_kernel<T, 1, U>), dim3((a.n + 15) / 16), dim3(512), 0, s, a);
+        hipLaunchKernelGGL((mx_rows_kernel<T, 1, U>), dim3(mx_ceil(a.n, 16)), dim3(512), 0, s, a);
     else
-        hipLaunchKernelGGL((mx_rows_kernel<T, 2, U / 2>), dim3((a.n + 15) / 16), dim3(512), 0, s, a);
+        hipLaunchKernelGGL((mx_rows_kernel<T, 2, U / 2>), dim3(mx_ceil(a.n, 16)), dim3(512), 0, s, a);
     return hipGetLastError();
 }
 

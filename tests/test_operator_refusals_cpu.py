@@ -197,6 +197,24 @@ def test_work_of_a_layer_covers_its_smaller_batches():
     assert need(0, 64, 64) == need(64, 0, 64) == 0
 
 
+@pytest.mark.parametrize("batch", [(1 << 32) - 256, (1 << 32) - 255, (1 << 32) - 64, (1 << 32) - 1])
+def test_work_of_a_layer_of_the_most_rows_or_outputs(batch):
+    """Rounding up to whole tiles goes past 32 bits."""
+    need = abi.load().skl_mxfp4_work_bytes
+    assert need(64, 64, batch) >= need(64, 64, 1 << 31) > 1 << 36
+    assert need(64, batch, 64) >= need(64, 1 << 31, 64) > 1 << 32
+
+
+@pytest.mark.parametrize("inputs,outputs,batch", [(1, 1, (1 << 32) - 1), (1, 1, (1 << 32) - 255), (64, 1, 1 << 29), (4096, 64, 1 << 25),
+                                                  (1, (1 << 32) - 1, 1), (1, (1 << 27) + 1, 32), (1, (1 << 32) - 1, 64)])
+def test_serve_of_more_than_a_launch_takes(inputs, outputs, batch):
+    """Refused whatever the workspace; addresses further from each other than any of the tensors is long."""
+    d, _ = desc(dtype=0, inputs=inputs, outputs=outputs, max_batch=batch, **{k: i << 50 for i, k in enumerate((
+        "out", "b", "grad", "d_prenorm", "d_prenorm_h", "preact", "predrop", "prenorm", "centered", "norm_rstd", "norm_w", "norm_b"), 1)})
+    assert abi.status("skl_dense_forward_mxfp4", CTX, C.byref(d), 13 << 50, batch, inputs, batch, 14 << 50, 15 << 50, 16 << 50,
+                      (1 << 64) - 1) == INVALID
+
+
 class NoContext:
     h, device = CTX, 0
 
