@@ -173,6 +173,15 @@ def test_serve(code, d, change):
     assert serve_status(d, **change) == code
 
 
+@pytest.mark.parametrize("norm", [1, 2, 3])
+def test_serve_of_a_workspace_in_the_norms_cache(norm):
+    """The product reads its workspace while it writes the pre-norm values."""
+    need = abi.load().skl_mxfp4_work_bytes(64, 32, 64)
+    at = 1 << 50
+    for prenorm in (at, at + 128, at + need - 2, at - 64 * 32 * 2 + 2):
+        assert need and serve_status(dict(norm=norm, max_batch=64, prenorm=prenorm), rows=64, batch=64, work=at, size=need) == INVALID
+
+
 def test_work_sizes():
     lib = abi.load()
     assert lib.skl_residual_work_bytes(0, 64) == lib.skl_residual_work_bytes(64, 0) == 0
