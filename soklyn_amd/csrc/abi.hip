@@ -1976,9 +1976,10 @@ int32_t skl_dense_forward_mxfp4(skl_ctx *ctx, const skl_dense_desc *b, const voi
                          {normed ? b->norm_b : nullptr, nb}};
     const Span out[] = {{b->out, e}, {need ? work : nullptr, need}, {normed ? b->prenorm : nullptr, e},
                         {normed ? b->centered : nullptr, e}, {normed ? b->preact : nullptr, e},
-                        {normed ? b->predrop : nullptr, e}};
+                        {normed ? b->predrop : nullptr, e},
+                        {normed ? b->norm_rstd : nullptr, (b->norm == SKL_NORM_BATCH ? b->outputs : batch) * t}};
     // (the product reads work while it writes out or prenorm)
-    SKL_CHECK(!spans_clash(out, 6, read, 6) && !outputs_clash(out, 2) && !outputs_clash(out + 1, 2), SKL_ERR_INVALID_CONFIGURATION);
+    SKL_CHECK(!spans_clash(out, 7, read, 6) && !outputs_clash(out, 2) && !outputs_clash(out + 1, 2), SKL_ERR_INVALID_CONFIGURATION);
     if ((r = check_tile(ctx, b))) return r;
     if ((r = enter(ctx))) return r;
     MxForwardArgs a{};

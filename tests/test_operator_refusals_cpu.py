@@ -182,6 +182,13 @@ def test_serve_of_a_workspace_in_the_norms_cache(norm):
         assert need and serve_status(dict(norm=norm, max_batch=64, prenorm=prenorm), rows=64, batch=64, work=at, size=need) == INVALID
 
 
+@pytest.mark.parametrize("norm,size", [(1, 2 * 8), (2, 2 * 8), (3, 2 * 32)])
+def test_serve_of_an_input_in_the_norms_deviations(norm, size):
+    at = 1 << 50
+    for x in (at, at + size - 2):
+        assert serve_status(dict(norm=norm, norm_rstd=at), x=x) == INVALID
+
+
 def test_work_sizes():
     lib = abi.load()
     assert lib.skl_residual_work_bytes(0, 64) == lib.skl_residual_work_bytes(64, 0) == 0
