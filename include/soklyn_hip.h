@@ -301,7 +301,9 @@ int32_t skl_dense_distill_error(skl_ctx *ctx, const skl_dense_desc *blk, const v
  * even one, past 6 to 6.  A block with an infinity or NaN has s = 255 and stands for
  * NaN.  Elements past k are 0.
  * The vectors are the rows of src [rows x cols] (down = 0) or its columns (down = 1:
- * the weights [inputs x outputs] of a block). */
+ * the weights [inputs x outputs] of a block).  Refused (SKL_ERR_INVALID_CONFIGURATION):
+ * vectors of more than 2^31 - 128 elements, 2^32 pieces of up to 256 elements of a vector,
+ * and down the columns 2^39 bytes of src with its rows rounded up to 128. */
 int32_t skl_mxfp4_quantise(skl_ctx *ctx, const void *src, uint32_t dtype, uint32_t rows, uint32_t cols,
                            uint32_t down, void *codes, void *scales);
 /* The values, rounded to dtype, into dst [rows x cols]. */

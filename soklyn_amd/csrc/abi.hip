@@ -1915,6 +1915,7 @@ static int32_t mx_cast(skl_ctx *ctx, const void *values, uint32_t dtype, uint32_
     const uint64_t k = down ? rows : cols, n = down ? cols : rows;
     SKL_CHECK(k <= 0x7fffff80u && n * ((k + 255) / 256) <= 0xffffffffu, SKL_ERR_INVALID_CONFIGURATION);
     if (rows == 0 || cols == 0) return SKL_OK;
+    SKL_CHECK(mx_cast_fits((uint32_t)n, (uint32_t)k, down != 0, dtype == SKL_F16 ? 2 : 4), SKL_ERR_INVALID_CONFIGURATION);
     SKL_CHECK(values && codes && scales, SKL_ERR_NULL_POINTER);
     SKL_CHECK(aligned16(codes) && aligned_to(scales, 4), SKL_ERR_HARDWARE_CONSTRAINT);
     MxCastArgs a{};

@@ -16,6 +16,13 @@ namespace skl {
 inline __host__ __device__ uint32_t mx_pad(uint32_t k) { return (k + 127u) / 128u * 128u; }
 inline __host__ __device__ uint32_t mx_ceil(uint32_t v, uint32_t by) { return v / by + (v % by != 0); }
 
+// Columns of a workgroup of the casts down the columns, which takes 128 rows of them, 256 threads.
+inline constexpr uint32_t mx_down_cols(size_t element) { return (uint32_t)(256 / element); }
+// A launch has less than 2^32 threads (along the rows workgroups loop).
+inline bool mx_cast_fits(uint32_t n, uint32_t k, bool down, size_t element) {
+    return !down || (uint64_t)mx_ceil(n, mx_down_cols(element)) * (mx_pad(k) / 128u) * 256u <= 0xffffffffu;
+}
+
 struct MxCastArgs {
     uint32_t n, k;          // vectors and their length
     void *values;           // T

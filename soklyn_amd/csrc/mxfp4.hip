@@ -68,7 +68,7 @@ template <int E> __host__ __device__ __forceinline__ MxRows mx_rows(uint32_t n, 
     r.lanes = mx_pad(k) / E;
     r.per_row = (r.lanes + 63) / 64;
     r.rows = r.lanes < 64 ? 64 / r.lanes : 1;
-    r.waves = (uint64_t)((n + r.rows - 1) / r.rows) * r.per_row;
+    r.waves = (uint64_t)mx_ceil(n, r.rows) * r.per_row;
     return r;
 }
 // For every lane that has elements of a vector use(vector, lane of the vector, what load(...) of
@@ -156,7 +156,7 @@ template <typename T> __global__ void __launch_bounds__(256) mx_quantise_down_ke
     typedef typename Unaligned<T, CV>::type Vec;
     __shared__ u32x4 codes[COLS][5];
     __shared__ uint8_t scales[COLS][4];
-    const uint32_t kp = mx_pad(a.k), ntiles = (a.n + COLS - 1) / COLS;
+    const uint32_t kp = mx_pad(a.k), ntiles = mx_ceil(a.n, COLS);
     const uint32_t ntile = blockIdx.x % ntiles, ktile = blockIdx.x / ntiles;
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
     const uint32_t k0 = ktile * 128u + wave * 32u, n0 = ntile * COLS, col = n0 + lane * CV;
@@ -206,7 +206,7 @@ template <typename T> __global__ void __launch_bounds__(256) mx_quantise_down_ke
 template <typename T> __global__ void __launch_bounds__(256) mx_dequantise_down_kernel(MxCastArgs a) {
     constexpr int CV = kDownCols<T>, COLS = 64 * CV;
     __shared__ u32x4 codes[COLS][5];
-    const uint32_t kp = mx_pad(a.k), ntiles = (a.n + COLS - 1) / COLS;
+    const uint32_t kp = mx_pad(a.k), ntiles = mx_ceil(a.n, COLS);
     const uint32_t ntile = blockIdx.x % ntiles, ktile = blockIdx.x / ntiles;
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
     const uint32_t k0 = ktile * 128u + wave * 32u, n0 = ntile * COLS, col = n0 + lane * CV;
@@ -504,8 +504,9 @@ template <typename T> hipError_t mx_forward_t(const MxForwardArgs &a, hipStream_
 template <typename T> hipError_t mx_cast(const MxCastArgs &a, bool down, bool back, hipStream_t s) {
     if (a.n == 0 || a.k == 0) return hipSuccess;
     if (down) {
-        constexpr uint32_t cols = 64 * kDownCols<T>;
-        const dim3 grid((a.n + cols - 1) / cols * (mx_pad(a.k) / 128));
+        constexpr uint32_t cols = mx_down_cols(sizeof(T));
+        static_assert(cols == 64 * kDownCols<T>, "what the kernels take");
+        const dim3 grid(mx_ceil(a.n, cols) * (mx_pad(a.k) / 128));
         hipLaunchKernelGGL((back ? mx_dequantise_down_kernel<T> : mx_quantise_down_kernel<T>), grid, dim3(256), 0, s, a);
     } else {
         const uint64_t waves = back ? mx_rows<kValues<T>>(a.n, a.k).waves : mx_rows<8>(a.n, a.k).waves;

@@ -150,6 +150,13 @@ def test_casts(back, code, change):
     assert cast_status(back, **change) == code
 
 
+@pytest.mark.parametrize("back", [False, True])
+@pytest.mark.parametrize("dtype,rows,cols", [(0, 1, 1 << 30), (1, 1, 1 << 31), (1, 128, (1 << 31) + 5), (0, 129, 1 << 29), (1, 1, (1 << 32) - 1),
+                                             (0, 1, (1 << 32) - 64)])
+def test_casts_down_more_than_a_launch_takes(back, dtype, rows, cols):
+    assert cast_status(back, dtype=dtype, rows=rows, cols=cols, down=1, src=1 << 50, codes=2 << 50, scales=3 << 50) == INVALID
+
+
 def serve_status(d=None, **change):
     blk, at = desc(**(d or {}))
     a = dict(ctx=CTX, blk=C.byref(blk), x=at(), rows=8, cols=64, batch=8, codes=at(), scales=at(), work=at(),
