@@ -25,12 +25,9 @@ fn main() {
             repo.join("soklyn_amd")
         }
     };
-    for src in [
-        "abi.hip", "gemm.hip", "gemm_wave.hip", "elementwise.hip", "epilogue.h", "gemm.h", "gemm_dma.h", "gemm_wave.h",
-        "device_math.h",
-    ] {
-        println!("cargo:rerun-if-changed={}", repo.join("soklyn_amd/csrc").join(src).display());
-    }
+    // (a folder: cargo looks at everything in it)
+    println!("cargo:rerun-if-changed={}", repo.join("soklyn_amd/csrc").display());
+    println!("cargo:rerun-if-changed={}", repo.join("soklyn_amd/build.py").display());
     println!("cargo:rerun-if-changed={}", repo.join("include/soklyn_hip.h").display());
     println!("cargo:rustc-link-search=native={}", lib_dir.display());
     println!("cargo:rustc-link-lib=dylib=soklyn_hip");

@@ -216,3 +216,15 @@ def test_checker_catches_a_field_added_to_the_header(tmp_path, monkeypatch):
         monkeypatch.setitem(globals(), "HEADER", str(p))
         with pytest.raises(AssertionError, match=msg):
             check()
+
+
+def test_the_build_script_watches_every_source():
+    """A file or its folder, which cargo looks through, for all that the library is built from."""
+    with open(os.path.join(ROOT, "rust", "build.rs")) as f:
+        code = re.sub(r"//[^\n]*", "", f.read())
+    watched = {os.path.normpath(p) for p in re.findall(r'rerun-if-changed=\{\}", repo\.join\("([^"]+)"\)\.display', code)}
+    csrc = os.path.join("soklyn_amd", "csrc")
+    named = {os.path.join(csrc, n) for n in re.findall(r'"([\w.]+\.(?:hip|h))"', code)}
+    for src in [os.path.join(csrc, n) for n in sorted(os.listdir(os.path.join(ROOT, csrc)))] + [
+            os.path.join("include", "soklyn_hip.h"), os.path.join("soklyn_amd", "build.py")]:
+        assert src in watched | named or os.path.dirname(src) in watched, src
