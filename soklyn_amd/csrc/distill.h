@@ -8,7 +8,7 @@
 
 namespace skl {
 
-constexpr uint32_t kDistillTop = 1024;   // teacher logits per row: three LDS words each
+constexpr uint32_t kDistillTop = 1024;   // teacher logits per row: four to six LDS words each
 
 struct DistillArgs {
     uint32_t rows, n, top;

@@ -47,8 +47,8 @@ __host__ __device__ constexpr uint32_t distill_words(int NT, int E, bool table, 
 }
 
 // NT threads to a row (16 or 64: several rows to a workgroup of 256).  They hold it in registers, E
-// elements each, from one read; MORE: what is longer than that is read three times (maximum, sums,
-// gradient).
+// elements each, from one read; MORE: what is longer than that is read for the maximum, for each of the two
+// sums that the row needs, and for the gradient: up to four times.
 //
 // What the teacher takes off a column.  TABLE: a table of the columns in LDS, filled by the slots (a
 // class that two of them name is seen when the second sets its bit in marks; then each slot looks
@@ -62,8 +62,10 @@ __host__ __device__ constexpr uint32_t distill_words(int NT, int E, bool table, 
 //
 // HBM bounds long rows (fp16: 2 bytes of a logit read, 10 written): 8192 rows of 8000 take 150 us,
 // 5.2 TB/s, 4096 of 30000 308 us, 4.8 TB/s, 2048 of 50257 274 us, 4.5 TB/s (there two workgroups to a
-// CU instead of one, with 64 registers a thread, are not ahead: 294 us against 288 in one run).  Few
-// short rows are launch and latency: 1024 rows of 1000 8.3 us.
+// CU instead of one, with 64 registers a thread, are not ahead: 294 us against 288 in one run).  MORE,
+// with 64 slots, teacher alone and with labels: 1024 rows of 128256 fp16 380 and 410 us (floor 308 at a
+// large copy's 5.12 TB/s), 512 of 256000 520 and 585 (307), fp32 485 and 512, 561 and 630: the reads past
+// the first.  Few short rows are launch and latency: 1024 rows of 1000 8.2 us.
 //
 // A softmax's exponent is (z - max) k and not fma(z, k, -max k): the rounding of max k is the same in
 // every term, but past 2^31 (large logits, a small temperature) takes the largest term itself out of

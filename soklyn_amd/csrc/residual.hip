@@ -58,6 +58,9 @@ __device__ __forceinline__ void row_stats(const float (&v)[E + 1], const RowMap<
 // One row per NT threads (several to a workgroup of 256 where a wave, or a quarter, holds one).
 // 8192 x 4096, fp16 with an fp32 stream, a gate for each row, RMS on both sides: 470 MB in 94.8 us,
 // 4.96 TB/s, of 5.1 for a large copy; one row of it 4.6 us, loads and two sums one behind the other.
+// Wider rows, one on each workgroup of 512, are further from it (RMS, one gate): 4096 x 8192 fp16
+// 83 us, 3.2 TB/s, fp32 126, 4.3 TB/s; 8192 x 5120, where three eighths of the threads' vectors are empty,
+// 168 and 169 us, 2.0 and 4.0 TB/s.
 template <typename T, typename R, int NT, int E>
 __global__ void __launch_bounds__(NT < 256 ? 256 : NT) join_kernel(JoinArgs a) {
     constexpr int RPG = NT < 256 ? 256 / NT : 1;
@@ -147,8 +150,11 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT) join_kernel(JoinArgs a) {
 // A workgroup walks rows blockIdx, blockIdx + grid, ... with its column sums in registers and the
 // next row's tensors on their way, and writes its sums as one plane of a.work [grid x kPlanes x
 // cols]; the next kernel adds the planes: 16384 x 2048 fp16, 671 MB in 137 + 6 us, 4.7 TB/s.  BIAS: a Layer norm is there, so that du and dn are summed.
-// Rows of more than 4096 columns leave no registers for the next row, nor for the sums but dn's,
-// which each thread then keeps in LDS.
+// Rows of more than 4096 columns: the sums but dn's, which do not fit the registers, are in LDS, each
+// thread its own, and a row's tensors are loaded where they are used, not a row ahead (of 256 registers BIAS
+// takes 236 to 244, the other form 192 to 200).  One workgroup to a CU then waits for dn and h, for dh
+// and for y: 4096 x 8192 fp16 with RMS on both sides 177 us, with Layer 191 (floor 131 at 5.12 TB/s),
+// fp32 193 and 207 (157); 8192 x 5120 fp16 245 and 264 (164), fp32 258 and 279 (197).
 template <typename T, typename R, int NT, int E, bool BIAS>
 __global__ void __launch_bounds__(NT < 256 ? 256 : NT) unjoin_kernel(UnjoinArgs a) {
     constexpr int RPG = NT < 256 ? 256 / NT : 1, S = NT < 64 ? 1 : NT / 64;
