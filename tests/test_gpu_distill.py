@@ -130,6 +130,28 @@ def test_sizes(ctx, half, rows, n, top):
     check(ctx, z, index, value, label, 2.0, 0.75)
 
 
+# the last width of each form and the next, rows that start at every remainder of 4
+@pytest.mark.parametrize("n", [61, 62, 63, 253, 254, 509, 510, 1021, 1022, 2045, 2046, 4093, 4094, 8189, 8190, 16381, 16382, 32765, 32766,
+                               65533, 65534])
+def test_edges_of_the_forms(ctx, n):
+    print(f"distill {n}", flush=True)
+    for half in (True, False):
+        z, index, value, label = inputs(6, n, 11, half, n)
+        check(ctx, z, index, value, label, 1.5, 0.25)
+
+
+@pytest.mark.parametrize("n", [61, 253, 257, 500, 509, 1000, 1021, 1999, 2045, 3000])
+def test_enough_rows_to_fill_the_gpu(ctx, n):
+    """Where rows are many a wave, or a quarter, has each of them by itself; every 97th is compared."""
+    rows = 4113
+    for half in (True, False):
+        z, index, value, label = inputs(rows, n, 7, half, n)
+        g, l = run(ctx, z, index, value, label, 2.0, 0.5)
+        some = slice(n % 97, rows, 97)
+        rg, tg, rl, tl = reference(z[some], index[some], value[some], label[some], 2.0, 0.5)
+        assert ((g[some] - rg).abs() <= tg).all() and ((l[some] - rl).abs() <= tl).all()
+
+
 @pytest.mark.parametrize("tau", [0.25, 1.0, 7.5])
 @pytest.mark.parametrize("alpha", [0.0, 0.3, 1.0])
 def test_temperatures_and_mixtures(ctx, tau, alpha):
@@ -170,7 +192,7 @@ def test_a_class_named_twice_adds_its_shares(ctx, n):
 
 # each form of the kernel, with a table of the columns and without
 @pytest.mark.parametrize("n,top", [(1, 2), (10, 4), (60, 33), (250, 64), (700, 8), (2000, 128), (4000, 64), (8000, 64), (9001, 300),
-                                   (40000, 64), (70001, 1024)])
+                                   (40000, 64), (70001, 1024), (5, 1024), (60, 65), (300, 1000), (3000, 1024)])
 def test_the_loss_is_a_divergence_where_classes_repeat(ctx, n, top):
     """sum Q (log Q - log p) over the classes, Q a class's shares added up: 0 where the layer has the
     teacher's distribution, and never below."""

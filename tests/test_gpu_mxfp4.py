@@ -201,6 +201,15 @@ def test_forward_sizes(ctx, half, M, K, N):
     check_forward(ctx, K, N, M, half, abi.ACT_SILU, seed=M + K + N)
 
 
+# batches on either side of each choice of tile, inputs of every remainder that their padding has
+@pytest.mark.parametrize("M,N", [(31, 33), (32, 4097), (33, 31), (63, 65), (64, 64 * 256), (65, 64 * 128), (64, 64 * 256 + 1), (127, 9000),
+                                 (1024, 1024), (1025, 1024), (3840, 2560), (3841, 2561)])
+def test_borders_of_the_tiles(ctx, M, N):
+    print(f"mxfp4 forward {M}x{N}, tile {tile_of(M, N)}", flush=True)
+    for half, K in ((True, 31), (False, 129), (True, 257)):
+        check_forward(ctx, K, N, M, half, abi.ACT_SILU, seed=M + N)
+
+
 @pytest.mark.parametrize("act", list(ACT_REF))
 def test_activations(ctx, act):
     for half in (True, False):

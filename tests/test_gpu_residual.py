@@ -232,6 +232,18 @@ def test_widths(ctx, rows, cols, half, half_stream):
     check_backward(c, h, stats)
 
 
+# the last width of each form and the next, in rows that end inside a workgroup and start at every remainder of 4
+@pytest.mark.parametrize("rows,cols", [(33, 63), (17, 64), (19, 65), (1, 66), (9, 255), (5, 256), (6, 257), (2600, 61), (1300, 509),
+                                       (530, 1023), (900, 1025), (300, 4095), (300, 4097)])
+@pytest.mark.parametrize("half,half_stream", [(True, True), (True, False), (False, False)])
+def test_edges_of_the_forms(ctx, rows, cols, half, half_stream):
+    print(f"join {rows}x{cols} half={half} half_stream={half_stream}", flush=True)
+    for norm, gates in ((LAYER, rows), (RMS, 1)):
+        c = Case(ctx, rows, cols, half, half_stream, norm, norm, gates, TANH, 1.25, seed=rows + cols)
+        h, _, stats = check_forward(c)
+        check_backward(c, h, stats)
+
+
 @pytest.mark.parametrize("rows,cols,post,pre,gates,half,half_stream", [
     (600, 5120, LAYER, LAYER, 1, True, True), (600, 5120, RMS, RMS, 1, True, False), (517, 8191, LAYER, RMS, 517, False, False),
     (530, 4101, NONE, LAYER, 1, True, True), (700, 6000, RMS, NONE, 1, False, False)])
