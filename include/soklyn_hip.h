@@ -325,6 +325,70 @@ int32_t skl_dense_forward_mxfp4(skl_ctx *ctx, const skl_dense_desc *blk, const v
 /* Host side; grows with the batch, and is 0 where the batch or the layer is small. */
 size_t skl_mxfp4_work_bytes(uint32_t inputs, uint32_t outputs, uint32_t batch);
 
+/* ---- gated feed-forward blocks (no counterpart in the reference) ------------- */
+/* Two blocks over one input, without norms, whose results are multiplied:
+ *   a = in . Wg + bg,  u = in . Wu + bu,  out = act(a) * u
+ * one kernel.  gate (any activation but Softmax) and up (Identity) have the same type,
+ * inputs and outputs; a NULL b is no bias.  in is [in_rows x inputs] T, its first `batch`
+ * rows are used; out is [batch x outputs] T.  Where gate->preact / up->preact are not
+ * NULL, a / u are kept there (rounded to T) for the backward.  out is computed from the
+ * fp32 sums and rounded once.  No output may overlap an input.
+ * work (16-byte aligned, or NULL): skl_product_work_bytes(dtype, batch, inputs, outputs,
+ * 2) bytes of the caller's for padded copies of ragged fp16 operands; with less, a kernel
+ * runs that takes them as stored (the same result but for the order of its sums).  What it
+ * holds does not outlive the call; calls that overlap in time need a work of their own.
+ * Weights of 2^31 bytes and more, and launches of 2^32 threads, are refused
+ * (SKL_ERR_INVALID_CONFIGURATION), here and in the calls below. */
+int32_t skl_gated_forward(skl_ctx *ctx, const skl_dense_desc *gate, const skl_dense_desc *up, const void *in,
+                          uint32_t in_rows, uint32_t in_cols, uint32_t batch, void *out, void *work,
+                          size_t work_bytes);
+/* Its backward, in the blocks' own buffers: from s (fp32 [batch x outputs]), the gradient
+ * of out with the loss scale in it, and the kept a and u,
+ *   gate->d_prenorm = s * u * act'(a),  up->d_prenorm = s * act(a)
+ * and their fp16 copies in d_prenorm_h (fp16 blocks).  skl_dense_backward on each of the
+ * two then updates its weights; grad is left as it is (nothing reads it without a norm). */
+int32_t skl_gated_error_from_sum(skl_ctx *ctx, const skl_dense_desc *gate, const skl_dense_desc *up, const float *s,
+                                 uint32_t batch);
+/* The same from the layer above, s = next.d_prenorm . next.W^T in the kernel's registers
+ * (fp16: next's d_prenorm_h and W, fp32 sums).  work: skl_product_work_bytes(dtype, batch,
+ * next->outputs, outputs, 1). */
+int32_t skl_gated_hidden_error(skl_ctx *ctx, const skl_dense_desc *gate, const skl_dense_desc *up,
+                               const skl_dense_desc *next, uint32_t batch, void *work, size_t work_bytes);
+/* dx[batch x inputs] fp32 = gate.d_prenorm . Wg^T + up.d_prenorm . Wu^T (fp16: of the
+ * fp16 copies), one sum.  work: skl_product_work_bytes(dtype, batch, outputs, inputs, 2). */
+int32_t skl_gated_input_grad(skl_ctx *ctx, const skl_dense_desc *gate, const skl_dense_desc *up, uint32_t batch,
+                             float *dx, void *work, size_t work_bytes);
+/* Host side: bytes of work for a product of `batch` rows of `inputs` with `matrices` (1 or
+ * 2) matrices to `outputs`; 0 where none is used. */
+size_t skl_product_work_bytes(uint32_t dtype, uint32_t batch, uint32_t inputs, uint32_t outputs, uint32_t matrices);
+
+/* ---- a block's result added to the residual stream, dropout (no counterpart) --- */
+/* z = in . W + b,  h = scale * x + drop(act(z)): a block without a norm (any activation but
+ * Softmax; a NULL b is no bias), its dropout and the residual stream in one kernel.  x and
+ * h are [batch x outputs] of stream_dtype (SKL_F32, or SKL_F16 with fp16 blocks); h may be
+ * x, in place; x NULL: h = drop(act(z)).  Where blk->preact is not NULL, z is kept there
+ * (rounded to T) for the backward; the block's other caches are not used.  h is computed
+ * from the fp32 sums and rounded once.
+ * Dropout (use_dropout; probability blk->mask_coeff, at least 0 and below 1) stores no mask:
+ * an element is kept, times 1 / (1 - p), or is 0 as skl_dense_forward draws it from the same
+ * seed, row and column.  work as above, skl_product_work_bytes(dtype, batch, inputs,
+ * outputs, 1). */
+int32_t skl_dense_forward_residual(skl_ctx *ctx, const skl_dense_desc *blk, const void *in, uint32_t in_rows,
+                                   uint32_t in_cols, uint32_t batch, uint32_t use_dropout, uint32_t seed,
+                                   uint32_t stream_dtype, float scale, const void *x, void *h, void *work,
+                                   size_t work_bytes);
+/* Its backward, from dh (fp32 [batch x outputs], the gradient of h with the loss scale in
+ * it): blk->d_prenorm = drop(dh) * act'(z), drawn again from use_dropout and seed, and its
+ * fp16 copy, as skl_dense_backward, skl_dense_input_grad and the layer below read them (grad
+ * is left as it is); dx = scale * dh where not NULL.  dx may be dh, in place.  preact is not
+ * read where the activation is Identity. */
+int32_t skl_dense_residual_error(skl_ctx *ctx, const skl_dense_desc *blk, const float *dh, uint32_t batch,
+                                 uint32_t use_dropout, uint32_t seed, float scale, float *dx);
+/* out = drop(in) of a matrix [rows x cols] of dtype, drawn as above (0 <= p < 1); out may be
+ * in.  On the gradient of out with the same p and seed it is its own backward. */
+int32_t skl_dropout(skl_ctx *ctx, uint32_t dtype, uint32_t rows, uint32_t cols, float p, uint32_t seed, const void *in,
+                    void *out);
+
 #ifdef __cplusplus
 }
 #endif

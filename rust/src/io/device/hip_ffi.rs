@@ -160,4 +160,23 @@ extern "C" {
                                    in_rows: u32, in_cols: u32, batch: u32, w_codes: *const c_void,
                                    w_scales: *const c_void, work: *mut c_void, work_bytes: usize) -> i32;
     pub fn skl_mxfp4_work_bytes(inputs: u32, outputs: u32, batch: u32) -> usize;
+    pub fn skl_gated_forward(ctx: *mut SklCtx, gate: *const SklDenseDesc, up: *const SklDenseDesc,
+                             input: *const c_void, in_rows: u32, in_cols: u32, batch: u32, out: *mut c_void,
+                             work: *mut c_void, work_bytes: usize) -> i32;
+    pub fn skl_gated_error_from_sum(ctx: *mut SklCtx, gate: *const SklDenseDesc, up: *const SklDenseDesc,
+                                    s: *const f32, batch: u32) -> i32;
+    pub fn skl_gated_hidden_error(ctx: *mut SklCtx, gate: *const SklDenseDesc, up: *const SklDenseDesc,
+                                  next: *const SklDenseDesc, batch: u32, work: *mut c_void,
+                                  work_bytes: usize) -> i32;
+    pub fn skl_gated_input_grad(ctx: *mut SklCtx, gate: *const SklDenseDesc, up: *const SklDenseDesc, batch: u32,
+                                dx: *mut f32, work: *mut c_void, work_bytes: usize) -> i32;
+    pub fn skl_product_work_bytes(dtype: u32, batch: u32, inputs: u32, outputs: u32, matrices: u32) -> usize;
+    pub fn skl_dense_forward_residual(ctx: *mut SklCtx, blk: *const SklDenseDesc, input: *const c_void,
+                                      in_rows: u32, in_cols: u32, batch: u32, use_dropout: u32, seed: u32,
+                                      stream_dtype: u32, scale: f32, x: *const c_void, h: *mut c_void,
+                                      work: *mut c_void, work_bytes: usize) -> i32;
+    pub fn skl_dense_residual_error(ctx: *mut SklCtx, blk: *const SklDenseDesc, dh: *const f32, batch: u32,
+                                    use_dropout: u32, seed: u32, scale: f32, dx: *mut f32) -> i32;
+    pub fn skl_dropout(ctx: *mut SklCtx, dtype: u32, rows: u32, cols: u32, p: f32, seed: u32,
+                       input: *const c_void, out: *mut c_void) -> i32;
 }

@@ -99,6 +99,20 @@ _SIGS = {
     "skl_dense_forward_mxfp4": (C.c_int32, [_VP, C.POINTER(SklDenseDesc), _VP, C.c_uint32, C.c_uint32,
                                             C.c_uint32, _VP, _VP, _VP, C.c_size_t]),
     "skl_mxfp4_work_bytes": (C.c_size_t, [C.c_uint32, C.c_uint32, C.c_uint32]),
+    "skl_gated_forward": (C.c_int32, [_VP, C.POINTER(SklDenseDesc), C.POINTER(SklDenseDesc), _VP, C.c_uint32,
+                                      C.c_uint32, C.c_uint32, _VP, _VP, C.c_size_t]),
+    "skl_gated_error_from_sum": (C.c_int32, [_VP, C.POINTER(SklDenseDesc), C.POINTER(SklDenseDesc), _VP, C.c_uint32]),
+    "skl_gated_hidden_error": (C.c_int32, [_VP, C.POINTER(SklDenseDesc), C.POINTER(SklDenseDesc),
+                                           C.POINTER(SklDenseDesc), C.c_uint32, _VP, C.c_size_t]),
+    "skl_gated_input_grad": (C.c_int32, [_VP, C.POINTER(SklDenseDesc), C.POINTER(SklDenseDesc), C.c_uint32, _VP, _VP,
+                                         C.c_size_t]),
+    "skl_product_work_bytes": (C.c_size_t, [C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32]),
+    "skl_dense_forward_residual": (C.c_int32, [_VP, C.POINTER(SklDenseDesc), _VP, C.c_uint32, C.c_uint32, C.c_uint32,
+                                               C.c_uint32, C.c_uint32, C.c_uint32, C.c_float, _VP, _VP, _VP,
+                                               C.c_size_t]),
+    "skl_dense_residual_error": (C.c_int32, [_VP, C.POINTER(SklDenseDesc), _VP, C.c_uint32, C.c_uint32, C.c_uint32,
+                                             C.c_float, _VP]),
+    "skl_dropout": (C.c_int32, [_VP, C.c_uint32, C.c_uint32, C.c_uint32, C.c_float, C.c_uint32, _VP, _VP]),
 }
 
 EXPORTED = tuple(_SIGS)
@@ -163,6 +177,30 @@ def need(name: str, t, dtype, shape: tuple, device: int) -> int:
         raise ValueError(f"{name}: a contiguous {dtype} tensor {list(shape)} on GPU {device} is wanted, "
                          f"got {t.dtype} {list(t.shape)} on {t.device}, strides {t.stride()}")
     return t.data_ptr()
+
+
+class Workspace:
+    """Device memory that the calls of one owner share: they follow each other on one stream.  It grows
+    on demand; smaller pieces stay (calls in flight and captured ones write there)."""
+
+    def __init__(self, ctx: "Context"):
+        self.device, self._pieces, self._sizes = ctx.device, [], {}
+
+    def get(self, size: int) -> tuple[int | None, int]:
+        """The address and size of a piece of at least `size` bytes."""
+        if not size:
+            return None, 0
+        if not self._pieces or self._pieces[-1].numel() < size:
+            import torch
+            self._pieces.append(torch.empty(size, device=f"cuda:{self.device}", dtype=torch.uint8))
+        return self._pieces[-1].data_ptr(), self._pieces[-1].numel()
+
+    def product(self, *sizes: int) -> tuple[int | None, int]:
+        """For skl_product_work_bytes(*sizes): dtype, batch, inputs, outputs, matrices."""
+        size = self._sizes.get(sizes)
+        if size is None:
+            size = self._sizes[sizes] = load().skl_product_work_bytes(*sizes)
+        return self.get(size) if size else (None, 0)
 
 
 class Context:

@@ -18,6 +18,7 @@
 
 #include "../../include/soklyn_hip.h"
 #include "distill.h"
+#include "ffn.h"
 #include "gemm_cost.h"
 #include "launch.h"
 #include "mxfp4.h"
@@ -591,6 +592,7 @@ GemmPlan plan_staged(const GemmLaunch &g) {
 struct PlanCtx {
     bool err, err_norm;        // hidden error, of a layer with a norm
     bool err_dma, err_wave;    // ... in the epilogue of the direct-to-LDS / K-splitting kernel
+    bool no_rag;               // operands that the direct-to-LDS kernel cannot take as stored
 };
 
 GemmPlan plan_route(const GemmLaunch &g, const GemmRoute &route) {
@@ -651,7 +653,7 @@ GemmPlan plan_gemm(const GemmLaunch &g, const GemmRoute &route, const PlanCtx &c
     // at most 16 columns: any larger tile is >90% padding; at most 16 k with the error in the
     // epilogue: the caller weighs it against the error kernel's own sum
     if (wave_ok && (g.N <= 16 || (g.K <= 16 && wave_err))) return wave;
-    const bool dma128_ok = plan_dma128(g, &dma128);
+    const bool dma128_ok = plan_dma128(g, &dma128) && !(c.no_rag && dma128.rag);
     if (dma128_ok) {
         const bool in_epilogue = c.err_dma && !dma128.rag;
         dma128.us = dma128_us(g, in_epilogue ? fused : w, dma128.rag) + (in_epilogue ? 0.0 : err);
@@ -2016,6 +2018,412 @@ int32_t skl_dense_forward_mxfp4(skl_ctx *ctx, const skl_dense_desc *b, const voi
         float *stats = n.norm == SKL_NORM_BATCH ? norm_scratch(ctx, norm_cols_scratch(n.m, n.n)) : nullptr;
         SKL_TRY(launch_norm_act(n, stats, ctx->norm.done, ctx->stream));
     }
+    return finish(ctx);
+}
+
+// ---- gated feed-forward blocks, the projection into the stream, dropout ---------------------
+
+namespace {
+
+size_t type_size(uint32_t dtype) { return dtype == SKL_F16 ? 2 : 4; }
+
+// What these operators check of a block alike.
+int32_t check_ffn_block(const skl_dense_desc *b) {
+    SKL_CHECK(b->dtype <= SKL_F16 && b->inputs > 0 && b->outputs > 0 && b->max_batch > 0, SKL_ERR_INVALID_CONFIGURATION);
+    SKL_CHECK(b->norm == SKL_NORM_DISABLED && b->act <= SKL_ACT_MISH && b->act != SKL_ACT_SOFTMAX,
+              SKL_ERR_INVALID_CONFIGURATION);
+    return SKL_OK;
+}
+
+int32_t check_gated(const skl_dense_desc *gate, const skl_dense_desc *up) {
+    int32_t r;
+    if ((r = check_ffn_block(gate)) || (r = check_ffn_block(up))) return r;
+    SKL_CHECK(gate->dtype == up->dtype && up->act == SKL_ACT_IDENTITY, SKL_ERR_INVALID_CONFIGURATION);
+    SKL_CHECK(gate->inputs == up->inputs && gate->outputs == up->outputs, SKL_ERR_MISMATCHED_DIMENSIONS);
+    return SKL_OK;
+}
+
+int32_t check_rows(const skl_dense_desc *b, uint32_t batch) {
+    SKL_CHECK(batch > 0, SKL_ERR_INVALID_BATCH_SIZE);
+    SKL_CHECK(batch <= b->max_batch, SKL_ERR_ALLOCATION_LIMIT);
+    return SKL_OK;
+}
+
+float leaky_of(const skl_dense_desc *b) { return b->act == SKL_ACT_LEAKY_RELU ? b->leaky : 0.0f; }
+
+// Copies of a product's operands zero-padded to the direct-to-LDS kernel's tiles, in the caller's
+// workspace.  parts: matrices side by side, along the output's columns for a pair and along k for a
+// chain, each padded for itself.
+struct Pads {
+    uint32_t mp, np, kp;      // as ProductLaunch's N and K: of one part
+    size_t a, b;              // bytes of one part's copy
+    uint32_t a_parts, b_parts;
+    size_t bytes(bool pad_a, bool pad_b) const { return (pad_a ? a * a_parts : 0) + (pad_b ? b * b_parts : 0); }
+};
+Pads product_pads(Product kind, uint32_t M, uint32_t N, uint32_t K) {
+    Pads p{};
+    p.mp = round_up(M, 256);
+    p.np = kind == Product::Pair ? round_up(N, 128) : round_up(N, 256);
+    p.kp = kind == Product::Chain ? round_up(K, 64) : round_up(K, 128);
+    p.a = (size_t)p.mp * p.kp * sizeof(half_t);
+    p.b = (size_t)p.np * p.kp * sizeof(half_t);
+    p.a_parts = kind == Product::Chain ? 2 : 1;
+    p.b_parts = kind == Product::Chain || kind == Product::Pair ? 2 : 1;
+    return p;
+}
+
+// The GEMM by which a product is planned: one of twice the columns (pair) or twice the k (chain).
+// Addresses stand for their alignment.
+GemmLaunch planned_gemm(const ProductLaunch &p) {
+    GemmLaunch g = p.g;
+    const bool two_b = p.kind == Product::Pair || p.kind == Product::Chain;
+    const void *b2 = p.kind == Product::Pair ? p.pair.b2 : p.chain.b2, *a2 = p.chain.a2;
+    auto both = [](const void *x, const void *y) {
+        return reinterpret_cast<const void *>(reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(y));
+    };
+    if (two_b) g.B = both(g.B, b2);
+    if (p.kind == Product::Chain) g.A = both(g.A, a2);
+    if (p.kind == Product::Pair) g.N *= 2;
+    if (p.kind == Product::Chain) g.K *= 2;
+    return g;
+}
+
+// Plans and launches a product whose g, kind and epilogue are set.  Copies go to the caller's work;
+// where it is too small for them another kernel runs that needs none.
+int32_t run_product(skl_ctx *ctx, ProductLaunch p, void *work, size_t work_bytes) {
+    const bool chain = p.kind == Product::Chain;
+    // offsets of the planned GEMM are 32-bit
+    SKL_CHECK(p.g.N <= 0x7fffffffu && p.g.K <= 0x7fffffffu, SKL_ERR_INVALID_CONFIGURATION);
+    const GemmLaunch g = planned_gemm(p);
+    PlanCtx how{};
+    how.no_rag = chain && p.g.K % 8 != 0;
+    GemmPlan plan = plan_gemm(g, ctx->route, how);
+    SKL_CHECK(!plan.refused && !plan.skinny && !(plan.rag && how.no_rag), SKL_ERR_INVALID_CONFIGURATION);
+    const Pads pads = product_pads(p.kind, p.g.M, p.g.N, p.g.K);
+    const bool staged = !plan.dma && !plan.wave;
+    if (staged || (plan.dma && !plan.rag && pads.bytes(plan.pad_a, plan.pad_b) > work_bytes)) {
+        SKL_CHECK(ctx->route.kind == Route::Planned, SKL_ERR_INVALID_CONFIGURATION);
+        GemmPlan other{};
+        uint32_t splits = 1;
+        double us = 0.0;
+        if (plan_dma128(g, &other) && !(how.no_rag && other.rag))
+            plan = other;
+        else
+            SKL_CHECK(plan_wave(g, gemm_wave_tile(g, &splits, &us), 0, 1, &plan), SKL_ERR_INVALID_CONFIGURATION);
+    }
+    p.g.time_start = ctx->gemm_start;
+    p.g.time_stop = ctx->gemm_stop;
+    p.dma = plan.dma;
+    p.g.rag = plan.rag;
+    if (!plan.dma) {
+        p.g.tile = plan.wave;
+        p.g.waves = plan.waves ? plan.waves : gemm_wave_waves(g, plan.wave);
+        SKL_CHECK(product_threads(p) <= 0xffffffffull, SKL_ERR_INVALID_CONFIGURATION);
+    } else {
+        p.g.tile = plan.tile;
+        p.g.mv = p.g.M;
+        p.g.nv = p.g.N;
+        char *at = reinterpret_cast<char *>(work);
+        auto pad = [&](const void *&src, uint32_t rows, uint32_t cols, uint32_t ld, uint32_t rows_p, uint32_t cols_p) {
+            const hipError_t e = launch_pad_h(src, rows, cols, ld, at, rows_p, cols_p, ctx->stream);
+            src = at;
+            at += (size_t)rows_p * cols_p * sizeof(half_t);
+            return e;
+        };
+        if (plan.pad_a) {
+            SKL_TRY(pad(p.g.A, p.g.M, p.g.K, p.g.lda, pads.mp, pads.kp));
+            if (chain) SKL_TRY(pad(p.chain.a2, p.g.M, p.g.K, p.g.lda, pads.mp, pads.kp));
+            p.g.lda = pads.kp;
+        }
+        if (plan.pad_b) {
+            // k-contiguous [N x K], or n-contiguous [K x N]
+            const uint32_t rows = p.g.b_kcontig ? p.g.N : p.g.K, cols = p.g.b_kcontig ? p.g.K : p.g.N;
+            const uint32_t rows_p = p.g.b_kcontig ? pads.np : pads.kp, cols_p = p.g.b_kcontig ? pads.kp : pads.np;
+            SKL_TRY(pad(p.g.B, rows, cols, p.g.ldb, rows_p, cols_p));
+            if (p.kind == Product::Pair) SKL_TRY(pad(p.pair.b2, rows, cols, p.g.ldb, rows_p, cols_p));
+            if (chain) SKL_TRY(pad(p.chain.b2, rows, cols, p.g.ldb, rows_p, cols_p));
+            p.g.ldb = cols_p;
+        }
+        if (!plan.rag) {   // whole tiles as they are, or padded
+            p.g.M = pads.mp;
+            p.g.N = pads.np;
+            p.g.K = pads.kp;
+        }
+    }
+    ctx->gemm_start = ctx->gemm_stop = nullptr;
+    SKL_TRY(launch_product(p, ctx->stream));
+    return SKL_OK;
+}
+
+GemmLaunch product_gemm(uint32_t dtype, Op op, uint32_t M, uint32_t N, uint32_t K, uint32_t lda, uint32_t ldb, const void *A,
+                        const void *B) {
+    GemmLaunch g{};
+    g.dtype = dtype;
+    g.M = M;
+    g.N = N;
+    g.K = K;
+    g.lda = lda;
+    g.ldb = ldb;
+    g.a_kcontig = true;
+    g.b_kcontig = op != Op::Fwd;
+    g.A = A;
+    g.B = B;
+    g.splits = 1;
+    g.op = op;
+    g.fwd.fuse_act = 1;   // (the planner's weight of an epilogue that does more than store)
+    return g;
+}
+
+int32_t check_work(const void *work) {
+    SKL_CHECK(aligned16(work), SKL_ERR_HARDWARE_CONSTRAINT);
+    return SKL_OK;
+}
+
+}  // namespace
+
+size_t skl_product_work_bytes(uint32_t dtype, uint32_t batch, uint32_t inputs, uint32_t outputs, uint32_t matrices) {
+    if (dtype != SKL_F16 || !batch || !inputs || !outputs || !matrices || matrices > 2) return 0;
+    // the direct-to-LDS kernel takes grids from 192 of its 256x256 tiles on; whole ones as they are
+    const uint64_t mp = ((uint64_t)batch + 255) / 256, np = ((uint64_t)outputs + 255) / 256;
+    if (mp * np * matrices < 192) return 0;
+    if (batch % 256 == 0 && inputs % 128 == 0 && outputs % 256 == 0) return 0;
+    const uint64_t kp = ((uint64_t)inputs + 127) / 128 * 128;
+    return (size_t)(mp + np) * 256 * kp * sizeof(half_t) * matrices;
+}
+
+int32_t skl_gated_forward(skl_ctx *ctx, const skl_dense_desc *gate, const skl_dense_desc *up, const void *in,
+                          uint32_t in_rows, uint32_t in_cols, uint32_t batch, void *out, void *work, size_t work_bytes) {
+    SKL_CHECK(ctx && gate && up, SKL_ERR_NULL_POINTER);
+    int32_t r;
+    if ((r = check_gated(gate, up))) return r;
+    if ((r = check_input(gate, in, in_rows, in_cols, batch))) return r;
+    if ((r = check_rows(gate, batch)) || (r = check_rows(up, batch))) return r;
+    SKL_CHECK(gate->w && up->w && out, SKL_ERR_NULL_POINTER);
+    if ((r = check_work(work))) return r;
+    const size_t t = type_size(gate->dtype), e = (size_t)batch * gate->outputs * t;
+    const size_t wb = (size_t)gate->inputs * gate->outputs * t, nb = gate->outputs * t;
+    const Span outs[] = {{out, e}, {gate->preact, e}, {up->preact, e}, {work, work ? work_bytes : 0}};
+    const Span ins[] = {{in, (size_t)batch * in_cols * t}, {gate->w, wb}, {up->w, wb}, {gate->b, nb}, {up->b, nb}};
+    SKL_CHECK(!spans_clash(outs, 4, ins, 5) && !outputs_clash(outs, 4), SKL_ERR_INVALID_CONFIGURATION);
+    if ((r = check_tile(ctx, gate))) return r;
+    if ((r = enter(ctx))) return r;
+    ProductLaunch p{};
+    p.kind = Product::Pair;
+    p.g = product_gemm(gate->dtype, Op::Fwd, batch, gate->outputs, gate->inputs, in_cols, gate->outputs, in, gate->w);
+    p.pair.b2 = up->w;
+    p.pair.bias = gate->b;
+    p.pair.bias2 = up->b;
+    p.pair.out = out;
+    p.pair.a = gate->preact;
+    p.pair.u = up->preact;
+    p.pair.act = gate->act;
+    p.pair.leaky = leaky_of(gate);
+    p.pair.ldc = gate->outputs;
+    if ((r = run_product(ctx, p, work, work ? work_bytes : 0))) return r;
+    return finish(ctx);
+}
+
+// What both errors of a gated block check and write; `s` stands for what the gradient comes from.
+static int32_t check_ungate(const skl_dense_desc *gate, const skl_dense_desc *up, uint32_t batch, const Span *from,
+                            size_t froms, const void *work, size_t work_bytes) {
+    SKL_CHECK(gate->is_training && up->is_training, SKL_ERR_TRAINING_MODE_REQUIRED);
+    int32_t r;
+    if ((r = check_rows(gate, batch)) || (r = check_rows(up, batch))) return r;
+    SKL_CHECK(gate->preact && up->preact && gate->d_prenorm && up->d_prenorm, SKL_ERR_NULL_POINTER);
+    const bool half = gate->dtype == SKL_F16;
+    SKL_CHECK(!half || (gate->d_prenorm_h && up->d_prenorm_h), SKL_ERR_NULL_POINTER);
+    const size_t e = (size_t)batch * gate->outputs, t = type_size(gate->dtype);
+    const Span outs[] = {{gate->d_prenorm, e * 4}, {up->d_prenorm, e * 4}, {half ? gate->d_prenorm_h : nullptr, e * 2},
+                         {half ? up->d_prenorm_h : nullptr, e * 2}, {work, work ? work_bytes : 0}};
+    const Span caches[] = {{gate->preact, e * t}, {up->preact, e * t}};
+    SKL_CHECK(!spans_clash(outs, 5, from, froms) && !spans_clash(outs, 5, caches, 2) && !outputs_clash(outs, 5),
+              SKL_ERR_INVALID_CONFIGURATION);
+    return SKL_OK;
+}
+
+static UngateEpi ungate_epi(const skl_dense_desc *gate, const skl_dense_desc *up) {
+    UngateEpi e{};
+    e.a = gate->preact;
+    e.u = up->preact;
+    e.d_gate = gate->d_prenorm;
+    e.d_up = up->d_prenorm;
+    if (gate->dtype == SKL_F16) {
+        e.d_gate_h = reinterpret_cast<half_t *>(gate->d_prenorm_h);
+        e.d_up_h = reinterpret_cast<half_t *>(up->d_prenorm_h);
+    }
+    e.act = gate->act;
+    e.leaky = leaky_of(gate);
+    e.ldc = gate->outputs;
+    return e;
+}
+
+int32_t skl_gated_error_from_sum(skl_ctx *ctx, const skl_dense_desc *gate, const skl_dense_desc *up, const float *s,
+                                 uint32_t batch) {
+    SKL_CHECK(ctx && gate && up && s, SKL_ERR_NULL_POINTER);
+    int32_t r;
+    if ((r = check_gated(gate, up))) return r;
+    const Span from[] = {{s, (size_t)batch * gate->outputs * 4}};
+    if ((r = check_ungate(gate, up, batch, from, 1, nullptr, 0))) return r;
+    if ((r = enter(ctx))) return r;
+    note_rewrite(ctx, gate);
+    note_rewrite(ctx, up);
+    ctx->cs.valid = false;
+    UngateArgs a{};
+    a.n = (uint64_t)batch * gate->outputs;
+    a.s = s;
+    a.e = ungate_epi(gate, up);
+    SKL_TRY(launch_ungate(a, gate->dtype, ctx->stream));
+    return finish(ctx);
+}
+
+int32_t skl_gated_hidden_error(skl_ctx *ctx, const skl_dense_desc *gate, const skl_dense_desc *up,
+                               const skl_dense_desc *next, uint32_t batch, void *work, size_t work_bytes) {
+    SKL_CHECK(ctx && gate && up && next, SKL_ERR_NULL_POINTER);
+    int32_t r;
+    if ((r = check_gated(gate, up))) return r;
+    SKL_CHECK(next->dtype == gate->dtype && next->outputs > 0, SKL_ERR_INVALID_CONFIGURATION);
+    SKL_CHECK(next->inputs == gate->outputs && next->max_batch >= batch, SKL_ERR_MISMATCHED_DIMENSIONS);
+    const void *dp = gate->dtype == SKL_F16 ? next->d_prenorm_h : next->d_prenorm;
+    SKL_CHECK(dp && next->w, SKL_ERR_NULL_POINTER);
+    if ((r = check_work(work))) return r;
+    const size_t t = type_size(gate->dtype);
+    const Span from[] = {{dp, (size_t)batch * next->outputs * t}, {next->w, (size_t)next->inputs * next->outputs * t}};
+    if ((r = check_ungate(gate, up, batch, from, 2, work, work_bytes))) return r;
+    if ((r = check_tile(ctx, gate))) return r;
+    if ((r = enter(ctx))) return r;
+    note_rewrite(ctx, gate);
+    note_rewrite(ctx, up);
+    ctx->cs.valid = false;
+    ProductLaunch p{};
+    p.kind = Product::Ungate;
+    p.g = product_gemm(gate->dtype, Op::InputGrad, batch, gate->outputs, next->outputs, next->outputs, next->outputs, dp,
+                       next->w);
+    p.ungate = ungate_epi(gate, up);
+    if ((r = run_product(ctx, p, work, work ? work_bytes : 0))) return r;
+    return finish(ctx);
+}
+
+int32_t skl_gated_input_grad(skl_ctx *ctx, const skl_dense_desc *gate, const skl_dense_desc *up, uint32_t batch, float *dx,
+                             void *work, size_t work_bytes) {
+    SKL_CHECK(ctx && gate && up && dx, SKL_ERR_NULL_POINTER);
+    int32_t r;
+    if ((r = check_gated(gate, up))) return r;
+    if ((r = check_rows(gate, batch)) || (r = check_rows(up, batch))) return r;
+    const bool half = gate->dtype == SKL_F16;
+    const void *dg = half ? gate->d_prenorm_h : gate->d_prenorm, *du = half ? up->d_prenorm_h : up->d_prenorm;
+    SKL_CHECK(dg && du && gate->w && up->w, SKL_ERR_NULL_POINTER);
+    if ((r = check_work(work))) return r;
+    const size_t t = type_size(gate->dtype), e = (size_t)batch * gate->outputs * t;
+    const size_t wb = (size_t)gate->inputs * gate->outputs * t;
+    const Span outs[] = {{dx, (size_t)batch * gate->inputs * 4}, {work, work ? work_bytes : 0}};
+    const Span ins[] = {{dg, e}, {du, e}, {gate->w, wb}, {up->w, wb}};
+    SKL_CHECK(!spans_clash(outs, 2, ins, 4) && !outputs_clash(outs, 2), SKL_ERR_INVALID_CONFIGURATION);
+    if ((r = check_tile(ctx, gate))) return r;
+    if ((r = enter(ctx))) return r;
+    ProductLaunch p{};
+    p.kind = Product::Chain;
+    p.g = product_gemm(gate->dtype, Op::InputGrad, batch, gate->inputs, gate->outputs, gate->outputs, gate->outputs, dg,
+                       gate->w);
+    p.chain.out = dx;
+    p.chain.a2 = du;
+    p.chain.b2 = up->w;
+    p.chain.ldc = gate->inputs;
+    if ((r = run_product(ctx, p, work, work ? work_bytes : 0))) return r;
+    return finish(ctx);
+}
+
+// A dropout probability is at least 0 and below 1 (NaN is neither).
+static bool drop_ok(float p) { return p >= 0.0f && p < 1.0f; }
+
+int32_t skl_dense_forward_residual(skl_ctx *ctx, const skl_dense_desc *b, const void *in, uint32_t in_rows,
+                                   uint32_t in_cols, uint32_t batch, uint32_t use_dropout, uint32_t seed,
+                                   uint32_t stream_dtype, float scale, const void *x, void *h, void *work,
+                                   size_t work_bytes) {
+    SKL_CHECK(ctx && b, SKL_ERR_NULL_POINTER);
+    int32_t r;
+    if ((r = check_ffn_block(b))) return r;
+    SKL_CHECK(stream_dtype <= b->dtype && std::isfinite(scale), SKL_ERR_INVALID_CONFIGURATION);
+    SKL_CHECK(!use_dropout || drop_ok(b->mask_coeff), SKL_ERR_INVALID_CONFIGURATION);
+    if ((r = check_input(b, in, in_rows, in_cols, batch))) return r;
+    if ((r = check_rows(b, batch))) return r;
+    SKL_CHECK(b->w && h, SKL_ERR_NULL_POINTER);
+    if ((r = check_work(work))) return r;
+    const size_t t = type_size(b->dtype), st = type_size(stream_dtype), e = (size_t)batch * b->outputs;
+    const Span outs[] = {{h, e * st}, {b->preact, e * t}, {work, work ? work_bytes : 0}};
+    const Span ins[] = {{x, e * st}, {in, (size_t)batch * in_cols * t}, {b->w, (size_t)b->inputs * b->outputs * t},
+                        {b->b, b->outputs * t}};
+    SKL_CHECK(!spans_clash(outs, 3, ins, 4, x) && !outputs_clash(outs, 3), SKL_ERR_INVALID_CONFIGURATION);
+    if ((r = check_tile(ctx, b))) return r;
+    if ((r = enter(ctx))) return r;
+    ProductLaunch p{};
+    p.kind = Product::Project;
+    p.stream_dtype = stream_dtype;
+    p.g = product_gemm(b->dtype, Op::Fwd, batch, b->outputs, b->inputs, in_cols, b->outputs, in, b->w);
+    p.project.bias = b->b;
+    p.project.x = x;
+    p.project.h = h;
+    p.project.preact = b->preact;
+    p.project.act = b->act;
+    p.project.leaky = leaky_of(b);
+    p.project.scale = scale;
+    p.project.ldc = b->outputs;
+    p.project.drop = drop_args(use_dropout != 0, b->mask_coeff, seed);
+    if ((r = run_product(ctx, p, work, work ? work_bytes : 0))) return r;
+    return finish(ctx);
+}
+
+int32_t skl_dense_residual_error(skl_ctx *ctx, const skl_dense_desc *b, const float *dh, uint32_t batch,
+                                 uint32_t use_dropout, uint32_t seed, float scale, float *dx) {
+    SKL_CHECK(ctx && b && dh, SKL_ERR_NULL_POINTER);
+    int32_t r;
+    if ((r = check_ffn_block(b))) return r;
+    SKL_CHECK(b->is_training, SKL_ERR_TRAINING_MODE_REQUIRED);
+    SKL_CHECK(std::isfinite(scale), SKL_ERR_INVALID_CONFIGURATION);
+    SKL_CHECK(!use_dropout || drop_ok(b->mask_coeff), SKL_ERR_INVALID_CONFIGURATION);
+    if ((r = check_rows(b, batch))) return r;
+    const bool half = b->dtype == SKL_F16;
+    SKL_CHECK(b->d_prenorm && (!half || b->d_prenorm_h), SKL_ERR_NULL_POINTER);
+    SKL_CHECK(b->act == SKL_ACT_IDENTITY || b->preact, SKL_ERR_NULL_POINTER);
+    const size_t e = (size_t)batch * b->outputs;
+    const Span outs[] = {{dx, e * 4}, {b->d_prenorm, e * 4}, {half ? b->d_prenorm_h : nullptr, e * 2}};
+    const Span ins[] = {{dh, e * 4}, {b->act == SKL_ACT_IDENTITY ? nullptr : b->preact, e * type_size(b->dtype)}};
+    SKL_CHECK(!spans_clash(outs, 3, ins, 2, dh) && !outputs_clash(outs, 3), SKL_ERR_INVALID_CONFIGURATION);
+    if ((r = enter(ctx))) return r;
+    note_rewrite(ctx, b);
+    ctx->cs.valid = false;
+    UnprojectArgs a{};
+    a.rows = batch;
+    a.cols = b->outputs;
+    a.dh = dh;
+    a.preact = b->preact;
+    a.d_prenorm = b->d_prenorm;
+    a.d_prenorm_h = half ? reinterpret_cast<half_t *>(b->d_prenorm_h) : nullptr;
+    a.dx = dx;
+    a.act = b->act;
+    a.leaky = leaky_of(b);
+    a.scale = scale;
+    a.drop = drop_args(use_dropout != 0, b->mask_coeff, seed);
+    SKL_TRY(launch_unproject(a, b->dtype, ctx->stream));
+    return finish(ctx);
+}
+
+int32_t skl_dropout(skl_ctx *ctx, uint32_t dtype, uint32_t rows, uint32_t cols, float p, uint32_t seed, const void *in,
+                    void *out) {
+    SKL_CHECK(ctx, SKL_ERR_NULL_POINTER);
+    SKL_CHECK(dtype <= SKL_F16 && drop_ok(p), SKL_ERR_INVALID_CONFIGURATION);
+    if (rows == 0 || cols == 0) return SKL_OK;
+    SKL_CHECK(in && out, SKL_ERR_NULL_POINTER);
+    const size_t e = (size_t)rows * cols * type_size(dtype);
+    SKL_CHECK(in == out || !overlaps(in, e, out, e), SKL_ERR_INVALID_CONFIGURATION);
+    int32_t r = enter(ctx);
+    if (r) return r;
+    DropoutArgs a{};
+    a.rows = rows;
+    a.cols = cols;
+    a.in = in;
+    a.out = out;
+    a.drop = drop_args(true, p, seed);
+    SKL_TRY(launch_dropout(a, dtype, ctx->stream));
     return finish(ctx);
 }
 

@@ -247,6 +247,7 @@ template <int NW, int NF, int MI = 32, int COLS = 256, bool RAG = false> struct 
     static constexpr int IPO = 64 / RPI / NW;
     static constexpr uint32_t KSB = P * (512 / MI);      // bytes per k-step (KSTEP k-rows)
     struct Frag { u32x2 v[NF][2]; };
+    static_assert(COLS != 64 || MI == 16, "rows of 64 columns: 16-row fragments");
     DmaSrc dma[2];                    // even / odd instructions (their swizzle differs for MI = 16, NW = 4)
     uint32_t step;                    // 2 NW k-rows per DMA instruction of a wave
     uint32_t kstep;                   // bytes per k-tile (64 k-rows)
@@ -254,7 +255,9 @@ template <int NW, int NF, int MI = 32, int COLS = 256, bool RAG = false> struct 
 
     // MI = 16 adds 2 ((r >> 3) & 1): the two 16-lane groups of a half-wave read
     // k-rows r and r + 8, which this moves to different banks
+    // (rows of 64 columns are half a bank row: rows r and r + 1 are apart already, r + 2 and r + 8 are moved)
     __device__ __forceinline__ static uint32_t swz(uint32_t r) {
+        if constexpr (COLS == 64) return (2u * ((r >> 1) & 1u)) ^ (4u * ((r >> 3) & 1u));
         return (4u * (r & 3u)) ^ (MI == 16 ? 2u * ((r >> 3) & 1u) : 0u);
     }
 
@@ -315,6 +318,65 @@ template <int NW, int NF, int MI = 32, int COLS = 256, bool RAG = false> struct 
     }
 };
 
+// Two m/n-contiguous operands of one tile (both projections of a gated block): the same columns of
+// each, half the tile's columns, one behind the other in LDS; fragments 0 .. NF / 2 - 1 are the
+// first's, the others the second's.
+template <class Op, int NF> struct OpPair {
+    static constexpr int H = NF / 2;
+    static constexpr int IPO = 2 * Op::IPO, RPF = Op::RPF;
+    struct Frag { typename Op::Frag a, b; };
+    Op a, b;
+    __device__ __forceinline__ void init(const half_t *p, const half_t *p2, uint32_t ld, uint32_t rows, uint32_t cols,
+                                         uint32_t mn0, uint32_t wbase, uint32_t wave, uint32_t lane, uint32_t lds_op) {
+        a.init(p, ld, rows, cols, mn0, wbase, wave, lane, lds_op);
+        b.init(p2, ld, rows, cols, mn0, wbase, wave, lane, lds_op + 64u * Op::P);
+    }
+    __device__ __forceinline__ void issue(int kt, int t, lds_char *dst) const {
+        if (t < Op::IPO)
+            a.issue(kt, t, dst);
+        else
+            b.issue(kt, t - Op::IPO, dst + 64u * Op::P);
+    }
+    __device__ __forceinline__ void read_frag(Frag &f, uint32_t stage_off, int ks, int i) const {
+        if (i < H)
+            a.read_frag(f.a, stage_off, ks, i);
+        else
+            b.read_frag(f.b, stage_off, ks, i - H);
+    }
+    __device__ __forceinline__ static u32x4 op(const Frag &f, int i) { return i < H ? Op::op(f.a, i) : Op::op(f.b, i - H); }
+    __device__ __forceinline__ static void pin_all(Frag &f) {
+        Op::pin_all(f.a);
+        Op::pin_all(f.b);
+    }
+};
+
+// A k-contiguous operand in two parts of k_part each, the second at an address of its own (the sum
+// of two products in one launch): k-tiles 0 .. tiles - 1 are the first's, the others the second's.
+// Which resource an instruction takes is scalar arithmetic on its k-tile.
+template <class Op> struct OpChain : Op {
+    __amdgpu_buffer_rsrc_t second;
+    int tiles;
+    __device__ __forceinline__ void init(const half_t *p, const half_t *p2, uint32_t ld, uint32_t rows, uint32_t k_part,
+                                         uint32_t mn0, uint32_t wbase, uint32_t wave, uint32_t lane, uint32_t lds_op) {
+        Op::init(p2, ld, rows, k_part, mn0, wbase, wave, lane, lds_op);
+        second = Op::dma.rsrc;
+        Op::init(p, ld, rows, k_part, mn0, wbase, wave, lane, lds_op);
+        tiles = (int)((k_part + 63u) / 64u);
+    }
+    __device__ __forceinline__ void issue(int kt, int t, lds_char *dst) const {
+        Op o = *this;
+        if (kt >= tiles) o.dma.rsrc = second;
+        o.issue(kt >= tiles ? kt - tiles : kt, t, dst);
+    }
+};
+
+// Epilogues of two products of one operand (kPair: the second's matrix is the parameters' b2) and of
+// the sum of two products (kChain: a2, b2).
+template <class E, class = void> struct EpiPair { static constexpr bool value = false; };
+template <class E> struct EpiPair<E, std::void_t<decltype(E::kPair)>> { static constexpr bool value = E::kPair; };
+template <class E, class = void> struct EpiChain { static constexpr bool value = false; };
+template <class E> struct EpiChain<E, std::void_t<decltype(E::kChain)>> { static constexpr bool value = E::kChain; };
+
 // Epilogues with running column sums (EpiErrK) declare kColSums, an Acc type,
 // finish(..., Acc &) and flush<NW>(), and run on whole tiles only; the others
 // have none.
@@ -372,6 +434,10 @@ template <bool KC, int NW, int NF, int MI, int R, bool RAG> struct DmaOpSel { ty
 template <int NW, int NF, int MI, int R, bool RAG> struct DmaOpSel<false, NW, NF, MI, R, RAG> {
     typedef OpN<NW, NF, MI, R, RAG> type;
 };
+// ... of an epilogue's second operand, and of either operand of a chain
+template <class Op, int NF, bool PAIR, bool CHAIN, class Half> struct DmaOpForm { typedef Op type; };
+template <class Op, int NF, class Half> struct DmaOpForm<Op, NF, true, false, Half> { typedef OpPair<Half, NF> type; };
+template <class Op, int NF, class Half> struct DmaOpForm<Op, NF, false, true, Half> { typedef OpChain<Op> type; };
 
 // Grid: (tiles, splits); each workgroup takes one (tile, split) pair (split-K grids
 // remap the pairs onto the XCDs, below).  Split y reduces k in [y k_per_split,
@@ -383,14 +449,22 @@ template <int NW, int NF, int MI, int R, bool RAG> struct DmaOpSel<false, NW, NF
 // rows on 4-byte boundaries): rows past an operand's end and k past K read as zero by the
 // resource's range check, columns past a row's end only reach outputs that are not stored;
 // only tiles that reach past the output go element by element.
+// A pair's tile is half as many output columns of each of its two matrices; a chain's K is the
+// length of each of its two parts (whole k-tiles but for RAG).
 template <class Epi, bool A_KC, bool B_KC, int NW, bool EDGE, int MI = 32, int BT = 256, bool RAG = false>
 __global__ void __launch_bounds__(64 * NW)
     __attribute__((amdgpu_waves_per_eu(DmaCfg<NW, MI, BT, BT>::WPE, DmaCfg<NW, MI, BT, BT>::WPE)))
     gemm_dma_kernel(GemmShape sh, const half_t *__restrict__ A, const half_t *__restrict__ B,
                     typename Epi::Params ep) {
     typedef DmaCfg<NW, MI, BT, BT> C;
-    typedef typename DmaOpSel<A_KC, NW, C::MT, MI, C::BM, RAG>::type OA;
-    typedef typename DmaOpSel<B_KC, NW, C::NTL, MI, C::BN, RAG>::type OB;
+    constexpr bool PAIR = EpiPair<Epi>::value, CHAIN = EpiChain<Epi>::value;
+    static_assert(!PAIR || (!B_KC && MI == 16), "a pair's matrices are n-contiguous");
+    static_assert(!CHAIN || (A_KC && B_KC), "a chain's operands are k-contiguous");
+    constexpr uint32_t TN = PAIR ? C::BN / 2 : C::BN;        // output columns of a tile
+    typedef typename DmaOpSel<A_KC, NW, C::MT, MI, C::BM, RAG>::type OA1;
+    typedef typename DmaOpSel<B_KC, NW, C::NTL, MI, C::BN, RAG>::type OB1;
+    typedef typename DmaOpForm<OA1, C::MT, false, CHAIN, void>::type OA;
+    typedef typename DmaOpForm<OB1, C::NTL, PAIR, CHAIN, OpN<NW, C::NTL / 2, MI, C::BN / 2, RAG>>::type OB;
     static_assert(!RAG || (EDGE && BT == 128), "operands as stored: 128x128 tiles with bounds");
     typedef DmaMma<MI> MM;
     static_assert(C::KS % 2 == 0, "k-steps alternate between two fragment sets");
@@ -428,16 +502,26 @@ __global__ void __launch_bounds__(64 * NW)
     } else {
         tile_coords(blockIdx.x, sh.tiles_m, sh.tiles_n, tm, tn);
     }
-    const uint32_t m0 = sh.m_base + tm * C::BM, n0 = tn * C::BN;
+    const uint32_t m0 = sh.m_base + tm * C::BM, n0 = tn * TN;
     const uint32_t kbeg = split * sh.k_per_split;
     const int kb = (int)(kbeg / C::BK);                                  // first k-tile of this split
-    const int nk = (int)((min(sh.K, kbeg + sh.k_per_split) - kbeg + (RAG ? C::BK - 1 : 0)) / C::BK);
+    const int nk = CHAIN ? 2 * (int)((sh.K + C::BK - 1) / C::BK)
+                         : (int)((min(sh.K, kbeg + sh.k_per_split) - kbeg + (RAG ? C::BK - 1 : 0)) / C::BK);
 
     const uint32_t lds0 = (uint32_t)(uintptr_t)lsm;   // LDS byte address of smem
     OA oa;
     OB ob;
-    oa.init(A, sh.lda, A_KC ? sh.M : sh.K, A_KC ? sh.K : sh.M, m0, wm * C::TWM, wave, lane, lds0);
-    ob.init(B, sh.ldb, B_KC ? sh.N : sh.K, B_KC ? sh.K : sh.N, n0, wn * C::TWN, wave, lane, lds0 + C::OPA);
+    if constexpr (CHAIN) {
+        oa.init(A, reinterpret_cast<const half_t *>(ep.a2), sh.lda, sh.M, sh.K, m0, wm * C::TWM, wave, lane, lds0);
+        ob.init(B, reinterpret_cast<const half_t *>(ep.b2), sh.ldb, sh.N, sh.K, n0, wn * C::TWN, wave, lane, lds0 + C::OPA);
+    } else {
+        oa.init(A, sh.lda, A_KC ? sh.M : sh.K, A_KC ? sh.K : sh.M, m0, wm * C::TWM, wave, lane, lds0);
+        if constexpr (PAIR)
+            ob.init(B, reinterpret_cast<const half_t *>(ep.b2), sh.ldb, sh.K, sh.N, n0, wn * C::TWN / 2, wave, lane,
+                    lds0 + C::OPA);
+        else
+            ob.init(B, sh.ldb, B_KC ? sh.N : sh.K, B_KC ? sh.K : sh.N, n0, wn * C::TWN, wave, lane, lds0 + C::OPA);
+    }
 
     auto issue = [&](int kt, int stage) {
         lds_char *st = lsm + stage * C::STAGEB + wave * 1024u;
@@ -692,6 +776,65 @@ __global__ void __launch_bounds__(64 * NW)
     }
     __syncthreads();
 
+    if constexpr (PAIR) {
+        // Both sums of an output element go through LDS, the first matrix's columns in front of the
+        // second's: a thread takes 8 columns of a row from each.
+        constexpr uint32_t L8 = TN / 8, R8 = 64 / L8;
+        static_assert(PROWS % (NW * R8) == 0, "rows of a pass");
+        float *E = reinterpret_cast<float *>(smem);
+        const uint32_t c8 = (lane % L8) * 8u, s8 = lane / L8;
+        const bool whole = !EDGE || (RAG && m0 + C::BM <= sh.mv && n0 + TN <= sh.nv && sh.whole);
+        typename Epi::Col8 col8{};
+        if (whole) col8 = Epi::column8(ep, n0 + c8);
+        constexpr int EQ = TN / 64;
+        typename Epi::Col1 col1[EQ];
+        if constexpr (EDGE) {
+#pragma unroll
+            for (int q = 0; q < EQ; ++q) {
+                const uint32_t n = n0 + lane + 64u * q;
+                col1[q] = n < sh.nv ? Epi::column1(ep, n) : typename Epi::Col1{};
+            }
+        }
+#pragma unroll
+        for (int pass = 0; pass < C::TWM / RPP; ++pass) {
+#pragma unroll
+            for (int ii = 0; ii < MTP; ++ii) {
+                const uint32_t r = wm * RPP + ii * 16 + (lane & 15u);
+#pragma unroll
+                for (int j = 0; j < C::NTL; ++j) {
+                    const uint32_t cc = (j < C::NTL / 2 ? 0u : TN) + wn * (C::TWN / 2) + (j % (C::NTL / 2)) * 16 + (lane >> 4) * 4;
+                    *reinterpret_cast<floatx4 *>(E + r * EPITCH + cc) = acc[pass * MTP + ii][j];
+                }
+            }
+            lds_barrier();
+            if (whole) {
+#pragma unroll 1
+                for (int b = 0; b < PROWS / (NW * (int)R8); ++b) {
+                    const uint32_t r = (wave + (uint32_t)NW * b) * R8 + s8;
+                    const uint32_t m = m0 + (r / RPP) * C::TWM + pass * RPP + r % RPP;
+                    const float *e = E + r * EPITCH + c8;
+                    Epi::finish8(ep, (uint64_t)m * Epi::ldc(ep) + n0 + c8, *reinterpret_cast<const floatx4 *>(e),
+                                 *reinterpret_cast<const floatx4 *>(e + 4), *reinterpret_cast<const floatx4 *>(e + TN),
+                                 *reinterpret_cast<const floatx4 *>(e + TN + 4), col8);
+                }
+            } else if constexpr (EDGE) {
+#pragma unroll 1
+                for (int b = 0; b < PROWS / NW; ++b) {
+                    const uint32_t r = wave + (uint32_t)NW * b;
+                    const uint32_t m = m0 + (r / RPP) * C::TWM + pass * RPP + r % RPP;
+                    if (m >= sh.mv) continue;
+#pragma unroll
+                    for (int q = 0; q < EQ; ++q) {
+                        const uint32_t cq = lane + 64u * q;
+                        if (n0 + cq < sh.nv) Epi::apply1(ep, m, n0 + cq, E[r * EPITCH + cq], E[r * EPITCH + TN + cq], col1[q]);
+                    }
+                }
+            }
+            if (pass + 1 < C::TWM / RPP) lds_barrier();
+        }
+        return;
+    } else {
+
     // Epilogue through LDS: passes of 128 rows (rows of accumulator block
     // i = pass * MTP + ii of both wave rows; two passes at 256 x 256, one at
     // 128 x 128).  A thread owns the fixed 4-column group c of the tile (a wave
@@ -830,6 +973,7 @@ __global__ void __launch_bounds__(64 * NW)
         const uint32_t nwg = gridDim.x * gridDim.y;
         for (uint32_t blk = blockIdx.x + gridDim.x * blockIdx.y; blk < ep.vec_blocks; blk += nwg)
             vec_opt_block<typename Epi::elem, 64 * NW>(ep.vec, blk);
+    }
     }
 }
 

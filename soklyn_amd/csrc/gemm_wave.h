@@ -438,16 +438,20 @@ __device__ __forceinline__ void wave_mfma(floatx4 (&acc)[MB][NB], const FA &fa, 
 
 // Grid: (tiles, splits); split y reduces k in [y k_per_split, (y + 1) k_per_split)
 // (k_per_split whole k-tiles).  WPE: waves per SIMD the registers are budgeted for.
+// A pair (both projections of a gated block) has its tile of each of two matrices; a chain (the sum
+// of two products) runs through the k-tiles of both, sh.K the length of each part.
 template <typename T, class Epi, bool A_KC, bool B_KC, bool REG, int MB, int NB, int W, int S, int WPE>
 __global__ void __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(WPE, WPE)))
     gemm_wave_kernel(GemmShape sh, const T *__restrict__ A, const T *__restrict__ B, typename Epi::Params ep) {
     typedef typename WaveOpSel<T, A_KC, 16 * MB, REG>::type OA;
     typedef typename WaveOpSel<T, B_KC, 16 * NB, REG>::type OB;
     static_assert(!REG || S == 1, "the register form keeps its next k-tile in registers");
+    constexpr bool PAIR = EpiPair<Epi>::value, CHAIN = EpiChain<Epi>::value;
+    constexpr int P = PAIR ? 2 : 1;                  // matrices, each with accumulators of its own
     constexpr uint32_t BM = 16 * MB, BN = 16 * NB, BKE = 128 / sizeof(T), NT = 64 * W;
-    constexpr uint32_t STAGE = (BM + BN) * 128;      // bytes per k-tile
-    constexpr int IPT = OA::IPO + OB::IPO;           // loads per k-tile
-    constexpr uint32_t EP = BN + 4;                  // floats per staged row
+    constexpr uint32_t STAGE = (BM + P * BN) * 128;  // bytes per k-tile
+    constexpr int IPT = OA::IPO + P * OB::IPO;       // loads per k-tile
+    constexpr uint32_t EP = P * BN + 4;              // floats per staged row
     constexpr uint32_t RING = W * S * STAGE, EPI = W * BM * EP * 4;
     __shared__ __attribute__((aligned(1024))) char smem[RING > EPI ? RING : EPI];
     lds_char *lsm = (lds_char *)(smem);
@@ -467,7 +471,8 @@ __global__ void __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(WPE
     const uint32_t m0 = tm * BM, n0 = tn * BN;
     const uint32_t kbeg = blockIdx.y * sh.k_per_split;
     const uint32_t kend = min(sh.K, kbeg + sh.k_per_split);
-    const uint32_t kt0 = wave, kt1 = (kend - kbeg + BKE - 1) / BKE;   // k-tiles of the slice
+    const uint32_t part = CHAIN ? (sh.K + BKE - 1) / BKE : 0;         // k-tiles of a chain's part
+    const uint32_t kt0 = wave, kt1 = CHAIN ? 2 * part : (kend - kbeg + BKE - 1) / BKE;   // k-tiles of the slice
 
     const uint32_t lds0 = (uint32_t)(uintptr_t)lsm + wave * (S * STAGE);
     OA oa;
@@ -476,14 +481,39 @@ __global__ void __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(WPE
     oa.init(A_KC ? A : A + (uint64_t)kbeg * sh.lda, sh.lda, sh.M, A_KC ? sh.K : kend - kbeg, m0, lane, lds0);
     ob.init(B_KC ? B : B + (uint64_t)kbeg * sh.ldb, sh.ldb, sh.N, B_KC ? sh.K : kend - kbeg, n0, lane, lds0 + BM * 128);
 
-    floatx4 acc[MB][NB];
-#pragma unroll
-    for (int i = 0; i < MB; ++i)
-#pragma unroll
-        for (int j = 0; j < NB; ++j) acc[i][j] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+    // a pair's second matrix, or the second part of a chain's operands
+    OA oa2;
+    OB ob2;
+    if constexpr (PAIR)
+        ob2.init(reinterpret_cast<const T *>(ep.b2), sh.ldb, sh.N, sh.K, n0, lane, lds0 + (BM + BN) * 128);
+    if constexpr (CHAIN) {
+        oa2.init(reinterpret_cast<const T *>(ep.a2), sh.lda, sh.M, sh.K, m0, lane, lds0);
+        ob2.init(reinterpret_cast<const T *>(ep.b2), sh.ldb, sh.N, sh.K, n0, lane, lds0 + BM * 128);
+    }
 
+    floatx4 acc[P][MB][NB];
+#pragma unroll
+    for (int p = 0; p < P; ++p)
+#pragma unroll
+        for (int i = 0; i < MB; ++i)
+#pragma unroll
+            for (int j = 0; j < NB; ++j) acc[p][i][j] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+
+    auto issue = [&](uint32_t kt, uint32_t stage) {
+        if constexpr (CHAIN) {
+            if (kt >= part) {
+                oa2.issue(kt - part, stage);
+                ob2.issue(kt - part, stage);
+                return;
+            }
+        }
+        oa.issue(kt, stage);
+        ob.issue(kt, stage);
+        if constexpr (PAIR) ob2.issue(kt, stage);
+    };
     // fragments of the k-tile in the stage, k past K zeroed where it is not by range
     auto frags = [&](auto &fa, auto &fb, uint32_t kt, uint32_t stage) {
+        if constexpr (CHAIN) kt = kt >= part ? kt - part : kt;
         fa.read(oa, stage);
         fb.read(ob, stage);
         if constexpr (A_KC) {
@@ -494,30 +524,38 @@ __global__ void __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(WPE
         }
     };
     if constexpr (REG) {
-        u32x4 ra[OA::IPO], rb[OB::IPO];
-        if (kt0 < kt1) {
-            oa.load(kt0, ra);
-            ob.load(kt0, rb);
-        }
+        u32x4 ra[OA::IPO], rb[OB::IPO], rb2[PAIR ? OB::IPO : 1];
+        auto load = [&](uint32_t kt) {
+            if constexpr (CHAIN) {
+                if (kt >= part) {
+                    oa2.load(kt - part, ra);
+                    ob2.load(kt - part, rb);
+                    return;
+                }
+            }
+            oa.load(kt, ra);
+            ob.load(kt, rb);
+            if constexpr (PAIR) ob2.load(kt, rb2);
+        };
+        if (kt0 < kt1) load(kt0);
         for (uint32_t kt = kt0; kt < kt1; kt += W) {
             oa.put(ra, lane);
             ob.put(rb, lane);
-            if (kt + W < kt1) {
-                oa.load(kt + W, ra);
-                ob.load(kt + W, rb);
-            }
+            if constexpr (PAIR) ob2.put(rb2, lane);
+            if (kt + W < kt1) load(kt + W);
             WaveFrags<T, A_KC, MB> fa;
             WaveFrags<T, B_KC, NB> fb;
             frags(fa, fb, kt, 0);   // a wave's LDS accesses complete in order
-            wave_mfma<MB, NB>(acc, fa, fb, T());
+            wave_mfma<MB, NB>(acc[0], fa, fb, T());
+            if constexpr (PAIR) {
+                fb.read(ob2, 0);
+                wave_mfma<MB, NB>(acc[1], fa, fb, T());
+            }
         }
     } else {
 #pragma unroll
         for (int s = 0; s < S; ++s)
-            if (kt0 + s * W < kt1) {
-                oa.issue(kt0 + s * W, s * STAGE);
-                ob.issue(kt0 + s * W, s * STAGE);
-            }
+            if (kt0 + s * W < kt1) issue(kt0 + s * W, s * STAGE);
         for (uint32_t kb = kt0; kb < kt1; kb += S * W) {
 #pragma unroll
             for (int s = 0; s < S; ++s) {
@@ -532,12 +570,12 @@ __global__ void __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(WPE
                 WaveFrags<T, A_KC, MB> fa;
                 WaveFrags<T, B_KC, NB> fb;
                 frags(fa, fb, kt, s * STAGE);
+                WaveFrags<T, B_KC, NB> fb2;
+                if constexpr (PAIR) fb2.read(ob2, s * STAGE);
                 __builtin_amdgcn_sched_barrier(0);
-                if (kt + S * W < kt1) {   // the stage is read: refill it
-                    oa.issue(kt + S * W, s * STAGE);
-                    ob.issue(kt + S * W, s * STAGE);
-                }
-                wave_mfma<MB, NB>(acc, fa, fb, T());
+                if (kt + S * W < kt1) issue(kt + S * W, s * STAGE);   // the stage is read: refill it
+                wave_mfma<MB, NB>(acc[0], fa, fb, T());
+                if constexpr (PAIR) wave_mfma<MB, NB>(acc[1], fa, fb2, T());
             }
         }
         wait_vmcnt<0>();
@@ -547,13 +585,45 @@ __global__ void __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(WPE
     // lane l of block (i, j): columns 4 (l / 16) .. + 3 of row l % 16
     float *E = reinterpret_cast<float *>(smem);
 #pragma unroll
-    for (int i = 0; i < MB; ++i)
+    for (int p = 0; p < P; ++p)
 #pragma unroll
-        for (int j = 0; j < NB; ++j)
-            *reinterpret_cast<floatx4 *>(E + (wave * BM + 16 * i + (lane & 15u)) * EP + 16 * j + 4 * (lane >> 4)) =
-                acc[i][j];
+        for (int i = 0; i < MB; ++i)
+#pragma unroll
+            for (int j = 0; j < NB; ++j)
+                *reinterpret_cast<floatx4 *>(E + (wave * BM + 16 * i + (lane & 15u)) * EP + p * BN + 16 * j +
+                                             4 * (lane >> 4)) = acc[p][i][j];
     lds_barrier();
-    if constexpr (EpiSums<Epi>::value) {
+    if constexpr (PAIR) {
+        if (sh.nv) {   // output rows on 4-element boundaries
+            for (uint32_t q = tid; q < BM * BN / 4; q += NT) {
+                const uint32_t r = q / (BN / 4), c = (q % (BN / 4)) * 4, m = m0 + r, n = n0 + c;
+                if (m >= sh.M || n >= sh.N) continue;
+                floatx4 g = *reinterpret_cast<const floatx4 *>(E + r * EP + c);
+                floatx4 u = *reinterpret_cast<const floatx4 *>(E + r * EP + BN + c);
+#pragma unroll
+                for (int w = 1; w < W; ++w) {
+                    g += *reinterpret_cast<const floatx4 *>(E + (w * BM + r) * EP + c);
+                    u += *reinterpret_cast<const floatx4 *>(E + (w * BM + r) * EP + BN + c);
+                }
+                Epi::finish(ep, (uint64_t)m * Epi::ldc(ep) + n, g, u, Epi::column(ep, n));   // ldc is whole groups
+            }
+        } else {
+            static_assert(NT % BN == 0, "one column per thread");
+            const uint32_t c = tid % BN, n = n0 + c;
+            if (n < sh.N) {
+                const typename Epi::Col1 col = Epi::column1(ep, n);
+                for (uint32_t r = tid / BN; r < BM && m0 + r < sh.M; r += NT / BN) {
+                    float g = E[r * EP + c], u = E[r * EP + BN + c];
+#pragma unroll
+                    for (int w = 1; w < W; ++w) {
+                        g += E[(w * BM + r) * EP + c];
+                        u += E[(w * BM + r) * EP + BN + c];
+                    }
+                    Epi::apply1(ep, m0 + r, n, g, u, col);
+                }
+            }
+        }
+    } else if constexpr (EpiSums<Epi>::value) {
         // the hidden error: 4 columns per lane (the launcher has checked their alignment), a
         // thread's group of columns fixed; the operands of up to 4 rows loaded before any use
         constexpr uint32_t QN = BM * BN / 4, GR = BN / 4, ACT = QN < NT ? QN : NT, ROWS = QN / ACT;

@@ -39,6 +39,9 @@ _READS = {
     "above": (("w", "d_prenorm", "d_prenorm_h"), ()),
     "update": (_UPDATE, _UPDATE_NORM),
     "hidden": (_UPDATE + ("predrop", "preact", "mask"), _UPDATE_NORM),
+    "project": (("w", "b", "preact"), ()),
+    "serve": (("w", "b"), ()),
+    "unproject": (("preact", "d_prenorm", "d_prenorm_h"), ()),
 }
 _SCALARS = tuple(n for n, _ in abi.SklDenseDesc._fields_[:11])
 _PTR_AT = {n: getattr(abi.SklDenseDesc, n).offset // 8 for n in abi.DESC_POINTERS}
@@ -127,6 +130,7 @@ class DeviceBlock:
         self.d_prenorm_h = zeros((M, N), torch.float16) if (half and is_training) else None
         self._desc = None
         self._local = threading.local()   # _fill's descriptors, one set per thread
+        self.work = abi.Workspace(ctx)    # of calls that are given none
 
     # -- descriptor -----------------------------------------------------------------
     def desc(self) -> abi.SklDenseDesc:
@@ -206,6 +210,30 @@ class DeviceBlock:
             out = torch.empty((batch, self.inputs), device=self.w.device, dtype=torch.float32)
         abi.call("skl_dense_input_grad", self.ctx.h, self._fill("input_grad"), batch, out.data_ptr())
         return out
+
+    def forward_residual(self, x: torch.Tensor, batch: int, stream: torch.Tensor | None, h: torch.Tensor, *,
+                         scale: float = 1.0, use_dropout: bool = False, seed: int = 0, keep: bool = True) -> torch.Tensor:
+        """h = scale * stream + drop(act(x W + b)), for a block without a norm; h may be stream, both [batch x
+        outputs] of fp32 (or fp16, fp16 blocks).  keep: the result in front of the activation stays in
+        preact, as residual_error reads it."""
+        rows, cols = x.shape
+        dev, wide, r = self.ctx.device, (batch, self.outputs), h.dtype
+        if r not in (torch.float32, self.tdtype):
+            raise ValueError(f"h: {torch.float32} or {self.tdtype} is wanted, got {r}")
+        work = self.work.product(int(self.half), batch, self.inputs, self.outputs, 1)
+        abi.call("skl_dense_forward_residual", self.ctx.h, self._fill("project" if keep else "serve"),
+                 abi.need("x", x, self.tdtype, (rows, cols), dev), rows, cols, batch, int(use_dropout), seed & 0xFFFFFFFF,
+                 int(r is torch.float16), scale, None if stream is None else abi.need("stream", stream, r, wide, dev),
+                 abi.need("h", h, r, wide, dev), *work)
+        return h
+
+    def residual_error(self, dh: torch.Tensor, batch: int, *, scale: float = 1.0, use_dropout: bool = False, seed: int = 0,
+                       dx: torch.Tensor | None = None):
+        """The block's error from dh (fp32), the gradient of forward_residual's h; dx = scale * dh where given."""
+        dev, wide = self.ctx.device, (batch, self.outputs)
+        abi.call("skl_dense_residual_error", self.ctx.h, self._fill("unproject"),
+                 abi.need("dh", dh, torch.float32, wide, dev), batch, int(use_dropout), seed & 0xFFFFFFFF, scale,
+                 None if dx is None else abi.need("dx", dx, torch.float32, wide, dev))
 
     # -- host views ----------------------------------------------------------------------
     def get(self, name: str) -> np.ndarray | None:

@@ -1,12 +1,20 @@
-"""Joins between the blocks of a residual network, over skl_residual_forward / _backward.
+"""Joins between the blocks of a residual network, over skl_residual_forward / _backward, and the
+projection into its stream, over skl_dense_forward_residual / skl_dense_residual_error.
 
     u = post(y);  h = scale * x + gate_act(gate) * u;  n = pre(h)
 
 `y` is the output of a block, `x` and `h` the residual stream before and behind it and `n` the
-input of the next block.  All calls run on the context's stream; tensors are contiguous and on
+input of the next block.
+
+    h = scale * stream + drop(act(x W + b))
+
+All calls run on the context's stream; tensors are contiguous and on
 its GPU, as for a DeviceBlock.
 """
 from __future__ import annotations
+
+import ctypes as C
+import threading
 
 import torch
 
@@ -109,3 +117,66 @@ class Join:
                            pdh, pdx, pdy, pdg, pdp, pw, size)
         if rc:
             raise abi.SklError("skl_residual_backward", rc)
+
+
+class Projection:
+    """A layer whose result, with dropout, is added to the stream: weights w [inputs x outputs] and bias b
+    [1 x outputs] (or None) of the blocks' type, held by reference.  No mask is stored: the backward draws
+    it again from the seed.  w may be None where only the backward is called.  Calls share a workspace and
+    follow each other on one stream."""
+
+    def __init__(self, ctx: abi.Context, w: torch.Tensor | None, b: torch.Tensor | None = None, *, outputs: int,
+                 half: bool = False, act: int = abi.ACT_IDENTITY, leaky: float = 0.0, dropout: float = 0.0,
+                 scale: float = 1.0):
+        self.ctx, self.outputs, self.half, self.act, self.leaky = ctx, outputs, half, act, leaky
+        self.dropout, self.scale = dropout, scale
+        self.dtype = torch.float16 if half else torch.float32
+        self.inputs = 1 if w is None else w.shape[0]
+        if w is not None:
+            abi.need("w", w, self.dtype, (self.inputs, outputs), ctx.device)
+        if b is not None:
+            abi.need("b", b, self.dtype, (1, outputs), ctx.device)
+        self.w, self.b, self.work = w, b, abi.Workspace(ctx)
+        self._local = threading.local()   # descriptors, one per thread
+
+    def _desc(self, rows: int) -> abi.SklDenseDesc:
+        d = getattr(self._local, "desc", None)
+        if d is None:
+            d = self._local.desc = abi.SklDenseDesc()
+            self._local.ref = C.byref(d)
+        d.dtype, d.inputs, d.outputs, d.max_batch = int(self.half), self.inputs, self.outputs, rows
+        d.act, d.leaky, d.mask_coeff, d.is_training = self.act, self.leaky, self.dropout, 1
+        d.w = None if self.w is None else self.w.data_ptr()
+        d.b = None if self.b is None else self.b.data_ptr()
+        return d
+
+    def forward(self, x: torch.Tensor, stream: torch.Tensor | None, h: torch.Tensor, *, preact: torch.Tensor | None = None,
+                seed: int = 0) -> torch.Tensor:
+        """h [rows x outputs] (fp32, or fp16 with fp16 layers) from x [rows x inputs] and the stream of h's type;
+        h may be stream.  preact [rows x outputs], where given, keeps x W + b for the backward."""
+        rows, dev, r = x.shape[0], self.ctx.device, h.dtype
+        wide = (rows, self.outputs)
+        if r is not torch.float32 and r is not self.dtype:
+            raise ValueError(f"h: {torch.float32} or {self.dtype} is wanted, got {r}")
+        d = self._desc(rows)
+        d.preact = None if preact is None else abi.need("preact", preact, self.dtype, wide, dev)
+        abi.call("skl_dense_forward_residual", self.ctx.h, self._local.ref,
+                 abi.need("x", x, self.dtype, (rows, self.inputs), dev), rows, self.inputs, rows, int(self.dropout != 0.0),
+                 seed & 0xFFFFFFFF, int(r is torch.float16), self.scale,
+                 None if stream is None else abi.need("stream", stream, r, wide, dev), abi.need("h", h, r, wide, dev),
+                 *self.work.product(int(self.half), rows, self.inputs, self.outputs, 1))
+        return h
+
+    def error(self, dh: torch.Tensor, preact: torch.Tensor | None, d_prenorm: torch.Tensor, *,
+              d_prenorm_h: torch.Tensor | None = None, dx: torch.Tensor | None = None, seed: int = 0):
+        """From dh (fp32), the gradient of h: that of x W + b in d_prenorm (fp32) and, for fp16 layers, its copy
+        d_prenorm_h; dx = scale * dh where given (it may be dh)."""
+        rows, dev, f32 = dh.shape[0], self.ctx.device, torch.float32
+        wide = (rows, self.outputs)
+        d = self._desc(rows)
+        d.preact = None if preact is None else abi.need("preact", preact, self.dtype, wide, dev)
+        d.d_prenorm = abi.need("d_prenorm", d_prenorm, f32, wide, dev)
+        d.d_prenorm_h = None if d_prenorm_h is None else abi.need("d_prenorm_h", d_prenorm_h, torch.float16, wide, dev)
+        abi.call("skl_dense_residual_error", self.ctx.h, self._local.ref, abi.need("dh", dh, f32, wide, dev), rows,
+                 int(self.dropout != 0.0), seed & 0xFFFFFFFF, self.scale,
+                 None if dx is None else abi.need("dx", dx, f32, wide, dev))
