@@ -184,7 +184,7 @@ class Workspace:
     on demand; smaller pieces stay (calls in flight and captured ones write there)."""
 
     def __init__(self, ctx: "Context"):
-        self.device, self._pieces, self._sizes = ctx.device, [], {}
+        self.ctx, self._pieces, self._sizes = ctx, [], {}
 
     def get(self, size: int) -> tuple[int | None, int]:
         """The address and size of a piece of at least `size` bytes."""
@@ -192,7 +192,7 @@ class Workspace:
             return None, 0
         if not self._pieces or self._pieces[-1].numel() < size:
             import torch
-            self._pieces.append(torch.empty(size, device=f"cuda:{self.device}", dtype=torch.uint8))
+            self._pieces.append(torch.empty(size, device=f"cuda:{self.ctx.device}", dtype=torch.uint8))
         return self._pieces[-1].data_ptr(), self._pieces[-1].numel()
 
     def product(self, *sizes: int) -> tuple[int | None, int]:

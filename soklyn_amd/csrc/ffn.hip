@@ -86,8 +86,8 @@ template <typename T, int V> __device__ __forceinline__ void ungate_at(const Ung
     for (int j = 0; j < V; ++j) {
         float v, d;
         ffn_act_slope<T>(a.e.act, g[j], a.e.leaky, v, d);
-        dg[j] = s[j] * u[j] * d;
-        du[j] = s[j] * v;
+        dg[j] = settled(s[j] * u[j] * d);
+        du[j] = settled(s[j] * v);
     }
     flat_store<float, V>(a.e.d_gate, i, dg);
     flat_store<float, V>(a.e.d_up, i, du);
@@ -123,6 +123,8 @@ template <typename T, int V> __device__ __forceinline__ void unproject_at(const 
 #pragma unroll
         for (int j = 0; j < V; ++j) d[j] = f[j] != 0.0f ? d[j] * f[j] : 0.0f;   // nothing passes a dropped element
     }
+#pragma unroll
+    for (int j = 0; j < V; ++j) d[j] = settled(d[j]);
     flat_store<float, V>(a.d_prenorm, i, d);
     if constexpr (sizeof(T) == 2) flat_store<half_t, V>(a.d_prenorm_h, i, d);
     if (a.dx) {

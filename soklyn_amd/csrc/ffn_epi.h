@@ -23,6 +23,13 @@ template <typename T> __device__ __forceinline__ void ffn_act_slope(uint32_t act
     d = activation_derivative<T>(act, 1.0f, v, z, leaky);
 }
 
+// A gradient as it is stored in fp32: without this its fp16 copy may be made from the product in front
+// of that rounding (one mixed-precision multiply), a step away from f16(gradient) now and then.
+__device__ __forceinline__ float settled(float v) {
+    asm("" : "+v"(v));
+    return v;
+}
+
 template <typename V> struct Vec4 { typedef f32x4 type; };
 template <> struct Vec4<half_t> { typedef f16x4 type; };
 template <typename T> __device__ __forceinline__ typename Vec4<T>::type load_nt(const void *p, uint64_t i) {
@@ -108,8 +115,8 @@ template <typename T> struct EpiUngateK {
         for (int j = 0; j < 4; ++j) {
             float v, d;
             ffn_act_slope<T>(e.act, (float)q.a[j], e.leaky, v, d);
-            dg[j] = s[j] * (float)q.u[j] * d;
-            du[j] = s[j] * v;
+            dg[j] = settled(s[j] * (float)q.u[j] * d);
+            du[j] = settled(s[j] * v);
         }
         __builtin_nontemporal_store(dg, reinterpret_cast<f32x4 *>(e.d_gate + idx));
         __builtin_nontemporal_store(du, reinterpret_cast<f32x4 *>(e.d_up + idx));
@@ -121,7 +128,7 @@ template <typename T> struct EpiUngateK {
     __device__ __forceinline__ static void one(const UngateEpi &e, uint64_t idx, float s) {
         float v, d;
         ffn_act_slope<T>(e.act, to_f32(ld_t<T>(e.a, idx)), e.leaky, v, d);
-        const float dg = s * to_f32(ld_t<T>(e.u, idx)) * d, du = s * v;
+        const float dg = settled(s * to_f32(ld_t<T>(e.u, idx)) * d), du = settled(s * v);
         e.d_gate[idx] = dg;
         e.d_up[idx] = du;
         if constexpr (sizeof(T) == 2) {

@@ -132,7 +132,8 @@ static hipError_t wave(const ProductLaunch &p, const typename Epi::Params &e, hi
             switch (code) {
             case 16 * 32 + 8: if constexpr (PAIR) return run_wave_t<T, Epi, BK, true, 1, 8, 1, 2>(p, e, s); break;
             case 16 * 32 + 16: if constexpr (!PAIR) return run_wave_t<T, Epi, BK, true, 1, 16, 1, 4>(p, e, s); break;
-            case 32 * 32 + 8: return run_wave_t<T, Epi, BK, true, 2, 8, 1, 4>(p, e, s);
+            // (a chain's two sets of addresses pass the registers of four waves to a SIMD)
+            case 32 * 32 + 8: return run_wave_t<T, Epi, BK, true, 2, 8, 1, EpiChain<Epi>::value ? 2 : 4>(p, e, s);
             case 64 * 32 + 4: return run_wave_t<T, Epi, BK, true, 4, 4, 1, 2>(p, e, s);
             }
             return hipErrorInvalidValue;
