@@ -734,6 +734,12 @@ __global__ void __launch_bounds__(64 * NW)
     }
     wait_vmcnt<0>();     // no DMA may land in the epilogue's staging area
     wait_lgkmcnt<0>();
+    // The last cross-barrier reads are in flight until here, into registers that nobody reads: used
+    // after the wait, or the compiler takes them as free and moves the epilogue's address arithmetic
+    // up into them, where a read that lands late overwrites it (a wild store).
+    OA::pin_all(fa[0]);
+    OB::pin_all(fb[0]);
+    __builtin_amdgcn_sched_barrier(0);
     if constexpr (AGPR_ASM) {
         // wait states before the epilogue's reads of the last MFMAs' accumulators (the
         // empty statements that claim to rewrite each accumulator keep those reads below)
