@@ -64,7 +64,7 @@ struct PadCopy {
 // instantiation, A/B comparisons): "staged", "dma", "dma128" (operands as stored), "skinny" or
 // "wave:TILE[:WAVES[:SLICES]]" (0: as planned).  A call whose GEMM that kernel does not take
 // fails, so a test that passes has run it.
-enum class Route : uint32_t { Planned, Staged, Dma, Dma128, Skinny, Wave };
+enum class Route : uint32_t { Planned, Staged, Dma, Dma128, Skinny, Wave, Copied };
 struct GemmRoute {
     Route kind;
     uint32_t tile, waves, splits;
@@ -592,7 +592,8 @@ GemmPlan plan_staged(const GemmLaunch &g) {
 struct PlanCtx {
     bool err, err_norm;        // hidden error, of a layer with a norm
     bool err_dma, err_wave;    // ... in the epilogue of the direct-to-LDS / K-splitting kernel
-    bool no_rag;               // operands that the direct-to-LDS kernel cannot take as stored
+    bool no_rag;               // not the direct-to-LDS kernel on operands as stored
+    bool heavy;                // an epilogue other than the store, about as dear as the hidden error's
 };
 
 GemmPlan plan_route(const GemmLaunch &g, const GemmRoute &route) {
@@ -604,6 +605,7 @@ GemmPlan plan_route(const GemmLaunch &g, const GemmRoute &route) {
     case Route::Dma: ok = plan_dma(g, Work::Store, &p, &us); break;
     case Route::Dma128: ok = plan_dma128(g, &p); break;
     case Route::Skinny: ok = plan_skinny(g, &p); break;
+    case Route::Copied: ok = false; break;   // the products that ffn.h has
     default:
         ok = plan_wave(g, route.tile, route.waves, g.op == Op::DwOpt && route.splits ? route.splits : 1, &p);
     }
@@ -618,7 +620,7 @@ GemmPlan plan_gemm(const GemmLaunch &g, const GemmRoute &route, const PlanCtx &c
     if (route.kind != Route::Planned) return plan_route(g, route);
     const bool dw = g.op == Op::DwOpt;
     const Work fused = c.err_norm ? Work::ErrNorm : Work::Err;
-    const Work w = dw ? Work::Dw : g.op == Op::Fwd ? Work::Fwd : Work::Store;
+    const Work w = dw ? Work::Dw : g.op == Op::Fwd ? Work::Fwd : c.heavy ? Work::Err : Work::Store;
     const double err = c.err ? err_us(g, c.err_norm) : 0.0;   // behind a stored sum
     const uint32_t t128 = ((g.M + 127) / 128) * ((g.N + 127) / 128);
     GemmPlan base{}, wave{}, skinny{}, dma128{};
@@ -672,6 +674,7 @@ void parse_route(const char *e, GemmRoute *r) {
     if (!strcmp(e, "dma")) r->kind = Route::Dma;
     if (!strcmp(e, "dma128")) r->kind = Route::Dma128;
     if (!strcmp(e, "skinny")) r->kind = Route::Skinny;
+    if (!strcmp(e, "copied")) r->kind = Route::Copied;
     unsigned t = 0, w = 0, sp = 0;
     if (sscanf(e, "wave:%u:%u:%u", &t, &w, &sp) >= 1) *r = GemmRoute{Route::Wave, t, w, sp};
 }
@@ -2051,25 +2054,40 @@ int32_t check_rows(const skl_dense_desc *b, uint32_t batch) {
 
 float leaky_of(const skl_dense_desc *b) { return b->act == SKL_ACT_LEAKY_RELU ? b->leaky : 0.0f; }
 
-// Copies of a product's operands zero-padded to the direct-to-LDS kernel's tiles, in the caller's
-// workspace.  parts: matrices side by side, along the output's columns for a pair and along k for a
-// chain, each padded for itself.
-struct Pads {
-    uint32_t mp, np, kp;      // as ProductLaunch's N and K: of one part
-    size_t a, b;              // bytes of one part's copy
+// Copies of a product's operands in the caller's workspace: zero-padded to whole 256x256 tiles (whole),
+// or only brought to rows of whole 16-byte pieces (for the direct-to-LDS kernel on operands as stored).
+// parts: matrices side by side, along the output's columns for a pair and along k for a chain, each
+// copied for itself.
+struct Copies {
+    bool a, b, whole;
+    uint32_t mp, np, kp;      // whole: the padded sizes (of one part)
+    uint32_t a_rows, a_cols, b_rows, b_cols;   // of a copy
     uint32_t a_parts, b_parts;
-    size_t bytes(bool pad_a, bool pad_b) const { return (pad_a ? a * a_parts : 0) + (pad_b ? b * b_parts : 0); }
+    size_t a_bytes() const { return (size_t)a_rows * a_cols * sizeof(half_t); }
+    size_t b_bytes() const { return (size_t)b_rows * b_cols * sizeof(half_t); }
+    size_t bytes() const { return (a ? a_bytes() * a_parts : 0) + (b ? b_bytes() * b_parts : 0); }
+    // the planner's price of a copy
+    double us() const {
+        return (a ? a_parts * (2.0 + 1e-6 * a_rows * a_cols) : 0.0) + (b ? b_parts * (2.0 + 1e-6 * b_rows * b_cols) : 0.0);
+    }
 };
-Pads product_pads(Product kind, uint32_t M, uint32_t N, uint32_t K) {
-    Pads p{};
-    p.mp = round_up(M, 256);
-    p.np = kind == Product::Pair ? round_up(N, 128) : round_up(N, 256);
-    p.kp = kind == Product::Chain ? round_up(K, 64) : round_up(K, 128);
-    p.a = (size_t)p.mp * p.kp * sizeof(half_t);
-    p.b = (size_t)p.np * p.kp * sizeof(half_t);
-    p.a_parts = kind == Product::Chain ? 2 : 1;
-    p.b_parts = kind == Product::Chain || kind == Product::Pair ? 2 : 1;
-    return p;
+Copies product_copies(const ProductLaunch &p, bool a, bool b, bool whole) {
+    const bool chain = p.kind == Product::Chain, pair = p.kind == Product::Pair, kc = p.g.b_kcontig;
+    Copies c{};
+    c.a = a;
+    c.b = b;
+    c.whole = whole;
+    c.mp = round_up(p.g.M, 256);
+    c.np = round_up(p.g.N, pair ? 128 : 256);
+    c.kp = round_up(p.g.K, chain ? 64 : 128);
+    const uint32_t k8 = round_up(p.g.K, 8), n8 = round_up(p.g.N, 8);
+    c.a_rows = whole ? c.mp : p.g.M;
+    c.a_cols = whole ? c.kp : k8;
+    c.b_rows = kc ? (whole ? c.np : p.g.N) : whole ? c.kp : k8;
+    c.b_cols = kc ? (whole ? c.kp : k8) : whole ? c.np : n8;
+    c.a_parts = chain ? 2 : 1;
+    c.b_parts = chain || pair ? 2 : 1;
+    return c;
 }
 
 // The GEMM by which a product is planned: one of twice the columns (pair) or twice the k (chain).
@@ -2088,6 +2106,39 @@ GemmLaunch planned_gemm(const ProductLaunch &p) {
     return g;
 }
 
+// fp16 operands that the direct-to-LDS kernel on 128x128 tiles cannot take as stored (odd rows, k in
+// part of a 16-byte piece): copies that it can, and the plan of the product over them.  False where
+// there are none, or they do not fit either.
+bool plan_copied(const ProductLaunch &p, Copies *c, GemmPlan *plan) {
+    if (p.g.dtype != SKL_F16 || !gemm_dma_enabled()) return false;
+    const GemmLaunch g = planned_gemm(p);
+    auto dword = [](const void *q, uint32_t ld) { return (reinterpret_cast<uintptr_t>(q) & 3u) == 0 && ld % 2 == 0; };
+    const bool k8 = p.g.K % 8 == 0;
+    *c = product_copies(p, !k8 || !dword(g.A, g.lda), (!k8 && g.b_kcontig) || !dword(g.B, g.ldb), false);
+    if (!k8 && !c->b) *c = product_copies(p, true, true, false);   // (k-rows past K have to be there: zeros)
+    if (!c->a && !c->b) return false;
+    ProductLaunch q = p;
+    const void *at = reinterpret_cast<const void *>(uintptr_t(256));
+    if (c->a) q.g.A = q.chain.a2 = at, q.g.lda = c->a_cols;
+    if (c->b) q.g.B = q.pair.b2 = q.chain.b2 = at, q.g.ldb = c->b_cols;
+    q.g.K = round_up(p.g.K, 8);
+    GemmPlan d{};
+    const GemmLaunch gq = planned_gemm(q);
+    if (!plan_dma128(gq, &d) || !d.rag) return false;
+    d.us = dma128_us(gq, gq.op == Op::Fwd ? Work::Fwd : Work::Store, true) + 1.44 * c->us();
+    *plan = d;
+    return true;
+}
+
+// Epilogues that read tensors of their own go element by element where the rows are not on 4 columns;
+// 128x128 tiles then need two workgroups to every CU to keep enough loads and stores in flight (from
+// the layer above, 2000 x 1531, K 1000: 32.6 us, 24.4 on the K-splitting kernel's 768 tiles; the
+// projection 38.7 and 32.3; 8000 x 2047, K 1531: 160 and 207).
+bool slow_rag(const ProductLaunch &p) {
+    const uint64_t tiles = (uint64_t)((p.g.M + 127) / 128) * ((p.g.N + 127) / 128);
+    return (p.kind == Product::Ungate || p.kind == Product::Project) && p.g.N % 4 != 0 && tiles < 512;
+}
+
 // Plans and launches a product whose g, kind and epilogue are set.  Copies go to the caller's work;
 // where it is too small for them another kernel runs that needs none.
 int32_t run_product(skl_ctx *ctx, ProductLaunch p, void *work, size_t work_bytes) {
@@ -2096,20 +2147,28 @@ int32_t run_product(skl_ctx *ctx, ProductLaunch p, void *work, size_t work_bytes
     SKL_CHECK(p.g.N <= 0x7fffffffu && p.g.K <= 0x7fffffffu, SKL_ERR_INVALID_CONFIGURATION);
     const GemmLaunch g = planned_gemm(p);
     PlanCtx how{};
-    how.no_rag = chain && p.g.K % 8 != 0;
-    GemmPlan plan = plan_gemm(g, ctx->route, how);
-    SKL_CHECK(!plan.refused && !plan.skinny && !(plan.rag && how.no_rag), SKL_ERR_INVALID_CONFIGURATION);
-    const Pads pads = product_pads(p.kind, p.g.M, p.g.N, p.g.K);
-    const bool staged = !plan.dma && !plan.wave;
-    if (staged || (plan.dma && !plan.rag && pads.bytes(plan.pad_a, plan.pad_b) > work_bytes)) {
-        SKL_CHECK(ctx->route.kind == Route::Planned, SKL_ERR_INVALID_CONFIGURATION);
-        GemmPlan other{};
-        uint32_t splits = 1;
-        double us = 0.0;
-        if (plan_dma128(g, &other) && !(how.no_rag && other.rag))
-            plan = other;
-        else
-            SKL_CHECK(plan_wave(g, gemm_wave_tile(g, &splits, &us), 0, 1, &plan), SKL_ERR_INVALID_CONFIGURATION);
+    how.heavy = p.kind == Product::Ungate;
+    how.no_rag = (chain && p.g.K % 8 != 0) || slow_rag(p);
+    GemmPlan plan = plan_gemm(g, ctx->route, how), other{};
+    Copies copies = product_copies(p, plan.pad_a, plan.pad_b, true), small{};
+    const bool planned = ctx->route.kind == Route::Planned, copied = ctx->route.kind == Route::Copied;
+    if ((planned || copied) && plan_copied(p, &small, &other) && small.bytes() <= work_bytes &&
+        (copied || (!slow_rag(p) && !plan.dma && other.us < ROUTE_MARGIN * plan.us))) {
+        plan = other;
+        copies = small;
+    } else {
+        SKL_CHECK(!copied && !plan.refused && !plan.skinny && !(plan.rag && chain && how.no_rag), SKL_ERR_INVALID_CONFIGURATION);
+        const bool staged = !plan.dma && !plan.wave;
+        if (staged || (plan.dma && !plan.rag && copies.bytes() > work_bytes)) {
+            SKL_CHECK(planned, SKL_ERR_INVALID_CONFIGURATION);
+            uint32_t splits = 1;
+            double us = 0.0;
+            if (plan_dma128(g, &other) && !(chain && how.no_rag && other.rag))
+                plan = other;
+            else
+                SKL_CHECK(plan_wave(g, gemm_wave_tile(g, &splits, &us), 0, 1, &plan), SKL_ERR_INVALID_CONFIGURATION);
+            copies = product_copies(p, plan.pad_a, plan.pad_b, true);
+        }
     }
     p.g.time_start = ctx->gemm_start;
     p.g.time_stop = ctx->gemm_stop;
@@ -2124,30 +2183,31 @@ int32_t run_product(skl_ctx *ctx, ProductLaunch p, void *work, size_t work_bytes
         p.g.mv = p.g.M;
         p.g.nv = p.g.N;
         char *at = reinterpret_cast<char *>(work);
-        auto pad = [&](const void *&src, uint32_t rows, uint32_t cols, uint32_t ld, uint32_t rows_p, uint32_t cols_p) {
+        auto copy = [&](const void *&src, uint32_t rows, uint32_t cols, uint32_t ld, uint32_t rows_p, uint32_t cols_p) {
             const hipError_t e = launch_pad_h(src, rows, cols, ld, at, rows_p, cols_p, ctx->stream);
             src = at;
             at += (size_t)rows_p * cols_p * sizeof(half_t);
             return e;
         };
-        if (plan.pad_a) {
-            SKL_TRY(pad(p.g.A, p.g.M, p.g.K, p.g.lda, pads.mp, pads.kp));
-            if (chain) SKL_TRY(pad(p.chain.a2, p.g.M, p.g.K, p.g.lda, pads.mp, pads.kp));
-            p.g.lda = pads.kp;
+        if (copies.a) {
+            SKL_TRY(copy(p.g.A, p.g.M, p.g.K, p.g.lda, copies.a_rows, copies.a_cols));
+            if (chain) SKL_TRY(copy(p.chain.a2, p.g.M, p.g.K, p.g.lda, copies.a_rows, copies.a_cols));
+            p.g.lda = copies.a_cols;
         }
-        if (plan.pad_b) {
+        if (copies.b) {
             // k-contiguous [N x K], or n-contiguous [K x N]
             const uint32_t rows = p.g.b_kcontig ? p.g.N : p.g.K, cols = p.g.b_kcontig ? p.g.K : p.g.N;
-            const uint32_t rows_p = p.g.b_kcontig ? pads.np : pads.kp, cols_p = p.g.b_kcontig ? pads.kp : pads.np;
-            SKL_TRY(pad(p.g.B, rows, cols, p.g.ldb, rows_p, cols_p));
-            if (p.kind == Product::Pair) SKL_TRY(pad(p.pair.b2, rows, cols, p.g.ldb, rows_p, cols_p));
-            if (chain) SKL_TRY(pad(p.chain.b2, rows, cols, p.g.ldb, rows_p, cols_p));
-            p.g.ldb = cols_p;
+            SKL_TRY(copy(p.g.B, rows, cols, p.g.ldb, copies.b_rows, copies.b_cols));
+            if (p.kind == Product::Pair) SKL_TRY(copy(p.pair.b2, rows, cols, p.g.ldb, copies.b_rows, copies.b_cols));
+            if (chain) SKL_TRY(copy(p.chain.b2, rows, cols, p.g.ldb, copies.b_rows, copies.b_cols));
+            p.g.ldb = copies.b_cols;
         }
         if (!plan.rag) {   // whole tiles as they are, or padded
-            p.g.M = pads.mp;
-            p.g.N = pads.np;
-            p.g.K = pads.kp;
+            p.g.M = copies.mp;
+            p.g.N = copies.np;
+            p.g.K = copies.kp;
+        } else if (copies.a || copies.b) {
+            p.g.K = round_up(p.g.K, 8);
         }
     }
     ctx->gemm_start = ctx->gemm_stop = nullptr;
@@ -2183,10 +2243,9 @@ int32_t check_work(const void *work) {
 
 size_t skl_product_work_bytes(uint32_t dtype, uint32_t batch, uint32_t inputs, uint32_t outputs, uint32_t matrices) {
     if (dtype != SKL_F16 || !batch || !inputs || !outputs || !matrices || matrices > 2) return 0;
-    // the direct-to-LDS kernel takes grids from 192 of its 256x256 tiles on; whole ones as they are
+    // few rows take the operands as they are; so do whole tiles
     const uint64_t mp = ((uint64_t)batch + 255) / 256, np = ((uint64_t)outputs + 255) / 256;
-    if (mp * np * matrices < 192) return 0;
-    if (batch % 256 == 0 && inputs % 128 == 0 && outputs % 256 == 0) return 0;
+    if (batch < 128 || (batch % 256 == 0 && inputs % 128 == 0 && outputs % 256 == 0)) return 0;
     const uint64_t kp = ((uint64_t)inputs + 127) / 128 * 128;
     return (size_t)(mp + np) * 256 * kp * sizeof(half_t) * matrices;
 }

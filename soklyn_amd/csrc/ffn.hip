@@ -82,12 +82,12 @@ template <typename T, int V> __device__ __forceinline__ void ungate_at(const Ung
     flat_load<float, V>(a.s, i, s);
     flat_load<T, V>(reinterpret_cast<const T *>(a.e.a), i, g);
     flat_load<T, V>(reinterpret_cast<const T *>(a.e.u), i, u);
+    float v[V], d[V];
+    ffn_act_slope<T>(a.e.act, g, a.e.leaky, v, d);
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-        float v, d;
-        ffn_act_slope<T>(a.e.act, g[j], a.e.leaky, v, d);
-        dg[j] = settled(s[j] * u[j] * d);
-        du[j] = settled(s[j] * v);
+        dg[j] = settled(s[j] * u[j] * d[j]);
+        du[j] = settled(s[j] * v[j]);
     }
     flat_store<float, V>(a.e.d_gate, i, dg);
     flat_store<float, V>(a.e.d_up, i, du);
@@ -110,12 +110,10 @@ template <typename T, int V> __device__ __forceinline__ void unproject_at(const 
     if (a.act) {
         float z[V];
         flat_load<T, V>(reinterpret_cast<const T *>(a.preact), i, z);
+        float v[V], slope[V];
+        ffn_act_slope<T>(a.act, z, a.leaky, v, slope);
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-            float v, slope;
-            ffn_act_slope<T>(a.act, z[j], a.leaky, v, slope);
-            d[j] *= slope;
-        }
+        for (int j = 0; j < V; ++j) d[j] *= slope[j];
     }
     if (a.drop.on) {
         float f[V];

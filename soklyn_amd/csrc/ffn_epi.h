@@ -14,13 +14,38 @@ namespace skl {
 
 // Activations of these operators, for both types from the hardware's exp2 and reciprocal but for
 // fp32 blocks' Mish; tanh by its series near 0 (tanhf is several times the work of the rest).
-template <typename T> __device__ __forceinline__ float ffn_act(uint32_t act, float z, float leaky) {
-    return act == 4 ? tanh_fast(z) : activation<T>(act, z, leaky);
+// N at a time: the choice of the activation outside the elements, whose chains of exp and reciprocal
+// then run beside each other.
+template <typename T, uint32_t ACT, bool SLOPE, int N>
+__device__ __forceinline__ void ffn_act_as(const float (&z)[N], float leaky, float (&v)[N], float (&d)[N]) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        v[j] = ACT == 4 ? tanh_fast(z[j]) : activation<T>(ACT, z[j], leaky);
+        if constexpr (SLOPE) d[j] = activation_derivative<T>(ACT, 1.0f, v[j], z[j], leaky);
+    }
 }
-// The activation's value and slope at z.
-template <typename T> __device__ __forceinline__ void ffn_act_slope(uint32_t act, float z, float leaky, float &v, float &d) {
-    v = ffn_act<T>(act, z, leaky);
-    d = activation_derivative<T>(act, 1.0f, v, z, leaky);
+template <typename T, bool SLOPE, int N>
+__device__ __forceinline__ void ffn_act_n(uint32_t act, const float (&z)[N], float leaky, float (&v)[N], float (&d)[N]) {
+    switch (act) {
+    case 1: return ffn_act_as<T, 1, SLOPE>(z, leaky, v, d);
+    case 2: return ffn_act_as<T, 2, SLOPE>(z, leaky, v, d);
+    case 3: return ffn_act_as<T, 3, SLOPE>(z, leaky, v, d);
+    case 4: return ffn_act_as<T, 4, SLOPE>(z, leaky, v, d);
+    case 6: return ffn_act_as<T, 6, SLOPE>(z, leaky, v, d);
+    case 7: return ffn_act_as<T, 7, SLOPE>(z, leaky, v, d);
+    default: return ffn_act_as<T, 0, SLOPE>(z, leaky, v, d);
+    }
+}
+// The activations of z in place, or its activations and slopes.
+template <typename T, int N> __device__ __forceinline__ void ffn_act(uint32_t act, float (&z)[N], float leaky) {
+    float v[N];
+    ffn_act_n<T, false>(act, z, leaky, v, v);
+#pragma unroll
+    for (int j = 0; j < N; ++j) z[j] = v[j];
+}
+template <typename T, int N>
+__device__ __forceinline__ void ffn_act_slope(uint32_t act, const float (&z)[N], float leaky, float (&v)[N], float (&d)[N]) {
+    ffn_act_n<T, true>(act, z, leaky, v, d);
 }
 
 // A gradient as it is stored in fp32: without this its fp16 copy may be made from the product in front
@@ -63,15 +88,11 @@ template <typename T> struct EpiPairK {
     __device__ __forceinline__ static Col8 column8(const PairEpi &e, uint32_t n) {
         return Col8{bias4(e.bias, n), bias4(e.bias, n + 4), bias4(e.bias2, n), bias4(e.bias2, n + 4)};
     }
-    __device__ __forceinline__ static f32x4 gated(const PairEpi &e, f32x4 a, f32x4 u) {
-        f32x4 o;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) o[j] = ffn_act<T>(e.act, a[j], e.leaky) * u[j];
-        return o;
-    }
     __device__ __forceinline__ static void finish(const PairEpi &e, uint64_t idx, floatx4 g, floatx4 u, const Col &c) {
         const f32x4 a = g + c.g, v = u + c.u;
-        store4_nt<T>(e.out, idx, gated(e, a, v));
+        float o[4] = {a[0], a[1], a[2], a[3]};
+        ffn_act<T>(e.act, o, e.leaky);
+        store4_nt<T>(e.out, idx, f32x4{o[0] * v[0], o[1] * v[1], o[2] * v[2], o[3] * v[3]});
         if (e.a) store4_nt<T>(e.a, idx, a);
         if (e.u) store4_nt<T>(e.u, idx, v);
     }
@@ -79,14 +100,19 @@ template <typename T> struct EpiPairK {
     __device__ __forceinline__ static void finish8(const PairEpi &e, uint64_t idx, floatx4 g0, floatx4 g1, floatx4 u0,
                                                    floatx4 u1, const Col8 &c) {
         const f32x4 a0 = g0 + c.g0, a1 = g1 + c.g1, v0 = u0 + c.u0, v1 = u1 + c.u1;
-        st8h_nt(e.out, idx, gated(e, a0, v0), gated(e, a1, v1));
+        float o[8] = {a0[0], a0[1], a0[2], a0[3], a1[0], a1[1], a1[2], a1[3]};
+        ffn_act<T>(e.act, o, e.leaky);
+        st8h_nt(e.out, idx, f32x4{o[0] * v0[0], o[1] * v0[1], o[2] * v0[2], o[3] * v0[3]},
+                f32x4{o[4] * v1[0], o[5] * v1[1], o[6] * v1[2], o[7] * v1[3]});
         if (e.a) st8h_nt(e.a, idx, a0, a1);
         if (e.u) st8h_nt(e.u, idx, v0, v1);
     }
     __device__ __forceinline__ static void apply1(const PairEpi &e, uint32_t m, uint32_t n, float g, float u, const Col1 &c) {
         const uint64_t idx = (uint64_t)m * e.ldc + n;
         const float a = g + c.g, v = u + c.u;
-        st_t<T>(e.out, idx, from_f32<T>(ffn_act<T>(e.act, a, e.leaky) * v));
+        float o[1] = {a};
+        ffn_act<T>(e.act, o, e.leaky);
+        st_t<T>(e.out, idx, from_f32<T>(o[0] * v));
         if (e.a) st_t<T>(e.a, idx, from_f32<T>(a));
         if (e.u) st_t<T>(e.u, idx, from_f32<T>(v));
     }
@@ -97,7 +123,9 @@ template <typename T> struct EpiPairK {
 template <typename T> struct EpiUngateK {
     typedef UngateEpi Params;
     typedef typename Vec4<T>::type V4;
+    static constexpr bool kReads = true;
     struct Pre { V4 a, u; };
+    struct Pre1 { T a, u; };
     struct Col {};
     struct Col1 {};
     __device__ __forceinline__ static uint32_t ldc(const UngateEpi &e) { return e.ldc; }
@@ -110,13 +138,14 @@ template <typename T> struct EpiUngateK {
     }
     __device__ __forceinline__ static void finish(const UngateEpi &e, uint64_t idx, uint32_t, uint32_t, floatx4 s, const Col &,
                                                   const Pre &q) {
+        const float a[4] = {(float)q.a[0], (float)q.a[1], (float)q.a[2], (float)q.a[3]};
+        float v[4], d[4];
+        ffn_act_slope<T>(e.act, a, e.leaky, v, d);
         f32x4 dg, du;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            float v, d;
-            ffn_act_slope<T>(e.act, (float)q.a[j], e.leaky, v, d);
-            dg[j] = settled(s[j] * (float)q.u[j] * d);
-            du[j] = settled(s[j] * v);
+            dg[j] = settled(s[j] * (float)q.u[j] * d[j]);
+            du[j] = settled(s[j] * v[j]);
         }
         __builtin_nontemporal_store(dg, reinterpret_cast<f32x4 *>(e.d_gate + idx));
         __builtin_nontemporal_store(du, reinterpret_cast<f32x4 *>(e.d_up + idx));
@@ -125,10 +154,16 @@ template <typename T> struct EpiUngateK {
             store4<half_t>(e.d_up_h, idx, du);
         }
     }
-    __device__ __forceinline__ static void one(const UngateEpi &e, uint64_t idx, float s) {
-        float v, d;
-        ffn_act_slope<T>(e.act, to_f32(ld_t<T>(e.a, idx)), e.leaky, v, d);
-        const float dg = settled(s * to_f32(ld_t<T>(e.u, idx)) * d), du = settled(s * v);
+    __device__ __forceinline__ static void load1(const UngateEpi &e, uint64_t idx, Pre1 &q) {
+        q.a = ld_t<T>(e.a, idx);
+        q.u = ld_t<T>(e.u, idx);
+    }
+    __device__ __forceinline__ static void finish1(const UngateEpi &e, uint64_t idx, uint32_t, uint32_t, float s, const Col1 &,
+                                                   const Pre1 &q) {
+        const float a[1] = {to_f32(q.a)};
+        float v[1], d[1];
+        ffn_act_slope<T>(e.act, a, e.leaky, v, d);
+        const float dg = settled(s * to_f32(q.u) * d[0]), du = settled(s * v[0]);
         e.d_gate[idx] = dg;
         e.d_up[idx] = du;
         if constexpr (sizeof(T) == 2) {
@@ -136,22 +171,11 @@ template <typename T> struct EpiUngateK {
             e.d_up_h[idx] = (half_t)du;
         }
     }
-    __device__ __forceinline__ static void apply1(const UngateEpi &e, uint32_t m, uint32_t n, float s, const Col1 &, uint32_t) {
-        one(e, (uint64_t)m * e.ldc + n, s);
-    }
-    __device__ __forceinline__ static void apply(const UngateEpi &e, const GemmShape &sh, uint32_t m, uint32_t n, floatx4 s,
-                                                 uint32_t) {
-        if (m >= sh.M) return;
+    __device__ __forceinline__ static void apply1(const UngateEpi &e, uint32_t m, uint32_t n, float s, const Col1 &c, uint32_t) {
         const uint64_t idx = (uint64_t)m * e.ldc + n;
-        if (n + 3 < sh.N) {
-            Pre q;
-            load(e, idx, m, q);
-            finish(e, idx, m, n, s, Col{}, q);
-            return;
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (n + j < sh.N) one(e, idx + j, s[j]);
+        Pre1 q;
+        load1(e, idx, q);
+        finish1(e, idx, m, n, s, c, q);
     }
 };
 
@@ -159,7 +183,9 @@ template <typename T> struct EpiUngateK {
 template <typename T, typename R> struct EpiProjectK {
     typedef ProjectEpi Params;
     typedef typename Vec4<R>::type V4;
+    static constexpr bool kReads = true;
     struct Pre { V4 x; };
+    struct Pre1 { R x; };
     struct Col { f32x4 bias; };
     struct Col1 { float bias; };
     __device__ __forceinline__ static uint32_t ldc(const ProjectEpi &e) { return e.ldc; }
@@ -181,9 +207,9 @@ template <typename T, typename R> struct EpiProjectK {
                                                   const Col &c, const Pre &q) {
         const f32x4 z = s + c.bias;
         if (e.preact) store4_nt<T>(e.preact, idx, z);
-        f32x4 v;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = ffn_act<T>(e.act, z[j], e.leaky);
+        float a[4] = {z[0], z[1], z[2], z[3]};
+        ffn_act<T>(e.act, a, e.leaky);
+        f32x4 v = {a[0], a[1], a[2], a[3]};
         if (e.drop.on) {
             const uint32_t rk = drop_rowkey(e.drop, m);
 #pragma unroll
@@ -195,28 +221,25 @@ template <typename T, typename R> struct EpiProjectK {
         }
         store4_nt<R>(e.h, idx, v);
     }
-    __device__ __forceinline__ static void apply1(const ProjectEpi &e, uint32_t m, uint32_t n, float s, const Col1 &c, uint32_t) {
-        const uint64_t idx = (uint64_t)m * e.ldc + n;
+    __device__ __forceinline__ static void load1(const ProjectEpi &e, uint64_t idx, Pre1 &q) {
+        q.x = e.x ? ld_t<R>(e.x, idx) : (R)0;
+    }
+    __device__ __forceinline__ static void finish1(const ProjectEpi &e, uint64_t idx, uint32_t m, uint32_t n, float s,
+                                                   const Col1 &c, const Pre1 &q) {
         const float z = s + c.bias;
         if (e.preact) st_t<T>(e.preact, idx, from_f32<T>(z));
-        float v = ffn_act<T>(e.act, z, e.leaky);
+        float a[1] = {z};
+        ffn_act<T>(e.act, a, e.leaky);
+        float v = a[0];
         if (e.drop.on) v = dropped(e, v, n * kDropColMul, drop_rowkey(e.drop, m));
-        if (e.x) v = fmaf(e.scale, to_f32(ld_t<R>(e.x, idx)), v);
+        if (e.x) v = fmaf(e.scale, to_f32(q.x), v);
         st_t<R>(e.h, idx, from_f32<R>(v));
     }
-    __device__ __forceinline__ static void apply(const ProjectEpi &e, const GemmShape &sh, uint32_t m, uint32_t n, floatx4 s,
-                                                 uint32_t) {
-        if (m >= sh.M) return;
-        if (n + 3 < sh.N) {
-            const uint64_t idx = (uint64_t)m * e.ldc + n;
-            Pre q;
-            load(e, idx, m, q);
-            finish(e, idx, m, n, s, column(e, n), q);
-            return;
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (n + j < sh.N) apply1(e, m, n + j, s[j], column1(e, n + j), 0);
+    __device__ __forceinline__ static void apply1(const ProjectEpi &e, uint32_t m, uint32_t n, float s, const Col1 &c, uint32_t) {
+        const uint64_t idx = (uint64_t)m * e.ldc + n;
+        Pre1 q;
+        load1(e, idx, q);
+        finish1(e, idx, m, n, s, c, q);
     }
 };
 

@@ -37,6 +37,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "device_math.h"
 
 namespace skl {
@@ -265,6 +267,25 @@ __device__ __forceinline__ void tile_coords(uint32_t wg, uint32_t tiles_m, uint3
     if ((total & 7u) == 0) t = (wg & 7u) * (total >> 3) + (wg >> 3);
     tile_coords_grouped(t, tiles_m, tiles_n, tm, tn);
 }
+
+// Epilogues of two products of one operand (kPair: the second's matrix is the parameters' b2) and of
+// the sum of two products (kChain: a2, b2).
+template <class E, class = void> struct EpiPair { static constexpr bool value = false; };
+template <class E> struct EpiPair<E, std::void_t<decltype(E::kPair)>> { static constexpr bool value = E::kPair; };
+template <class E, class = void> struct EpiChain { static constexpr bool value = false; };
+template <class E> struct EpiChain<E, std::void_t<decltype(E::kChain)>> { static constexpr bool value = E::kChain; };
+
+// Epilogues that read tensors of their own per element (kReads).
+template <class E, class = void> struct EpiReads { static constexpr bool value = false; };
+template <class E> struct EpiReads<E, std::void_t<decltype(E::kReads)>> { static constexpr bool value = E::kReads; };
+template <class E, bool READS> struct EpiReadsPre {
+    struct Pre {};
+    struct Pre1 {};
+};
+template <class E> struct EpiReadsPre<E, true> {
+    typedef typename E::Pre Pre;
+    typedef typename E::Pre1 Pre1;
+};
 
 // The K loop: double-buffered LDS, register prefetch one K-tile ahead,
 // unrolled by two so each half works on a compile-time buffer.

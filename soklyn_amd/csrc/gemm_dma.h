@@ -370,13 +370,6 @@ template <class Op> struct OpChain : Op {
     }
 };
 
-// Epilogues of two products of one operand (kPair: the second's matrix is the parameters' b2) and of
-// the sum of two products (kChain: a2, b2).
-template <class E, class = void> struct EpiPair { static constexpr bool value = false; };
-template <class E> struct EpiPair<E, std::void_t<decltype(E::kPair)>> { static constexpr bool value = E::kPair; };
-template <class E, class = void> struct EpiChain { static constexpr bool value = false; };
-template <class E> struct EpiChain<E, std::void_t<decltype(E::kChain)>> { static constexpr bool value = E::kChain; };
-
 // Epilogues with running column sums (EpiErrK) declare kColSums, an Acc type,
 // finish(..., Acc &) and flush<NW>(), and run on whole tiles only; the others
 // have none.
@@ -789,7 +782,7 @@ __global__ void __launch_bounds__(64 * NW)
         static_assert(PROWS % (NW * R8) == 0, "rows of a pass");
         float *E = reinterpret_cast<float *>(smem);
         const uint32_t c8 = (lane % L8) * 8u, s8 = lane / L8;
-        const bool whole = !EDGE || (RAG && m0 + C::BM <= sh.mv && n0 + TN <= sh.nv && sh.whole);
+        const bool whole = !EDGE || (m0 + C::BM <= sh.mv && n0 + TN <= sh.nv && sh.whole);
         typename Epi::Col8 col8{};
         if (whole) col8 = Epi::column8(ep, n0 + c8);
         constexpr int EQ = TN / 64;
@@ -864,8 +857,9 @@ __global__ void __launch_bounds__(64 * NW)
     shv.M = sh.mv;
     shv.N = sh.nv;
     const typename Epi::Params eps = Epi::at_split(ep, split);
-    // RAG: this tile lies inside the output and its rows are whole vectors
-    const bool whole = !EDGE || (RAG && m0 + C::BM <= shv.M && n0 + C::BN <= shv.N && sh.whole);
+    // this tile lies inside the output and its rows are whole vectors
+    constexpr bool READS = EpiReads<Epi>::value, BOUNDED = RAG || READS || CHAIN;
+    const bool whole = !EDGE || (BOUNDED && m0 + C::BM <= shv.M && n0 + C::BN <= shv.N && sh.whole);
     const typename Epi::Col col = whole ? Epi::column(eps, n0 + c) : typename Epi::Col{};
     // EDGE: lane l's columns n0 + l + 64 q, their per-column operands loaded once
     constexpr int EQ = C::BN / 64;
@@ -901,7 +895,44 @@ __global__ void __launch_bounds__(64 * NW)
             }
         }
         lds_barrier();
-        if constexpr (EDGE) if (!whole) {
+        if constexpr (EDGE && READS) if (!whole) {
+            // as below, the loads of UB rows issued before any of them is used
+            constexpr int UB = 4;
+            static_assert(PROWS / NW % UB == 0, "rows of a wave");
+#pragma unroll 1
+            for (int b0 = 0; b0 < PROWS / NW; b0 += UB) {
+                typename Epi::Pre1 pre[UB][EQ];
+                auto place = [&](int b, uint32_t &r) {
+                    r = wave + (uint32_t)NW * b;
+                    return m0 + (r / RPP) * C::TWM + pass * RPP + r % RPP;
+                };
+#pragma unroll
+                for (int u = 0; u < UB; ++u) {
+                    uint32_t r;
+                    const uint32_t m = place(b0 + u, r);
+#pragma unroll
+                    for (int q = 0; q < EQ; ++q) {
+                        const uint32_t n = n0 + lane + 64u * q;
+                        Epi::load1(ep, (uint64_t)min(m, shv.M - 1u) * Epi::ldc(ep) + min(n, shv.N - 1u), pre[u][q]);
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < UB; ++u) {
+                    uint32_t r;
+                    const uint32_t m = place(b0 + u, r);
+#pragma unroll
+                    for (int q = 0; q < EQ; ++q) {
+                        const uint32_t n = n0 + lane + 64u * q;
+                        if (m < shv.M && n < shv.N)
+                            Epi::finish1(ep, (uint64_t)m * Epi::ldc(ep) + n, m, n, E[r * EPITCH + lane + 64u * q], col1[q],
+                                         pre[u][q]);
+                    }
+                }
+            }
+            if (pass + 1 < C::TWM / RPP) lds_barrier();
+            continue;
+        }
+        if constexpr (EDGE && !READS) if (!whole) {
             // element by element, lane l taking columns l, l + 64, ... of the
             // row: each store instruction covers 64 consecutive columns
             // whatever the output's alignment; the per-column operands (bias)

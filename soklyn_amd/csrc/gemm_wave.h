@@ -436,6 +436,11 @@ __device__ __forceinline__ void wave_mfma(floatx4 (&acc)[MB][NB], const FA &fa, 
     }
 }
 
+// Epilogues that read tensors of their own per element (kReads) declare Pre, load, finish for 4 columns
+// and Pre1, load1, finish1 for one; their loads are issued before the tile's own (64x64 tiles: behind
+// the k loop), all at once for up to 4 groups or 8 elements of a thread, otherwise in batches of that many: one at a time, each behind
+// the stores of the last, they waited for HBM row by row (2000 x 1531, K 777, fp16: 45 us, LATER now).
+
 // Grid: (tiles, splits); split y reduces k in [y k_per_split, (y + 1) k_per_split)
 // (k_per_split whole k-tiles).  WPE: waves per SIMD the registers are budgeted for.
 // A pair (both projections of a gated block) has its tile of each of two matrices; a chain (the sum
@@ -490,6 +495,40 @@ __global__ void __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(WPE
         oa2.init(reinterpret_cast<const T *>(ep.a2), sh.lda, sh.M, sh.K, m0, lane, lds0);
         ob2.init(reinterpret_cast<const T *>(ep.b2), sh.ldb, sh.N, sh.K, n0, lane, lds0 + BM * 128);
     }
+
+    // the epilogue's own operands of the thread's first rows
+    constexpr bool READS = EpiReads<Epi>::value;
+    constexpr uint32_t QN4 = BM * BN / 4, ACT4 = QN4 < NT ? QN4 : NT, U4 = QN4 / ACT4, B4 = U4 < 4 ? U4 : 4;
+    constexpr uint32_t U1 = BM * BN > NT ? BM * BN / NT : 1, B1 = U1 < 8 ? U1 : 8;
+    typename EpiReadsPre<Epi, READS>::Pre pre4[READS ? B4 : 1];
+    typename EpiReadsPre<Epi, READS>::Pre1 pre1[READS ? B1 : 1];
+    auto load4 = [&](uint32_t u0) {
+        if constexpr (READS) {
+#pragma unroll
+            for (uint32_t u = 0; u < B4; ++u) {
+                const uint32_t q = tid + (u0 + u) * ACT4, m = m0 + q / (BN / 4), n = n0 + (q % (BN / 4)) * 4;
+                // (past the edges the last rows and columns again: no branch between the loads)
+                Epi::load(ep, (uint64_t)min(m, sh.M - 1u) * Epi::ldc(ep) + min(n, sh.N - 4u), m, pre4[u]);
+            }
+        }
+    };
+    auto load1 = [&](uint32_t u0) {
+        if constexpr (READS) {
+#pragma unroll
+            for (uint32_t u = 0; u < B1; ++u) {
+                const uint32_t r = tid / BN + (u0 + u) * (NT / BN), m = m0 + r, n = n0 + tid % BN;
+                Epi::load1(ep, (uint64_t)min(m, sh.M - 1u) * Epi::ldc(ep) + min(n, sh.N - 1u), pre1[u]);
+            }
+        }
+    };
+    auto load_first = [&] {
+        if (sh.nv)
+            load4(0);
+        else
+            load1(0);
+    };
+    constexpr bool EARLY = READS && !REG && MB <= 2;   // 64x64 tiles and the register form have no registers to spare
+    if constexpr (EARLY) load_first();
 
     floatx4 acc[P][MB][NB];
 #pragma unroll
@@ -580,6 +619,7 @@ __global__ void __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(WPE
         }
         wait_vmcnt<0>();
     }
+    if constexpr (READS && !EARLY) load_first();
     lds_barrier();   // every wave is done with its ring: the partial tiles go over it
 
     // lane l of block (i, j): columns 4 (l / 16) .. + 3 of row l % 16
@@ -620,6 +660,39 @@ __global__ void __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(WPE
                         u += E[(w * BM + r) * EP + BN + c];
                     }
                     Epi::apply1(ep, m0 + r, n, g, u, col);
+                }
+            }
+        }
+    } else if constexpr (READS) {
+        if (sh.nv) {
+#pragma unroll 1
+            for (uint32_t u0 = 0; u0 < U4; u0 += B4) {
+                if (u0) load4(u0);
+#pragma unroll
+                for (uint32_t u = 0; u < B4; ++u) {
+                    const uint32_t q = tid + (u0 + u) * ACT4, r = q / (BN / 4), c = (q % (BN / 4)) * 4, m = m0 + r, n = n0 + c;
+                    if (tid >= ACT4 || m >= sh.M || n >= sh.N) continue;
+                    floatx4 v = *reinterpret_cast<const floatx4 *>(E + r * EP + c);
+#pragma unroll 4
+                    for (int w = 1; w < W; ++w) v += *reinterpret_cast<const floatx4 *>(E + (w * BM + r) * EP + c);
+                    Epi::finish(ep, (uint64_t)m * Epi::ldc(ep) + n, m, n, v, Epi::column(ep, n), pre4[u]);   // whole groups
+                }
+            }
+        } else {
+            static_assert(NT % BN == 0, "one column per thread");
+            const uint32_t c = tid % BN, n = n0 + c;
+            const typename Epi::Col1 col = n < sh.N ? Epi::column1(ep, n) : typename Epi::Col1{};
+#pragma unroll 1
+            for (uint32_t u0 = 0; u0 < U1; u0 += B1) {
+                if (u0) load1(u0);
+#pragma unroll
+                for (uint32_t u = 0; u < B1; ++u) {
+                    const uint32_t r = tid / BN + (u0 + u) * (NT / BN), m = m0 + r;
+                    if (r >= BM || m >= sh.M || n >= sh.N) continue;
+                    float v = E[r * EP + c];
+#pragma unroll
+                    for (int w = 1; w < W; ++w) v += E[(w * BM + r) * EP + c];
+                    Epi::finish1(ep, (uint64_t)m * Epi::ldc(ep) + n, m, n, v, col, pre1[u]);
                 }
             }
         }
