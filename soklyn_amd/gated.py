@@ -34,24 +34,31 @@ class Gated:
             if w is not None:
                 abi.need(name, w, t, shape, ctx.device)
         self.wg, self.wu, self.bg, self.bu, self.work = wg, wu, bg, bu, abi.Workspace(ctx)
+        lib = abi.load()
+        self._call = lib.skl_gated_forward, lib.skl_gated_error_from_sum, lib.skl_gated_hidden_error, lib.skl_gated_input_grad
         self._local = threading.local()   # descriptors, one set per thread
 
     def _descs(self, rows: int):
         """This thread's descriptors of gate, up and the layer above, with the weights as they are now."""
         own = self._local.__dict__
-        if not own:
-            own["d"] = d = (abi.SklDenseDesc(), abi.SklDenseDesc(), abi.SklDenseDesc())
-            own["refs"] = tuple(C.byref(x) for x in d)
-            for x in d:
-                x.is_training = 1
+        key = rows, self.inputs, self.outputs, self.half, self.act, self.leaky
+        if own.get("key") != key:
+            if not own:
+                own["d"] = tuple(abi.SklDenseDesc() for _ in range(3))
+                own["refs"] = tuple(C.byref(x) for x in own["d"])
+            for d in own["d"]:
+                d.is_training, d.dtype, d.inputs, d.outputs, d.max_batch = 1, int(self.half), self.inputs, self.outputs, rows
+            own["d"][0].act, own["d"][0].leaky = self.act, self.leaky
+            own["key"] = key
         gate, up, above = own["d"]
-        half = int(self.half)
         for d, w, b in ((gate, self.wg, self.bg), (up, self.wu, self.bu)):
-            d.dtype, d.inputs, d.outputs, d.max_batch = half, self.inputs, self.outputs, rows
-            d.w = None if w is None else w.data_ptr()
+            if w is not None:
+                d.w = w.data_ptr()
             d.b = None if b is None else b.data_ptr()
-        gate.act, gate.leaky = self.act, self.leaky
         return gate, up, above, own["refs"]
+
+    def _work(self, *sizes):
+        return self.work.product(1, *sizes) if self.half else (None, 0)   # fp32 operands are taken as they are
 
     def _at(self, name, t, dtype, shape):
         return None if t is None else abi.need(name, t, dtype, shape, self.ctx.device)
@@ -64,8 +71,10 @@ class Gated:
         wide = (rows, self.outputs)
         gate, up, _, (rg, ru, _) = self._descs(rows)
         gate.preact, up.preact = self._at("a", a, t, wide), self._at("u", u, t, wide)
-        abi.call("skl_gated_forward", self.ctx.h, rg, ru, self._at("x", x, t, (rows, self.inputs)), rows, self.inputs, rows,
-                 self._at("out", out, t, wide), *self.work.product(int(self.half), rows, self.inputs, self.outputs, 2))
+        rc = self._call[0](self.ctx.h, rg, ru, self._at("x", x, t, (rows, self.inputs)), rows, self.inputs, rows,
+                           self._at("out", out, t, wide), *self._work(rows, self.inputs, self.outputs, 2))
+        if rc:
+            raise abi.SklError("skl_gated_forward", rc)
         return out
 
     def _errors(self, rows, a, u, dg, du, dg_h, du_h):
@@ -83,7 +92,9 @@ class Gated:
         of out, and the kept a and u."""
         rows = s.shape[0]
         _, (rg, ru, _) = self._errors(rows, a, u, dg, du, dg_h, du_h)
-        abi.call("skl_gated_error_from_sum", self.ctx.h, rg, ru, self._at("s", s, _F32, (rows, self.outputs)), rows)
+        rc = self._call[1](self.ctx.h, rg, ru, self._at("s", s, _F32, (rows, self.outputs)), rows)
+        if rc:
+            raise abi.SklError("skl_gated_error_from_sum", rc)
 
     def hidden_error(self, above_d: torch.Tensor, above_w: torch.Tensor, a: torch.Tensor, u: torch.Tensor, *,
                      dg: torch.Tensor, du: torch.Tensor, dg_h: torch.Tensor | None = None,
@@ -92,12 +103,13 @@ class Gated:
         blocks' type."""
         (rows, n), t = above_d.shape, self.dtype
         above, (rg, ru, rn) = self._errors(rows, a, u, dg, du, dg_h, du_h)
-        above.dtype, above.inputs, above.outputs, above.max_batch = int(self.half), self.outputs, n, rows
+        above.inputs, above.outputs = self.outputs, n
         above.w = self._at("above_w", above_w, t, (self.outputs, n))
         d = self._at("above_d", above_d, t, (rows, n))
         above.d_prenorm, above.d_prenorm_h = (None, d) if self.half else (d, None)
-        abi.call("skl_gated_hidden_error", self.ctx.h, rg, ru, rn, rows,
-                 *self.work.product(int(self.half), rows, n, self.outputs, 1))
+        rc = self._call[2](self.ctx.h, rg, ru, rn, rows, *self._work(rows, n, self.outputs, 1))
+        if rc:
+            raise abi.SklError("skl_gated_hidden_error", rc)
 
     def input_grad(self, dg: torch.Tensor, du: torch.Tensor, dx: torch.Tensor) -> torch.Tensor:
         """dx [rows x inputs] (fp32) from the gradients of both projections' results, of the blocks' type."""
@@ -106,8 +118,10 @@ class Gated:
         for d, g, n in ((gate, dg, "dg"), (up, du, "du")):
             p = self._at(n, g, t, (rows, self.outputs))
             d.d_prenorm, d.d_prenorm_h = (None, p) if half else (p, None)
-        abi.call("skl_gated_input_grad", self.ctx.h, rg, ru, rows, self._at("dx", dx, _F32, (rows, self.inputs)),
-                 *self.work.product(int(half), rows, self.outputs, self.inputs, 2))
+        rc = self._call[3](self.ctx.h, rg, ru, rows, self._at("dx", dx, _F32, (rows, self.inputs)),
+                           *self._work(rows, self.outputs, self.inputs, 2))
+        if rc:
+            raise abi.SklError("skl_gated_input_grad", rc)
         return dx
 
 

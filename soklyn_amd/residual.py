@@ -137,16 +137,21 @@ class Projection:
         if b is not None:
             abi.need("b", b, self.dtype, (1, outputs), ctx.device)
         self.w, self.b, self.work = w, b, abi.Workspace(ctx)
+        self._call = abi.load().skl_dense_forward_residual, abi.load().skl_dense_residual_error
         self._local = threading.local()   # descriptors, one per thread
 
     def _desc(self, rows: int) -> abi.SklDenseDesc:
-        d = getattr(self._local, "desc", None)
-        if d is None:
-            d = self._local.desc = abi.SklDenseDesc()
-            self._local.ref = C.byref(d)
-        d.dtype, d.inputs, d.outputs, d.max_batch = int(self.half), self.inputs, self.outputs, rows
-        d.act, d.leaky, d.mask_coeff, d.is_training = self.act, self.leaky, self.dropout, 1
-        d.w = None if self.w is None else self.w.data_ptr()
+        own = self._local.__dict__
+        key = rows, self.half, self.inputs, self.outputs, self.act, self.leaky, self.dropout
+        if own.get("key") != key:
+            d = own["desc"] = abi.SklDenseDesc()
+            own["ref"] = C.byref(d)
+            d.dtype, d.inputs, d.outputs, d.max_batch = int(self.half), self.inputs, self.outputs, rows
+            d.act, d.leaky, d.mask_coeff, d.is_training = self.act, self.leaky, self.dropout, 1
+            own["key"] = key
+        d = own["desc"]
+        if self.w is not None:
+            d.w = self.w.data_ptr()
         d.b = None if self.b is None else self.b.data_ptr()
         return d
 
@@ -160,11 +165,13 @@ class Projection:
             raise ValueError(f"h: {torch.float32} or {self.dtype} is wanted, got {r}")
         d = self._desc(rows)
         d.preact = None if preact is None else abi.need("preact", preact, self.dtype, wide, dev)
-        abi.call("skl_dense_forward_residual", self.ctx.h, self._local.ref,
-                 abi.need("x", x, self.dtype, (rows, self.inputs), dev), rows, self.inputs, rows, int(self.dropout != 0.0),
-                 seed & 0xFFFFFFFF, int(r is torch.float16), self.scale,
-                 None if stream is None else abi.need("stream", stream, r, wide, dev), abi.need("h", h, r, wide, dev),
-                 *self.work.product(int(self.half), rows, self.inputs, self.outputs, 1))
+        work = self.work.product(1, rows, self.inputs, self.outputs, 1) if self.half else (None, 0)
+        rc = self._call[0](self.ctx.h, self._local.ref, abi.need("x", x, self.dtype, (rows, self.inputs), dev), rows,
+                           self.inputs, rows, self.dropout != 0.0, seed & 0xFFFFFFFF, r is torch.float16, self.scale,
+                           None if stream is None else abi.need("stream", stream, r, wide, dev),
+                           abi.need("h", h, r, wide, dev), *work)
+        if rc:
+            raise abi.SklError("skl_dense_forward_residual", rc)
         return h
 
     def error(self, dh: torch.Tensor, preact: torch.Tensor | None, d_prenorm: torch.Tensor, *,
@@ -177,6 +184,7 @@ class Projection:
         d.preact = None if preact is None else abi.need("preact", preact, self.dtype, wide, dev)
         d.d_prenorm = abi.need("d_prenorm", d_prenorm, f32, wide, dev)
         d.d_prenorm_h = None if d_prenorm_h is None else abi.need("d_prenorm_h", d_prenorm_h, torch.float16, wide, dev)
-        abi.call("skl_dense_residual_error", self.ctx.h, self._local.ref, abi.need("dh", dh, f32, wide, dev), rows,
-                 int(self.dropout != 0.0), seed & 0xFFFFFFFF, self.scale,
-                 None if dx is None else abi.need("dx", dx, f32, wide, dev))
+        rc = self._call[1](self.ctx.h, self._local.ref, abi.need("dh", dh, f32, wide, dev), rows, self.dropout != 0.0,
+                           seed & 0xFFFFFFFF, self.scale, None if dx is None else abi.need("dx", dx, f32, wide, dev))
+        if rc:
+            raise abi.SklError("skl_dense_residual_error", rc)
