@@ -70,6 +70,7 @@ WAVES_ODD = ["wave:16:16", "wave:32:8", "wave:64:4"]
 # (rows, k, columns): whole tiles, ragged ones, and for padded copies grids of 192 tiles
 KERNELS = ([(r, torch.float16, 70, 200, 68) for r in WAVES16] + [(r, torch.float16, 70, 77, 67) for r in WAVES_ODD] +
            [(r, torch.float32, 70, 203, 67) for r in WAVES32] + [(r, torch.float32, 130, 64, 64) for r in WAVES32] +
+           [("copied", torch.float16, 300, 77, 131), ("copied", torch.float16, 129, 1001, 259)] +
            [("dma128", torch.float16, 256, 128, 256), ("dma128", torch.float16, 300, 72, 130),
             ("dma128", torch.float16, 129, 200, 264), ("dma", torch.float16, 4096, 128, 1536),
             ("dma", torch.float16, 4000, 100, 1500), ("dma", torch.float16, 4096, 65, 1531)])
@@ -78,6 +79,13 @@ KERNELS = ([(r, torch.float16, 70, 200, 68) for r in WAVES16] + [(r, torch.float
 @pytest.mark.parametrize("route,t,m,k,n", KERNELS)
 def test_forward_kernels(monkeypatch, ctx, route, t, m, k, n):
     forward_case(routed(monkeypatch, ctx, route), m, k, n, t, abi.ACT_SILU, True, True)
+
+
+@pytest.mark.parametrize("m,k,n", [(200, 80, 131), (130, 77, 132), (257, 75, 260)])
+@pytest.mark.parametrize("place", [lambda v: v, odd_base], ids=["aligned", "off"])
+def test_forward_copies_of_one_operand(monkeypatch, ctx, m, k, n, place):
+    """Odd rows of the weights alone, part of a 16-byte piece of k alone, and bases off their boundaries."""
+    forward_case(routed(monkeypatch, ctx, "copied"), m, k, n, torch.float16, abi.ACT_SILU, False, True, place)
 
 
 def error_case(ctx, m, n, above, t, act, place=lambda v: v):
