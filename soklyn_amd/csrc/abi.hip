@@ -2145,6 +2145,14 @@ int32_t run_product(skl_ctx *ctx, ProductLaunch p, void *work, size_t work_bytes
     const bool chain = p.kind == Product::Chain;
     // offsets of the planned GEMM are 32-bit
     SKL_CHECK(p.g.N <= 0x7fffffffu && p.g.K <= 0x7fffffffu, SKL_ERR_INVALID_CONFIGURATION);
+    if (ctx->route.kind == Route::Planned && product_rows_ok(p) &&
+        product_rows_bytes(p.g.M, p.g.N, p.kind == Product::Pair ? 2 : 1) <= work_bytes) {
+        p.g.time_start = ctx->gemm_start;
+        p.g.time_stop = ctx->gemm_stop;
+        ctx->gemm_start = ctx->gemm_stop = nullptr;
+        SKL_TRY(launch_product_rows(p, work, ctx->stream));
+        return SKL_OK;
+    }
     const GemmLaunch g = planned_gemm(p);
     PlanCtx how{};
     how.heavy = p.kind == Product::Ungate;
@@ -2242,7 +2250,9 @@ int32_t check_work(const void *work) {
 }  // namespace
 
 size_t skl_product_work_bytes(uint32_t dtype, uint32_t batch, uint32_t inputs, uint32_t outputs, uint32_t matrices) {
-    if (dtype != SKL_F16 || !batch || !inputs || !outputs || !matrices || matrices > 2) return 0;
+    if (dtype > SKL_F16 || !batch || !inputs || !outputs || !matrices || matrices > 2) return 0;
+    if (product_rows_size(dtype, batch, outputs, inputs, matrices)) return product_rows_bytes(batch, outputs, matrices);
+    if (dtype != SKL_F16) return 0;
     // few rows take the operands as they are; so do whole tiles
     const uint64_t mp = ((uint64_t)batch + 255) / 256, np = ((uint64_t)outputs + 255) / 256;
     if (batch < 128 || (batch % 256 == 0 && inputs % 128 == 0 && outputs % 256 == 0)) return 0;

@@ -81,6 +81,14 @@ struct ProductLaunch {
     ChainEpi chain;
 };
 hipError_t launch_product(const ProductLaunch &p, hipStream_t s);
+// The kernels for few rows of a Pair or Project (ffn_rows.hip), which want product_rows_bytes of
+// workspace: whether sizes are theirs, and a product with its alignments.
+hipError_t launch_product_rows(const ProductLaunch &p, void *work, hipStream_t s);
+bool product_rows_size(uint32_t dtype, uint32_t M, uint32_t N, uint32_t K, uint32_t matrices);
+bool product_rows_ok(const ProductLaunch &p);
+size_t product_rows_bytes(uint32_t M, uint32_t N, uint32_t matrices);
+// Every tensor of the epilogue starts its rows on 4 elements.
+bool product_rows4(const ProductLaunch &p);
 // Threads of the K-splitting kernel's launch.
 uint64_t product_threads(const ProductLaunch &p);
 

@@ -28,6 +28,8 @@ static bool rows_on(const ProductLaunch &p, uint32_t group) {
     return false;
 }
 
+bool product_rows4(const ProductLaunch &p) { return rows_on(p, 4); }
+
 // ---- direct-to-LDS ---------------------------------------------------------------------
 template <class Epi, bool BK, int NW, bool EDGE, int BT, bool RAG>
 static hipError_t run_dma(const ProductLaunch &p, const typename Epi::Params &e, bool whole, hipStream_t s) {

@@ -1,0 +1,247 @@
+// ffn_rows.hip — the forward products of ffn.h for up to 16 rows (gfx950): a stream over the weights.
+//
+// k goes in up to eight slices, each to an XCD or to neighbours that halve its columns (workgroup L runs
+// on XCD L % 8), so that an XCD reads whole or half rows of W [k x n] and 256 workgroups are in flight;
+// within a slice a workgroup owns 16 VN columns of each matrix of a pair and its waves share the slice's k, 32 k (fp16) or 16 k (fp32) to a step.  The weights go from
+// memory to registers as they are stored, VN columns of a k-row to a lane, 16 lanes to the row.  fp16
+// lanes turn 8 k-rows into fragments by permutes, one MFMA (16x16x32) for each of their VN columns,
+// whose n index is then VN (lane % 16) + j; fp32 lanes hold a fragment (16x16x4) as loaded.  The waves'
+// sums are added in LDS, the slices' by a second launch, both in a fixed order, in front of the epilogue.
+//
+// What bounds it: HBM, the weights read once (floor at the 5.12 TB/s of a copy).  One row, the K-splitting
+// kernel's tiles of 16 to 64 columns over all of k in brackets, where each XCD has a narrow strip of every
+// row and few waves share a long k: pair fp16 8192 x 4096 30 us (52; floor 26), 4096 x 8192 30 (36; 26),
+// 11008 x 4096 37 (68; 35), 3000 x 3000 14 (24; 7); fp32 4096 x 8192 54 (66; 52); projection fp16
+// 8192 x 4096 18 (28; 13), 3000 x 3000 9 (13; 3.5).  The second launch costs 3 to 4 us of it: below 3000
+// elements of k in all matrices the other's one launch is ahead (projection 2048 x 2048: 9.2 and 6.2).
+#include "ffn.h"
+#include "ffn_epi.h"
+#include "gemm.h"
+
+namespace skl {
+
+constexpr uint32_t kSlices = 8;   // the most
+constexpr uint32_t kRowsMax = 16;
+constexpr uint32_t kOut = 0x80000000u;   // an offset past every operand: reads as zero
+
+template <int N> struct Words { typedef uint32_t type __attribute__((ext_vector_type(N))); };
+
+template <int N> __device__ __forceinline__ typename Words<N>::type rows_load(__amdgpu_buffer_rsrc_t r, uint32_t off) {
+    if constexpr (N == 2) return __builtin_bit_cast(typename Words<2>::type, __builtin_amdgcn_raw_buffer_load_b64(r, (int)off, 0, 0));
+    else return __builtin_bit_cast(typename Words<4>::type, __builtin_amdgcn_raw_buffer_load_b128(r, (int)off, 0, 0));
+}
+
+// The weights of one step of one matrix: L loads of VN columns, fp16 k-rows 8 (lane / 16) + i,
+// fp32 k-rows 4 i + lane / 16.
+template <typename T, int VN> struct RowsW {
+    static constexpr int L = sizeof(T) == 2 ? 8 : 4;
+    static constexpr int NW = VN * (int)sizeof(T) / 4;   // words of a load
+    typename Words<NW>::type v[L];
+    __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t r, uint32_t off, uint32_t row) {
+#pragma unroll
+        for (int i = 0; i < L; ++i) v[i] = rows_load<NW>(r, off + (sizeof(T) == 2 ? i : 4 * i) * row);
+    }
+    // fp16: the fragment of the lane's column j, its 8 k
+    __device__ __forceinline__ u32x4 frag(int j) const {
+        const uint32_t sel = (j & 1) ? 0x07060302u : 0x05040100u;
+        u32x4 f;
+#pragma unroll
+        for (int p = 0; p < 4; ++p) f[p] = __builtin_amdgcn_perm(v[2 * p + 1][j >> 1], v[2 * p][j >> 1], sel);
+        return f;
+    }
+};
+
+// x of one step, row lane % 16: fp16 k 8 (lane / 16) .. + 7, fp32 k 4 i + lane / 16, i < 4.
+template <typename T> struct RowsX {
+    u32x4 v;
+    // left: k of the row from the step's first on (fp16: from the lane's first); past it zeros, as the bytes there
+    // are the next row's
+    __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t r, uint32_t off, int left) {
+        if constexpr (sizeof(T) == 2) {
+            v = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, (int)(left > 0 ? off : kOut), 0, 0));
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                v[i] = __builtin_amdgcn_raw_buffer_load_b32(r, (int)(left > 4 * i ? off + 16 * i : kOut), 0, 0);
+        }
+    }
+};
+
+// planes: [sh.k_per_split slices][P][M][N] fp32
+template <typename T, int P, int VN, int W, int D>
+__global__ void __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(W / 4, W / 4)))
+    rows_kernel(GemmShape sh, const T *__restrict__ A, const T *__restrict__ B, const T *__restrict__ B2, float *planes) {
+    constexpr uint32_t CW = 16 * VN, KS = sizeof(T) == 2 ? 32 : 16, NT = 64 * W, EP = CW + 4;
+    __shared__ __attribute__((aligned(16))) float E[W * 16 * EP];
+    const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    // XCDs 8 / slices to a slice, each with a contiguous part of its column groups
+    const uint32_t share = 8u / sh.k_per_split, slice = blockIdx.x % 8u / share, groups = (sh.N + CW - 1) / CW;
+    const uint32_t mine = (groups + share - 1) / share, group = blockIdx.x % share * mine + blockIdx.x / 8u;
+    if (blockIdx.x / 8u >= mine || group >= groups) return;
+    const uint32_t n0 = group * CW, g = lane >> 4, c = lane & 15u;
+    const uint32_t all = (sh.K + KS - 1) / KS, per = (all + sh.k_per_split - 1) / sh.k_per_split;
+    const uint32_t first = min(slice * per, all), end = min(first + per, all);
+
+    const uint32_t wbytes = sh.K * sh.ldb * (uint32_t)sizeof(T), row = sh.ldb * (uint32_t)sizeof(T);
+    __amdgpu_buffer_rsrc_t rw[P], rx;
+    rw[0] = __builtin_amdgcn_make_buffer_rsrc(const_cast<T *>(B), (short)0, (int)wbytes, 0x00020000);
+    if constexpr (P == 2) rw[1] = __builtin_amdgcn_make_buffer_rsrc(const_cast<T *>(B2), (short)0, (int)wbytes, 0x00020000);
+    rx = __builtin_amdgcn_make_buffer_rsrc(const_cast<T *>(A), (short)0, (int)(((sh.M - 1) * sh.lda + sh.K) * (uint32_t)sizeof(T)),
+                                           0x00020000);
+    // k-row of the lane's first load; columns past the last are not read
+    const uint32_t krow = sizeof(T) == 2 ? 8u * g : g, ncol = n0 + VN * c;
+    const uint32_t woff = ncol < sh.N ? krow * row + ncol * (uint32_t)sizeof(T) : kOut;
+    const uint32_t xoff = c < sh.M ? (c * sh.lda + krow) * (uint32_t)sizeof(T) : kOut;
+
+    floatx4 acc[P][VN];
+#pragma unroll
+    for (int p = 0; p < P; ++p)
+#pragma unroll
+        for (int j = 0; j < VN; ++j) acc[p][j] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+
+    RowsW<T, VN> w[D][P];
+    RowsX<T> x[D];
+    auto load = [&](int d, uint32_t s) {   // steps past the slice's last read zeros on both sides, as do k past K
+        const uint32_t k0 = s * KS;
+        const bool in = s < end;
+#pragma unroll
+        for (int p = 0; p < P; ++p) w[d][p].load(rw[p], in && woff != kOut ? woff + k0 * row : kOut, row);
+        x[d].load(rx, xoff + k0 * (uint32_t)sizeof(T), in && xoff != kOut ? (int)sh.K - (int)(k0 + (sizeof(T) == 2 ? krow : 0u)) : 0);
+    };
+    auto work = [&](int d) {
+        if constexpr (sizeof(T) == 2) {
+#pragma unroll
+            for (int p = 0; p < P; ++p)
+#pragma unroll
+                for (int j = 0; j < VN; ++j)
+                    acc[p][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(halfx8, w[d][p].frag(j)),
+                                                                       __builtin_bit_cast(halfx8, x[d].v), acc[p][j], 0, 0, 0);
+        } else {
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+#pragma unroll
+                for (int p = 0; p < P; ++p)
+#pragma unroll
+                    for (int j = 0; j < VN; ++j)
+                        acc[p][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, (uint32_t)w[d][p].v[q][j]),
+                                                                         __builtin_bit_cast(float, (uint32_t)x[d].v[q]), acc[p][j], 0, 0, 0);
+        }
+    };
+#pragma unroll
+    for (int d = 0; d < D; ++d) load(d, first + wave + d * W);
+    for (uint32_t s = first + wave; s < end; s += D * W) {
+#pragma unroll
+        for (int d = 0; d < D; ++d) {
+            work(d);
+            load(d, s + (D + d) * W);
+        }
+    }
+    // lane l, register r of block j: row l % 16, column VN (4 (l / 16) + r) + j
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+        if (p) lds_barrier();
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int j = 0; j < VN; j += 4)
+                *reinterpret_cast<floatx4 *>(E + (wave * 16 + c) * EP + VN * (4 * g + r) + j) =
+                    floatx4{acc[p][j][r], acc[p][j + 1][r], acc[p][j + 2][r], acc[p][j + 3][r]};
+        lds_barrier();
+        for (uint32_t q = tid; q < 16 * CW / 4; q += NT) {
+            const uint32_t m = q / (CW / 4), cc = (q % (CW / 4)) * 4, n = n0 + cc;
+            if (m >= sh.M || n >= sh.N) continue;
+            floatx4 v = *reinterpret_cast<const floatx4 *>(E + m * EP + cc);
+#pragma unroll
+            for (int k = 1; k < W; ++k) v += *reinterpret_cast<const floatx4 *>(E + (k * 16 + m) * EP + cc);
+            *reinterpret_cast<floatx4 *>(planes + ((uint64_t)(slice * P + p) * sh.M + m) * sh.N + n) = v;
+        }
+    }
+}
+
+// The sums of the S slices' planes, 4 columns to a thread, and the epilogue.
+template <class Epi, int P, int S> __global__ void __launch_bounds__(256) rows_join_kernel(GemmShape sh, const float *planes, typename Epi::Params ep) {
+    const uint32_t per = sh.N / 4, q = blockIdx.x * 256 + threadIdx.x, m = q / per, n = q % per * 4;
+    if (m >= sh.M) return;
+    floatx4 v[S][P];
+#pragma unroll
+    for (uint32_t s = 0; s < S; ++s)
+#pragma unroll
+        for (int p = 0; p < P; ++p)
+            v[s][p] = *reinterpret_cast<const floatx4 *>(planes + ((uint64_t)(s * P + p) * sh.M + m) * sh.N + n);
+    const uint64_t idx = (uint64_t)m * Epi::ldc(ep) + n;
+    typename EpiReadsPre<Epi, EpiReads<Epi>::value>::Pre pre;
+    if constexpr (EpiReads<Epi>::value) Epi::load(ep, idx, m, pre);
+    const typename Epi::Col col = Epi::column(ep, n);
+#pragma unroll
+    for (uint32_t s = 1; s < S; ++s)
+#pragma unroll
+        for (int p = 0; p < P; ++p) v[0][p] += v[s][p];
+    if constexpr (P == 2)
+        Epi::finish(ep, idx, v[0][0], v[0][1], col);
+    else
+        Epi::finish(ep, idx, m, n, v[0][0], col, pre);
+}
+
+// Slices of k: as many as 256 workgroups allow.
+static uint32_t rows_slices(uint32_t dtype, uint32_t N) {
+    const uint32_t cw = dtype == 1 ? 128 : 64, groups = (N + cw - 1) / cw;
+    return groups <= 32 ? 8 : groups <= 64 ? 4 : groups <= 128 ? 2 : 1;
+}
+
+size_t product_rows_bytes(uint32_t M, uint32_t N, uint32_t matrices) {
+    return (size_t)kSlices * matrices * M * N * sizeof(float);
+}
+
+bool product_rows_size(uint32_t dtype, uint32_t M, uint32_t N, uint32_t K, uint32_t matrices) {
+    const uint64_t t = dtype == 1 ? 2 : 4;
+    return M && M <= kRowsMax && N >= 256 && (uint64_t)matrices * K >= 3000 && N % (dtype == 1 ? 8 : 4) == 0 && K % (dtype == 1 ? 8 : 4) == 0 &&
+           (K + 64ull) * N * t < (1ull << 31);
+}
+
+bool product_rows_ok(const ProductLaunch &p) {
+    const GemmLaunch &g = p.g;
+    if (p.kind != Product::Pair && p.kind != Product::Project) return false;
+    const bool pair = p.kind == Product::Pair;
+    const uint64_t t = g.dtype == 1 ? 2 : 4;
+    auto on = [](const void *q) { return (reinterpret_cast<uintptr_t>(q) & 15u) == 0; };
+    return product_rows_size(g.dtype, g.M, g.N, g.K, pair ? 2 : 1) && on(g.A) && g.lda * t % 16 == 0 &&
+           (uint64_t)g.M * g.lda * t < (1ull << 31) && on(g.B) && (!pair || on(p.pair.b2)) && product_rows4(p);
+}
+
+template <typename T, class Epi> static hipError_t rows_t(const ProductLaunch &p, const typename Epi::Params &e, float *planes, hipStream_t s) {
+    constexpr int P = EpiPair<Epi>::value ? 2 : 1, VN = sizeof(T) == 2 ? 8 : 4, W = 8, D = 2;
+    GemmShape sh{};
+    sh.M = p.g.M;
+    sh.N = p.g.N;
+    sh.K = p.g.K;
+    sh.lda = p.g.lda;
+    sh.ldb = p.g.ldb;
+    const T *b2 = nullptr;
+    if constexpr (P == 2) b2 = reinterpret_cast<const T *>(e.b2);
+    sh.k_per_split = rows_slices(p.g.dtype, sh.N);
+    const uint32_t share = 8 / sh.k_per_split, groups = (sh.N + 16 * VN - 1) / (16 * VN);
+    launch_timed(p.g, rows_kernel<T, P, VN, W, D>, dim3((groups + share - 1) / share * 8), dim3(64 * W), s, sh,
+                 reinterpret_cast<const T *>(p.g.A), reinterpret_cast<const T *>(p.g.B), b2, planes);
+    const dim3 join((uint32_t)(((uint64_t)sh.M * (sh.N / 4) + 255) / 256));
+    switch (sh.k_per_split) {
+    case 8: rows_join_kernel<Epi, P, 8><<<join, 256, 0, s>>>(sh, planes, e); break;
+    case 4: rows_join_kernel<Epi, P, 4><<<join, 256, 0, s>>>(sh, planes, e); break;
+    case 2: rows_join_kernel<Epi, P, 2><<<join, 256, 0, s>>>(sh, planes, e); break;
+    default: rows_join_kernel<Epi, P, 1><<<join, 256, 0, s>>>(sh, planes, e);
+    }
+    return hipGetLastError();
+}
+
+hipError_t launch_product_rows(const ProductLaunch &p, void *work, hipStream_t s) {
+    if (!product_rows_ok(p)) return hipErrorInvalidValue;
+    float *planes = reinterpret_cast<float *>(work);
+    if (p.g.dtype == 1) {
+        if (p.kind == Product::Pair) return rows_t<half_t, EpiPairK<half_t>>(p, p.pair, planes, s);
+        return p.stream_dtype == 1 ? rows_t<half_t, EpiProjectK<half_t, half_t>>(p, p.project, planes, s)
+                                   : rows_t<half_t, EpiProjectK<half_t, float>>(p, p.project, planes, s);
+    }
+    return p.kind == Product::Pair ? rows_t<float, EpiPairK<float>>(p, p.pair, planes, s)
+                                   : rows_t<float, EpiProjectK<float, float>>(p, p.project, planes, s);
+}
+
+}  // namespace skl

@@ -58,7 +58,7 @@ class Gated:
         return gate, up, above, own["refs"]
 
     def _work(self, *sizes):
-        return self.work.product(1, *sizes) if self.half else (None, 0)   # fp32 operands are taken as they are
+        return self.work.product(int(self.half), *sizes)
 
     def _at(self, name, t, dtype, shape):
         return None if t is None else abi.need(name, t, dtype, shape, self.ctx.device)

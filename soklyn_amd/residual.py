@@ -165,7 +165,7 @@ class Projection:
             raise ValueError(f"h: {torch.float32} or {self.dtype} is wanted, got {r}")
         d = self._desc(rows)
         d.preact = None if preact is None else abi.need("preact", preact, self.dtype, wide, dev)
-        work = self.work.product(1, rows, self.inputs, self.outputs, 1) if self.half else (None, 0)
+        work = self.work.product(int(self.half), rows, self.inputs, self.outputs, 1)
         rc = self._call[0](self.ctx.h, self._local.ref, abi.need("x", x, self.dtype, (rows, self.inputs), dev), rows,
                            self.inputs, rows, self.dropout != 0.0, seed & 0xFFFFFFFF, r is torch.float16, self.scale,
                            None if stream is None else abi.need("stream", stream, r, wide, dev),

@@ -88,6 +88,33 @@ def test_forward_copies_of_one_operand(monkeypatch, ctx, m, k, n, place):
     forward_case(routed(monkeypatch, ctx, "copied"), m, k, n, torch.float16, abi.ACT_SILU, False, True, place)
 
 
+# up to 16 rows over a long k: eight slices of it (up to 4096 columns of fp16, 2048 of fp32), four, two, one; k
+# that ends inside a step, slices without any, and sizes on both sides of the rule's borders
+FEW_ROWS = [(1, 3000, 256), (3, 4096, 1000), (16, 3008, 2056), (16, 1500, 260), (17, 3000, 264), (2, 3001, 264), (5, 2999, 256),
+            (9, 1504, 8200), (1, 1500, 16400), (7, 1512, 32776), (16, 40000, 256), (1, 6004, 252)]
+
+
+@pytest.mark.parametrize("t", TYPES, ids=IDS)
+@pytest.mark.parametrize("m,k,n", FEW_ROWS)
+def test_forward_few_rows(ctx, m, k, n, t):
+    forward_case(ctx, m, k, n, t, abi.ACT_SILU, n % 3 == 0, m % 2 == 0)
+    if n < 300:
+        forward_case(ctx, m, k, n, t, abi.ACT_SILU, True, True, odd_base)
+
+
+def test_forward_few_rows_beside_nan(ctx):
+    """Rows past the batch, which follow the last one in memory, are not read into its sums."""
+    k, n, t = 3004, 256, torch.float32
+    wg, wu, _, _ = weights(k, n, t, 1, False)
+    for m in (1, 4):
+        x = values((16, k), t, 2)
+        x[m:] = float("nan")
+        out = filled((m, n), t)
+        Gated(ctx, wg, wu, outputs=n).forward(x[:m], out)
+        torch.cuda.synchronize()
+        check(out, gated_ref(x[:m], wg, wu, None, None, abi.ACT_SILU)["out"], t, "out")
+
+
 def error_case(ctx, m, n, above, t, act, place=lambda v: v):
     a, u = place(values((m, n), t, 3)), place(values((m, n), t, 4))
     half = t == torch.float16

@@ -10,7 +10,7 @@ from soklyn_amd import abi, dropout
 from soklyn_amd.devblock import DeviceBlock
 from soklyn_amd.residual import Projection
 from tests.ffn_helpers import ACTS, LEAKY, U, act_off, check, factors, filled, half_step, keeps, odd_base, product, slope, values, within
-from tests.test_gpu_gated import KERNELS, routed
+from tests.test_gpu_gated import FEW_ROWS, KERNELS, routed
 
 pytestmark = pytest.mark.gpu
 F32, F16 = torch.float32, torch.float16
@@ -72,6 +72,14 @@ def test_forward_kernels(monkeypatch, ctx, route, t, m, k, n):
         n *= 2   # one matrix fills the grid that two do
     for r in (F32, F16) if t is F16 else (F32,):
         project_case(c, m, k, n, t, r, act=abi.ACT_SILU)
+
+
+@pytest.mark.parametrize("t,r", PAIRS, ids=IDS)
+@pytest.mark.parametrize("m,k,n", FEW_ROWS)
+def test_forward_few_rows(ctx, m, k, n, t, r):
+    k *= 2 if k < 3000 else 1
+    project_case(ctx, m, k, n, t, r, act=abi.ACT_SILU, bias=n % 3 == 0, drop=0.25 if m % 2 else 0.0, keep=m % 2 == 0,
+                 in_place=n % 2 == 0)
 
 
 def unproject_case(ctx, m, n, t, act=abi.ACT_IDENTITY, drop=0.25, scale=0.75, dx="own", place=lambda v: v, seed=77):
