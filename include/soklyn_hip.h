@@ -334,8 +334,9 @@ size_t skl_mxfp4_work_bytes(uint32_t inputs, uint32_t outputs, uint32_t batch);
  * NULL, a / u are kept there (rounded to T) for the backward.  out is computed from the
  * fp32 sums and rounded once.  No output may overlap an input.
  * work (16-byte aligned, or NULL): skl_product_work_bytes(dtype, batch, inputs, outputs,
- * 2) bytes of the caller's for padded copies of ragged fp16 operands; with less, a kernel
- * runs that takes them as stored (the same result but for the order of its sums).  What it
+ * 2) bytes of the caller's for padded copies of ragged fp16 operands, or for the sums over
+ * slices of a long k where the rows are few; with less, a kernel runs that does without
+ * (the same result but for the order of its sums).  What it
  * holds does not outlive the call; calls that overlap in time need a work of their own.
  * Weights of 2^31 bytes and more, and launches of 2^32 threads, are refused
  * (SKL_ERR_INVALID_CONFIGURATION), here and in the calls below. */

@@ -62,7 +62,8 @@ struct PadCopy {
 
 // SOKLYN_GEMM_ROUTE at skl_ctx_create names the kernel of the context's GEMMs (tests of one
 // instantiation, A/B comparisons): "staged", "dma", "dma128" (operands as stored), "skinny" or
-// "wave:TILE[:WAVES[:SLICES]]" (0: as planned).  A call whose GEMM that kernel does not take
+// "wave:TILE[:WAVES[:SLICES]]" (0: as planned), "copied" (products with work of the caller's: padded
+// copies of their operands).  A call whose GEMM that kernel does not take
 // fails, so a test that passes has run it.
 enum class Route : uint32_t { Planned, Staged, Dma, Dma128, Skinny, Wave, Copied };
 struct GemmRoute {

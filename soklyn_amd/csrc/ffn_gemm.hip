@@ -46,7 +46,7 @@ static hipError_t run_dma(const ProductLaunch &p, const typename Epi::Params &e,
     sh.tiles_n = (g.N + TN - 1) / TN;
     sh.mv = g.mv;
     sh.nv = g.nv;
-    sh.whole = EDGE ? whole : 0;
+    sh.whole = whole;
     launch_timed(g, gemm_dma_kernel<Epi, true, BK, NW, EDGE, 16, BT, RAG>, dim3(sh.tiles_m * sh.tiles_n), dim3(64 * NW), s,
                  sh, reinterpret_cast<const half_t *>(g.A), reinterpret_cast<const half_t *>(g.B), e);
     return hipGetLastError();

@@ -1,9 +1,9 @@
-// ffn_rows.hip — the forward products of ffn.h for up to 16 rows (gfx950): a stream over the weights.
+// ffn_rows.hip — the forward products of ffn.h for up to 32 rows (gfx950): a stream over the weights.
 //
 // k goes in up to eight slices, each to an XCD or to neighbours that halve its columns (workgroup L runs
 // on XCD L % 8), so that an XCD reads whole or half rows of W [k x n] and 256 workgroups are in flight;
-// within a slice a workgroup owns 16 VN columns of each matrix of a pair and its waves share the slice's k, 32 k (fp16) or 16 k (fp32) to a step.  The weights go from
-// memory to registers as they are stored, VN columns of a k-row to a lane, 16 lanes to the row.  fp16
+// within a slice a workgroup owns 16 VN columns of each matrix of a pair and its waves share the slice's
+// k, 32 k (fp16) or 16 k (fp32) to a step.  The weights go from memory to registers as they are stored, VN columns of a k-row to a lane, 16 lanes to the row.  fp16
 // lanes turn 8 k-rows into fragments by permutes, one MFMA (16x16x32) for each of their VN columns,
 // whose n index is then VN (lane % 16) + j; fp32 lanes hold a fragment (16x16x4) as loaded.  The waves'
 // sums are added in LDS, the slices' by a second launch, both in a fixed order, in front of the epilogue.
@@ -14,6 +14,10 @@
 // 11008 x 4096 37 (68; 35), 3000 x 3000 14 (24; 7); fp32 4096 x 8192 54 (66; 52); projection fp16
 // 8192 x 4096 18 (28; 13), 3000 x 3000 9 (13; 3.5).  The second launch costs 3 to 4 us of it: below 3000
 // elements of k in all matrices the other's one launch is ahead (projection 2048 x 2048: 9.2 and 6.2).
+// 17 to 32 rows have two blocks of rows to a fragment of the weights; fp16 lanes then own 4 columns, as
+// the sums of 8 would not leave registers for the loads ahead.  32 rows: pair fp16 8192 x 4096 36 (57),
+// 4096 x 8192 34 (38), 11008 x 4096 44 (76), fp32 4096 x 8192 60 (75); projection fp16 8192 x 4096 22
+// (37), 4096 x 1024 8.9 (9.2).
 #include "ffn.h"
 #include "ffn_epi.h"
 #include "gemm.h"
@@ -21,7 +25,6 @@
 namespace skl {
 
 constexpr uint32_t kSlices = 8;   // the most
-constexpr uint32_t kRowsMax = 16;
 constexpr uint32_t kOut = 0x80000000u;   // an offset past every operand: reads as zero
 
 template <int N> struct Words { typedef uint32_t type __attribute__((ext_vector_type(N))); };
@@ -68,11 +71,11 @@ template <typename T> struct RowsX {
 };
 
 // planes: [sh.k_per_split slices][P][M][N] fp32
-template <typename T, int P, int VN, int W, int D>
+template <typename T, int P, int VN, int MB, int W, int D>
 __global__ void __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(W / 4, W / 4)))
     rows_kernel(GemmShape sh, const T *__restrict__ A, const T *__restrict__ B, const T *__restrict__ B2, float *planes) {
-    constexpr uint32_t CW = 16 * VN, KS = sizeof(T) == 2 ? 32 : 16, NT = 64 * W, EP = CW + 4;
-    __shared__ __attribute__((aligned(16))) float E[W * 16 * EP];
+    constexpr uint32_t CW = 16 * VN, KS = sizeof(T) == 2 ? 32 : 16, NT = 64 * W, EP = CW + 4, BM = 16 * MB;
+    __shared__ __attribute__((aligned(16))) float E[W * BM * EP];
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     // XCDs 8 / slices to a slice, each with a contiguous part of its column groups
     const uint32_t share = 8u / sh.k_per_split, slice = blockIdx.x % 8u / share, groups = (sh.N + CW - 1) / CW;
@@ -91,31 +94,45 @@ __global__ void __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(W /
     // k-row of the lane's first load; columns past the last are not read
     const uint32_t krow = sizeof(T) == 2 ? 8u * g : g, ncol = n0 + VN * c;
     const uint32_t woff = ncol < sh.N ? krow * row + ncol * (uint32_t)sizeof(T) : kOut;
-    const uint32_t xoff = c < sh.M ? (c * sh.lda + krow) * (uint32_t)sizeof(T) : kOut;
+    uint32_t xoff[MB];
+#pragma unroll
+    for (uint32_t i = 0; i < MB; ++i) {
+        const uint32_t m = 16 * i + c;
+        xoff[i] = m < sh.M ? (m * sh.lda + krow) * (uint32_t)sizeof(T) : kOut;
+    }
 
-    floatx4 acc[P][VN];
+    floatx4 acc[P][VN][MB];
 #pragma unroll
     for (int p = 0; p < P; ++p)
 #pragma unroll
-        for (int j = 0; j < VN; ++j) acc[p][j] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int j = 0; j < VN; ++j)
+#pragma unroll
+            for (int i = 0; i < MB; ++i) acc[p][j][i] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
 
     RowsW<T, VN> w[D][P];
-    RowsX<T> x[D];
+    RowsX<T> x[D][MB];
     auto load = [&](int d, uint32_t s) {   // steps past the slice's last read zeros on both sides, as do k past K
         const uint32_t k0 = s * KS;
         const bool in = s < end;
 #pragma unroll
         for (int p = 0; p < P; ++p) w[d][p].load(rw[p], in && woff != kOut ? woff + k0 * row : kOut, row);
-        x[d].load(rx, xoff + k0 * (uint32_t)sizeof(T), in && xoff != kOut ? (int)sh.K - (int)(k0 + (sizeof(T) == 2 ? krow : 0u)) : 0);
+#pragma unroll
+        for (int i = 0; i < MB; ++i)
+            x[d][i].load(rx, xoff[i] + k0 * (uint32_t)sizeof(T),
+                         in && xoff[i] != kOut ? (int)sh.K - (int)(k0 + (sizeof(T) == 2 ? krow : 0u)) : 0);
     };
     auto work = [&](int d) {
         if constexpr (sizeof(T) == 2) {
 #pragma unroll
             for (int p = 0; p < P; ++p)
 #pragma unroll
-                for (int j = 0; j < VN; ++j)
-                    acc[p][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(halfx8, w[d][p].frag(j)),
-                                                                       __builtin_bit_cast(halfx8, x[d].v), acc[p][j], 0, 0, 0);
+                for (int j = 0; j < VN; ++j) {
+                    const halfx8 f = __builtin_bit_cast(halfx8, w[d][p].frag(j));
+#pragma unroll
+                    for (int i = 0; i < MB; ++i)
+                        acc[p][j][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, __builtin_bit_cast(halfx8, x[d][i].v),
+                                                                              acc[p][j][i], 0, 0, 0);
+                }
         } else {
 #pragma unroll
             for (int q = 0; q < 4; ++q)
@@ -123,8 +140,11 @@ __global__ void __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(W /
                 for (int p = 0; p < P; ++p)
 #pragma unroll
                     for (int j = 0; j < VN; ++j)
-                        acc[p][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, (uint32_t)w[d][p].v[q][j]),
-                                                                         __builtin_bit_cast(float, (uint32_t)x[d].v[q]), acc[p][j], 0, 0, 0);
+#pragma unroll
+                        for (int i = 0; i < MB; ++i)
+                            acc[p][j][i] = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                                __builtin_bit_cast(float, (uint32_t)w[d][p].v[q][j]),
+                                __builtin_bit_cast(float, (uint32_t)x[d][i].v[q]), acc[p][j][i], 0, 0, 0);
         }
     };
 #pragma unroll
@@ -136,23 +156,25 @@ __global__ void __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(W /
             load(d, s + (D + d) * W);
         }
     }
-    // lane l, register r of block j: row l % 16, column VN (4 (l / 16) + r) + j
+    // lane l, register r of block (j, i): row 16 i + l % 16, column VN (4 (l / 16) + r) + j
 #pragma unroll
     for (int p = 0; p < P; ++p) {
         if (p) lds_barrier();
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
+        for (int i = 0; i < MB; ++i)
 #pragma unroll
-            for (int j = 0; j < VN; j += 4)
-                *reinterpret_cast<floatx4 *>(E + (wave * 16 + c) * EP + VN * (4 * g + r) + j) =
-                    floatx4{acc[p][j][r], acc[p][j + 1][r], acc[p][j + 2][r], acc[p][j + 3][r]};
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+                for (int j = 0; j < VN; j += 4)
+                    *reinterpret_cast<floatx4 *>(E + (wave * BM + 16 * i + c) * EP + VN * (4 * g + r) + j) =
+                        floatx4{acc[p][j][i][r], acc[p][j + 1][i][r], acc[p][j + 2][i][r], acc[p][j + 3][i][r]};
         lds_barrier();
-        for (uint32_t q = tid; q < 16 * CW / 4; q += NT) {
+        for (uint32_t q = tid; q < BM * CW / 4; q += NT) {
             const uint32_t m = q / (CW / 4), cc = (q % (CW / 4)) * 4, n = n0 + cc;
             if (m >= sh.M || n >= sh.N) continue;
             floatx4 v = *reinterpret_cast<const floatx4 *>(E + m * EP + cc);
 #pragma unroll
-            for (int k = 1; k < W; ++k) v += *reinterpret_cast<const floatx4 *>(E + (k * 16 + m) * EP + cc);
+            for (int k = 1; k < W; ++k) v += *reinterpret_cast<const floatx4 *>(E + (k * BM + m) * EP + cc);
             *reinterpret_cast<floatx4 *>(planes + ((uint64_t)(slice * P + p) * sh.M + m) * sh.N + n) = v;
         }
     }
@@ -182,9 +204,11 @@ template <class Epi, int P, int S> __global__ void __launch_bounds__(256) rows_j
         Epi::finish(ep, idx, m, n, v[0][0], col, pre);
 }
 
+// Columns of a lane: 16 bytes of them, half of that where fp16 has two blocks of rows to sum for.
+static uint32_t rows_vn(uint32_t dtype, uint32_t M) { return dtype == 1 && M <= 16 ? 8 : 4; }
 // Slices of k: as many as 256 workgroups allow.
-static uint32_t rows_slices(uint32_t dtype, uint32_t N) {
-    const uint32_t cw = dtype == 1 ? 128 : 64, groups = (N + cw - 1) / cw;
+static uint32_t rows_slices(uint32_t dtype, uint32_t M, uint32_t N) {
+    const uint32_t cw = 16 * rows_vn(dtype, M), groups = (N + cw - 1) / cw;
     return groups <= 32 ? 8 : groups <= 64 ? 4 : groups <= 128 ? 2 : 1;
 }
 
@@ -192,9 +216,15 @@ size_t product_rows_bytes(uint32_t M, uint32_t N, uint32_t matrices) {
     return (size_t)kSlices * matrices * M * N * sizeof(float);
 }
 
+// Past 16 rows, 32 columns of one fp32 matrix to a wave do too little for the two blocks of x (the fp32
+// MFMAs bound it: projection 4096 x 8192, 32 rows, 42 us, the K-splitting kernel 30), and a pair of
+// short k and few columns has too few steps to a wave (2048 x 2048 fp16, 32 rows: 11.6 and 9.6; 2048 x
+// 8192: 21.8 and 31.2).
 bool product_rows_size(uint32_t dtype, uint32_t M, uint32_t N, uint32_t K, uint32_t matrices) {
     const uint64_t t = dtype == 1 ? 2 : 4;
-    return M && M <= kRowsMax && N >= 256 && (uint64_t)matrices * K >= 3000 && N % (dtype == 1 ? 8 : 4) == 0 && K % (dtype == 1 ? 8 : 4) == 0 &&
+    const uint32_t lane = dtype == 1 ? 8 : 4;
+    const bool rows = M <= 16 || (M <= 32 && (dtype == 1 || matrices == 2) && (K >= 3000 || N >= 4096));
+    return M && rows && N >= 256 && (uint64_t)matrices * K >= 3000 && N % lane == 0 && K % lane == 0 &&
            (K + 64ull) * N * t < (1ull << 31);
 }
 
@@ -208,8 +238,9 @@ bool product_rows_ok(const ProductLaunch &p) {
            (uint64_t)g.M * g.lda * t < (1ull << 31) && on(g.B) && (!pair || on(p.pair.b2)) && product_rows4(p);
 }
 
-template <typename T, class Epi> static hipError_t rows_t(const ProductLaunch &p, const typename Epi::Params &e, float *planes, hipStream_t s) {
-    constexpr int P = EpiPair<Epi>::value ? 2 : 1, VN = sizeof(T) == 2 ? 8 : 4, W = 8, D = 2;
+template <typename T, class Epi, int MB>
+static hipError_t rows_mb(const ProductLaunch &p, const typename Epi::Params &e, float *planes, hipStream_t s) {
+    constexpr int P = EpiPair<Epi>::value ? 2 : 1, VN = sizeof(T) == 2 && MB == 1 ? 8 : 4, W = 8, D = 2;
     GemmShape sh{};
     sh.M = p.g.M;
     sh.N = p.g.N;
@@ -218,9 +249,9 @@ template <typename T, class Epi> static hipError_t rows_t(const ProductLaunch &p
     sh.ldb = p.g.ldb;
     const T *b2 = nullptr;
     if constexpr (P == 2) b2 = reinterpret_cast<const T *>(e.b2);
-    sh.k_per_split = rows_slices(p.g.dtype, sh.N);
+    sh.k_per_split = rows_slices(p.g.dtype, sh.M, sh.N);
     const uint32_t share = 8 / sh.k_per_split, groups = (sh.N + 16 * VN - 1) / (16 * VN);
-    launch_timed(p.g, rows_kernel<T, P, VN, W, D>, dim3((groups + share - 1) / share * 8), dim3(64 * W), s, sh,
+    launch_timed(p.g, rows_kernel<T, P, VN, MB, W, D>, dim3((groups + share - 1) / share * 8), dim3(64 * W), s, sh,
                  reinterpret_cast<const T *>(p.g.A), reinterpret_cast<const T *>(p.g.B), b2, planes);
     const dim3 join((uint32_t)(((uint64_t)sh.M * (sh.N / 4) + 255) / 256));
     switch (sh.k_per_split) {
@@ -230,6 +261,13 @@ template <typename T, class Epi> static hipError_t rows_t(const ProductLaunch &p
     default: rows_join_kernel<Epi, P, 1><<<join, 256, 0, s>>>(sh, planes, e);
     }
     return hipGetLastError();
+}
+
+template <typename T, class Epi>
+static hipError_t rows_t(const ProductLaunch &p, const typename Epi::Params &e, float *planes, hipStream_t s) {
+    if constexpr (sizeof(T) == 2 || EpiPair<Epi>::value)
+        if (p.g.M > 16) return rows_mb<T, Epi, 2>(p, e, planes, s);
+    return rows_mb<T, Epi, 1>(p, e, planes, s);
 }
 
 hipError_t launch_product_rows(const ProductLaunch &p, void *work, hipStream_t s) {

@@ -91,7 +91,8 @@ def test_forward_copies_of_one_operand(monkeypatch, ctx, m, k, n, place):
 # up to 16 rows over a long k: eight slices of it (up to 4096 columns of fp16, 2048 of fp32), four, two, one; k
 # that ends inside a step, slices without any, and sizes on both sides of the rule's borders
 FEW_ROWS = [(1, 3000, 256), (3, 4096, 1000), (16, 3008, 2056), (16, 1500, 260), (17, 3000, 264), (2, 3001, 264), (5, 2999, 256),
-            (9, 1504, 8200), (1, 1500, 16400), (7, 1512, 32776), (16, 40000, 256), (1, 6004, 252)]
+            (9, 1504, 8200), (1, 1500, 16400), (7, 1512, 32776), (16, 40000, 256), (1, 6004, 252),
+            (32, 3000, 256), (31, 1504, 4104), (18, 3008, 1000), (32, 1500, 16388), (33, 3000, 256)]
 
 
 @pytest.mark.parametrize("t", TYPES, ids=IDS)
