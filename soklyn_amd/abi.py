@@ -192,8 +192,12 @@ class Workspace:
             return None, 0
         if not self._pieces or self._pieces[-1].numel() < size:
             import torch
-            self._pieces.append(torch.empty(size, device=f"cuda:{self.ctx.device}", dtype=torch.uint8))
-        return self._pieces[-1].data_ptr(), self._pieces[-1].numel()
+            # of the context's stream: what held the memory before is done there, and so is this owner
+            # when another allocation gets it
+            with torch.cuda.stream(torch.cuda.ExternalStream(load().skl_ctx_stream(self.ctx.h), self.ctx.device)):
+                self._pieces.append(torch.empty(size, device=f"cuda:{self.ctx.device}", dtype=torch.uint8))
+        piece = self._pieces[-1]
+        return piece.data_ptr(), piece.numel()
 
     def product(self, *sizes: int) -> tuple[int | None, int]:
         """For skl_product_work_bytes(*sizes): dtype, batch, inputs, outputs, matrices."""

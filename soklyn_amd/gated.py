@@ -27,16 +27,19 @@ class Gated:
                  bu: torch.Tensor | None = None, *, outputs: int, half: bool = False, act: int = abi.ACT_SILU,
                  leaky: float = 0.0):
         self.ctx, self.outputs, self.half, self.act, self.leaky = ctx, outputs, half, act, leaky
-        self.dtype = t = _F16 if half else _F32
+        self.dtype = _F16 if half else _F32
         self.inputs = 1 if wg is None else wg.shape[0]
-        for name, w, shape in (("wg", wg, (self.inputs, outputs)), ("wu", wu, (self.inputs, outputs)),
-                               ("bg", bg, (1, outputs)), ("bu", bu, (1, outputs))):
-            if w is not None:
-                abi.need(name, w, t, shape, ctx.device)
         self.wg, self.wu, self.bg, self.bu, self.work = wg, wu, bg, bu, abi.Workspace(ctx)
+        self._weights()
         lib = abi.load()
         self._call = lib.skl_gated_forward, lib.skl_gated_error_from_sum, lib.skl_gated_hidden_error, lib.skl_gated_input_grad
         self._local = threading.local()   # descriptors, one set per thread
+
+    def _weights(self):
+        """The addresses of the weights and biases, of the sizes that they have to have."""
+        wide, row = (self.inputs, self.outputs), (1, self.outputs)
+        return (self._at("wg", self.wg, self.dtype, wide), self._at("bg", self.bg, self.dtype, row),
+                self._at("wu", self.wu, self.dtype, wide), self._at("bu", self.bu, self.dtype, row))
 
     def _descs(self, rows: int):
         """This thread's descriptors of gate, up and the layer above, with the weights as they are now."""
@@ -51,10 +54,7 @@ class Gated:
             own["d"][0].act, own["d"][0].leaky = self.act, self.leaky
             own["key"] = key
         gate, up, above = own["d"]
-        for d, w, b in ((gate, self.wg, self.bg), (up, self.wu, self.bu)):
-            if w is not None:
-                d.w = w.data_ptr()
-            d.b = None if b is None else b.data_ptr()
+        gate.w, gate.b, up.w, up.b = self._weights()
         return gate, up, above, own["refs"]
 
     def _work(self, *sizes):

@@ -132,13 +132,16 @@ class Projection:
         self.dropout, self.scale = dropout, scale
         self.dtype = torch.float16 if half else torch.float32
         self.inputs = 1 if w is None else w.shape[0]
-        if w is not None:
-            abi.need("w", w, self.dtype, (self.inputs, outputs), ctx.device)
-        if b is not None:
-            abi.need("b", b, self.dtype, (1, outputs), ctx.device)
         self.w, self.b, self.work = w, b, abi.Workspace(ctx)
+        self._weights()
         self._call = abi.load().skl_dense_forward_residual, abi.load().skl_dense_residual_error
         self._local = threading.local()   # descriptors, one per thread
+
+    def _weights(self):
+        """The addresses of w and b, of the sizes that they have to have."""
+        t, n, dev = self.dtype, self.outputs, self.ctx.device
+        return (None if self.w is None else abi.need("w", self.w, t, (self.inputs, n), dev),
+                None if self.b is None else abi.need("b", self.b, t, (1, n), dev))
 
     def _desc(self, rows: int) -> abi.SklDenseDesc:
         own = self._local.__dict__
@@ -150,9 +153,7 @@ class Projection:
             d.act, d.leaky, d.mask_coeff, d.is_training = self.act, self.leaky, self.dropout, 1
             own["key"] = key
         d = own["desc"]
-        if self.w is not None:
-            d.w = self.w.data_ptr()
-        d.b = None if self.b is None else self.b.data_ptr()
+        d.w, d.b = self._weights()
         return d
 
     def forward(self, x: torch.Tensor, stream: torch.Tensor | None, h: torch.Tensor, *, preact: torch.Tensor | None = None,

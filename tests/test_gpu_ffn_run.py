@@ -228,6 +228,95 @@ def test_two_graphs_of_copied_operands(ctx):
             c.close()
 
 
+def test_graphs_of_few_rows(ctx):
+    """The sums over slices of k are in workspaces: calls captured before any eager one, each object with its own,
+    replayed in flight together, with larger and smaller eager calls of the same objects in between."""
+    t, k, n = F16, 4096, 520
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    cs = [abi.Context(0, 16, stream=s.cuda_stream) for s in streams]
+    try:
+        work = []
+        for i, (c, s) in enumerate(zip(cs, streams)):
+            g = torch.Generator(device="cuda").manual_seed(i)
+            x, wg, wu, wp, x32 = (torch.randn(sh, generator=g, device="cuda").to(t) * 0.02
+                                  for sh in ((3, k), (k, n), (k, n), (k, n), (32, k)))
+            gate, project = Gated(c, wg, wu, outputs=n, half=True), Projection(c, wp, None, outputs=n, half=True, dropout=0.5)
+            mid, h = torch.empty((3, n), dtype=t, device="cuda"), torch.randn((3, n), generator=g, device="cuda")
+            torch.cuda.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=s, capture_error_mode="thread_local"):
+                gate.forward(x, mid)
+                project.forward(x, h, h, seed=i)
+            work.append((graph, gate, project, x, mid, h, x32, s, i))
+        for rep in range(4):
+            want = []
+            for _, gate, project, x, mid, h, x32, s, i in work:
+                x.mul_(-1.25)
+                torch.cuda.synchronize()
+                a, b = torch.empty_like(mid), torch.empty_like(h)
+                gate.forward(x, a)
+                project.forward(x, h, b, seed=i)
+                rows = 32 if rep % 2 else 1
+                gate.forward(x32[:rows], torch.empty((rows, n), dtype=t, device="cuda"))
+                want.append((a, b))
+                mid.fill_(float("nan"))
+            torch.cuda.synchronize()
+            for graph, *_, s, _ in work:
+                with torch.cuda.stream(s):
+                    graph.replay()
+            torch.cuda.synchronize()
+            for (_, _, _, _, mid, h, *_), (a, b) in zip(work, want):
+                assert torch.equal(mid, a) and torch.equal(h, b), rep
+    finally:
+        torch.cuda.synchronize()
+        for c in cs:
+            c.close()
+
+
+def test_workspaces_belong_to_the_context_s_stream(ctx):
+    """What a dropped object held goes to allocations of its context's stream alone, behind its last kernels."""
+    side = torch.cuda.Stream()
+    other = abi.Context(0, 16, stream=side.cuda_stream)
+    try:
+        size = 96 << 20
+        piece = abi.Workspace(other)
+        at, have = piece.get(size)
+        assert have == size and piece.get(1000)[0] == at
+        torch.cuda.synchronize()
+        del piece
+        elsewhere = torch.empty(size, dtype=torch.uint8, device="cuda")
+        assert elsewhere.data_ptr() != at
+        with torch.cuda.stream(side):
+            assert torch.empty(size, dtype=torch.uint8, device="cuda").data_ptr() == at
+    finally:
+        torch.cuda.synchronize()
+        other.close()
+
+
+def test_weights_exchanged_for_others(ctx):
+    """An object's weights may be exchanged; ones of another size, type or layout are refused."""
+    wg, wu, w2 = (torch.randn((64, 40), device="cuda") for _ in range(3))
+    x, out, h = torch.randn((5, 64), device="cuda"), torch.empty((5, 40), device="cuda"), torch.zeros((5, 40), device="cuda")
+    op, pr = Gated(ctx, wg, wu, outputs=40, act=abi.ACT_IDENTITY), Projection(ctx, wg, None, outputs=40)
+    op.wg = pr.w = w2
+    op.forward(x, out)
+    pr.forward(x, None, h)
+    torch.cuda.synchronize()
+    a, u = x.double() @ w2.double(), x.double() @ wu.double()
+    size, other = x.double().abs() @ w2.double().abs(), x.double().abs() @ wu.double().abs()
+    assert bool(((h.double() - a).abs() <= 128 * U * size).all())
+    assert bool(((out.double() - a * u).abs() <= 4 * 128 * U * size * other).all())
+    for bad in (w2[:32], w2.half(), w2.t(), torch.cat([w2, w2])):
+        op.wg = pr.w = bad
+        with pytest.raises(ValueError):
+            op.forward(x, out)
+        with pytest.raises(ValueError):
+            pr.forward(x, None, h)
+    op.wg, op.outputs = w2, 400
+    with pytest.raises(ValueError):
+        op.forward(x, torch.empty((5, 400), device="cuda"))
+
+
 def test_two_contexts_at_once(ctx):
     """Steps of two contexts on streams of their own, in flight together, give what each gives alone."""
     side = torch.cuda.Stream()
