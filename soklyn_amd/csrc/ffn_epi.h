@@ -150,8 +150,8 @@ template <typename T> struct EpiUngateK {
         __builtin_nontemporal_store(dg, reinterpret_cast<f32x4 *>(e.d_gate + idx));
         __builtin_nontemporal_store(du, reinterpret_cast<f32x4 *>(e.d_up + idx));
         if constexpr (sizeof(T) == 2) {
-            store4<half_t>(e.d_gate_h, idx, dg);
-            store4<half_t>(e.d_up_h, idx, du);
+            store4_nt<half_t>(e.d_gate_h, idx, dg);   // (past the caches: 16384 x 4096, K 2048: 421 -> 395 us)
+            store4_nt<half_t>(e.d_up_h, idx, du);
         }
     }
     __device__ __forceinline__ static void load1(const UngateEpi &e, uint64_t idx, Pre1 &q) {
