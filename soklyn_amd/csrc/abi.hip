@@ -2140,14 +2140,13 @@ bool slow_rag(const ProductLaunch &p) {
     return (p.kind == Product::Ungate || p.kind == Product::Project) && p.g.N % 4 != 0 && tiles < 512;
 }
 
-// A pair's 32x16 tiles take 16 columns of a k-row from each matrix, 32 or 64 bytes, its 64x32 tiles twice
-// as many; the planner prices both as tiles of one matrix of twice the columns.  fp16, enough work to fill
-// the card with 64x32 tiles: 200 x 1024, K 2048 9.7 us (12.4), 500 x 1025, K 777 15.1 (23.9), but 200 x 1024,
-// K 777 10.8 (8.6).  fp32, six rounds of them: 3000 x 1025, K 2048 239 (452), 3000 x 1024 198 (224), but
-// 1000 x 1025 106 (89).
+// A pair's 32x16 tiles take 16 columns of a k-row from each matrix, in fp16 32 bytes, its 64x32 tiles twice
+// as many; the planner prices both as tiles of one matrix of twice the columns.  With work for the whole
+// card 64x32 are ahead (fp16 200 x 1024, K 2048: 9.7 us, 32x16 11.8; 500 x 1025, K 777: 15.0, 23.6; but
+// 200 x 1024, K 1200: 10.4, 8.4).
 bool wide_pair(const ProductLaunch &p) {
     const uint64_t tiles = (uint64_t)((p.g.M + 63) / 64) * ((p.g.N + 31) / 32);
-    return p.kind == Product::Pair && (p.g.dtype == SKL_F16 ? tiles * p.g.K >= 120000 : tiles >= 1500);
+    return p.kind == Product::Pair && p.g.dtype == SKL_F16 && tiles * p.g.K >= 160000;
 }
 
 // Plans and launches a product whose g, kind and epilogue are set.  Copies go to the caller's work;

@@ -1,4 +1,16 @@
 // ffn_gemm.hip — launchers of the products in ffn.h on the direct-to-LDS and K-splitting kernels.
+//
+//   Pair     out = act(A Wg + bg) * (A Wu + bu)     a tile of both matrices beside each other: A is read once
+//   Ungate   s = A B^T, dg = s u act'(a), du = s act(a)     s stays in registers
+//   Project  h = scale x + drop(act(A W + b))
+//   Chain    dx = A B^T + a2 b2^T                   one k loop over both parts, one store
+//
+// fp16, 16384 rows (2 M N K of one or two products; HBM as 5.1 TB/s):
+//   Pair 2048 -> 4096, a and u kept      466 us: 1.18 PF/s, the library's 8192^3 product 1.14-1.2
+//   Chain 2 x 4096 -> 2048               428 us: 1.28 PF/s
+//   Project 4096 -> 2048, fp32 stream    260 us: 1.06 PF/s
+//   Ungate 2048 -> 4096                  393 us: 0.70 PF/s and 2.9 TB/s; the k loops alone 176, the epilogues'
+//     6 tensors alone 226.  All workgroups of a round load, multiply and store together, so the two add up.
 #include "ffn.h"
 #include "ffn_epi.h"
 #include "gemm_dma.h"
@@ -54,7 +66,9 @@ static hipError_t run_dma(const ProductLaunch &p, const typename Epi::Params &e,
 
 // 256x256 tiles on 8 waves, but for the plain store of a chain, which takes one wave per SIMD where
 // the tiles are whole; 128x128 on 4; both also over padded copies (mv, nv the real output), 128x128
-// over operands as stored.
+// over operands as stored.  The epilogues of the others want the threads of 8 waves (4 waves of 128x128:
+// 2-4% slower), and 128x128 tiles, two workgroups to a CU, lose more in the k loop than their epilogues
+// gain beside it (Pair 545 us, Project 308, Ungate 442).
 template <class Epi, bool BK>
 static hipError_t dma(const ProductLaunch &p, const typename Epi::Params &e, hipStream_t s) {
     const GemmLaunch &g = p.g;
