@@ -181,8 +181,8 @@ __global__ void __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(W /
 }
 
 // The sums of the S slices' planes, 4 columns to a thread, and the epilogue.
-template <class Epi, int P, int S> __global__ void __launch_bounds__(256) rows_join_kernel(GemmShape sh, const float *planes, typename Epi::Params ep) {
-    const uint32_t per = sh.N / 4, q = blockIdx.x * 256 + threadIdx.x, m = q / per, n = q % per * 4;
+template <class Epi, int P, int S> __global__ void __launch_bounds__(64) rows_join_kernel(GemmShape sh, const float *planes, typename Epi::Params ep) {
+    const uint32_t per = sh.N / 4, q = blockIdx.x * 64 + threadIdx.x, m = q / per, n = q % per * 4;
     if (m >= sh.M) return;
     floatx4 v[S][P];
 #pragma unroll
@@ -253,12 +253,12 @@ static hipError_t rows_mb(const ProductLaunch &p, const typename Epi::Params &e,
     const uint32_t share = 8 / sh.k_per_split, groups = (sh.N + 16 * VN - 1) / (16 * VN);
     launch_timed(p.g, rows_kernel<T, P, VN, MB, W, D>, dim3((groups + share - 1) / share * 8), dim3(64 * W), s, sh,
                  reinterpret_cast<const T *>(p.g.A), reinterpret_cast<const T *>(p.g.B), b2, planes);
-    const dim3 join((uint32_t)(((uint64_t)sh.M * (sh.N / 4) + 255) / 256));
+    const dim3 join((uint32_t)(((uint64_t)sh.M * (sh.N / 4) + 63) / 64));
     switch (sh.k_per_split) {
-    case 8: rows_join_kernel<Epi, P, 8><<<join, 256, 0, s>>>(sh, planes, e); break;
-    case 4: rows_join_kernel<Epi, P, 4><<<join, 256, 0, s>>>(sh, planes, e); break;
-    case 2: rows_join_kernel<Epi, P, 2><<<join, 256, 0, s>>>(sh, planes, e); break;
-    default: rows_join_kernel<Epi, P, 1><<<join, 256, 0, s>>>(sh, planes, e);
+    case 8: rows_join_kernel<Epi, P, 8><<<join, 64, 0, s>>>(sh, planes, e); break;
+    case 4: rows_join_kernel<Epi, P, 4><<<join, 64, 0, s>>>(sh, planes, e); break;
+    case 2: rows_join_kernel<Epi, P, 2><<<join, 64, 0, s>>>(sh, planes, e); break;
+    default: rows_join_kernel<Epi, P, 1><<<join, 64, 0, s>>>(sh, planes, e);
     }
     return hipGetLastError();
 }
