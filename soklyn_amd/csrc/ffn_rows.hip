@@ -1,4 +1,4 @@
-// ffn_rows.hip — the forward products of ffn.h for up to 32 rows (gfx950): a stream over the weights.
+// ffn_rows.hip — the forward products of ffn.h for up to 64 rows (gfx950): a stream over the weights.
 //
 // k goes in up to eight slices, each to an XCD or to neighbours that halve its columns (workgroup L runs
 // on XCD L % 8), so that an XCD reads whole or half rows of W [k x n] and 256 workgroups are in flight;
@@ -14,10 +14,11 @@
 // 11008 x 4096 37 (68; 35), 3000 x 3000 14 (24; 7); fp32 4096 x 8192 54 (66; 52); projection fp16
 // 8192 x 4096 18 (28; 13), 3000 x 3000 9 (13; 3.5).  The second launch costs 3 to 4 us of it: below 3000
 // elements of k in all matrices the other's one launch is ahead (projection 2048 x 2048: 9.2 and 6.2).
-// 17 to 32 rows have two blocks of rows to a fragment of the weights; fp16 lanes then own 4 columns, as
+// 17 to 32 rows have two blocks of rows to a fragment of the weights, more have four; fp16 lanes then own 4 columns, as
 // the sums of 8 would not leave registers for the loads ahead.  32 rows: pair fp16 8192 x 4096 36 (57),
 // 4096 x 8192 34 (38), 11008 x 4096 44 (76), fp32 4096 x 8192 60 (75); projection fp16 8192 x 4096 22
-// (37), 4096 x 1024 8.9 (9.2).
+// (37), 4096 x 1024 8.9 (9.2).  64 rows, fp16: pair 8192 x 4096 43 (74), 4096 x 8192 39 (42), projection
+// 8192 x 4096 27 (34).
 #include "ffn.h"
 #include "ffn_epi.h"
 #include "gemm.h"
@@ -216,14 +217,17 @@ size_t product_rows_bytes(uint32_t M, uint32_t N, uint32_t matrices) {
     return (size_t)kSlices * matrices * M * N * sizeof(float);
 }
 
-// Past 16 rows, 32 columns of one fp32 matrix to a wave do too little for the two blocks of x (the fp32
+// Past 32 rows, four blocks of rows have registers in fp16 only, and one matrix wants enough columns and
+// k for its two launches (projection, 64 rows: 3000 x 3000 13.2 us, one launch 11.0; 4096 x 1024 9.8 and
+// 9.2; 4096 x 8192 25.4 and 28.0).  Past 16 rows, 32 columns of one fp32 matrix to a wave do too little for the two blocks of x (the fp32
 // MFMAs bound it: projection 4096 x 8192, 32 rows, 42 us, the K-splitting kernel 30), and a pair of
 // short k and few columns has too few steps to a wave (2048 x 2048 fp16, 32 rows: 11.6 and 9.6; 2048 x
 // 8192: 21.8 and 31.2).
 bool product_rows_size(uint32_t dtype, uint32_t M, uint32_t N, uint32_t K, uint32_t matrices) {
     const uint64_t t = dtype == 1 ? 2 : 4;
     const uint32_t lane = dtype == 1 ? 8 : 4;
-    const bool rows = M <= 16 || (M <= 32 && (dtype == 1 || matrices == 2) && (K >= 3000 || N >= 4096));
+    const bool rows = M <= 16 || (M <= 32 && (dtype == 1 || matrices == 2) && (K >= 3000 || N >= 4096)) ||
+                      (M <= 64 && dtype == 1 && K >= 3000 && (matrices == 2 || (K >= 4000 && N >= 4000)));
     return M && rows && N >= 256 && (uint64_t)matrices * K >= 3000 && N % lane == 0 && K % lane == 0 &&
            (K + 64ull) * N * t < (1ull << 31);
 }
@@ -266,7 +270,9 @@ static hipError_t rows_mb(const ProductLaunch &p, const typename Epi::Params &e,
 template <typename T, class Epi>
 static hipError_t rows_t(const ProductLaunch &p, const typename Epi::Params &e, float *planes, hipStream_t s) {
     if constexpr (sizeof(T) == 2 || EpiPair<Epi>::value)
-        if (p.g.M > 16) return rows_mb<T, Epi, 2>(p, e, planes, s);
+        if (p.g.M > 16 && p.g.M <= 32) return rows_mb<T, Epi, 2>(p, e, planes, s);
+    if constexpr (sizeof(T) == 2)
+        if (p.g.M > 32) return rows_mb<T, Epi, 4>(p, e, planes, s);
     return rows_mb<T, Epi, 1>(p, e, planes, s);
 }
 

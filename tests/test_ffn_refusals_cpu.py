@@ -217,7 +217,8 @@ def test_work_bytes():
     need = abi.load().skl_product_work_bytes
     assert need(0, 4001, 130, 1500, 2) == 0            # fp32 takes operands as they are
     assert need(0, 16, 4096, 1024, 1) == 8 * 16 * 1024 * 4   # few rows over a long k: its slices' sums
-    assert need(1, 16, 4096, 8192, 2) == 8 * 16 * 8192 * 4 * 2 and need(1, 33, 4096, 8192, 2) == 0
+    assert need(1, 16, 4096, 8192, 2) == 8 * 16 * 8192 * 4 * 2 and need(1, 65, 4096, 8192, 2) == 0
+    assert need(1, 64, 4096, 8192, 2) == 8 * 64 * 8192 * 4 * 2 and need(1, 64, 4096, 1024, 1) == need(0, 33, 4096, 8192, 2) == 0
     assert need(1, 32, 4096, 1024, 1) == 8 * 32 * 1024 * 4 and need(0, 32, 4096, 1024, 1) == 0
     assert need(1, 64, 130, 1500, 2) == 0              # too few tiles for padded copies
     assert need(1, 16384, 2048, 4096, 2) == 0          # whole tiles

@@ -92,7 +92,8 @@ def test_forward_copies_of_one_operand(monkeypatch, ctx, m, k, n, place):
 # that ends inside a step, slices without any, and sizes on both sides of the rule's borders
 FEW_ROWS = [(1, 3000, 256), (3, 4096, 1000), (16, 3008, 2056), (16, 1500, 260), (17, 3000, 264), (2, 3001, 264), (5, 2999, 256),
             (9, 1504, 8200), (1, 1500, 16400), (7, 1512, 32776), (16, 40000, 256), (1, 6004, 252),
-            (32, 3000, 256), (31, 1504, 4104), (18, 3008, 1000), (32, 1500, 16388), (33, 3000, 256)]
+            (32, 3000, 256), (31, 1504, 4104), (18, 3008, 1000), (32, 1500, 16388), (33, 3000, 256),
+            (64, 3008, 264), (49, 4000, 4000)]
 
 
 @pytest.mark.parametrize("t", TYPES, ids=IDS)
@@ -320,3 +321,21 @@ def test_workspace_makes_no_difference_but_for_order(ctx):
     for out in got:
         check(out, ref, t, "out")
     within(got[0], got[1].double(), 2 * ref[1] + 2 * half_step(ref[0], t), "both")
+
+
+@pytest.mark.parametrize("t", TYPES, ids=IDS)
+def test_few_rows_with_a_workspace_too_small(ctx, t):
+    """... and so does one of few rows, whose sums over slices of k do not fit; what lies behind the given bytes stays."""
+    m, k, n = 7, 4096, 520
+    need = abi.load().skl_product_work_bytes(int(t == torch.float16), m, k, n, 2)
+    wg, wu, _, _ = weights(k, n, t, 1, False)
+    x = values((m, k), t, 2)
+    g = Gated(ctx, wg, wu, outputs=n, half=t == torch.float16)
+    work = torch.full((need + 4096,), 171, dtype=torch.uint8, device="cuda")
+    for size in (0, 16, need - 16, need):
+        g.work.product = lambda *_: (work.data_ptr(), size)
+        out = filled((m, n), t)
+        g.forward(x, out)
+        torch.cuda.synchronize()
+        check(out, gated_ref(x, wg, wu, None, None, abi.ACT_SILU)["out"], t, "out")
+        assert bool((work[size:] == 171).all()), size
