@@ -2131,12 +2131,17 @@ bool plan_copied(const ProductLaunch &p, Copies *c, GemmPlan *plan) {
     return true;
 }
 
-// Epilogues that read tensors of their own go element by element where the rows are not on 4 columns;
-// 128x128 tiles then need two workgroups to every CU to keep enough loads and stores in flight (from
-// the layer above, 2000 x 1531, K 1000: 32.6 us, 24.4 on the K-splitting kernel's 768 tiles; the
-// projection 38.7 and 32.3; 8000 x 2047, K 1531: 160 and 207).
-bool slow_rag(const ProductLaunch &p) {
+// Epilogues that read tensors of their own keep too few loads and stores in flight from few 128x128
+// tiles, a gated block's error with its six tensors most: from the layer above 1000 x 2048, K 400: 19.1 us,
+// 11.1 on the K-splitting kernel's 64x64 tiles; 500 x 6000, K 800: 31.1, 24.0; 801 x 5008, K 600: 31.2, 27.7;
+// but 4000 x 1432, K 400 (384 tiles): 36.0, 39.0.  (Of whole tiles: 1024 x 2048, K 512, 128 of them: 15.1,
+// 10.2; 2048 x 2048, 256: 18.7, 19.9.)  Where the rows are not on 4 columns they go element by
+// element, and two workgroups to every CU are wanted (2000 x 1531, K 1000: 32.6, 24.4; the projection
+// 38.7, 32.3; 8000 x 2047, K 1531: 160, 207).
+bool slow_dma(const ProductLaunch &p) {
     const uint64_t tiles = (uint64_t)((p.g.M + 127) / 128) * ((p.g.N + 127) / 128);
+    const bool whole = p.g.M % 128 == 0 && p.g.N % 128 == 0 && p.g.K % 128 == 0;
+    if (p.kind == Product::Ungate && tiles < (whole ? 200u : 300u)) return true;
     return (p.kind == Product::Ungate || p.kind == Product::Project) && p.g.N % 4 != 0 && tiles < 512;
 }
 
@@ -2166,22 +2171,23 @@ int32_t run_product(skl_ctx *ctx, ProductLaunch p, void *work, size_t work_bytes
     const GemmLaunch g = planned_gemm(p);
     PlanCtx how{};
     how.heavy = p.kind == Product::Ungate;
-    how.no_rag = (chain && p.g.K % 8 != 0) || slow_rag(p);
+    const bool slow = slow_dma(p);
+    how.no_rag = (chain && p.g.K % 8 != 0) || slow;
     GemmPlan plan = plan_gemm(g, ctx->route, how), other{};
     Copies copies = product_copies(p, plan.pad_a, plan.pad_b, true), small{};
     const bool planned = ctx->route.kind == Route::Planned, copied = ctx->route.kind == Route::Copied;
     if ((planned || copied) && plan_copied(p, &small, &other) && small.bytes() <= work_bytes &&
-        (copied || (!slow_rag(p) && !plan.dma && other.us < ROUTE_MARGIN * plan.us))) {
+        (copied || (!slow && !plan.dma && other.us < ROUTE_MARGIN * plan.us))) {
         plan = other;
         copies = small;
     } else {
         SKL_CHECK(!copied && !plan.refused && !plan.skinny && !(plan.rag && chain && how.no_rag), SKL_ERR_INVALID_CONFIGURATION);
-        const bool staged = !plan.dma && !plan.wave;
-        if (staged || (plan.dma && !plan.rag && copies.bytes() > work_bytes)) {
+        const bool staged = !plan.dma && !plan.wave, few = planned && slow && plan.dma && plan.tile == 128;
+        if (staged || few || (plan.dma && !plan.rag && copies.bytes() > work_bytes)) {
             SKL_CHECK(planned, SKL_ERR_INVALID_CONFIGURATION);
             uint32_t splits = 1;
             double us = 0.0;
-            if (plan_dma128(g, &other) && !(chain && how.no_rag && other.rag))
+            if (!slow && plan_dma128(g, &other) && !(how.no_rag && other.rag))
                 plan = other;
             else
                 SKL_CHECK(plan_wave(g, gemm_wave_tile(g, &splits, &us), 0, 1, &plan), SKL_ERR_INVALID_CONFIGURATION);
