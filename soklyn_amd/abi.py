@@ -179,25 +179,35 @@ def need(name: str, t, dtype, shape: tuple, device: int) -> int:
     return t.data_ptr()
 
 
+class Tracked:
+    """Counts its attributes' changes, so that calls look again at what they have looked at before."""
+    changes = 0
+
+    def __setattr__(self, name, value):
+        object.__setattr__(self, name, value)
+        object.__setattr__(self, "changes", self.changes + 1)
+
+
 class Workspace:
     """Device memory that the calls of one owner share: they follow each other on one stream.  It grows
     on demand; smaller pieces stay (calls in flight and captured ones write there)."""
 
     def __init__(self, ctx: "Context"):
-        self.ctx, self._pieces, self._sizes = ctx, [], {}
+        self.ctx, self._pieces, self._sizes, self._last = ctx, [], {}, (None, 0)
 
     def get(self, size: int) -> tuple[int | None, int]:
         """The address and size of a piece of at least `size` bytes."""
         if not size:
             return None, 0
-        if not self._pieces or self._pieces[-1].numel() < size:
+        if self._last[1] < size:
             import torch
             # of the context's stream: what held the memory before is done there, and so is this owner
             # when another allocation gets it
             with torch.cuda.stream(torch.cuda.ExternalStream(load().skl_ctx_stream(self.ctx.h), self.ctx.device)):
-                self._pieces.append(torch.empty(size, device=f"cuda:{self.ctx.device}", dtype=torch.uint8))
-        piece = self._pieces[-1]
-        return piece.data_ptr(), piece.numel()
+                piece = torch.empty(size, device=f"cuda:{self.ctx.device}", dtype=torch.uint8)
+            self._pieces.append(piece)
+            self._last = piece.data_ptr(), size
+        return self._last
 
     def product(self, *sizes: int) -> tuple[int | None, int]:
         """For skl_product_work_bytes(*sizes): dtype, batch, inputs, outputs, matrices."""

@@ -18,7 +18,7 @@ from .devblock import DeviceBlock
 _F32, _F16 = torch.float32, torch.float16
 
 
-class Gated:
+class Gated(abi.Tracked):
     """The weights wg and wu [inputs x outputs] and biases [1 x outputs] (or None) of both projections, held by
     reference; act is the gate's activation.  The weights may be None where only error_from_sum and hidden_error
     are called.  Calls share a workspace and follow each other on one stream."""
@@ -30,22 +30,22 @@ class Gated:
         self.dtype = _F16 if half else _F32
         self.inputs = 1 if wg is None else wg.shape[0]
         self.wg, self.wu, self.bg, self.bu, self.work = wg, wu, bg, bu, abi.Workspace(ctx)
-        self._weights()
+        self._check_weights()
         lib = abi.load()
         self._call = lib.skl_gated_forward, lib.skl_gated_error_from_sum, lib.skl_gated_hidden_error, lib.skl_gated_input_grad
         self._local = threading.local()   # descriptors, one set per thread
 
-    def _weights(self):
-        """The addresses of the weights and biases, of the sizes that they have to have."""
+    def _check_weights(self):
         wide, row = (self.inputs, self.outputs), (1, self.outputs)
-        return (self._at("wg", self.wg, self.dtype, wide), self._at("bg", self.bg, self.dtype, row),
-                self._at("wu", self.wu, self.dtype, wide), self._at("bu", self.bu, self.dtype, row))
+        for name, shape in (("wg", wide), ("wu", wide), ("bg", row), ("bu", row)):
+            self._at(name, getattr(self, name), self.dtype, shape)
 
-    def _descs(self, rows: int):
-        """This thread's descriptors of gate, up and the layer above, with the weights as they are now."""
+    def _descs(self, rows: int, weights: bool = True):
+        """This thread's descriptors of gate, up and the layer above; weights: with the weights where they are now."""
         own = self._local.__dict__
-        key = rows, self.inputs, self.outputs, self.half, self.act, self.leaky
+        key = rows, self.changes
         if own.get("key") != key:
+            self._check_weights()
             if not own:
                 own["d"] = tuple(abi.SklDenseDesc() for _ in range(3))
                 own["refs"] = tuple(C.byref(x) for x in own["d"])
@@ -54,7 +54,10 @@ class Gated:
             own["d"][0].act, own["d"][0].leaky = self.act, self.leaky
             own["key"] = key
         gate, up, above = own["d"]
-        gate.w, gate.b, up.w, up.b = self._weights()
+        if weights:
+            for d, w, b in ((gate, self.wg, self.bg), (up, self.wu, self.bu)):
+                d.w = None if w is None else w.data_ptr()
+                d.b = None if b is None else b.data_ptr()
         return gate, up, above, own["refs"]
 
     def _work(self, *sizes):
@@ -79,7 +82,7 @@ class Gated:
 
     def _errors(self, rows, a, u, dg, du, dg_h, du_h):
         t, wide = self.dtype, (rows, self.outputs)
-        gate, up, above, refs = self._descs(rows)
+        gate, up, above, refs = self._descs(rows, False)
         for d, kept, g, h, n in ((gate, a, dg, dg_h, ("a", "dg", "dg_h")), (up, u, du, du_h, ("u", "du", "du_h"))):
             d.preact = self._at(n[0], kept, t, wide)
             d.d_prenorm = self._at(n[1], g, _F32, wide)
