@@ -317,6 +317,24 @@ def test_weights_exchanged_for_others(ctx):
         op.forward(x, torch.empty((5, 400), device="cuda"))
 
 
+def test_weights_moved_in_place(ctx):
+    """A weight whose memory is another one's now is read there."""
+    wg, wu, other = (torch.randn((64, 40), device="cuda") for _ in range(3))
+    x, got, want = torch.randn((5, 64), device="cuda"), torch.empty((5, 40), device="cuda"), torch.empty((5, 40), device="cuda")
+    op, pr = Gated(ctx, wg, wu, outputs=40), Projection(ctx, wg, None, outputs=40)
+    op.forward(x, got)
+    pr.forward(x, None, got)
+    torch.cuda.synchronize()
+    wg.data = other.clone()
+    torch.cuda.synchronize()
+    for of, new in ((op, Gated(ctx, other, wu, outputs=40)), (pr, Projection(ctx, other, None, outputs=40))):
+        args = (x, got) if of is op else (x, None, got)
+        of.forward(*args)
+        new.forward(*args[:-1], want)
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+
+
 def test_two_contexts_at_once(ctx):
     """Steps of two contexts on streams of their own, in flight together, give what each gives alone."""
     side = torch.cuda.Stream()
