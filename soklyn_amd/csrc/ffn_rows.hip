@@ -8,17 +8,19 @@
 // whose n index is then VN (lane % 16) + j; fp32 lanes hold a fragment (16x16x4) as loaded.  The waves'
 // sums are added in LDS, the slices' by a second launch, both in a fixed order, in front of the epilogue.
 //
-// What bounds it: HBM, the weights read once (floor at the 5.12 TB/s of a copy).  One row, the K-splitting
-// kernel's tiles of 16 to 64 columns over all of k in brackets, where each XCD has a narrow strip of every
-// row and few waves share a long k: pair fp16 8192 x 4096 30 us (52; floor 26), 4096 x 8192 30 (36; 26),
-// 11008 x 4096 37 (68; 35), 3000 x 3000 14 (24; 7); fp32 4096 x 8192 54 (66; 52); projection fp16
-// 8192 x 4096 18 (28; 13), 3000 x 3000 9 (13; 3.5).  The second launch costs 3 to 4 us of it: below 3000
-// elements of k in all matrices the other's one launch is ahead (projection 2048 x 2048: 9.2 and 6.2).
-// 17 to 32 rows have two blocks of rows to a fragment of the weights, more have four; fp16 lanes then own 4 columns, as
-// the sums of 8 would not leave registers for the loads ahead.  32 rows: pair fp16 8192 x 4096 36 (57),
-// 4096 x 8192 34 (38), 11008 x 4096 44 (76), fp32 4096 x 8192 60 (75); projection fp16 8192 x 4096 22
-// (37), 4096 x 1024 8.9 (9.2).  64 rows, fp16: pair 8192 x 4096 43 (74), 4096 x 8192 39 (42), projection
-// 8192 x 4096 27 (34).
+// What bounds it: HBM, the weights read once (floor at the 5.12 TB/s of a copy).  One row, weights from
+// memory, the K-splitting kernel's tiles of 16 to 64 columns over all of k in brackets, where each XCD has
+// a narrow strip of every row and few waves share a long k: pair fp16 8192 x 4096 30 us (63; floor 26),
+// 4096 x 8192 29 (36; 26), 11008 x 4096 37 (83; 35), 3000 x 3000 14 (21; 7), 4096 x 1024 13 (27; 3); fp32
+// 4096 x 8192 52 (66; 52); projection fp16 8192 x 4096 18 (28; 13), 3000 x 3000 9.3 (10; 3.5).  The second
+// launch costs 3 to 4 us of it: below 3000 elements of k in all matrices the other's one launch is ahead
+// (projection 2048 x 2048: 9.2 and 6.2), and so it can be where caches hold the weights (pair 4096 x 1024,
+// called again at once: 9.6 and 7.5), which a network's layers between two calls do not leave there.
+// 17 to 32 rows have two blocks of rows to a fragment of the weights, more have four; fp16 lanes then own 4
+// columns, as the sums of 8 would not leave registers for the loads ahead.  32 rows: pair fp16 8192 x 4096
+// 37 (69), 4096 x 8192 33 (38), 11008 x 4096 45 (93), fp32 4096 x 8192 61 (75); projection fp16 8192 x 4096
+// 22 (38), 4096 x 1024 9.4 (14).  64 rows, fp16: pair 8192 x 4096 42 (74), 4096 x 8192 39 (41), projection
+// 8192 x 4096 27 (35).
 #include "ffn.h"
 #include "ffn_epi.h"
 #include "gemm.h"
