@@ -2091,22 +2091,6 @@ Copies product_copies(const ProductLaunch &p, bool a, bool b, bool whole) {
     return c;
 }
 
-// The GEMM by which a product is planned: one of twice the columns (pair) or twice the k (chain).
-// Addresses stand for their alignment.
-GemmLaunch planned_gemm(const ProductLaunch &p) {
-    GemmLaunch g = p.g;
-    const bool two_b = p.kind == Product::Pair || p.kind == Product::Chain;
-    const void *b2 = p.kind == Product::Pair ? p.pair.b2 : p.chain.b2, *a2 = p.chain.a2;
-    auto both = [](const void *x, const void *y) {
-        return reinterpret_cast<const void *>(reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(y));
-    };
-    if (two_b) g.B = both(g.B, b2);
-    if (p.kind == Product::Chain) g.A = both(g.A, a2);
-    if (p.kind == Product::Pair) g.N *= 2;
-    if (p.kind == Product::Chain) g.K *= 2;
-    return g;
-}
-
 // fp16 operands that the direct-to-LDS kernel on 128x128 tiles cannot take as stored (odd rows, k in
 // part of a 16-byte piece): copies that it can, and the plan of the product over them.  False where
 // there are none, or they do not fit either.

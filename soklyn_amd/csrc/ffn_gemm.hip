@@ -42,6 +42,23 @@ static bool rows_on(const ProductLaunch &p, uint32_t group) {
 
 bool product_rows4(const ProductLaunch &p) { return rows_on(p, 4); }
 
+GemmLaunch planned_gemm(const ProductLaunch &p) {
+    GemmLaunch g = p.g;
+    auto both = [](const void *x, const void *y) {
+        return reinterpret_cast<const void *>(reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(y));
+    };
+    if (p.kind == Product::Pair) {
+        g.B = both(g.B, p.pair.b2);
+        g.N *= 2;
+    }
+    if (p.kind == Product::Chain) {
+        g.A = both(g.A, p.chain.a2);
+        g.B = both(g.B, p.chain.b2);
+        g.K *= 2;
+    }
+    return g;
+}
+
 // ---- direct-to-LDS ---------------------------------------------------------------------
 template <class Epi, bool BK, int NW, bool EDGE, int BT, bool RAG>
 static hipError_t run_dma(const ProductLaunch &p, const typename Epi::Params &e, bool whole, hipStream_t s) {
@@ -86,10 +103,13 @@ static hipError_t dma(const ProductLaunch &p, const typename Epi::Params &e, hip
 static hipError_t launch_dma(const ProductLaunch &p, hipStream_t s) {
     const GemmLaunch &g = p.g;
     if (g.dtype != 1 || !g.M || !g.N || !g.K) return hipErrorInvalidValue;
-    if (!g.rag) {
+    const GemmLaunch all = planned_gemm(p);
+    if (g.rag) {
+        if (g.K % 8 || !gemm_dma_rag_ok(all)) return hipErrorInvalidValue;
+    } else {
         const uint32_t t = g.tile == 128 ? 128 : 256, tn = p.kind == Product::Pair ? t / 2 : t;
-        if (g.M % t || g.N % tn || g.K % (p.kind == Product::Chain ? 64 : 128) || g.lda % 8 || g.ldb % 8 || !on16(g.A) ||
-            !on16(g.B))
+        if (g.M % t || g.N % tn || g.K % (p.kind == Product::Chain ? 64 : 128) || g.lda % 8 || g.ldb % 8 || !on16(all.A) ||
+            !on16(all.B))
             return hipErrorInvalidValue;
     }
     switch (p.kind) {
@@ -116,7 +136,7 @@ static uint64_t wave_tiles(const ProductLaunch &p) {
 }
 // (16 waves of a pair's 16x16 tiles would not leave the registers for the sum over them)
 static uint32_t wave_waves(const ProductLaunch &p) {
-    return p.kind == Product::Pair && p.g.tile == 16 ? 8 : p.g.waves ? p.g.waves : gemm_wave_waves(p.g, p.g.tile);
+    return p.kind == Product::Pair && p.g.tile == 16 ? 8 : p.g.waves ? p.g.waves : gemm_wave_waves(planned_gemm(p), p.g.tile);
 }
 uint64_t product_threads(const ProductLaunch &p) { return wave_tiles(p) * 64 * wave_waves(p); }
 
@@ -144,7 +164,7 @@ static hipError_t wave(const ProductLaunch &p, const typename Epi::Params &e, hi
     constexpr bool PAIR = EpiPair<Epi>::value;
     const uint32_t code = p.g.tile * 32 + wave_waves(p);
     if constexpr (sizeof(T) == 2) {
-        if (!wave_dword_rows(p.g)) {
+        if (!wave_dword_rows(planned_gemm(p))) {
             switch (code) {
             case 16 * 32 + 8: if constexpr (PAIR) return run_wave_t<T, Epi, BK, true, 1, 8, 1, 2>(p, e, s); break;
             case 16 * 32 + 16: if constexpr (!PAIR) return run_wave_t<T, Epi, BK, true, 1, 16, 1, 4>(p, e, s); break;
