@@ -180,7 +180,7 @@ def need(name: str, t, dtype, shape: tuple, device: int) -> int:
 
 
 class Tracked:
-    """Counts its attributes' changes, so that calls look again at what they have looked at before."""
+    """Counts its attributes' changes, so that a descriptor filled for some calls is filled again behind one."""
     changes = 0
 
     def __setattr__(self, name, value):

@@ -30,22 +30,22 @@ class Gated(abi.Tracked):
         self.dtype = _F16 if half else _F32
         self.inputs = 1 if wg is None else wg.shape[0]
         self.wg, self.wu, self.bg, self.bu, self.work = wg, wu, bg, bu, abi.Workspace(ctx)
-        self._check_weights()
+        self._weights()
         lib = abi.load()
         self._call = lib.skl_gated_forward, lib.skl_gated_error_from_sum, lib.skl_gated_hidden_error, lib.skl_gated_input_grad
         self._local = threading.local()   # descriptors, one set per thread
 
-    def _check_weights(self):
-        wide, row = (self.inputs, self.outputs), (1, self.outputs)
-        for name, shape in (("wg", wide), ("wu", wide), ("bg", row), ("bu", row)):
-            self._at(name, getattr(self, name), self.dtype, shape)
+    def _weights(self):
+        """The addresses of wg, wu, bg and bu, looked at each time: a tensor held by reference may have become another."""
+        t, wide, row = self.dtype, (self.inputs, self.outputs), (1, self.outputs)
+        return (self._at("wg", self.wg, t, wide), self._at("wu", self.wu, t, wide), self._at("bg", self.bg, t, row),
+                self._at("bu", self.bu, t, row))
 
     def _descs(self, rows: int, weights: bool = True):
-        """This thread's descriptors of gate, up and the layer above; weights: with the weights where they are now."""
+        """This thread's descriptors of gate, up and the layer above; weights: with the weights as they are now."""
         own = self._local.__dict__
         key = rows, self.changes
         if own.get("key") != key:
-            self._check_weights()
             if not own:
                 own["d"] = tuple(abi.SklDenseDesc() for _ in range(3))
                 own["refs"] = tuple(C.byref(x) for x in own["d"])
@@ -55,9 +55,7 @@ class Gated(abi.Tracked):
             own["key"] = key
         gate, up, above = own["d"]
         if weights:
-            for d, w, b in ((gate, self.wg, self.bg), (up, self.wu, self.bu)):
-                d.w = None if w is None else w.data_ptr()
-                d.b = None if b is None else b.data_ptr()
+            gate.w, up.w, gate.b, up.b = self._weights()
         return gate, up, above, own["refs"]
 
     def _work(self, *sizes):

@@ -133,28 +133,27 @@ class Projection(abi.Tracked):
         self.dtype = torch.float16 if half else torch.float32
         self.inputs = 1 if w is None else w.shape[0]
         self.w, self.b, self.work = w, b, abi.Workspace(ctx)
-        self._check_weights()
+        self._weights()
         self._call = abi.load().skl_dense_forward_residual, abi.load().skl_dense_residual_error
         self._local = threading.local()   # descriptors, one per thread
 
-    def _check_weights(self):
-        for name, t, rows in (("w", self.w, self.inputs), ("b", self.b, 1)):
-            if t is not None:
-                abi.need(name, t, self.dtype, (rows, self.outputs), self.ctx.device)
+    def _weights(self):
+        """The addresses of w and b, looked at each time: a tensor held by reference may have become another."""
+        t, n, dev = self.dtype, self.outputs, self.ctx.device
+        return (None if self.w is None else abi.need("w", self.w, t, (self.inputs, n), dev),
+                None if self.b is None else abi.need("b", self.b, t, (1, n), dev))
 
     def _desc(self, rows: int) -> abi.SklDenseDesc:
         own = self._local.__dict__
         key = rows, self.changes
         if own.get("key") != key:
-            self._check_weights()
             d = own["desc"] = abi.SklDenseDesc()
             own["ref"] = C.byref(d)
             d.dtype, d.inputs, d.outputs, d.max_batch = int(self.half), self.inputs, self.outputs, rows
             d.act, d.leaky, d.mask_coeff, d.is_training = self.act, self.leaky, self.dropout, 1
             own["key"] = key
         d = own["desc"]
-        d.w = None if self.w is None else self.w.data_ptr()
-        d.b = None if self.b is None else self.b.data_ptr()
+        d.w, d.b = self._weights()
         return d
 
     def forward(self, x: torch.Tensor, stream: torch.Tensor | None, h: torch.Tensor, *, preact: torch.Tensor | None = None,
