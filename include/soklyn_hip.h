@@ -332,7 +332,9 @@ size_t skl_mxfp4_work_bytes(uint32_t inputs, uint32_t outputs, uint32_t batch);
  * inputs and outputs; a NULL b is no bias.  in is [in_rows x inputs] T, its first `batch`
  * rows are used; out is [batch x outputs] T.  Where gate->preact / up->preact are not
  * NULL, a / u are kept there (rounded to T) for the backward.  out is computed from the
- * fp32 sums and rounded once.  No output may overlap an input.
+ * fp32 sums and rounded once.  No output may overlap an input.  The activations here and in
+ * the calls below are the blocks', but that Mish of a z whose e^z overflows is z (slope 1),
+ * where a block follows the reference's NaN.
  * work (16-byte aligned, or NULL): skl_product_work_bytes(dtype, batch, inputs, outputs,
  * 2) bytes of the caller's for padded copies of ragged fp16 operands, or for the sums over
  * slices of a long k where the rows are few; with less, a kernel runs that does without

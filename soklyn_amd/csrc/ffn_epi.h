@@ -13,15 +13,18 @@
 namespace skl {
 
 // Activations of these operators, for both types from the hardware's exp2 and reciprocal but for
-// fp32 blocks' Mish; tanh by its series near 0 (tanhf is several times the work of the rest).
+// fp32 blocks' Mish; tanh by its series near 0 (tanhf is several times the work of the rest).  Mish is z
+// and its slope 1 above 20, where tanh(softplus(z)) is off 1 by 2 e^-40 at most: the blocks' forms say
+// NaN from 88.7 on, where e^z overflows, as the reference does; these operators have none to follow.
 // N at a time: the choice of the activation outside the elements, whose chains of exp and reciprocal
 // then run beside each other.
 template <typename T, uint32_t ACT, bool SLOPE, int N>
 __device__ __forceinline__ void ffn_act_as(const float (&z)[N], float leaky, float (&v)[N], float (&d)[N]) {
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-        v[j] = ACT == 4 ? tanh_fast(z[j]) : activation<T>(ACT, z[j], leaky);
-        if constexpr (SLOPE) d[j] = activation_derivative<T>(ACT, 1.0f, v[j], z[j], leaky);
+        const bool far = ACT == 7 && z[j] > 20.0f;
+        v[j] = ACT == 4 ? tanh_fast(z[j]) : far ? z[j] : activation<T>(ACT, z[j], leaky);
+        if constexpr (SLOPE) d[j] = far ? 1.0f : activation_derivative<T>(ACT, 1.0f, v[j], z[j], leaky);
     }
 }
 template <typename T, bool SLOPE, int N>
