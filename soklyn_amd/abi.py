@@ -190,7 +190,8 @@ class Tracked:
 
 class Workspace:
     """Device memory that the calls of one owner share: they follow each other on one stream.  It grows
-    on demand; smaller pieces stay (calls in flight and captured ones write there)."""
+    on demand; smaller pieces stay (calls in flight and captured ones write there).  Each piece behind the
+    first is twice the last or more, so that all of them are less than four times the largest call's."""
 
     def __init__(self, ctx: "Context"):
         self.ctx, self._pieces, self._sizes, self._last = ctx, [], {}, (None, 0)
@@ -204,15 +205,21 @@ class Workspace:
             # of the context's stream: what held the memory before is done there, and so is this owner
             # when another allocation gets it
             with torch.cuda.stream(torch.cuda.ExternalStream(load().skl_ctx_stream(self.ctx.h), self.ctx.device)):
-                piece = torch.empty(size, device=f"cuda:{self.ctx.device}", dtype=torch.uint8)
+                where = dict(device=f"cuda:{self.ctx.device}", dtype=torch.uint8)
+                try:
+                    piece = torch.empty(max(size, 2 * self._last[1]), **where)
+                except torch.OutOfMemoryError:
+                    piece = torch.empty(size, **where)
             self._pieces.append(piece)
-            self._last = piece.data_ptr(), size
+            self._last = piece.data_ptr(), piece.numel()
         return self._last
 
     def product(self, *sizes: int) -> tuple[int | None, int]:
         """For skl_product_work_bytes(*sizes): dtype, batch, inputs, outputs, matrices."""
         size = self._sizes.get(sizes)
         if size is None:
+            if len(self._sizes) >= 1024:
+                self._sizes.clear()
             size = self._sizes[sizes] = load().skl_product_work_bytes(*sizes)
         return self.get(size) if size else (None, 0)
 
