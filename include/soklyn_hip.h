@@ -353,17 +353,22 @@ int32_t skl_gated_forward(skl_ctx *ctx, const skl_dense_desc *gate, const skl_de
 int32_t skl_gated_error_from_sum(skl_ctx *ctx, const skl_dense_desc *gate, const skl_dense_desc *up, const float *s,
                                  uint32_t batch);
 /* The same from the layer above, s = next.d_prenorm . next.W^T in the kernel's registers
- * (fp16: next's d_prenorm_h and W, fp32 sums).  work: skl_product_work_bytes(dtype, batch,
- * next->outputs, outputs, 1). */
+ * (fp16: next's d_prenorm_h and W, fp32 sums).  work: skl_product_grad_work_bytes(dtype,
+ * batch, next->outputs, outputs, 1). */
 int32_t skl_gated_hidden_error(skl_ctx *ctx, const skl_dense_desc *gate, const skl_dense_desc *up,
                                const skl_dense_desc *next, uint32_t batch, void *work, size_t work_bytes);
 /* dx[batch x inputs] fp32 = gate.d_prenorm . Wg^T + up.d_prenorm . Wu^T (fp16: of the
- * fp16 copies), one sum.  work: skl_product_work_bytes(dtype, batch, outputs, inputs, 2). */
+ * fp16 copies), one sum.  work: skl_product_grad_work_bytes(dtype, batch, outputs,
+ * inputs, 2). */
 int32_t skl_gated_input_grad(skl_ctx *ctx, const skl_dense_desc *gate, const skl_dense_desc *up, uint32_t batch,
                              float *dx, void *work, size_t work_bytes);
-/* Host side: bytes of work for a product of `batch` rows of `inputs` with `matrices` (1 or
- * 2) matrices to `outputs`; 0 where none is used. */
+/* Host side: bytes of work for a forward product (the gated forward, a projection) of
+ * `batch` rows of `inputs` with `matrices` (1 or 2) matrices to `outputs`, and for a backward
+ * one; 0 where sizes and type have no use for any (a call may have none either, for where its
+ * tensors lie). */
 size_t skl_product_work_bytes(uint32_t dtype, uint32_t batch, uint32_t inputs, uint32_t outputs, uint32_t matrices);
+size_t skl_product_grad_work_bytes(uint32_t dtype, uint32_t batch, uint32_t inputs, uint32_t outputs,
+                                   uint32_t matrices);
 
 /* ---- a block's result added to the residual stream, dropout (no counterpart) --- */
 /* z = in . W + b,  h = scale * x + drop(act(z)): a block without a norm (any activation but

@@ -171,6 +171,7 @@ extern "C" {
     pub fn skl_gated_input_grad(ctx: *mut SklCtx, gate: *const SklDenseDesc, up: *const SklDenseDesc, batch: u32,
                                 dx: *mut f32, work: *mut c_void, work_bytes: usize) -> i32;
     pub fn skl_product_work_bytes(dtype: u32, batch: u32, inputs: u32, outputs: u32, matrices: u32) -> usize;
+    pub fn skl_product_grad_work_bytes(dtype: u32, batch: u32, inputs: u32, outputs: u32, matrices: u32) -> usize;
     pub fn skl_dense_forward_residual(ctx: *mut SklCtx, blk: *const SklDenseDesc, input: *const c_void,
                                       in_rows: u32, in_cols: u32, batch: u32, use_dropout: u32, seed: u32,
                                       stream_dtype: u32, scale: f32, x: *const c_void, h: *mut c_void,

@@ -107,6 +107,7 @@ _SIGS = {
     "skl_gated_input_grad": (C.c_int32, [_VP, C.POINTER(SklDenseDesc), C.POINTER(SklDenseDesc), C.c_uint32, _VP, _VP,
                                          C.c_size_t]),
     "skl_product_work_bytes": (C.c_size_t, [C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32]),
+    "skl_product_grad_work_bytes": (C.c_size_t, [C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32]),
     "skl_dense_forward_residual": (C.c_int32, [_VP, C.POINTER(SklDenseDesc), _VP, C.c_uint32, C.c_uint32, C.c_uint32,
                                                C.c_uint32, C.c_uint32, C.c_uint32, C.c_float, _VP, _VP, _VP,
                                                C.c_size_t]),
@@ -216,11 +217,18 @@ class Workspace:
 
     def product(self, *sizes: int) -> tuple[int | None, int]:
         """For skl_product_work_bytes(*sizes): dtype, batch, inputs, outputs, matrices."""
-        size = self._sizes.get(sizes)
+        return self._sized("skl_product_work_bytes", sizes)
+
+    def gradient(self, *sizes: int) -> tuple[int | None, int]:
+        """For skl_product_grad_work_bytes(*sizes)."""
+        return self._sized("skl_product_grad_work_bytes", sizes)
+
+    def _sized(self, how: str, sizes: tuple[int, ...]) -> tuple[int | None, int]:
+        size = self._sizes.get((how, sizes))
         if size is None:
             if len(self._sizes) >= 1024:
                 self._sizes.clear()
-            size = self._sizes[sizes] = load().skl_product_work_bytes(*sizes)
+            size = self._sizes[how, sizes] = getattr(load(), how)(*sizes)
         return self.get(size) if size else (None, 0)
 
 

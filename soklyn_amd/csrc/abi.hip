@@ -2254,9 +2254,14 @@ int32_t check_work(const void *work) {
 }  // namespace
 
 size_t skl_product_work_bytes(uint32_t dtype, uint32_t batch, uint32_t inputs, uint32_t outputs, uint32_t matrices) {
-    if (dtype > SKL_F16 || !batch || !inputs || !outputs || !matrices || matrices > 2) return 0;
-    if (product_rows_size(dtype, batch, outputs, inputs, matrices)) return product_rows_bytes(batch, outputs, matrices);
-    if (dtype != SKL_F16) return 0;
+    if (dtype <= SKL_F16 && batch && inputs && outputs && (matrices == 1 || matrices == 2) &&
+        product_rows_size(dtype, batch, outputs, inputs, matrices))
+        return product_rows_bytes(batch, outputs, matrices);
+    return skl_product_grad_work_bytes(dtype, batch, inputs, outputs, matrices);
+}
+
+size_t skl_product_grad_work_bytes(uint32_t dtype, uint32_t batch, uint32_t inputs, uint32_t outputs, uint32_t matrices) {
+    if (dtype != SKL_F16 || !batch || !inputs || !outputs || !matrices || matrices > 2) return 0;
     // few rows take the operands as they are; so do whole tiles
     const uint64_t mp = ((uint64_t)batch + 255) / 256, np = ((uint64_t)outputs + 255) / 256;
     if (batch < 128 || (batch % 256 == 0 && inputs % 128 == 0 && outputs % 256 == 0)) return 0;

@@ -58,9 +58,6 @@ class Gated(abi.Tracked):
             gate.w, up.w, gate.b, up.b = self._weights()
         return gate, up, above, own["refs"]
 
-    def _work(self, *sizes):
-        return self.work.product(int(self.half), *sizes)
-
     def _at(self, name, t, dtype, shape):
         return None if t is None else abi.need(name, t, dtype, shape, self.ctx.device)
 
@@ -73,7 +70,8 @@ class Gated(abi.Tracked):
         gate, up, _, (rg, ru, _) = self._descs(rows)
         gate.preact, up.preact = self._at("a", a, t, wide), self._at("u", u, t, wide)
         rc = self._call[0](self.ctx.h, rg, ru, self._at("x", x, t, (rows, self.inputs)), rows, self.inputs, rows,
-                           self._at("out", out, t, wide), *self._work(rows, self.inputs, self.outputs, 2))
+                           self._at("out", out, t, wide),
+                           *self.work.product(int(self.half), rows, self.inputs, self.outputs, 2))
         if rc:
             raise abi.SklError("skl_gated_forward", rc)
         return out
@@ -108,7 +106,7 @@ class Gated(abi.Tracked):
         above.w = self._at("above_w", above_w, t, (self.outputs, n))
         d = self._at("above_d", above_d, t, (rows, n))
         above.d_prenorm, above.d_prenorm_h = (None, d) if self.half else (d, None)
-        rc = self._call[2](self.ctx.h, rg, ru, rn, rows, *self._work(rows, n, self.outputs, 1))
+        rc = self._call[2](self.ctx.h, rg, ru, rn, rows, *self.work.gradient(int(self.half), rows, n, self.outputs, 1))
         if rc:
             raise abi.SklError("skl_gated_hidden_error", rc)
 
@@ -120,7 +118,7 @@ class Gated(abi.Tracked):
             p = self._at(n, g, t, (rows, self.outputs))
             d.d_prenorm, d.d_prenorm_h = (None, p) if half else (p, None)
         rc = self._call[3](self.ctx.h, rg, ru, rows, self._at("dx", dx, _F32, (rows, self.inputs)),
-                           *self._work(rows, self.outputs, self.inputs, 2))
+                           *self.work.gradient(int(self.half), rows, self.outputs, self.inputs, 2))
         if rc:
             raise abi.SklError("skl_gated_input_grad", rc)
         return dx
@@ -151,7 +149,7 @@ class GatedBlock:
     def hidden_error(self, nxt: DeviceBlock, batch: int):
         g = self.gate
         abi.call("skl_gated_hidden_error", self.ctx.h, g._fill("unproject"), self.up._fill("unproject"), nxt._fill("above"),
-                 batch, *self.work.product(int(g.half), batch, nxt.outputs, g.outputs, 1))
+                 batch, *self.work.gradient(int(g.half), batch, nxt.outputs, g.outputs, 1))
 
     def input_grad(self, batch: int, out: torch.Tensor | None = None) -> torch.Tensor:
         g, dev = self.gate, self.ctx.device
@@ -159,7 +157,7 @@ class GatedBlock:
             out = torch.empty((batch, g.inputs), device=g.w.device, dtype=_F32)
         abi.call("skl_gated_input_grad", self.ctx.h, g._fill("above"), self.up._fill("above"), batch,
                  abi.need("out", out, _F32, (batch, g.inputs), dev),
-                 *self.work.product(int(g.half), batch, g.outputs, g.inputs, 2))
+                 *self.work.gradient(int(g.half), batch, g.outputs, g.inputs, 2))
         return out
 
     def backward(self, x: torch.Tensor, tc: abi.SklTrainCtx, step: int):

@@ -62,3 +62,33 @@ def test_sizes_looked_up_are_forgotten(taken):
     for m in range(1, 5001):
         assert w.product(0, m, 40, 24, 1) == (None, 0)
     assert len(w._sizes) <= 1024
+
+
+def test_few_rows_reserve_sums_for_the_forward_alone(taken):
+    """The sums over slices of k of few rows are the forward products' (which they alone use); the backward ones take
+    their operands as they are."""
+    from soklyn_amd.gated import Gated
+    got, _ = taken
+    ctx = NoContext()
+    ctx.device = -1   # its tensors are on the CPU
+    rows, inputs, outputs = 8, 256, 1504
+    ones = torch.ones
+    seen = []
+    for k, n, call in ((inputs, outputs, lambda op: op.input_grad(ones(rows, n), ones(rows, n), ones(rows, k))),
+                       (outputs, inputs, lambda op: op.hidden_error(ones(rows, 3000), ones(n, 3000), *(ones(rows, n),) * 2,
+                                                                    **{v: ones(rows, n) for v in ("dg", "du")}))):
+        op = Gated(ctx, ones(k, n), ones(k, n), outputs=n)
+        op._call = tuple(lambda *a: seen.append(a[-2:]) or 0 for _ in op._call)
+        call(op)
+    assert seen == [(None, 0)] * 2 and not got
+
+
+def test_work_of_backward_products():
+    if not os.path.exists(abi.LIB_PATH):
+        pytest.skip("libsoklyn_hip.so not built")
+    forward, back = abi.load().skl_product_work_bytes, abi.load().skl_product_grad_work_bytes
+    for rows in (1, 16, 32, 64, 127):
+        assert back(0, rows, 4096, 8192, 2) == back(1, rows, 4096, 8192, 2) == back(1, rows, 4001, 259, 1) == 0
+    for sizes in ((1, 4001, 130, 1500, 2), (1, 129, 1001, 259, 1), (1, 128, 4096, 8192, 2), (1, 16384, 2048, 4096, 2),
+                  (0, 4001, 130, 1500, 2), (1, 4001, 0, 1500, 2), (1, 4001, 130, 1500, 3)):
+        assert back(*sizes) == forward(*sizes)   # copies of ragged operands
