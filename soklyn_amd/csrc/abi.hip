@@ -430,8 +430,8 @@ uint32_t dw_dma_splits(uint32_t tiles, uint32_t Kp, uint64_t out_elems, uint32_t
 // 12544 x 1536 GEMMs (294 tiles) one 256x256 round plus a 128x128 launch ran
 // 3-4 us slower than 128x128 alone (a launch of fewer 128x128 workgroups than
 // CUs takes as long as a full round of them), hence two rounds at least.
-// *rounds: the estimate, without the band where there is one.
-uint32_t dma_tile(Op op, uint32_t Mp, uint32_t Np, uint32_t splits, uint32_t *band, double *rounds,
+// *rounds: the estimate, without the band where there is one.  one_launch: no band.
+uint32_t dma_tile(Op op, uint32_t Mp, uint32_t Np, uint32_t splits, bool one_launch, uint32_t *band, double *rounds,
                   double *band_rounds) {
     *band = 0;
     const uint32_t R = Mp / 256, Cn = Np / 256;   // 256x256 tile rows and columns
@@ -442,7 +442,7 @@ uint32_t dma_tile(Op op, uint32_t Mp, uint32_t Np, uint32_t splits, uint32_t *ba
     const uint32_t forced = gemm_dma_tile_forced();
     const uint32_t tile = forced ? forced : splits <= 1 && r128 < 0.95 * r256 ? 128u : 256u;
     *rounds = *band_rounds = tile == 128 ? r128 : r256;
-    if (forced || splits > 1 || (op != Op::Fwd && op != Op::InputGrad)) return tile;
+    if (forced || one_launch || splits > 1 || (op != Op::Fwd && op != Op::InputGrad)) return tile;
     double best = *rounds;
     uint32_t best_rows = 0;
     for (uint32_t k = 2; k < (uint32_t)r256; ++k) {
@@ -501,7 +501,7 @@ bool plan_skinny(const GemmLaunch &g, GemmPlan *out) {
 // The direct-to-LDS kernel on operands padded to its tiles where they are not whole, for
 // grids that fill the GPU.  *us: its estimated time, the copies included, for a hidden error
 // that of the whole call.
-bool plan_dma(const GemmLaunch &g, Work w, GemmPlan *out, double *us) {
+bool plan_dma(const GemmLaunch &g, Work w, GemmPlan *out, double *us, bool one_launch = false) {
     if (g.dtype != SKL_F16 || !gemm_dma_enabled() || !g.M || !g.N || !g.K) return false;
     const bool dw = g.op == Op::DwOpt;
     const uint32_t Mp = round_up(g.M, 256), Np = round_up(g.N, 256), Kp = round_up(g.K, 128);
@@ -526,7 +526,7 @@ bool plan_dma(const GemmLaunch &g, Work w, GemmPlan *out, double *us) {
     p.Np = Np;
     p.Kp = Kp;
     p.splits = splits;
-    p.tile = dma_tile(g.op, Mp, Np, splits, &p.band, &rounds, &band_rounds);
+    p.tile = dma_tile(g.op, Mp, Np, splits, one_launch, &p.band, &rounds, &band_rounds);
     if (dw && dw_tile == 128 && !gemm_dma_tile_forced()) p.tile = 128;
     // A: k-contiguous [M x K] or m-contiguous [K x M]; B likewise with N
     p.pad_a = g.a_kcontig ? !dma_operand_ok(g.A, g.M, g.K, g.lda, 256, 128)
@@ -595,15 +595,16 @@ struct PlanCtx {
     bool err_dma, err_wave;    // ... in the epilogue of the direct-to-LDS / K-splitting kernel
     bool no_rag;               // not the direct-to-LDS kernel on operands as stored
     bool heavy;                // an epilogue other than the store, about as dear as the hidden error's
+    bool one_launch;           // no band of 256x256 tiles in front of 128x128 ones
 };
 
-GemmPlan plan_route(const GemmLaunch &g, const GemmRoute &route) {
+GemmPlan plan_route(const GemmLaunch &g, const GemmRoute &route, const PlanCtx &c) {
     GemmPlan p{};
     double us;
     bool ok = true;
     switch (route.kind) {
     case Route::Staged: p = plan_staged(g); break;
-    case Route::Dma: ok = plan_dma(g, Work::Store, &p, &us); break;
+    case Route::Dma: ok = plan_dma(g, Work::Store, &p, &us, c.one_launch); break;
     case Route::Dma128: ok = plan_dma128(g, &p); break;
     case Route::Skinny: ok = plan_skinny(g, &p); break;
     case Route::Copied: ok = false; break;   // the products that ffn.h has
@@ -618,7 +619,7 @@ GemmPlan plan_route(const GemmLaunch &g, const GemmRoute &route) {
 // streaming dW) against 128x128 direct-to-LDS tiles and the K-splitting kernel, by
 // gemm_cost.h.
 GemmPlan plan_gemm(const GemmLaunch &g, const GemmRoute &route, const PlanCtx &c = PlanCtx{}) {
-    if (route.kind != Route::Planned) return plan_route(g, route);
+    if (route.kind != Route::Planned) return plan_route(g, route, c);
     const bool dw = g.op == Op::DwOpt;
     const Work fused = c.err_norm ? Work::ErrNorm : Work::Err;
     const Work w = dw ? Work::Dw : g.op == Op::Fwd ? Work::Fwd : c.heavy ? Work::Err : Work::Store;
@@ -626,7 +627,7 @@ GemmPlan plan_gemm(const GemmLaunch &g, const GemmRoute &route, const PlanCtx &c
     const uint32_t t128 = ((g.M + 127) / 128) * ((g.N + 127) / 128);
     GemmPlan base{}, wave{}, skinny{}, dma128{};
     double base_us = 0.0;
-    const bool dma = plan_dma(g, c.err_dma ? fused : w, &base, &base_us);
+    const bool dma = plan_dma(g, c.err_dma ? fused : w, &base, &base_us, c.one_launch);
     if (dma && gemm_dma_tile_forced()) return base;
     if (dma) {
         base_us += c.err_dma ? 0.0 : err;
@@ -2138,36 +2139,38 @@ bool wide_pair(const ProductLaunch &p) {
     return p.kind == Product::Pair && p.g.dtype == SKL_F16 && tiles * p.g.K >= 160000;
 }
 
-// Plans and launches a product whose g, kind and epilogue are set.  Copies go to the caller's work;
-// where it is too small for them another kernel runs that needs none.
-int32_t run_product(skl_ctx *ctx, ProductLaunch p, void *work, size_t work_bytes) {
-    const bool chain = p.kind == Product::Chain;
+// The kernel of a product whose g, kind and epilogue are set, in p.dma and p.g (rag, tile, waves); `copies`
+// of its operands go to the caller's work, and where it is too small for them another kernel runs that needs
+// none.  rows: the kernels for few rows instead, nothing else is set.
+int32_t plan_product(const GemmRoute &route, ProductLaunch *p, size_t work_bytes, Copies *copies, bool *rows) {
+    const bool chain = p->kind == Product::Chain, pair = p->kind == Product::Pair;
+    const bool planned = route.kind == Route::Planned, copied = route.kind == Route::Copied;
     // offsets of the planned GEMM are 32-bit
-    SKL_CHECK(p.g.N <= 0x7fffffffu && p.g.K <= 0x7fffffffu, SKL_ERR_INVALID_CONFIGURATION);
-    if (ctx->route.kind == Route::Planned && product_rows_ok(p) &&
-        product_rows_bytes(p.g.M, p.g.N, p.kind == Product::Pair ? 2 : 1) <= work_bytes) {
-        p.g.time_start = ctx->gemm_start;
-        p.g.time_stop = ctx->gemm_stop;
-        ctx->gemm_start = ctx->gemm_stop = nullptr;
-        SKL_TRY(launch_product_rows(p, work, ctx->stream));
-        return SKL_OK;
-    }
-    const GemmLaunch g = planned_gemm(p);
+    SKL_CHECK(p->g.N <= 0x7fffffffu && p->g.K <= 0x7fffffffu, SKL_ERR_INVALID_CONFIGURATION);
+    *rows = planned && product_rows_ok(*p) && product_rows_bytes(p->g.M, p->g.N, pair ? 2 : 1) <= work_bytes;
+    if (*rows) return SKL_OK;
+    const GemmLaunch g = planned_gemm(*p);
     PlanCtx how{};
-    how.heavy = p.kind == Product::Ungate;
-    const bool slow = slow_dma(p);
-    how.no_rag = (chain && p.g.K % 8 != 0) || slow;
-    GemmPlan plan = plan_gemm(g, ctx->route, how), other{};
-    Copies copies = product_copies(p, plan.pad_a, plan.pad_b, true), small{};
-    const bool planned = ctx->route.kind == Route::Planned, copied = ctx->route.kind == Route::Copied;
-    if ((planned || copied) && plan_copied(p, &small, &other) && small.bytes() <= work_bytes &&
+    how.heavy = p->kind == Product::Ungate;
+    // A product is one launch, and is priced as one.  A pair over copies keeps the price with a band: the
+    // kernels on operands as stored are slower for a pair than the lines of one matrix say (us, 256x256 tiles over
+    // copies against the kernel that the price of one launch would give: 8872 x 2856, K 1752 0.80 times the speed,
+    // 13233 x 3320, K 776 0.90; of whole tiles 14592 x 1408, K 1280 119.5, 113.3; projection 25344 x 1408, K 640
+    // 126.1, 101.5; chain 13056 x 2816, K 1152 1.04 times).
+    how.one_launch = !pair || (p->g.M % 256 == 0 && p->g.N % 128 == 0 && p->g.K % 128 == 0);
+    const bool slow = slow_dma(*p);
+    how.no_rag = (chain && p->g.K % 8 != 0) || slow;
+    GemmPlan plan = plan_gemm(g, route, how), other{};
+    Copies small{};
+    *copies = product_copies(*p, plan.pad_a, plan.pad_b, true);
+    if ((planned || copied) && plan_copied(*p, &small, &other) && small.bytes() <= work_bytes &&
         (copied || (!slow && !plan.dma && other.us < ROUTE_MARGIN * plan.us))) {
         plan = other;
-        copies = small;
+        *copies = small;
     } else {
         SKL_CHECK(!copied && !plan.refused && !plan.skinny && !(plan.rag && chain && how.no_rag), SKL_ERR_INVALID_CONFIGURATION);
         const bool staged = !plan.dma && !plan.wave, few = planned && slow && plan.dma && plan.tile == 128;
-        if (staged || few || (plan.dma && !plan.rag && copies.bytes() > work_bytes)) {
+        if (staged || few || (plan.dma && !plan.rag && copies->bytes() > work_bytes)) {
             SKL_CHECK(planned, SKL_ERR_INVALID_CONFIGURATION);
             uint32_t splits = 1;
             double us = 0.0;
@@ -2175,23 +2178,38 @@ int32_t run_product(skl_ctx *ctx, ProductLaunch p, void *work, size_t work_bytes
                 plan = other;
             else
                 SKL_CHECK(plan_wave(g, gemm_wave_tile(g, &splits, &us), 0, 1, &plan), SKL_ERR_INVALID_CONFIGURATION);
-            copies = product_copies(p, plan.pad_a, plan.pad_b, true);
+            *copies = product_copies(*p, plan.pad_a, plan.pad_b, true);
         }
     }
+    p->dma = plan.dma;
+    p->g.rag = plan.rag;
+    p->g.tile = plan.tile;
+    if (plan.dma) return SKL_OK;
+    p->g.tile = plan.wave;
+    p->g.waves = plan.waves ? plan.waves : gemm_wave_waves(g, plan.wave);
+    if (planned && plan.wave == 32 && wide_pair(*p)) {
+        p->g.tile = 64;
+        p->g.waves = 4;
+    }
+    SKL_CHECK(product_threads(*p) <= 0xffffffffull, SKL_ERR_INVALID_CONFIGURATION);
+    return SKL_OK;
+}
+
+// Plans and launches a product.
+int32_t run_product(skl_ctx *ctx, ProductLaunch p, void *work, size_t work_bytes) {
+    const bool chain = p.kind == Product::Chain;
+    Copies copies{};
+    bool rows = false;
+    int32_t r;
+    if ((r = plan_product(ctx->route, &p, work_bytes, &copies, &rows))) return r;
     p.g.time_start = ctx->gemm_start;
     p.g.time_stop = ctx->gemm_stop;
-    p.dma = plan.dma;
-    p.g.rag = plan.rag;
-    if (!plan.dma) {
-        p.g.tile = plan.wave;
-        p.g.waves = plan.waves ? plan.waves : gemm_wave_waves(g, plan.wave);
-        if (planned && plan.wave == 32 && wide_pair(p)) {
-            p.g.tile = 64;
-            p.g.waves = 4;
-        }
-        SKL_CHECK(product_threads(p) <= 0xffffffffull, SKL_ERR_INVALID_CONFIGURATION);
-    } else {
-        p.g.tile = plan.tile;
+    if (rows) {
+        ctx->gemm_start = ctx->gemm_stop = nullptr;
+        SKL_TRY(launch_product_rows(p, work, ctx->stream));
+        return SKL_OK;
+    }
+    if (p.dma) {
         p.g.mv = p.g.M;
         p.g.nv = p.g.N;
         char *at = reinterpret_cast<char *>(work);
@@ -2214,7 +2232,7 @@ int32_t run_product(skl_ctx *ctx, ProductLaunch p, void *work, size_t work_bytes
             if (chain) SKL_TRY(copy(p.chain.b2, rows, cols, p.g.ldb, copies.b_rows, copies.b_cols));
             p.g.ldb = copies.b_cols;
         }
-        if (!plan.rag) {   // whole tiles as they are, or padded
+        if (!p.g.rag) {   // whole tiles as they are, or padded
             p.g.M = copies.mp;
             p.g.N = copies.np;
             p.g.K = copies.kp;
@@ -2537,6 +2555,35 @@ const char *skl_diag_gemm_route(uint32_t dtype, uint32_t op, uint32_t M, uint32_
         snprintf(text, sizeof(text), "wave:%u:%u:%u", p.wave, p.waves ? p.waves : gemm_wave_waves(g, p.wave), p.splits);
     else
         snprintf(text, sizeof(text), "%s:%u:%u", kind, p.dma ? p.tile : 0u, p.splits);
+    return text;
+}
+
+// The same for the products of ffn.h: kind 0 the gated forward, 1 its error from the layer above, 2 the
+// projection, 3 the input gradient, each of an output M x N, its workspace given.  off: operands that lie one
+// element off a boundary (1 the left one, 2 its weights, 4 and 8 the second ones of a pair or chain).
+const char *skl_diag_product_route(uint32_t kind, uint32_t dtype, uint32_t M, uint32_t N, uint32_t K, uint32_t off) {
+    static thread_local char text[64];
+    const size_t t = type_size(dtype);
+    auto at = [&](uint32_t bit) { return reinterpret_cast<const void *>(uintptr_t(256) + (off & bit ? t : 0)); };   // never read
+    ProductLaunch p{};
+    p.kind = kind == 0 ? Product::Pair : kind == 1 ? Product::Ungate : kind == 2 ? Product::Project : Product::Chain;
+    const bool forward = kind == 0 || kind == 2;
+    p.g = product_gemm(dtype, forward ? Op::Fwd : Op::InputGrad, M, N, K, K, forward ? N : K, at(1), at(2));
+    p.chain.a2 = at(4);
+    p.pair.b2 = p.chain.b2 = at(8);
+    p.pair.ldc = p.ungate.ldc = p.project.ldc = p.chain.ldc = N;
+    const uint32_t matrices = kind == 0 || kind == 3 ? 2 : 1;
+    const size_t work = (forward ? skl_product_work_bytes : skl_product_grad_work_bytes)(dtype, M, K, N, matrices);
+    Copies copies{};
+    bool rows = false;
+    if (plan_product(GemmRoute{}, &p, work, &copies, &rows))
+        snprintf(text, sizeof(text), "refused");
+    else if (rows)
+        snprintf(text, sizeof(text), "rows");
+    else if (p.dma)
+        snprintf(text, sizeof(text), "dma:%u%s%s", p.g.tile, p.g.rag ? ":stored" : "", copies.a || copies.b ? ":copied" : "");
+    else
+        snprintf(text, sizeof(text), "wave:%u:%u%s", p.g.tile, p.g.waves, product_registers(p) ? ":registers" : "");
     return text;
 }
 

@@ -84,6 +84,8 @@ hipError_t launch_product(const ProductLaunch &p, hipStream_t s);
 // The GEMM as which a product is planned and its kernel's form chosen: of twice the columns (Pair) or
 // twice the k (Chain).  Its addresses stand for the alignment of all operands, the second ones too.
 GemmLaunch planned_gemm(const ProductLaunch &p);
+// The K-splitting kernel takes the operands through registers: rows off 4-byte boundaries.
+bool product_registers(const ProductLaunch &p);
 // The kernels for few rows of a Pair or Project (ffn_rows.hip), which want product_rows_bytes of
 // workspace: whether sizes are theirs, and a product with its alignments.
 hipError_t launch_product_rows(const ProductLaunch &p, void *work, hipStream_t s);

@@ -59,6 +59,8 @@ GemmLaunch planned_gemm(const ProductLaunch &p) {
     return g;
 }
 
+bool product_registers(const ProductLaunch &p) { return !wave_dword_rows(planned_gemm(p)); }
+
 // ---- direct-to-LDS ---------------------------------------------------------------------
 template <class Epi, bool BK, int NW, bool EDGE, int BT, bool RAG>
 static hipError_t run_dma(const ProductLaunch &p, const typename Epi::Params &e, bool whole, hipStream_t s) {
@@ -164,7 +166,7 @@ static hipError_t wave(const ProductLaunch &p, const typename Epi::Params &e, hi
     constexpr bool PAIR = EpiPair<Epi>::value;
     const uint32_t code = p.g.tile * 32 + wave_waves(p);
     if constexpr (sizeof(T) == 2) {
-        if (!wave_dword_rows(planned_gemm(p))) {
+        if (product_registers(p)) {
             switch (code) {
             case 16 * 32 + 8: if constexpr (PAIR) return run_wave_t<T, Epi, BK, true, 1, 8, 1, 2>(p, e, s); break;
             case 16 * 32 + 16: if constexpr (!PAIR) return run_wave_t<T, Epi, BK, true, 1, 16, 1, 4>(p, e, s); break;
