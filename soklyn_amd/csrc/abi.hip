@@ -2121,22 +2121,27 @@ bool plan_copied(const ProductLaunch &p, Copies *c, GemmPlan *plan) {
 // 11.1 on the K-splitting kernel's 64x64 tiles; 500 x 6000, K 800: 31.1, 24.0; 801 x 5008, K 600: 31.2, 27.7;
 // but 4000 x 1432, K 400 (384 tiles): 36.0, 39.0.  (Of whole tiles: 1024 x 2048, K 512, 128 of them: 15.1,
 // 10.2; 2048 x 2048, 256: 18.7, 19.9.)  Where the rows are not on 4 columns they go element by
-// element, and two workgroups to every CU are wanted (2000 x 1531, K 1000: 32.6, 24.4; the projection
-// 38.7, 32.3; 8000 x 2047, K 1531: 160, 207).
+// element, and nearly two workgroups to every CU are wanted (2000 x 1531, K 1000: 32.6, 24.4; the projection
+// 38.7, 32.3; 8000 x 2047, K 1531: 160, 207).  Over 1800 random sizes the K-splitting kernel's time is of the
+// other's: error 0.85 to 0.94 at 200 to 300 tiles and 0.89 to 1.13 at 300 to 400; of odd rows 0.72 to 0.98 and 0.89
+// to 1.18, then 1.07 to 1.28 at 400 to 512, from K 300 on (projection 1.06 to 1.4).
 bool slow_dma(const ProductLaunch &p) {
     const uint64_t tiles = (uint64_t)((p.g.M + 127) / 128) * ((p.g.N + 127) / 128);
     const bool whole = p.g.M % 128 == 0 && p.g.N % 128 == 0 && p.g.K % 128 == 0;
     if (p.kind == Product::Ungate && tiles < (whole ? 200u : 300u)) return true;
-    return (p.kind == Product::Ungate || p.kind == Product::Project) && p.g.N % 4 != 0 && tiles < 512;
+    return (p.kind == Product::Ungate || p.kind == Product::Project) && p.g.N % 4 != 0 && tiles < 400;
 }
 
 // A pair's 32x16 tiles take 16 columns of a k-row from each matrix, in fp16 32 bytes, its 64x32 tiles twice
-// as many; the planner prices both as tiles of one matrix of twice the columns.  With work for the whole
-// card 64x32 are ahead (fp16 200 x 1024, K 2048: 9.7 us, 32x16 11.8; 500 x 1025, K 777: 15.0, 23.6; but
-// 200 x 1024, K 1200: 10.4, 8.4).
+// as many; the planner prices both as tiles of one matrix of twice the columns.  From 128 of the larger tiles on
+// these are ahead whatever K, from 64 on with a long one; fewer leave CUs idle.  Their time is, over 1900 random
+// sizes, of the smaller tiles' (K up to 200, to 800, above): below 64 tiles 1, 1.02, 1.3; to 128 1, 1, 0.89; to
+// 192 0.99, 0.89, 0.68; to 256 0.98, 0.79, 0.57; above 0.56, 0.52, 0.43; with operands through registers to 64 tiles
+// 1.05, 1.2, 2; to 128 1.03, 1.2, 1.25; to 192 0.97, 0.91, 0.9; to 256 0.83, 0.78, 0.7.
 bool wide_pair(const ProductLaunch &p) {
     const uint64_t tiles = (uint64_t)((p.g.M + 63) / 64) * ((p.g.N + 31) / 32);
-    return p.kind == Product::Pair && p.g.dtype == SKL_F16 && tiles * p.g.K >= 160000;
+    return p.kind == Product::Pair && p.g.dtype == SKL_F16 &&
+           (tiles >= 128 || (tiles >= 64 && p.g.K >= 800 && !product_registers(p)));
 }
 
 // The kernel of a product whose g, kind and epilogue are set, in p.dma and p.g (rag, tile, waves); `copies`

@@ -219,19 +219,35 @@ size_t product_rows_bytes(uint32_t M, uint32_t N, uint32_t matrices) {
     return (size_t)kSlices * matrices * M * N * sizeof(float);
 }
 
-// Past 32 rows, four blocks of rows have registers in fp16 only, and one matrix wants enough columns and
-// k for its two launches (projection, 64 rows: 3000 x 3000 13.2 us, one launch 11.0; 4096 x 1024 9.8 and
-// 9.2; 4096 x 8192 25.4 and 28.0).  Past 16 rows, 32 columns of one fp32 matrix to a wave do too little for the two blocks of x (the fp32
-// MFMAs bound it: projection 4096 x 8192, 32 rows, 42 us, the K-splitting kernel 30), and a pair of
-// short k and few columns has too few steps to a wave (2048 x 2048 fp16, 32 rows: 11.6 and 9.6; 2048 x
-// 8192: 21.8 and 31.2).
+// Where the two launches are ahead of the K-splitting kernel's one: k long enough for eight slices of it (that
+// kernel's 16x16 tiles take a step more behind every 1024 k, a pair's behind every 512, and so it loses what it
+// was ahead in some places).  Both measured with weights from memory, k of 512 to 16384 and 64 to 8192 columns (us, the
+// K-splitting kernel behind the stroke).  Short k are ahead only for a pair of enough columns:
+//   one row     fp16 pair 3008 x 64 8.7/9.4, 2048 x 256 9.1/8.3, 2904 x 256 9.9/12.1, 2048 x 512 10.9/14.2, 1504 x 512
+//               8.9/7.6, 1504 x 1024 10.6/10.8; fp32 pair 2048 x 64 8.3/8.5, 1504 x 256 9.0/9.4, 1024 x 1024 9.6/10.2
+//               projection fp16 3008 x 64 6.4/6.7, 2048 x 512 6.9/5.9, fp32 3008 x 64 7.5/8.0
+// Past 16 rows the sums of the blocks of rows take more of the registers, and the fp32 MFMAs bound one matrix
+// (4096 x 8192, 32 rows: 42/30); past 32 rows four blocks have registers in fp16 only:
+//   32 rows     fp16 pair 3008 x 256 10.5/11.4, 2048 x 1024 12.6/13.5, 1504 x 8192 19.0/17.3; fp32 pair 3008 x 256
+//               19.6/20.7, 2048 x 4096 24.2/22.1; fp16 projection 3480 x 264 8.1/9.6, 3008 x 512 8.2/7.3, 3008 x 1024 9.6/10.8
+//   64 rows     fp16 pair 3880 x 384 13.7/16.2, 3008 x 256 12.7/10.4, 3008 x 512 14.9/17.4; projection 8192 x 256
+//               14.0/18.9, 4096 x 2048 13.8/18.2, 4096 x 1024 11.9/12.3, 3008 x 4096 16.5/15.0
 bool product_rows_size(uint32_t dtype, uint32_t M, uint32_t N, uint32_t K, uint32_t matrices) {
-    const uint64_t t = dtype == 1 ? 2 : 4;
-    const uint32_t lane = dtype == 1 ? 8 : 4;
-    const bool rows = M <= 16 || (M <= 32 && (dtype == 1 || matrices == 2) && (K >= 3000 || N >= 4096)) ||
-                      (M <= 64 && dtype == 1 && K >= 3000 && (matrices == 2 || (K >= 4000 && N >= 4000)));
-    return M && rows && N >= 256 && (uint64_t)matrices * K >= 3000 && N % lane == 0 && K % lane == 0 &&
-           (K + 64ull) * N * t < (1ull << 31);
+    const bool half = dtype == 1, pair = matrices == 2;
+    const uint64_t t = half ? 2 : 4;
+    const uint32_t lane = half ? 8 : 4;
+    bool ahead = false;
+    if (M <= 16)
+        ahead = N >= 64 && (K >= 3000 || (pair && (half ? (K >= 1500 && (uint64_t)K * N >= 1u << 20) || (K >= 2100 && N >= 256)
+                                                        : K >= 2000 || (K >= 1500 && N >= 256))));
+    else if (M <= 32 && pair)
+        ahead = N >= 256 && (K >= 3000 || (half && K >= 2000 && N >= 512));
+    else if (M <= 32)
+        ahead = half && N >= 256 && K >= (N >= 1000 ? 3000 : 3100);
+    else if (M <= 64 && half)
+        ahead = pair ? N >= 256 && K >= (N >= 512 ? 3000 : 3100)
+                     : N >= 256 && (K >= 8000 || (K >= 4000 && N >= 2000));
+    return M && ahead && N % lane == 0 && K % lane == 0 && (K + 64ull) * N * t < (1ull << 31);
 }
 
 bool product_rows_ok(const ProductLaunch &p) {

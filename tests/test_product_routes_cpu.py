@@ -51,3 +51,33 @@ def test_one_launch(route, kind, M, N, K, kernel):
 @pytest.mark.parametrize("M,N,K", [(8872, 2856, 1752), (13233, 3320, 776), (12833, 1528, 3800)])
 def test_pairs_over_copies(route, M, N, K):
     assert route(GATED, F16, M, N, K) == "dma:256:copied"
+
+
+# few rows: the stream over the weights where it is measured ahead of the K-splitting kernel, on both sides of its borders
+@pytest.mark.parametrize("kind,dtype,M,N,K,rows", [
+    (GATED, F16, 1, 64, 3000, True), (GATED, F16, 1, 56, 3000, False), (GATED, F16, 1, 256, 2048, False), (GATED, F16, 16, 512, 2048, True),
+    (GATED, F16, 16, 512, 1504, False), (GATED, F16, 16, 1024, 1504, True), (GATED, F16, 1, 4096, 1024, False),
+    (GATED, F32, 16, 64, 2000, True), (GATED, F32, 1, 512, 1504, True), (GATED, F32, 1, 256, 1504, True), (GATED, F32, 1, 248, 1504, False), (GATED, F16, 16, 256, 2904, True), (PROJECT, F16, 1, 64, 3000, True),
+    (PROJECT, F16, 1, 4096, 2048, False), (PROJECT, F32, 16, 4096, 2048, False), (PROJECT, F32, 17, 4096, 8192, False),
+    (GATED, F16, 17, 512, 2048, True), (GATED, F16, 32, 8192, 1504, False), (GATED, F32, 32, 4096, 2048, False),
+    (GATED, F32, 32, 256, 3000, True), (GATED, F32, 33, 4096, 8192, False), (PROJECT, F16, 32, 512, 3008, False), (PROJECT, F16, 32, 264, 3480, True), (GATED, F16, 48, 384, 3880, True),
+    (PROJECT, F16, 32, 1024, 3008, True), (GATED, F16, 33, 256, 3008, False), (GATED, F16, 64, 512, 3008, True),
+    (PROJECT, F16, 64, 4096, 3008, False), (PROJECT, F16, 64, 2048, 4096, True), (PROJECT, F16, 64, 256, 8192, True),
+    (GATED, F16, 65, 4096, 8192, False), (ERROR, F16, 1, 4096, 8192, False), (GRAD, F16, 1, 4096, 8192, False)])
+def test_few_rows(route, kind, dtype, M, N, K, rows):
+    assert (route(kind, dtype, M, N, K) == "rows") == rows
+
+
+# a pair's tiles: 64x32 once there are enough of them
+@pytest.mark.parametrize("M,N,K,off,tile", [(632, 1256, 69, 0, 64), (256, 2432, 448, 0, 64), (200, 480, 2700, 0, 32), (182, 544, 3000, 0, 32),
+                                            (300, 416, 1200, 0, 64), (300, 416, 1200, WEIGHTS, 32), (448, 281, 2560, 0, 32)])
+def test_tiles_of_a_pair(route, M, N, K, off, tile):
+    how = route(GATED, F16, M, N, K, off=off)
+    assert how.startswith(f"wave:{tile}:"), how
+
+
+# 128x128 tiles of an error or projection of odd rows: from 400 on
+@pytest.mark.parametrize("kind,M,N,K,dma", [(ERROR, 2752, 2835, 4032, True), (ERROR, 2000, 1531, 1000, False), (PROJECT, 2752, 2835, 4032, True),
+                                            (PROJECT, 2000, 1531, 1000, False)])
+def test_odd_rows(route, kind, M, N, K, dma):
+    assert route(kind, F16, M, N, K).startswith("dma") == dma
