@@ -217,19 +217,21 @@ class Workspace:
 
     def product(self, *sizes: int) -> tuple[int | None, int]:
         """For skl_product_work_bytes(*sizes): dtype, batch, inputs, outputs, matrices."""
-        return self._sized("skl_product_work_bytes", sizes)
+        size = self._sizes.get(sizes)
+        return self._first("skl_product_work_bytes", sizes, sizes) if size is None else self.get(size) if size else (None, 0)
 
     def gradient(self, *sizes: int) -> tuple[int | None, int]:
         """For skl_product_grad_work_bytes(*sizes)."""
-        return self._sized("skl_product_grad_work_bytes", sizes)
-
-    def _sized(self, how: str, sizes: tuple[int, ...]) -> tuple[int | None, int]:
-        size = self._sizes.get((how, sizes))
+        size = self._sizes.get(("gradient", sizes))
         if size is None:
-            if len(self._sizes) >= 1024:
-                self._sizes.clear()
-            size = self._sizes[how, sizes] = getattr(load(), how)(*sizes)
+            return self._first("skl_product_grad_work_bytes", ("gradient", sizes), sizes)
         return self.get(size) if size else (None, 0)
+
+    def _first(self, how: str, key: tuple, sizes: tuple) -> tuple[int | None, int]:
+        if len(self._sizes) >= 1024:
+            self._sizes.clear()
+        size = self._sizes[key] = getattr(load(), how)(*sizes)
+        return self.get(size)
 
 
 class Context:

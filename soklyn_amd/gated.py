@@ -37,9 +37,11 @@ class Gated(abi.Tracked):
 
     def _weights(self):
         """The addresses of wg, wu, bg and bu, looked at each time: a tensor held by reference may have become another."""
-        t, wide, row = self.dtype, (self.inputs, self.outputs), (1, self.outputs)
-        return (self._at("wg", self.wg, t, wide), self._at("wu", self.wu, t, wide), self._at("bg", self.bg, t, row),
-                self._at("bu", self.bu, t, row))
+        t, n, dev, need = self.dtype, self.outputs, self.ctx.device, abi.need
+        wg, wu, bg, bu = self.wg, self.wu, self.bg, self.bu
+        wide, row = (self.inputs, n), (1, n)
+        return (None if wg is None else need("wg", wg, t, wide, dev), None if wu is None else need("wu", wu, t, wide, dev),
+                None if bg is None else need("bg", bg, t, row, dev), None if bu is None else need("bu", bu, t, row, dev))
 
     def _descs(self, rows: int, weights: bool = True):
         """This thread's descriptors of gate, up and the layer above; weights: with the weights as they are now."""
@@ -65,13 +67,14 @@ class Gated(abi.Tracked):
                 u: torch.Tensor | None = None) -> torch.Tensor:
         """out [rows x outputs] from x [rows x inputs]; a and u (of out's shape), where given, are kept for the
         backward."""
-        rows, t = x.shape[0], self.dtype
-        wide = (rows, self.outputs)
+        ctx, rows, t, k, n, need = self.ctx, x.shape[0], self.dtype, self.inputs, self.outputs, abi.need
+        dev, wide = ctx.device, (rows, n)
         gate, up, _, (rg, ru, _) = self._descs(rows)
-        gate.preact, up.preact = self._at("a", a, t, wide), self._at("u", u, t, wide)
-        rc = self._call[0](self.ctx.h, rg, ru, self._at("x", x, t, (rows, self.inputs)), rows, self.inputs, rows,
-                           self._at("out", out, t, wide),
-                           *self.work.product(int(self.half), rows, self.inputs, self.outputs, 2))
+        gate.preact = None if a is None else need("a", a, t, wide, dev)
+        up.preact = None if u is None else need("u", u, t, wide, dev)
+        rc = self._call[0](ctx.h, rg, ru, need("x", x, t, (rows, k), dev), rows, k, rows,
+                           None if out is None else need("out", out, t, wide, dev),
+                           *self.work.product(int(self.half), rows, k, n, 2))
         if rc:
             raise abi.SklError("skl_gated_forward", rc)
         return out
@@ -112,13 +115,14 @@ class Gated(abi.Tracked):
 
     def input_grad(self, dg: torch.Tensor, du: torch.Tensor, dx: torch.Tensor) -> torch.Tensor:
         """dx [rows x inputs] (fp32) from the gradients of both projections' results, of the blocks' type."""
-        rows, t, half = dg.shape[0], self.dtype, self.half
+        ctx, rows, t, n, half, need = self.ctx, dg.shape[0], self.dtype, self.outputs, self.half, abi.need
+        dev, wide = ctx.device, (rows, n)
         gate, up, _, (rg, ru, _) = self._descs(rows)
-        for d, g, n in ((gate, dg, "dg"), (up, du, "du")):
-            p = self._at(n, g, t, (rows, self.outputs))
-            d.d_prenorm, d.d_prenorm_h = (None, p) if half else (p, None)
-        rc = self._call[3](self.ctx.h, rg, ru, rows, self._at("dx", dx, _F32, (rows, self.inputs)),
-                           *self.work.gradient(int(self.half), rows, self.outputs, self.inputs, 2))
+        pg, pu = need("dg", dg, t, wide, dev), None if du is None else need("du", du, t, wide, dev)
+        gate.d_prenorm, gate.d_prenorm_h, up.d_prenorm, up.d_prenorm_h = (None, pg, None, pu) if half else (pg, None, pu, None)
+        rc = self._call[3](ctx.h, rg, ru, rows,
+                           None if dx is None else need("dx", dx, _F32, (rows, self.inputs), dev),
+                           *self.work.gradient(int(half), rows, n, self.inputs, 2))
         if rc:
             raise abi.SklError("skl_gated_input_grad", rc)
         return dx

@@ -139,9 +139,9 @@ class Projection(abi.Tracked):
 
     def _weights(self):
         """The addresses of w and b, looked at each time: a tensor held by reference may have become another."""
-        t, n, dev = self.dtype, self.outputs, self.ctx.device
-        return (None if self.w is None else abi.need("w", self.w, t, (self.inputs, n), dev),
-                None if self.b is None else abi.need("b", self.b, t, (1, n), dev))
+        t, n, dev, w, b = self.dtype, self.outputs, self.ctx.device, self.w, self.b
+        return (None if w is None else abi.need("w", w, t, (self.inputs, n), dev),
+                None if b is None else abi.need("b", b, t, (1, n), dev))
 
     def _desc(self, rows: int) -> abi.SklDenseDesc:
         own = self._local.__dict__
