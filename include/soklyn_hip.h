@@ -142,8 +142,9 @@ const char *skl_status_string(int32_t status);
  * next DenseBlock call that launches one records start_event and stop_event
  * (hipEvent_t, created by the caller) at its own start and end, through its
  * dispatch (no marker packets enter the stream); the GEMM alone, not the
- * operand staging, element-wise or reduction kernels around it.  The hook then
- * clears itself.  NULL, NULL clears it.  Not an entry-point call in the sense
+ * operand staging, element-wise or reduction kernels around it (of few rows of a
+ * gated forward or a projection, the sums over slices of k without the kernel that
+ * joins them).  The hook then clears itself.  NULL, NULL clears it.  Not an entry-point call in the sense
  * of skl_dense_backward's column-sum reuse. */
 int32_t skl_ctx_time_next_gemm(skl_ctx *ctx, void *start_event, void *stop_event);
 
@@ -328,8 +329,9 @@ size_t skl_mxfp4_work_bytes(uint32_t inputs, uint32_t outputs, uint32_t batch);
 /* ---- gated feed-forward blocks (no counterpart in the reference) ------------- */
 /* Two blocks over one input, without norms, whose results are multiplied:
  *   a = in . Wg + bg,  u = in . Wu + bu,  out = act(a) * u
- * one kernel.  gate (any activation but Softmax) and up (Identity) have the same type,
- * inputs and outputs; a NULL b is no bias.  in is [in_rows x inputs] T, its first `batch`
+ * in one pass: one kernel, up to 64 rows over a long k two (sums of slices of k, then the
+ * rest), over ragged fp16 operands up to three copies in front of it.  gate (any activation
+ * but Softmax) and up (Identity) have the same type, inputs and outputs; a NULL b is no bias.  in is [in_rows x inputs] T, its first `batch`
  * rows are used; out is [batch x outputs] T.  Where gate->preact / up->preact are not
  * NULL, a / u are kept there (rounded to T) for the backward.  out is computed from the
  * fp32 sums and rounded once.  No output may overlap an input.  The activations here and in
@@ -338,8 +340,9 @@ size_t skl_mxfp4_work_bytes(uint32_t inputs, uint32_t outputs, uint32_t batch);
  * work (16-byte aligned, or NULL): skl_product_work_bytes(dtype, batch, inputs, outputs,
  * 2) bytes of the caller's for padded copies of ragged fp16 operands, or for the sums over
  * slices of a long k where the rows are few; with less, a kernel runs that does without
- * (the same result but for the order of its sums).  What it
- * holds does not outlive the call; calls that overlap in time need a work of their own.
+ * (the same result but for the order of its sums).  What it holds does not outlive the call;
+ * calls that overlap in time need a work of their own, and a captured one keeps its as long
+ * as its graph.
  * Weights of 2^31 bytes and more, and launches of 2^32 threads, are refused
  * (SKL_ERR_INVALID_CONFIGURATION), here and in the calls below. */
 int32_t skl_gated_forward(skl_ctx *ctx, const skl_dense_desc *gate, const skl_dense_desc *up, const void *in,
@@ -372,7 +375,7 @@ size_t skl_product_grad_work_bytes(uint32_t dtype, uint32_t batch, uint32_t inpu
 
 /* ---- a block's result added to the residual stream, dropout (no counterpart) --- */
 /* z = in . W + b,  h = scale * x + drop(act(z)): a block without a norm (any activation but
- * Softmax; a NULL b is no bias), its dropout and the residual stream in one kernel.  x and
+ * Softmax; a NULL b is no bias), its dropout and the residual stream in one pass, as above.  x and
  * h are [batch x outputs] of stream_dtype (SKL_F32, or SKL_F16 with fp16 blocks); h may be
  * x, in place; x NULL: h = drop(act(z)).  Where blk->preact is not NULL, z is kept there
  * (rounded to T) for the backward; the block's other caches are not used.  h is computed

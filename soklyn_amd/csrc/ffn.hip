@@ -26,12 +26,14 @@ static uint32_t flat_groups(uint64_t items, uint32_t each) {
 static bool on16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 template <typename T, int V> struct FlatVec { T v[V]; };
-template <typename T, int V> using FlatBits = uint32_t __attribute__((ext_vector_type(V * sizeof(T) / 4)));   // 8 or 16 bytes
+// 8 or 16 bytes
+template <typename T, int V> using FlatBits = uint32_t __attribute__((ext_vector_type(V * sizeof(T) / 4)));
 template <typename T, int V> __device__ __forceinline__ void flat_load(const T *p, uint64_t i, float (&to)[V]) {
     if constexpr (V == 1) {
         to[0] = to_f32(p[i]);
     } else {
-        const FlatVec<T, V> v = __builtin_bit_cast(FlatVec<T, V>, __builtin_nontemporal_load(reinterpret_cast<const FlatBits<T, V> *>(p + i)));
+        const FlatVec<T, V> v =
+            __builtin_bit_cast(FlatVec<T, V>, __builtin_nontemporal_load(reinterpret_cast<const FlatBits<T, V> *>(p + i)));
 #pragma unroll
         for (int j = 0; j < V; ++j) to[j] = to_f32(v.v[j]);
     }

@@ -1,9 +1,11 @@
 // ffn_rows.hip — the forward products of ffn.h for up to 64 rows (gfx950): a stream over the weights.
 //
 // k goes in up to eight slices, each to an XCD or to neighbours that halve its columns (workgroup L runs
-// on XCD L % 8), so that an XCD reads whole or half rows of W [k x n] and 256 workgroups are in flight;
-// within a slice a workgroup owns 16 VN columns of each matrix of a pair and its waves share the slice's
-// k, 32 k (fp16) or 16 k (fp32) to a step.  The weights go from memory to registers as they are stored, VN columns of a k-row to a lane, 16 lanes to the row.  fp16
+// on XCD L % 8), so that an XCD reads whole or half rows of W [k x n]; within a slice a workgroup owns 16 VN
+// columns of each matrix of a pair and its waves share the slice's k, 32 k (fp16) or 16 k (fp32) to a step.
+// With eight slices 256 workgroups are in flight from 4096 columns on (VN 8; VN 4: 2048), and fewer below:
+// 64 of 1024 columns.  The weights go from memory to registers as they are stored, VN columns of a k-row to a
+// lane, 16 lanes to the row.  fp16
 // lanes turn 8 k-rows into fragments by permutes, one MFMA (16x16x32) for each of their VN columns,
 // whose n index is then VN (lane % 16) + j; fp32 lanes hold a fragment (16x16x4) as loaded.  The waves'
 // sums are added in LDS, the slices' by a second launch, both in a fixed order, in front of the epilogue.
@@ -12,10 +14,11 @@
 // memory, the K-splitting kernel's tiles of 16 to 64 columns over all of k in brackets, where each XCD has
 // a narrow strip of every row and few waves share a long k: pair fp16 8192 x 4096 30 us (63; floor 26),
 // 4096 x 8192 29 (36; 26), 11008 x 4096 37 (83; 35), 3000 x 3000 14 (21; 7), 4096 x 1024 13 (27; 3); fp32
-// 4096 x 8192 52 (66; 52); projection fp16 8192 x 4096 18 (28; 13), 3000 x 3000 9.3 (10; 3.5).  The second
-// launch costs 3 to 4 us of it: below 3000 elements of k in all matrices the other's one launch is ahead
-// (projection 2048 x 2048: 9.2 and 6.2), and so it can be where caches hold the weights (pair 4096 x 1024,
-// called again at once: 9.6 and 7.5), which a network's layers between two calls do not leave there.
+// 4096 x 8192 52 (66; 52); projection fp16 8192 x 4096 18 (28; 13), 3000 x 3000 9.3 (10; 3.5).  Narrower layers
+// stay 2 to 4 times over the floor: too few workgroups for the memory, and 3 to 4 us of the second launch.  For
+// that launch the other kernel is ahead where k is short (product_rows_size), and it can be where caches hold
+// the weights (pair 4096 x 1024, called again at once: 9.6 and 7.5), which a network's layers between two
+// calls do not leave there.
 // 17 to 32 rows have two blocks of rows to a fragment of the weights, more have four; fp16 lanes then own 4
 // columns, as the sums of 8 would not leave registers for the loads ahead.  32 rows: pair fp16 8192 x 4096
 // 37 (69), 4096 x 8192 33 (38), 11008 x 4096 45 (93), fp32 4096 x 8192 61 (75); projection fp16 8192 x 4096
@@ -184,7 +187,8 @@ __global__ void __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(W /
 }
 
 // The sums of the S slices' planes, 4 columns to a thread, and the epilogue.
-template <class Epi, int P, int S> __global__ void __launch_bounds__(64) rows_join_kernel(GemmShape sh, const float *planes, typename Epi::Params ep) {
+template <class Epi, int P, int S>
+__global__ void __launch_bounds__(64) rows_join_kernel(GemmShape sh, const float *planes, typename Epi::Params ep) {
     const uint32_t per = sh.N / 4, q = blockIdx.x * 64 + threadIdx.x, m = q / per, n = q % per * 4;
     if (m >= sh.M) return;
     floatx4 v[S][P];

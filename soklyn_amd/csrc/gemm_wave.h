@@ -438,9 +438,9 @@ __device__ __forceinline__ void wave_mfma(floatx4 (&acc)[MB][NB], const FA &fa, 
 
 // Epilogues that read tensors of their own per element (kReads) declare Pre, load, finish for 4 columns
 // and Pre1, load1, finish1 for one; their loads are issued before the tile's own (64x64 tiles: behind
-// the k loop), all at once for up to 4 groups or 8 elements of a thread, otherwise in batches of that many: one at a time, each behind
-// the stores of the last, they waited for HBM row by row (two read tensors, 2000 x 1531, K 777, fp16: 45 us,
-// 35 in batches).
+// the k loop), all at once for up to 4 groups or 8 elements of a thread, otherwise in batches of that
+// many: one at a time, each behind the stores of the last, they waited for HBM row by row (two read
+// tensors, 2000 x 1531, K 777, fp16: 45 us, 35 in batches).
 
 // Grid: (tiles, splits); split y reduces k in [y k_per_split, (y + 1) k_per_split)
 // (k_per_split whole k-tiles).  WPE: waves per SIMD the registers are budgeted for.

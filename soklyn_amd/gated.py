@@ -21,7 +21,8 @@ _F32, _F16 = torch.float32, torch.float16
 class Gated(abi.Tracked):
     """The weights wg and wu [inputs x outputs] and biases [1 x outputs] (or None) of both projections, held by
     reference; act is the gate's activation.  The weights may be None where only error_from_sum and hidden_error
-    are called.  Calls share a workspace and follow each other on one stream."""
+    are called.  Calls share a workspace and follow each other on one stream; the object, which holds it,
+    outlives the graphs that its calls were captured into."""
 
     def __init__(self, ctx: abi.Context, wg: torch.Tensor | None, wu: torch.Tensor | None, bg: torch.Tensor | None = None,
                  bu: torch.Tensor | None = None, *, outputs: int, half: bool = False, act: int = abi.ACT_SILU,

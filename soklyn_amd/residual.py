@@ -123,7 +123,8 @@ class Projection(abi.Tracked):
     """A layer whose result, with dropout, is added to the stream: weights w [inputs x outputs] and bias b
     [1 x outputs] (or None) of the blocks' type, held by reference.  No mask is stored: the backward draws
     it again from the seed.  w may be None where only the backward is called.  Calls share a workspace and
-    follow each other on one stream."""
+    follow each other on one stream; the object, which holds it, outlives the graphs that its calls were
+    captured into."""
 
     def __init__(self, ctx: abi.Context, w: torch.Tensor | None, b: torch.Tensor | None = None, *, outputs: int,
                  half: bool = False, act: int = abi.ACT_IDENTITY, leaky: float = 0.0, dropout: float = 0.0,
